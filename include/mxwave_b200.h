@@ -52,6 +52,12 @@ extern "C" {
 #define MXW_DAMP_ABSOLUTE 0
 #define MXW_DAMP_RELATIVE 1
 
+/* Activations of mxw_linear_mxfp4 (GELU is the erf form). */
+#define MXW_ACT_NONE 0
+#define MXW_ACT_RELU 1
+#define MXW_ACT_SILU 2
+#define MXW_ACT_GELU 3
+
 /* Bits of the device flag word written by the kernels. */
 #define MXW_FLAG_NONFINITE 1 /* the input held a NaN or infinity                 */
 #define MXW_FLAG_TIMEOUT 2   /* a bounded on-device wait gave up; output invalid */
@@ -261,6 +267,31 @@ MXW_API int mxw_finalize_moments(const float* sum_abs, const float* sum_sq, int6
  */
 MXW_API int mxw_finalize_block_hessian(const float* gram, int full, int64_t cols, int64_t ldg,
                                int64_t count, double damp, int mode, float* out, void* stream);
+
+/*
+ * y = act(x W^T + bias) + residual with W [outs, inner] held in MXFP4 as
+ * mxw_quantize_mxfp4 writes it (packed [outs, inner/2], scales [outs,
+ * inner/32]): the product that a model quantized by this library runs, without
+ * dequantizing W.  No counterpart in the reference, whose consumers dequantize
+ * (mxwave/core.py:254-278).
+ *   x         [rows, inner] bf16 or f16 (`dtype`), row stride ldx
+ *   bias      [outs] of x's type, or NULL;  act: MXW_ACT_*
+ *   residual  [rows, outs] of x's type, row stride ldr, or NULL
+ *   y         [rows, outs] of x's type, contiguous; y == residual is allowed
+ *             when ldr == outs
+ *   workspace device memory, 16-byte aligned, of at least
+ *             mxw_linear_workspace_size(rows, inner, dtype) bytes; calls that
+ *             share one must not overlap on the device
+ * inner % 32 == 0; packed 8-byte aligned.  fp32 accumulation; the fixed order
+ * of additions makes results reproducible.  A row of x that holds a NaN or an
+ * infinity gives NaN in all its outputs; so does a scale byte 255.
+ * flags: MXW_FLAG_TIMEOUT or NULL.
+ */
+MXW_API size_t mxw_linear_workspace_size(int64_t rows, int64_t inner, int dtype);
+MXW_API int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t inner, int64_t ldx,
+                             const uint8_t* packed, const uint8_t* scales, int64_t outs, const void* bias, int act,
+                             const void* residual, int64_t ldr, void* y, void* workspace, size_t workspace_bytes,
+                             uint32_t* flags, void* stream);
 
 #ifdef __cplusplus
 }

@@ -29,6 +29,11 @@ MXW_METHOD_RTN = 1
 MXW_DAMP_ABSOLUTE = 0
 MXW_DAMP_RELATIVE = 1
 
+MXW_ACT_NONE = 0
+MXW_ACT_RELU = 1
+MXW_ACT_SILU = 2
+MXW_ACT_GELU = 3
+
 MXW_FLAG_NONFINITE = 1
 MXW_FLAG_TIMEOUT = 2
 MXW_FLAG_RARE = 4
@@ -66,6 +71,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mxw_repack_gguf_mxfp4": (_int, [_vp, _vp, _i64, _i64, _vp, _vp]),
     "mxw_error_sums_noalloc": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp,
                                       _vp]),
+    "mxw_linear_workspace_size": (ctypes.c_size_t, [_i64, _i64, _int]),
+    "mxw_linear_mxfp4": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _int, _vp, _i64, _vp, _vp,
+                                ctypes.c_size_t, _vp, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,75 @@
+// Block-scaled tcgen05 products (kind::mxf8f6f4) in inline PTX, sm_100a: the
+// tensor cores read E2M1 and E4M3 operands with one E8M0 scale per 32 elements
+// of the contraction, which is MXFP4 as the quantizer stores it.
+#pragma once
+
+#include <stdint.h>
+
+#include "tcgen05.cuh"
+#include "tma.cuh"
+
+namespace mxw {
+
+// Instruction descriptor, kind::mxf8f6f4: A = E2M1, B = E4M3, E8M0 scales,
+// fp32 D, both operands K-major.  The two scale ids (which byte of a TMEM
+// scale word the instruction takes) are OR-ed in by mx_idesc_scale_byte.
+__host__ __device__ constexpr uint32_t make_idesc_e2m1_e4m3(int m, int n) {
+  return (5u << 7)                                   // A format: E2M1
+         | (0u << 10)                                // B format: E4M3
+         | (static_cast<uint32_t>(n >> 3) << 17)     // N / 8
+         | (1u << 23)                                // scale format: E8M0
+         | (static_cast<uint32_t>(m >> 4) << 24);    // M / 16
+}
+
+__device__ __forceinline__ uint32_t mx_idesc_scale_byte(uint32_t idesc, uint32_t byte) {
+  return idesc | (byte << 4) | (byte << 29);
+}
+
+// D[128 x N] (+)= (A 2^sa) (B 2^sb)^T over 32 elements of K.
+__device__ __forceinline__ void mma_mxf8f6f4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// Copies the scales of 128 operand rows x 4 blocks (512 bytes of shared memory,
+// [row % 32][row / 32][block]) to four TMEM columns of all four lane quarters.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
+  const uint64_t desc = make_smem_desc_k_noswz(saddr, 0, 128);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Untiled asynchronous copies into shared memory.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(smem_dst)),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t saddr, const void* src, uint32_t src_bytes) {
+  static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16, "cp.async copies 4, 8 or 16 bytes");
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(saddr), "l"(src), "r"(src_bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(saddr), "l"(src), "r"(src_bytes), "n"(BYTES)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Programmatic dependent launch: wait for the kernel before this one in the
+// stream; let the next one be scheduled.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependents_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+}  // namespace mxw

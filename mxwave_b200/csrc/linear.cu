@@ -1,0 +1,517 @@
+// K8: matrix product with MXFP4 weights, y = act(x W^T + bias) + residual.
+//
+// W [N, K] is what the quantizer wrote: E2M1 codes and one E8M0 exponent per
+// 32 inputs.  That is an operand format of the tensor cores (kind::mxf8f6f4),
+// so the codes go to them as they are and nothing is dequantized.  The other
+// operand has to be 8 bits wide, so x is split exactly into a sum of E4M3
+// terms with E8M0 block scales (E4M3 carries 4 significant bits: two terms for
+// bf16's 8, three for f16's 11):
+//   s = 2^(floor(log2 amax) - 7) of the block of 32,  t0 = e4m3(x / s),
+//   t1 = e4m3((x / s - t0) 2^5),  t2 = e4m3(((x / s - t0) 2^5 - t1) 2^5)
+// with scales s, s 2^-5, s 2^-10.  Every remainder is exact in fp32.  An
+// element at least 2^-13 of its block's largest is represented exactly; a
+// smaller one to within 2^-22 of the block's largest (E4M3's subnormals).
+// Products and sums are fp32 in TMEM.  A block that holds a NaN or an infinity
+// gets the NaN scale: every output of that row of x is NaN.
+//
+// Two launches:
+//   linear_terms_kernel   x -> terms and scales, as images of the shared-memory
+//                         tiles the product reads (K-major, 128-byte swizzle)
+//   linear_kernel         the product with its epilogue
+// CTA tile: 128 outputs (M, W's rows) x NT rows of x (N).  Four warps copy W's
+// codes with 8-byte cp.async into the 16-byte slots that E2M1 operands take in
+// shared memory (8 bytes of codes, 8 of padding) and its scales into the
+// tensor cores' scale layout; the terms come as bulk copies.  One thread of
+// a fifth warp issues the products.  When there are too few tiles for the SMs
+// the CTAs of a cluster split K and add their fp32 partial tiles over
+// distributed shared memory in rank order, so results do not change from run
+// to run.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cooperative_groups.h>
+
+#include "blockscale.cuh"
+#include "common.cuh"
+#include "runtime.h"
+
+namespace cg = cooperative_groups;
+
+namespace mxw {
+
+constexpr int kLinM = 128;       // outputs per tile
+constexpr int kLinK = 128;       // inputs per stage
+constexpr int kLinLoaders = 128;  // threads that copy W, and the epilogue's
+constexpr int kLinThreads = kLinLoaders + 32;
+constexpr int kLinWBytes = kLinM * kLinK;  // E2M1 in shared memory: 16 bytes per 16 codes
+constexpr int kLinSfBytes = 512;           // scales of 128 rows x 4 blocks
+
+template <int NT, int TERMS>
+struct LinearTile {
+  static constexpr int kTermBytes = NT * kLinK;
+  static constexpr int kSfTiles = (NT + 127) / 128;  // 128-row groups of the x scales
+  static constexpr int kTermSfBytes = kSfTiles * kLinSfBytes;
+  static constexpr int kXBytes = TERMS * (kTermBytes + kTermSfBytes);  // one chunk of x in the workspace
+  static constexpr int kStageBytes = kLinWBytes + kLinSfBytes + kXBytes;
+  static constexpr int kBudget = NT <= 32 ? 110 * 1024 : 220 * 1024;  // two CTAs per SM for small tiles
+  static constexpr int kStages = kBudget / ((kStageBytes + 1023) / 1024 * 1024) < 8
+                                     ? kBudget / ((kStageBytes + 1023) / 1024 * 1024)
+                                     : 8;
+  static_assert(kStages >= 2, "a stage must fit twice");
+  static constexpr int kStageStride = (kStageBytes + 1023) / 1024 * 1024;
+  static constexpr int kSmem = kStages * kStageStride + 1024 + 256;
+  // TMEM: the accumulator, then the scales of two stages.
+  static constexpr uint32_t kSfCols = 4 * (1 + TERMS * kSfTiles);
+  static constexpr uint32_t kCols = NT + 2 * kSfCols;
+  static constexpr uint32_t kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+};
+
+struct LinearParams {
+  const uint8_t* packed;
+  const uint8_t* scales;
+  const uint8_t* terms;  // [token tiles][chunks][kXBytes]
+  const void* bias;
+  const void* residual;
+  int64_t ldr;
+  void* y;
+  int64_t rows, outs, inner;
+  int chunks;
+  int act;
+  int words;  // the scales of a row start on a 4-byte boundary
+  uint32_t* flags;
+};
+
+// ------------------------------------------------------------- terms of x
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
+  const __half2 hh = *reinterpret_cast<__half2*>(&h);
+  return make_float2(__low2float(hh), __high2float(hh));
+}
+
+struct TermsParams {
+  const void* x;
+  int64_t ldx, rows, inner;
+  int chunks;
+  uint8_t* terms;
+};
+
+// Sixteen threads take the 128 inputs of one (row, chunk), eight each; four
+// neighbours share a block.  VEC: rows start on 16-byte boundaries.
+template <bool BF16, int NT, bool VEC>
+__global__ void __launch_bounds__(256) linear_terms_kernel(const TermsParams P) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Tile = LinearTile<NT, TERMS>;
+  grid_dependents_launch();
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
+  const int part = threadIdx.x & 15;
+  const int64_t padded = (P.rows + NT - 1) / NT * NT;
+  const bool in_grid = unit < padded * P.chunks;  // uniform over the sixteen threads
+  const int64_t row = in_grid ? unit / P.chunks : 0;
+  const int chunk = in_grid ? static_cast<int>(unit % P.chunks) : 0;
+  const int64_t k0 = static_cast<int64_t>(chunk) * kLinK + part * 8;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  if (in_grid && row < P.rows && k0 < P.inner) {  // inner % 32 == 0: eight inputs are in or out together
+    const uint16_t* src = static_cast<const uint16_t*>(P.x) + row * P.ldx + k0;
+    uint16_t raw[8];
+    if constexpr (VEC) {
+      *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) raw[i] = src[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = BF16 ? bits_f32(static_cast<uint32_t>(raw[i]) << 16) : __half2float(*reinterpret_cast<__half*>(&raw[i]));
+  }
+  uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  // byte = 127 + floor(log2 amax) - 7, at least 0; 255 (NaN) for a non-finite block.
+  const int ebits = static_cast<int>(amax >> 23);
+  int byte = max(ebits - 7, 0);
+  if (ebits == 255) byte = 255;
+  const float mult = ebits == 255 ? 0.0f : exp2i(127 - byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = ebits == 255 ? 0.0f : __fmul_rn(v[i], mult);
+  if (!in_grid) return;
+  const int r = static_cast<int>(row % NT);
+  uint8_t* base = P.terms + ((row / NT) * P.chunks + chunk) * static_cast<int64_t>(Tile::kXBytes);
+  // 16-byte slot part / 2 of the row's 128 bytes, swizzled over eight rows.
+  uint8_t* dst = base + r * 128 + (((part >> 1) ^ (r & 7)) << 4) + ((part & 1) << 3);
+  uint8_t* sf = base + TERMS * Tile::kTermBytes + (r >> 7) * kLinSfBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (part >> 2);
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint2*>(dst + t * Tile::kTermBytes) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    if ((part & 3) == 0) sf[t * Tile::kTermSfBytes] = static_cast<uint8_t>(byte);
+    if (t + 1 < TERMS) {
+      const int step = byte == 255 ? 0 : min(byte, 5);  // scales do not go below 2^-127
+      const float up = static_cast<float>(1 << step);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 q = e4m3x2_to_f32x2(w[i]);
+        v[2 * i] = __fmul_rn(__fsub_rn(v[2 * i], q.x), up);
+        v[2 * i + 1] = __fmul_rn(__fsub_rn(v[2 * i + 1], q.y), up);
+      }
+      byte -= step;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- epilogue
+
+__device__ __forceinline__ float activate(float v, int act) {
+  switch (act) {
+    case MXW_ACT_RELU:
+      return v > 0.0f ? v : (v != v ? v : 0.0f);
+    case MXW_ACT_SILU:
+      return v / (1.0f + __expf(-v));
+    case MXW_ACT_GELU:
+      return 0.5f * v * erfcf(-0.70710678118654752f * v);
+    default:
+      return v;
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ float load16(const void* p, int64_t i) {
+  const uint16_t b = static_cast<const uint16_t*>(p)[i];
+  return BF16 ? bits_f32(static_cast<uint32_t>(b) << 16) : __half2float(*reinterpret_cast<const __half*>(&b));
+}
+template <bool BF16>
+__device__ __forceinline__ void store16(void* p, int64_t i, float v) {
+  if constexpr (BF16)
+    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else
+    static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// ----------------------------------------------------------------- product
+
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(kLinThreads) linear_kernel(const LinearParams P) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Tile = LinearTile<NT, TERMS>;
+  constexpr int ST = Tile::kStages;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * Tile::kStageStride);
+  uint64_t* empty = full + ST;
+  uint64_t* done = empty + ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* fail = reinterpret_cast<int*>(tmem_slot + 1);
+
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kLinM;
+  const int64_t tile = blockIdx.z;
+  const int c_begin = static_cast<int>(static_cast<int64_t>(P.chunks) * rank / ranks);
+  const int n_chunks = static_cast<int>(static_cast<int64_t>(P.chunks) * (rank + 1) / ranks) - c_begin;
+
+  if (tid == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&full[s], kLinLoaders + 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    *fail = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4) tmem_alloc(tmem_slot, Tile::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    // --------------------------------------------------------------- copies
+    bool ok = true;
+    bool waited = false;  // for the terms of x, which the launch before this one writes
+    const uint8_t* xsrc = P.terms + (tile * P.chunks + c_begin) * static_cast<int64_t>(Tile::kXBytes);
+    int issued = 0;
+    for (int i = 0; i < n_chunks + ST - 2; ++i) {
+      if (i < n_chunks && ok) {
+        const int s = i % ST;
+        if (i >= ST && !mbar_wait(&empty[s], static_cast<uint32_t>((i / ST - 1) & 1))) ok = false;
+        if (ok) {
+          uint8_t* st = smem + s * Tile::kStageStride;  // [W codes][x terms][x scales][W scales]
+          const uint32_t sw = smem_u32(st);
+          const int64_t kbyte = static_cast<int64_t>(c_begin + i) * (kLinK / 2);
+          // 8 pieces of 16 codes per row, 4 rows per warp and step.
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = 16 * j + (tid >> 3), p = tid & 7;
+            const bool in = n0 + r < P.outs && kbyte + 8 * p < P.inner / 2;
+            const uint8_t* src = P.packed + (in ? (n0 + r) * (P.inner / 2) + kbyte + 8 * p : 0);
+            cp_async<8>(sw + r * 128 + ((p ^ (r & 7)) << 4), src, in ? 8u : 0u);
+          }
+          {
+            const int r = tid;
+            const int64_t b0 = static_cast<int64_t>(c_begin + i) * (kLinK / 32);
+            const int64_t nb = P.inner / 32;
+            uint8_t* dst = st + kLinWBytes + Tile::kXBytes + (r & 31) * 16 + (r >> 5) * 4;
+            const bool in = n0 + r < P.outs;
+            const uint8_t* src = P.scales + (in ? (n0 + r) * nb + b0 : 0);
+            if (P.words) {
+              cp_async<4>(smem_u32(dst), src, in ? 4u : 0u);
+            } else {
+              uint32_t w = 0;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (in && b0 + q < nb) w |= static_cast<uint32_t>(src[q]) << (8 * q);
+              *reinterpret_cast<uint32_t*>(dst) = w;
+            }
+          }
+          if (tid == 0) {
+            if (!waited) grid_dependency_wait();
+            waited = true;
+            mbar_arrive_expect_tx(&full[s], Tile::kXBytes);
+            bulk_load(st + kLinWBytes, xsrc, Tile::kXBytes, &full[s]);
+            xsrc += Tile::kXBytes;
+          }
+          ++issued;
+        }
+      }
+      cp_async_commit();
+      cp_async_wait<ST - 2>();
+      const int ready = i - (ST - 2);
+      if (ready >= 0 && ready < issued) {
+        fence_proxy_async_smem();
+        mbar_arrive(&full[ready % ST]);
+      }
+    }
+    if (!ok) {
+      // Stages never filled: the issuer's own wait gives up.  Copies in flight
+      // have to land before the CTA may end.
+      cp_async_wait<0>();
+      if (tid == 0)
+        for (int j = issued > ST ? issued - ST : 0; j < issued; ++j)
+          mbar_wait(&full[j % ST], static_cast<uint32_t>((j / ST) & 1));
+      atomicOr(fail, 1);
+    }
+  } else if (lane == 0) {
+    // ------------------------------------------------------------- products
+    constexpr uint32_t idesc = make_idesc_e2m1_e4m3(kLinM, NT);
+    bool ok = true;
+    for (int i = 0; i < n_chunks; ++i) {
+      const int s = i % ST;
+      if (!mbar_wait(&full[s], static_cast<uint32_t>((i / ST) & 1))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sw = smem_u32(smem + s * Tile::kStageStride);
+      const uint32_t sx = sw + kLinWBytes;
+      const uint32_t sfa = tmem + NT + (i & 1) * Tile::kSfCols;
+      const uint32_t sfb = sfa + 4;
+      tmem_cp_scales(sfa, sx + Tile::kXBytes);
+#pragma unroll
+      for (int t = 0; t < TERMS * Tile::kSfTiles; ++t)
+        tmem_cp_scales(sfb + 4 * t, sx + TERMS * Tile::kTermBytes + t * kLinSfBytes);
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int kk = 0; kk < kLinK / 32; ++kk) {
+          // 32 inputs are 32 bytes of a swizzled 128-byte row.
+          const uint64_t ad = make_smem_desc_mn_sw128(sw + kk * 32, 16, 1024);
+          const uint64_t bd = make_smem_desc_mn_sw128(sx + t * Tile::kTermBytes + kk * 32, 16, 1024);
+          mma_mxf8f6f4(tmem, ad, bd, mx_idesc_scale_byte(idesc, kk), sfa, sfb + 4 * t * Tile::kSfTiles,
+                       (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
+        }
+      mma_commit(&empty[s]);
+    }
+    mma_commit(done);
+    if (!ok) atomicOr(fail, 1);
+  }
+
+  // ---------------------------------------------------------------- epilogue
+  __syncwarp();
+  if (warp < 4 && !__all_sync(0xffffffffu, mbar_wait(done, 0))) atomicOr(fail, 1);
+  tc_fence_after();
+  const int64_t n = n0 + tid;  // this thread's output (warps 0..3)
+  const int64_t t0 = tile * NT;
+  float bias = 0.0f;
+  if (warp < 4 && P.bias && n < P.outs) bias = load16<BF16>(P.bias, n);
+  if (ranks == 1) {
+    if (warp < 4) {
+#pragma unroll 1
+      for (int c = 0; c < NT; c += 16) {
+        if (t0 + c >= P.rows) break;
+        float v[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + c, v);
+        if (n < P.outs) {
+#pragma unroll
+          for (int u = 0; u < 16; ++u) {
+            const int64_t t = t0 + c + u;
+            if (t < P.rows) {
+              float o = activate(__fadd_rn(v[u], bias), P.act);
+              if (P.residual) o = __fadd_rn(o, load16<BF16>(P.residual, t * P.ldr + n));
+              store16<BF16>(P.y, t * P.outs + n, o);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    float* part = reinterpret_cast<float*>(smem);  // [NT][128], in the drained stages
+    if (warp < 4) {
+#pragma unroll 1
+      for (int c = 0; c < NT; c += 16) {
+        float v[16];
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + c, v);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) part[(c + u) * 128 + tid] = v[u];
+      }
+    }
+    cluster_sync_all();
+    if (warp < 4 && n < P.outs) {
+      for (int c = rank; c < NT && t0 + c < P.rows; c += ranks) {
+        float v = 0.0f;
+        for (int k = 0; k < ranks; ++k) v = __fadd_rn(v, cluster.map_shared_rank(part, k)[c * 128 + tid]);
+        float o = activate(__fadd_rn(v, bias), P.act);
+        const int64_t t = t0 + c;
+        if (P.residual) o = __fadd_rn(o, load16<BF16>(P.residual, t * P.ldr + n));
+        store16<BF16>(P.y, t * P.outs + n, o);
+      }
+    }
+    cluster_sync_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Tile::kTmemCols);
+  }
+  if (tid == 0 && *fail && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
+}
+
+// -------------------------------------------------------------------- host
+
+// Rows of x per tile: the smallest tile that takes them all, so that W is read
+// once, up to what two stages of shared memory hold.
+static int linear_tile(int64_t rows, int dtype) {
+  if (rows <= 16) return 16;
+  if (rows <= 32) return 32;
+  if (rows <= 64) return 64;
+  return rows <= 128 || dtype == MXW_F16 ? 128 : 256;
+}
+
+template <bool BF16, int NT>
+static int launch_linear(const TermsParams& T, LinearParams P, cudaStream_t s) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Tile = LinearTile<NT, TERMS>;
+  const int64_t tiles = (P.rows + NT - 1) / NT;
+  const int64_t units = tiles * NT * P.chunks;
+  const bool vec = T.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(T.x) % 16 == 0;
+  const unsigned grid = static_cast<unsigned>((units * 16 + 255) / 256);
+  if (vec)
+    linear_terms_kernel<BF16, NT, true><<<grid, 256, 0, s>>>(T);
+  else
+    linear_terms_kernel<BF16, NT, false><<<grid, 256, 0, s>>>(T);
+  int status = check_launch();
+  if (status != MXW_OK) return status;
+
+  auto kernel = linear_kernel<BF16, NT>;
+  status = set_max_smem(reinterpret_cast<const void*>(kernel), Tile::kSmem);
+  if (status != MXW_OK) return status;
+  const int64_t row_tiles = (P.outs + kLinM - 1) / kLinM;
+  int split = 1;
+  while (split < 8 && row_tiles * tiles * split * 2 <= 2 * num_sms() && split * 4 <= P.chunks) split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(row_tiles), static_cast<unsigned>(tiles));
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = Tile::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(split), 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, P);
+  return err == cudaSuccess ? MXW_OK : record_cuda_error(err);
+}
+
+template <bool BF16>
+static int launch_linear_rows(const TermsParams& T, const LinearParams& P, cudaStream_t s) {
+  switch (linear_tile(P.rows, BF16 ? MXW_BF16 : MXW_F16)) {
+    case 16:
+      return launch_linear<BF16, 16>(T, P, s);
+    case 32:
+      return launch_linear<BF16, 32>(T, P, s);
+    case 64:
+      return launch_linear<BF16, 64>(T, P, s);
+    case 128:
+      return launch_linear<BF16, 128>(T, P, s);
+    default:
+      if constexpr (BF16) return launch_linear<BF16, 256>(T, P, s);
+      return MXW_EUNSUPPORTED;
+  }
+}
+
+}  // namespace mxw
+
+using namespace mxw;
+
+extern "C" size_t mxw_linear_workspace_size(int64_t rows, int64_t inner, int dtype) {
+  if (rows <= 0 || inner <= 0 || (dtype != MXW_BF16 && dtype != MXW_F16)) return 0;
+  const int64_t nt = linear_tile(rows, dtype);
+  const int64_t per_chunk = (dtype == MXW_BF16 ? 2 : 3) * (nt * kLinK + (nt + 127) / 128 * kLinSfBytes);
+  return static_cast<size_t>((rows + nt - 1) / nt * ((inner + kLinK - 1) / kLinK) * per_chunk);
+}
+
+extern "C" int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t inner, int64_t ldx,
+                                const uint8_t* packed, const uint8_t* scales, int64_t outs, const void* bias, int act,
+                                const void* residual, int64_t ldr, void* y, void* workspace, size_t workspace_bytes,
+                                uint32_t* flags, void* stream) {
+  if (rows < 0 || outs < 0 || inner <= 0 || inner % 32 != 0 || ldx < inner) return MXW_EINVAL;
+  if (dtype != MXW_BF16 && dtype != MXW_F16) return MXW_EINVAL;
+  if (act < MXW_ACT_NONE || act > MXW_ACT_GELU) return MXW_EINVAL;
+  if (residual && ldr < outs) return MXW_EINVAL;
+  if (rows == 0 || outs == 0) return MXW_OK;
+  if (!x || !packed || !scales || !y || !workspace) return MXW_EINVAL;
+  if (reinterpret_cast<uintptr_t>(packed) % 8 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return MXW_EINVAL;
+  if (workspace_bytes < mxw_linear_workspace_size(rows, inner, dtype)) return MXW_EINVAL;
+  // Grid limits: 65535 tiles of 128 outputs and of 128 rows; 2^31 blocks of terms.
+  if (outs > 65535ll * kLinM || rows > 65535ll * 128 || inner > (1ll << 30)) return MXW_EUNSUPPORTED;
+  if ((rows + 256) * ((inner + kLinK - 1) / kLinK) / 16 >= (1ll << 31) - 1) return MXW_EUNSUPPORTED;
+  TermsParams T{};
+  T.x = x;
+  T.ldx = ldx;
+  T.rows = rows;
+  T.inner = inner;
+  T.chunks = static_cast<int>((inner + kLinK - 1) / kLinK);
+  T.terms = static_cast<uint8_t*>(workspace);
+  LinearParams P{};
+  P.packed = packed;
+  P.scales = scales;
+  P.terms = T.terms;
+  P.bias = bias;
+  P.residual = residual;
+  P.ldr = ldr;
+  P.y = y;
+  P.rows = rows;
+  P.outs = outs;
+  P.inner = inner;
+  P.chunks = T.chunks;
+  P.act = act;
+  P.words = inner % 128 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
+  P.flags = flags;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == MXW_BF16 ? launch_linear_rows<true>(T, P, s) : launch_linear_rows<false>(T, P, s);
+}

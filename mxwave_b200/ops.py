@@ -23,6 +23,17 @@ Operators (reference function each one backs):
 * ``finalize_moments(sums, count, root) -> fp32`` -- calibration.py:262-266.
 * ``finalize_block_hessian(gram, full, count, damp, mode) -> fp32`` --
   calibration.py:267-270 with core.py:61-69.
+
+Serving operators (no counterpart in the reference; ``mxwave_b200.linear``
+holds their public functions and argument checks):
+
+* ``linear_mxfp4(x, packed, scales, bias?, residual?, act) -> y`` -- the product
+  with quantized weights.
+
+These have an implementation function of the same name with a leading
+underscore, which the public functions call directly for plain eager CUDA
+tensors: dispatching a custom operator costs more host time than their
+smallest calls take on the device.
 """
 
 from __future__ import annotations
@@ -235,6 +246,66 @@ def _(gram, full, count, damp, mode):
     return gram.new_empty((cols // 32, 32, 32), dtype=torch.float32)
 
 
+# ----------------------------------------------------------------- serving
+
+
+def plain_eager(t: Tensor) -> bool:
+    """Whether a call on `t` may skip the operator dispatch: an ordinary tensor, and
+    nothing (FakeTensor, tracing, compilation, another dispatch mode) is watching."""
+    return type(t) is Tensor and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
+
+
+class _on_device:
+    """``torch.cuda.device(d)`` that does nothing when `d` is current already."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, device: torch.device) -> None:
+        self.index = device.index
+
+    def __enter__(self) -> None:
+        self.previous = torch._C._cuda_getDevice()
+        if self.previous != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *exc: object) -> None:
+        if self.previous != self.index:
+            torch._C._cuda_setDevice(self.previous)
+
+
+def _raw_stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _linear_mxfp4(x: Tensor, packed: Tensor, scales: Tensor, bias: Tensor | None, residual: Tensor | None,
+                  act: int) -> Tensor:
+    rows, inner = x.shape
+    outs = packed.shape[0]
+    y = torch.empty((rows, outs), dtype=x.dtype, device=x.device)
+    if rows == 0 or outs == 0:
+        return y
+    lib = _lib.load()
+    code = _DTYPE_CODES[x.dtype]
+    nbytes = lib.mxw_linear_workspace_size(rows, inner, code)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    with _on_device(x.device):
+        status = lib.mxw_linear_mxfp4(
+            x.data_ptr(), code, rows, inner, x.stride(0) if rows > 1 else inner, packed.data_ptr(), scales.data_ptr(),
+            outs, _ptr(bias), act, _ptr(residual), residual.stride(0) if residual is not None and rows > 1 else outs,
+            y.data_ptr(), workspace.data_ptr(), nbytes, None, _raw_stream(x.device),
+        )
+    _lib.check(status, "mxw_linear_mxfp4")
+    return y
+
+
+linear_mxfp4 = torch.library.custom_op("mxwave_b200::linear_mxfp4", _linear_mxfp4, mutates_args=())
+
+
+@linear_mxfp4.register_fake
+def _(x, packed, scales, bias, residual, act):
+    return x.new_empty((x.shape[0], packed.shape[0]))
+
+
 OPS = (
     quantize_mxfp4,
     dequant_mxfp4,
@@ -243,6 +314,7 @@ OPS = (
     accumulate_xtx_,
     finalize_moments,
     finalize_block_hessian,
+    linear_mxfp4,
 )
 
 __all__ = [
@@ -253,5 +325,6 @@ __all__ = [
     "dequant_mxfp4",
     "finalize_block_hessian",
     "finalize_moments",
+    "linear_mxfp4",
     "quantize_mxfp4",
 ]
