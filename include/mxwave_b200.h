@@ -293,6 +293,73 @@ MXW_API int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t inn
                              const void* residual, int64_t ldr, void* y, void* workspace, size_t workspace_bytes,
                              uint32_t* flags, void* stream);
 
+/*
+ * A paged key/value cache in MXFP4.  One layer of it is
+ *   codes  [pages][2 (key, value)][heads][page_tokens][dim / 2]
+ *   scales [pages][2][heads][page_tokens][dim / 32]
+ * both 16-byte aligned, each row encoded as a weight row (E2M1, element 2j in
+ * the low nibble; E8M0 per 32).  page_tokens is 16, 32, 64 or 128, dim 64 or
+ * 128.  Slot s is token s % page_tokens of page s / page_tokens.
+ * No counterpart in the reference, which quantizes weights only.
+ *
+ * mxw_kv_append encodes key and value rows [tokens][heads][dim] (unit stride
+ * over dim; token and head strides in elements) of `dtype` under the rule of
+ * MXW_METHOD_RTN (core.py:91-104) and writes them to their slots.  Slots
+ * outside the pool are skipped (padding: -1); slots of one call are distinct.
+ * mxw_kv_gather reads rows back as values of `dtype`, [tokens][heads][dim]
+ * contiguous, 16-byte aligned; zeros for slots outside the pool.
+ */
+MXW_API int mxw_kv_append(uint8_t* codes, uint8_t* scales, int64_t pages, int64_t heads, int64_t page_tokens,
+                          int64_t dim, const void* key, const void* value, int dtype, int64_t key_token,
+                          int64_t key_head, int64_t value_token, int64_t value_head, const int64_t* slots,
+                          int64_t tokens, void* stream);
+MXW_API int mxw_kv_gather(const uint8_t* codes, const uint8_t* scales, int64_t pages, int64_t heads,
+                          int64_t page_tokens, int64_t dim, const int64_t* slots, int64_t tokens, int dtype,
+                          void* key, void* value, void* stream);
+
+/*
+ * Copies pages source[i] -> target[i], i < n, in each of `layers` layers
+ * (codes [layers][pages][code_bytes], scales [layers][pages][scale_bytes], both
+ * sizes multiples of 16).  `source` and `target` are HOST arrays, read before
+ * the call returns; they travel as kernel arguments, so a captured launch
+ * keeps them.  No target may be a source or appear twice (MXW_EINVAL).
+ */
+MXW_API int mxw_copy_pages(uint8_t* codes, uint8_t* scales, int64_t layers, int64_t pages, int64_t code_bytes,
+                           int64_t scale_bytes, const int64_t* source, const int64_t* target, int64_t n, void* stream);
+
+/*
+ * Softmax attention of packed queries over one layer of such a cache:
+ *   out[i, h] = sum_j softmax_j(softmax_scale q[i, h] . k[j, h'] + mask) v[j, h']
+ *   query   [tokens][heads][dim] bf16 or f16 (`dtype`; token and head strides in
+ *           elements); heads is a multiple of kv_heads, h' = h / (heads / kv_heads)
+ *   table   [seqs][table_width] int32 (row stride table_ld): each sequence's pages
+ *   lengths [seqs] int32: its cached tokens, the new ones included (at most
+ *           table_width * page_tokens are read)
+ *   start   [seqs + 1] int32: its queries are rows start[b] .. start[b + 1]
+ *           - 1, the last tokens of the sequence
+ * causal: query i sees keys up to its own position; window > 0 (causal only):
+ * the last `window` of those.  max_length and max_queries bound lengths and the
+ * queries of a sequence; they size the launch (results hold if they are wrong,
+ * speed does not).  Pages outside [0, pages) are not read: their keys are left
+ * out.  A query without a key gives zeros and -infinity; so do rows of `out`
+ * that no sequence covers.
+ *   out [tokens][heads][dim] of `dtype`; lse [tokens][heads] fp32 (natural log
+ *   of the sum of exponentials) or NULL.
+ * workspace: device memory, 16-byte aligned, of at least
+ * mxw_paged_attention_workspace_size bytes for the same arguments; calls that
+ * share one must not overlap on the device.
+ * fp32 statistics and sums in a fixed order.
+ */
+MXW_API size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,
+                                                  int64_t max_length, int64_t max_queries);
+MXW_API int mxw_paged_attention(const void* query, int dtype, int64_t tokens, int64_t heads, int64_t q_token,
+                                int64_t q_head, const uint8_t* codes, const uint8_t* scales, int64_t pages,
+                                int64_t kv_heads, int64_t page_tokens, int64_t dim, const int32_t* table,
+                                int64_t table_ld, int64_t table_width, const int32_t* lengths, const int32_t* start,
+                                int64_t seqs, int64_t max_length, int64_t max_queries, double softmax_scale,
+                                int causal, int64_t window, void* out, float* lse, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,6 +74,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mxw_linear_workspace_size": (ctypes.c_size_t, [_i64, _i64, _int]),
     "mxw_linear_mxfp4": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _int, _vp, _i64, _vp, _vp,
                                 ctypes.c_size_t, _vp, _vp]),
+    "mxw_kv_append": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64,
+                             _vp]),
+    "mxw_kv_gather": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _int, _vp, _vp, _vp]),
+    "mxw_copy_pages": (_int, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp]),
+    "mxw_paged_attention_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "mxw_paged_attention": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64,
+                                   _i64, _vp, _vp, _i64, _i64, _i64, ctypes.c_double, _int, _i64, _vp, _vp, _vp,
+                                   ctypes.c_size_t, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,365 @@
+// K9: a paged key/value cache in MXFP4: writing rows, reading them back, and
+// copying pages.
+//
+// One layer of the cache is
+//   codes  [pages][2 (key, value)][kv heads][page tokens][dim / 2]
+//   scales [pages][2][kv heads][page tokens][dim / 32]
+// with every row encoded as the quantizer encodes a weight row (E2M1, element
+// 2j in the low nibble; E8M0 per 32 elements) under its `rtn` rule:
+//   e = floor(log2 amax) - 2, plus 1 when amax >= 1.75 2^floor(log2 amax)
+// clamped to [-127, 127].  Token `slot` lives in page slot / page_tokens.
+//
+// All three kernels move bytes once and are bound by HBM; a row's 4.25 bits per
+// element leave too little arithmetic to matter.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdlib.h>
+
+#include "common.cuh"
+#include "runtime.h"
+
+namespace mxw {
+
+constexpr int kKvThreads = 256;
+
+struct KvRows {
+  uint8_t* codes;
+  uint8_t* scales;
+  const int64_t* slots;
+  int64_t tokens, n_slots;  // slots of the pool
+  int heads, dim, page;
+  int units;      // eight-element pieces of a token: 2 heads dim / 8
+  int per_block;  // tokens per block
+};
+
+// Where piece `r` of a token lies: part (0 key, 1 value), head, first element.
+struct KvPiece {
+  int part, head, d;
+};
+__device__ __forceinline__ KvPiece kv_piece(const KvRows& P, int r) {
+  const int shift = P.dim == 128 ? 4 : 3;
+  const int hh = r >> shift;
+  const int part = hh >= P.heads ? 1 : 0;
+  return {part, hh - part * P.heads, (r & ((1 << shift) - 1)) * 8};
+}
+
+// The row's index among all rows of the pool.
+__device__ __forceinline__ int64_t kv_row(const KvRows& P, int64_t slot, const KvPiece& p) {
+  const int64_t page = slot / P.page, offset = slot - page * P.page;
+  return ((page * 2 + p.part) * P.heads + p.head) * P.page + offset;
+}
+
+template <int DT>
+__device__ __forceinline__ float kv_load(const void* p, int64_t i) {
+  if constexpr (DT == MXW_BF16) return bits_f32(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
+  if constexpr (DT == MXW_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return static_cast<const float*>(p)[i];
+}
+
+// Eight elements of one row; VEC: 16-byte aligned.
+template <int DT, bool VEC>
+__device__ __forceinline__ void kv_load8(const void* p, int64_t i, float (&v)[8]) {
+  if constexpr (VEC && DT == MXW_F32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else if constexpr (VEC) {
+    uint16_t raw[8];
+    *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = kv_load<DT>(raw, k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = kv_load<DT>(p, i + k);
+  }
+}
+
+struct KvSource {
+  const void *key, *value;
+  int64_t key_token, key_head, value_token, value_head;  // strides in elements
+};
+
+// Eight elements per thread, a block of 32 per four neighbours: the largest
+// magnitude over two shuffles, one 4-byte store of codes each, and the first
+// of them stores the scale.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvRows P, const KvSource S) {
+  const int sub = static_cast<int>(threadIdx.x) / P.units;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * P.per_block + sub;
+  const int first = P.per_block == 1 ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) - sub * P.units;
+  const bool mine = (P.per_block == 1 || sub < P.per_block) && token < P.tokens;
+  const int64_t slot = mine ? P.slots[P.per_block == 1 ? blockIdx.x : token] : -1;
+  const bool kept = slot >= 0 && slot < P.n_slots;
+  // The loop count is the block's, so that the shuffles see whole warps.
+  for (int r0 = 0; r0 < P.units; r0 += P.per_block == 1 ? kKvThreads : P.units) {
+    const int r = first + r0;
+    const bool on = kept && r < P.units;
+    const KvPiece p = kv_piece(P, on ? r : 0);
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (on) {
+      const int64_t at = p.part ? token * S.value_token + p.head * S.value_head + p.d
+                                : token * S.key_token + p.head * S.key_head + p.d;
+      kv_load8<DT, VEC>(p.part ? S.value : S.key, at, v);
+    }
+    uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = max(amax, f32_bits(v[k]) & 0x7fffffffu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // Exponent of the block (the quantizer's rtn rule, its non-finite cases
+    // included: -127 for a NaN or zero maximum, 127 for an infinite one).
+    int e;
+    if (amax > 0x7f800000u || amax == 0u) {
+      e = -127;
+    } else if (amax == 0x7f800000u) {
+      e = 127;
+    } else {
+      const uint32_t safe = max(amax, 0x00800000u);
+      e = static_cast<int>(safe >> 23) - 129 + ((safe & 0x7fffffu) >= 0x600000u ? 1 : 0);
+      e = max(e, -127);
+    }
+    if (on) {
+      const float inv = exp2i(-e);
+      uint32_t word = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a = __fadd_rn(__fmul_rn(v[2 * k], inv), 0.0f), b = __fadd_rn(__fmul_rn(v[2 * k + 1], inv), 0.0f);
+        if (a != a) a = 6.0f;  // a NaN takes the last code, without a sign
+        if (b != b) b = 6.0f;
+        word |= e2m1x2(a, b) << (8 * k);
+      }
+      const int64_t row = kv_row(P, slot, p);
+      *reinterpret_cast<uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2) = word;
+      if ((r & 3) == 0) P.scales[row * (P.dim / 32) + p.d / 32] = static_cast<uint8_t>(e + 127);
+    }
+  }
+}
+
+__device__ __forceinline__ void kv_store8(float* p, const float (&v)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void kv_store8(__nv_bfloat16* p, const float (&v)[8]) {
+  __nv_bfloat162 h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+}
+__device__ __forceinline__ void kv_store8(__half* p, const float (&v)[8]) {
+  __half2 h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(h);
+}
+
+// Rows read back as values, [tokens][heads][dim] each; zeros for a slot that
+// lies outside the pool.
+template <typename OUT>
+__global__ void __launch_bounds__(kKvThreads) kv_gather_kernel(const KvRows P, OUT* key, OUT* value) {
+  const int sub = static_cast<int>(threadIdx.x) / P.units;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * P.per_block + (P.per_block == 1 ? 0 : sub);
+  if (token >= P.tokens || (P.per_block > 1 && sub >= P.per_block)) return;
+  const int64_t slot = P.slots[token];
+  const bool kept = slot >= 0 && slot < P.n_slots;
+  const int first = static_cast<int>(threadIdx.x) - (P.per_block == 1 ? 0 : sub * P.units);
+  for (int r = first; r < P.units; r += P.per_block == 1 ? kKvThreads : P.units) {
+    const KvPiece p = kv_piece(P, r);
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (kept) {
+      const int64_t row = kv_row(P, slot, p);
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2);
+      const float sc = exp2i(static_cast<int>(P.scales[row * (P.dim / 32) + p.d / 32]) - 127);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f2 q = unpack2(e2m1x2_to_f32x2((word >> (8 * k)) & 0xffu));
+        v[2 * k] = __fmul_rn(q.x, sc);
+        v[2 * k + 1] = __fmul_rn(q.y, sc);
+      }
+    }
+    kv_store8((p.part ? value : key) + (token * P.heads + p.head) * P.dim + p.d, v);
+  }
+}
+
+// --------------------------------------------------------------- page copies
+//
+// The pairs travel as a kernel argument: no copy to the device, nothing to
+// keep alive until the launch runs, and the call can be captured in a graph.
+// Two sizes: 16 KB of arguments cost a launch more than 512 bytes do.
+template <int N>
+struct PagePairs {
+  int32_t source[N], target[N];
+};
+
+struct PageCopy {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t pages, layers;
+  int64_t code_vec, scale_vec;  // 16-byte vectors of one page
+  int n;
+};
+
+constexpr int kCopyVecs = 4;  // vectors per thread: enough loads in flight to cover HBM's latency
+
+template <int N>
+__global__ void __launch_bounds__(kKvThreads) copy_pages_kernel(const PageCopy P, const __grid_constant__ PagePairs<N> pairs) {
+  const int64_t layer = blockIdx.z;
+  const int i = blockIdx.y;
+  const int64_t vecs = P.code_vec + P.scale_vec;
+  const int64_t src = layer * P.pages + pairs.source[i], dst = layer * P.pages + pairs.target[i];
+  uint4* codes = reinterpret_cast<uint4*>(P.codes);
+  uint4* scales = reinterpret_cast<uint4*>(P.scales);
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kKvThreads * kCopyVecs) + threadIdx.x;
+  uint4 v[kCopyVecs];
+#pragma unroll
+  for (int k = 0; k < kCopyVecs; ++k) {
+    const int64_t j = base + k * kKvThreads;
+    if (j < P.code_vec)
+      v[k] = codes[src * P.code_vec + j];
+    else if (j < vecs)
+      v[k] = scales[src * P.scale_vec + j - P.code_vec];
+  }
+#pragma unroll
+  for (int k = 0; k < kCopyVecs; ++k) {
+    const int64_t j = base + k * kKvThreads;
+    if (j < P.code_vec)
+      codes[dst * P.code_vec + j] = v[k];
+    else if (j < vecs)
+      scales[dst * P.scale_vec + j - P.code_vec] = v[k];
+  }
+}
+
+template <int N>
+static int launch_copy(PageCopy P, const int64_t* source, const int64_t* target, int64_t n, cudaStream_t s) {
+  const unsigned blocks =
+      static_cast<unsigned>((P.code_vec + P.scale_vec + kKvThreads * kCopyVecs - 1) / (kKvThreads * kCopyVecs));
+  PagePairs<N> pairs;
+  for (int64_t done = 0; done < n; done += N) {
+    P.n = static_cast<int>(std::min<int64_t>(N, n - done));
+    for (int i = 0; i < N; ++i) {
+      pairs.source[i] = i < P.n ? static_cast<int32_t>(source[done + i]) : 0;
+      pairs.target[i] = i < P.n ? static_cast<int32_t>(target[done + i]) : 0;
+    }
+    copy_pages_kernel<N><<<dim3(blocks, static_cast<unsigned>(P.n), static_cast<unsigned>(P.layers)), kKvThreads, 0, s>>>(
+        P, pairs);
+    const int status = check_launch();
+    if (status != MXW_OK) return status;
+  }
+  return MXW_OK;
+}
+
+static bool kv_shape_ok(int64_t pages, int64_t heads, int64_t page, int64_t dim) {
+  if (dim != 64 && dim != 128) return false;
+  if (page != 16 && page != 32 && page != 64 && page != 128) return false;
+  return pages >= 0 && pages <= 0x7fffffff && heads >= 1 && heads <= 1024;
+}
+
+static KvRows kv_rows(uint8_t* codes, uint8_t* scales, const int64_t* slots, int64_t tokens, int64_t pages,
+                      int64_t heads, int64_t page, int64_t dim) {
+  KvRows P{};
+  P.codes = codes;
+  P.scales = scales;
+  P.slots = slots;
+  P.tokens = tokens;
+  P.n_slots = pages * page;
+  P.heads = static_cast<int>(heads);
+  P.dim = static_cast<int>(dim);
+  P.page = static_cast<int>(page);
+  P.units = static_cast<int>(2 * heads * dim / 8);
+  P.per_block = std::max(1, kKvThreads / P.units);
+  return P;
+}
+
+template <int DT>
+static void launch_append(const KvRows& P, const KvSource& S, bool vec, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((P.tokens + P.per_block - 1) / P.per_block);
+  if (vec)
+    kv_append_kernel<DT, true><<<grid, kKvThreads, 0, s>>>(P, S);
+  else
+    kv_append_kernel<DT, false><<<grid, kKvThreads, 0, s>>>(P, S);
+}
+
+}  // namespace mxw
+
+using namespace mxw;
+
+extern "C" int mxw_kv_append(uint8_t* codes, uint8_t* scales, int64_t pages, int64_t heads, int64_t page_tokens,
+                             int64_t dim, const void* key, const void* value, int dtype, int64_t key_token,
+                             int64_t key_head, int64_t value_token, int64_t value_head, const int64_t* slots,
+                             int64_t tokens, void* stream) {
+  if (!kv_shape_ok(pages, heads, page_tokens, dim) || tokens < 0) return MXW_EINVAL;
+  if (dtype != MXW_BF16 && dtype != MXW_F16 && dtype != MXW_F32) return MXW_EINVAL;
+  if (key_token < 0 || key_head < 0 || value_token < 0 || value_head < 0) return MXW_EINVAL;
+  if (tokens == 0 || pages == 0) return MXW_OK;
+  if (!codes || !scales || !key || !value || !slots) return MXW_EINVAL;
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0) return MXW_EINVAL;
+  if (tokens > 0x7fffffff) return MXW_EUNSUPPORTED;
+  const KvRows P = kv_rows(codes, scales, slots, tokens, pages, heads, page_tokens, dim);
+  const KvSource S{key, value, key_token, key_head, value_token, value_head};
+  const int64_t strides = key_token | key_head | value_token | value_head;
+  const bool vec = strides % 8 == 0 && reinterpret_cast<uintptr_t>(key) % 16 == 0 && reinterpret_cast<uintptr_t>(value) % 16 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MXW_BF16)
+    launch_append<MXW_BF16>(P, S, vec, s);
+  else if (dtype == MXW_F16)
+    launch_append<MXW_F16>(P, S, vec, s);
+  else
+    launch_append<MXW_F32>(P, S, vec, s);
+  return check_launch();
+}
+
+extern "C" int mxw_kv_gather(const uint8_t* codes, const uint8_t* scales, int64_t pages, int64_t heads,
+                             int64_t page_tokens, int64_t dim, const int64_t* slots, int64_t tokens, int dtype,
+                             void* key, void* value, void* stream) {
+  if (!kv_shape_ok(pages, heads, page_tokens, dim) || tokens < 0) return MXW_EINVAL;
+  if (dtype != MXW_BF16 && dtype != MXW_F16 && dtype != MXW_F32) return MXW_EINVAL;
+  if (tokens == 0) return MXW_OK;
+  if ((pages > 0 && (!codes || !scales)) || !slots || !key || !value) return MXW_EINVAL;
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(key) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(value) % 16 != 0)
+    return MXW_EINVAL;
+  if (tokens > 0x7fffffff) return MXW_EUNSUPPORTED;
+  const KvRows P = kv_rows(const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales), slots, tokens, pages, heads,
+                           page_tokens, dim);
+  const unsigned grid = static_cast<unsigned>((tokens + P.per_block - 1) / P.per_block);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == MXW_BF16)
+    kv_gather_kernel<<<grid, kKvThreads, 0, s>>>(P, static_cast<__nv_bfloat16*>(key), static_cast<__nv_bfloat16*>(value));
+  else if (dtype == MXW_F16)
+    kv_gather_kernel<<<grid, kKvThreads, 0, s>>>(P, static_cast<__half*>(key), static_cast<__half*>(value));
+  else
+    kv_gather_kernel<<<grid, kKvThreads, 0, s>>>(P, static_cast<float*>(key), static_cast<float*>(value));
+  return check_launch();
+}
+
+extern "C" int mxw_copy_pages(uint8_t* codes, uint8_t* scales, int64_t layers, int64_t pages, int64_t code_bytes,
+                              int64_t scale_bytes, const int64_t* source, const int64_t* target, int64_t n,
+                              void* stream) {
+  if (layers < 0 || pages < 0 || pages > 0x7fffffff || n < 0) return MXW_EINVAL;
+  if (code_bytes <= 0 || scale_bytes <= 0 || code_bytes % 16 != 0 || scale_bytes % 16 != 0) return MXW_EINVAL;
+  if (layers == 0 || n == 0) return MXW_OK;
+  if (!codes || !scales || !source || !target) return MXW_EINVAL;
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0) return MXW_EINVAL;
+  if (layers > 65535 || code_bytes + scale_bytes > (1ll << 40)) return MXW_EUNSUPPORTED;
+  for (int64_t i = 0; i < n; ++i)
+    if (source[i] < 0 || source[i] >= pages || target[i] < 0 || target[i] >= pages) return MXW_EINVAL;
+  // Copies of one call run in no order: a target may be neither a source nor another copy's target.
+  uint8_t* seen = static_cast<uint8_t*>(calloc(static_cast<size_t>(pages), 1));
+  if (!seen) return MXW_EUNSUPPORTED;
+  bool clash = false;
+  for (int64_t i = 0; i < n; ++i) {
+    clash |= seen[target[i]] != 0;
+    seen[target[i]] = 1;
+  }
+  for (int64_t i = 0; i < n; ++i) clash |= seen[source[i]] != 0;
+  free(seen);
+  if (clash) return MXW_EINVAL;
+  PageCopy P{};
+  P.codes = codes;
+  P.scales = scales;
+  P.pages = pages;
+  P.layers = layers;
+  P.code_vec = code_bytes / 16;
+  P.scale_vec = scale_bytes / 16;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return n <= 64 ? launch_copy<64>(P, source, target, n, s) : launch_copy<2000>(P, source, target, n, s);
+}

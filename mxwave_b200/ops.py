@@ -25,10 +25,18 @@ Operators (reference function each one backs):
   calibration.py:267-270 with core.py:61-69.
 
 Serving operators (no counterpart in the reference; ``mxwave_b200.linear``
-holds their public functions and argument checks):
+and ``mxwave_b200.kvcache`` hold their public functions and argument checks):
 
 * ``linear_mxfp4(x, packed, scales, bias?, residual?, act) -> y`` -- the product
   with quantized weights.
+* ``kv_append_mxfp4_(codes, scales, key, value, slots)`` and
+  ``kv_gather_mxfp4(codes, scales, slots, dtype) -> (key, value)`` -- rows of a
+  paged cache in MXFP4 (``mxwave_b200.kvcache``).
+* ``copy_pages_(codes, scales, source, target)`` -- page copies in every layer;
+  ``source`` and ``target`` are host tensors.
+* ``paged_attention_mxfp4(query, codes, scales, table, lengths, query_start,
+  max_length, max_queries, softmax_scale, causal, window, want_lse) -> (out,
+  lse)``; lse is empty unless wanted.
 
 These have an implementation function of the same name with a leading
 underscore, which the public functions call directly for plain eager CUDA
@@ -306,6 +314,113 @@ def _(x, packed, scales, bias, residual, act):
     return x.new_empty((x.shape[0], packed.shape[0]))
 
 
+def _kv_append_mxfp4_(codes: Tensor, scales: Tensor, key: Tensor, value: Tensor, slots: Tensor) -> None:
+    tokens = key.shape[0]
+    if tokens == 0 or codes.shape[0] == 0:
+        return
+    lib = _lib.load()
+    pages, _two, heads, page, half = codes.shape
+    with _on_device(codes.device):
+        status = lib.mxw_kv_append(
+            codes.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, key.data_ptr(), value.data_ptr(),
+            _DTYPE_CODES[key.dtype], key.stride(0), key.stride(1), value.stride(0), value.stride(1), slots.data_ptr(),
+            tokens, _raw_stream(codes.device),
+        )
+    _lib.check(status, "mxw_kv_append")
+
+
+kv_append_mxfp4_ = torch.library.custom_op("mxwave_b200::kv_append_mxfp4_", _kv_append_mxfp4_,
+                                           mutates_args=("codes", "scales"))
+
+
+@kv_append_mxfp4_.register_fake
+def _(codes, scales, key, value, slots):
+    return None
+
+
+def _kv_gather_mxfp4(codes: Tensor, scales: Tensor, slots: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
+    pages, _two, heads, page, half = codes.shape
+    tokens = slots.shape[0]
+    key = torch.empty((tokens, heads, 2 * half), dtype=dtype, device=codes.device)
+    value = torch.empty_like(key)
+    if tokens == 0:
+        return key, value
+    lib = _lib.load()
+    with _on_device(codes.device):
+        status = lib.mxw_kv_gather(codes.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, slots.data_ptr(),
+                                   tokens, _DTYPE_CODES[dtype], key.data_ptr(), value.data_ptr(),
+                                   _raw_stream(codes.device))
+    _lib.check(status, "mxw_kv_gather")
+    return key, value
+
+
+kv_gather_mxfp4 = torch.library.custom_op("mxwave_b200::kv_gather_mxfp4", _kv_gather_mxfp4, mutates_args=())
+
+
+@kv_gather_mxfp4.register_fake
+def _(codes, scales, slots, dtype):
+    shape = (slots.shape[0], codes.shape[2], 2 * codes.shape[4])
+    return codes.new_empty(shape, dtype=dtype), codes.new_empty(shape, dtype=dtype)
+
+
+def _copy_pages_(codes: Tensor, scales: Tensor, source: Tensor, target: Tensor) -> None:
+    layers, pages = codes.shape[:2]
+    n = source.shape[0]
+    if n == 0 or layers == 0:
+        return
+    lib = _lib.load()
+    with _on_device(codes.device):
+        status = lib.mxw_copy_pages(codes.data_ptr(), scales.data_ptr(), layers, pages, codes[0, 0].numel(),
+                                    scales[0, 0].numel(), source.data_ptr(), target.data_ptr(), n,
+                                    _raw_stream(codes.device))
+    _lib.check(status, "mxw_copy_pages")
+
+
+copy_pages_ = torch.library.custom_op("mxwave_b200::copy_pages_", _copy_pages_, mutates_args=("codes", "scales"))
+
+
+@copy_pages_.register_fake
+def _(codes, scales, source, target):
+    return None
+
+
+def _paged_attention_mxfp4(query: Tensor, codes: Tensor, scales: Tensor, table: Tensor, lengths: Tensor,
+                           query_start: Tensor, max_length: int, max_queries: int, softmax_scale: float, causal: bool,
+                           window: int, want_lse: bool) -> tuple[Tensor, Tensor]:
+    tokens, heads, dim = query.shape
+    pages, _two, kv_heads, page, _half = codes.shape
+    seqs, width = table.shape
+    lse = torch.empty((tokens, heads) if want_lse else (0,), dtype=torch.float32, device=query.device)
+    if tokens == 0 or seqs == 0 or max_queries == 0:
+        return torch.zeros((tokens, heads, dim), dtype=query.dtype, device=query.device), lse.fill_(float("-inf"))
+    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=query.device)
+    lib = _lib.load()
+    with _on_device(query.device):
+        nbytes = lib.mxw_paged_attention_workspace_size(seqs, heads, kv_heads, dim, max_length, max_queries)
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+        status = lib.mxw_paged_attention(
+            query.data_ptr(), _DTYPE_CODES[query.dtype], tokens, heads, query.stride(0), query.stride(1),
+            codes.data_ptr(), scales.data_ptr(), pages, kv_heads, page, dim, table.data_ptr(), table.stride(0), width,
+            lengths.data_ptr(), query_start.data_ptr(), seqs, max_length, max_queries, softmax_scale, causal, window,
+            out.data_ptr(), lse.data_ptr() if want_lse else None, workspace.data_ptr(), nbytes,
+            _raw_stream(query.device),
+        )
+    _lib.check(status, "mxw_paged_attention")
+    return out, lse
+
+
+paged_attention_mxfp4 = torch.library.custom_op("mxwave_b200::paged_attention_mxfp4", _paged_attention_mxfp4,
+                                                mutates_args=())
+
+
+@paged_attention_mxfp4.register_fake
+def _(query, codes, scales, table, lengths, query_start, max_length, max_queries, softmax_scale, causal, window,
+      want_lse):
+    tokens, heads, _dim = query.shape
+    return (query.new_empty(query.shape),
+            query.new_empty((tokens, heads) if want_lse else (0,), dtype=torch.float32))
+
+
 OPS = (
     quantize_mxfp4,
     dequant_mxfp4,
@@ -315,6 +430,10 @@ OPS = (
     finalize_moments,
     finalize_block_hessian,
     linear_mxfp4,
+    kv_append_mxfp4_,
+    kv_gather_mxfp4,
+    copy_pages_,
+    paged_attention_mxfp4,
 )
 
 __all__ = [
@@ -322,9 +441,13 @@ __all__ = [
     "accumulate_activation_stats_",
     "accumulate_moments_",
     "accumulate_xtx_",
+    "copy_pages_",
     "dequant_mxfp4",
     "finalize_block_hessian",
     "finalize_moments",
+    "kv_append_mxfp4_",
+    "kv_gather_mxfp4",
     "linear_mxfp4",
+    "paged_attention_mxfp4",
     "quantize_mxfp4",
 ]
