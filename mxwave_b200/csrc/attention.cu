@@ -29,10 +29,10 @@
 //     of the largest, nothing lost above 2^-31.  Their sum is taken in fp32
 //     before the rounding.  m is raised only when a score passes it by 8
 //     (binary), which spares most tiles the reduction and the rescaling.
-//   * Four warps of a block take tiles of 16 keys in turn, each with its own
+//   * Four warps of a block take steps of 32 keys in turn, each with its own
 //     running maximum and sum, its own ring of asynchronous copies and no
 //     synchronisation with the others until the end of a segment.
-// Work split: the (sequence, head, row group) units are cut into tiles of 64
+// Work split: the (sequence, head, row group) units are cut into tiles of 128
 // keys, all tiles are laid end to end, and each block takes an equal share of
 // them, whatever the lengths.  A unit that several blocks share leaves partial
 // results (normalised rows and their log-sum-exp) in the workspace, two slots
@@ -48,9 +48,11 @@ namespace mxw {
 
 constexpr int kAttWarps = 4;
 constexpr int kAttThreads = kAttWarps * 32;
-constexpr int kAttKeys = 16;                      // keys per warp step
+constexpr int kAttHalf = 16;                      // keys per matrix instruction
+constexpr int kAttKeys = 2 * kAttHalf;            // keys per warp step
 constexpr int kAttTile = kAttWarps * kAttKeys;    // keys per block step
-constexpr int kAttStages = 4;
+constexpr int kAttStages = 3;
+constexpr int kAttJoinThreads = 256;
 constexpr float kAttLift = 7.0f;    // probabilities are held as 2^(x - m + 7)
 constexpr float kAttSlack = 8.0f;   // and x may pass m by 8 before m is raised: at most 2^15
 
@@ -65,6 +67,7 @@ struct AttParams {
   const int32_t* lengths;
   const int32_t* start;
   int64_t tokens;
+  int q_vec;  // 16-byte loads of the queries are aligned
   int seqs, heads, kv_heads, group, page_shift;
   float scale_log2;  // softmax scale times log2(e)
   int causal, window;
@@ -77,8 +80,8 @@ struct AttParams {
 struct AttSeq {
   int q0, queries;  // its rows of the packed queries
   int length;       // cached tokens
-  int lo;           // first key that some query sees, rounded down to a tile step
-  int tiles;        // tiles of 64 keys from lo on, at least one
+  int lo;           // first key that some query sees, rounded down to 16
+  int tiles;        // tiles of 128 keys from lo on, at least one
   int row_groups;   // groups of 8 NT rows per key/value head
 };
 
@@ -90,7 +93,7 @@ __device__ __forceinline__ AttSeq att_seq(const AttParams& P, int b) {
   s.queries = static_cast<int>(max(static_cast<int64_t>(0), min(last, P.tokens) - s.q0));
   const int64_t held = P.table_width << P.page_shift;
   s.length = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(P.lengths[b]), held)));
-  s.lo = P.window > 0 ? max(0, s.length - s.queries - P.window + 1) / kAttKeys * kAttKeys : 0;
+  s.lo = P.window > 0 ? max(0, s.length - s.queries - P.window + 1) / kAttHalf * kAttHalf : 0;
   s.tiles = max(1, (s.length - s.lo + kAttTile - 1) / kAttTile);
   s.row_groups = (s.queries * P.group + ROWS - 1) / ROWS;
   return s;
@@ -101,6 +104,7 @@ __device__ __forceinline__ int64_t att_work(const AttParams& P, const AttSeq& s)
 }
 
 // Sum over the block (all threads get it); `red` holds one word per warp.
+template <int THREADS>
 __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -109,36 +113,46 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* red) {
   __syncthreads();
   int64_t sum = 0;
 #pragma unroll
-  for (int w = 0; w < kAttWarps; ++w) sum += red[w];
+  for (int w = 0; w < THREADS / 32; ++w) sum += red[w];
   return sum;
 }
 
 // All tiles, and the tiles of the sequences before `upto`.
-template <int ROWS>
+template <int ROWS, int THREADS>
 __device__ __forceinline__ void att_totals(const AttParams& P, int upto, int64_t* red, int64_t& total, int64_t& before) {
   int64_t all = 0, part = 0;
-  for (int b = threadIdx.x; b < P.seqs; b += kAttThreads) {
+  for (int b = threadIdx.x; b < P.seqs; b += THREADS) {
     const int64_t w = att_work(P, att_seq<ROWS>(P, b));
     all += w;
     if (b < upto) part += w;
   }
-  total = block_sum(all, red);
-  before = block_sum(part, red);
+  total = block_sum<THREADS>(all, red);
+  before = upto > 0 ? block_sum<THREADS>(part, red) : 0;
 }
 
-__device__ __forceinline__ int64_t att_first_tile(int64_t total, int64_t block, int64_t blocks) {
-  return total / blocks * block + total % blocks * block / blocks;
-}
+// Equal shares of `total` tiles: the first total % blocks of them are one larger.
+struct AttShares {
+  int64_t each, more;
+  __device__ __forceinline__ AttShares(int64_t total, int64_t blocks) : each(total / blocks), more(total % blocks) {}
+  __device__ __forceinline__ int64_t first(int64_t block) const { return each * block + min(block, more); }
+  __device__ __forceinline__ int64_t block_of(int64_t tile) const {
+    const int64_t large = (each + 1) * more;
+    return tile < large ? tile / (each + 1) : more + (tile - large) / each;
+  }
+};
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t e2m1x2_to_f16x2(uint32_t byte) {
-  uint32_t h;
-  asm("{\n\t.reg .b8 t;\n\tcvt.u8.u32 t, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, t;\n\t}" : "=r"(h) : "r"(byte));
-  return h;
+// The f16 pairs of a word's four bytes.
+__device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t word, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(word));
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -167,27 +181,20 @@ __device__ __forceinline__ uint32_t f16_pow2_13_minus(int n) {
   return n <= 27 ? static_cast<uint32_t>(28 - n) << 10 : 0x400u >> min(n - 27, 31);
 }
 
-// The f16 pair of byte q of a word.
-#define MXW_PAIR(word, q) e2m1x2_to_f16x2((word) >> (8 * (q)))
-
 template <int D, int NT>
 struct AttShape {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kCodes = kAttKeys * D / 2;    // bytes of 16 rows
-  static constexpr int kScales = kAttKeys * D / 32;
-  static constexpr int kStage = 2 * (kCodes + kScales);
+  static constexpr int kCodes = kAttHalf * D / 2;    // bytes of 16 rows
+  static constexpr int kScales = kAttHalf * D / 32;
+  static constexpr int kHalf = 2 * (kCodes + kScales);  // 16 keys and values: [K codes][V codes][K scales][V scales]
+  static constexpr int kStage = 2 * kHalf;
   static constexpr int kRing = kAttStages * kStage;
-  static constexpr int kJoin = kAttWarps * kRows * D * 4;  // fp32 rows of each warp
-  static constexpr int kSmem = kAttWarps * kRing + kJoin;
+  static constexpr int kJoin = kAttWarps * kRows * D * 4;  // fp32 rows of each warp, in the drained rings
+  static constexpr int kSmem = kAttWarps * kRing > kJoin ? kAttWarps * kRing : kJoin;
   static constexpr int kBlocks = NT == 1 ? 4 : 3;  // per SM: 128 and 168 registers a thread
   static constexpr int kSlot = kRows * D + kRows;  // floats of a partial result
 };
 
-template <bool BF16>
-__device__ __forceinline__ float att_load_q(const void* q, int64_t i) {
-  const uint16_t b = static_cast<const uint16_t*>(q)[i];
-  return BF16 ? bits_f32(static_cast<uint32_t>(b) << 16) : __half2float(*reinterpret_cast<const __half*>(&b));
-}
 template <bool BF16>
 __device__ __forceinline__ void att_store(void* p, int64_t i, float v) {
   if constexpr (BF16)
@@ -216,6 +223,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
   constexpr int ROWS = Shape::kRows;
   constexpr int QREGS = D / 8;       // f16 pairs of a query row per lane
   constexpr int STEPS = D / 16;      // k16 steps of S, and 16-channel groups of O
+  constexpr int BLOCKS = D / 32;     // scales per row
   extern __shared__ __align__(128) uint8_t att_smem[];
   __shared__ int64_t red[kAttWarps];
   __shared__ float row_m[kAttWarps][ROWS], row_l[kAttWarps][ROWS];
@@ -223,42 +231,41 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = att_smem + warp * Shape::kRing;
-  float* join = reinterpret_cast<float*>(att_smem + kAttWarps * Shape::kRing);  // [warp][row][D]
+  float* join = reinterpret_cast<float*>(att_smem);  // [warp][row][D]
   const uint32_t ring_s = smem_u32(ring);
 
   att_clear_rest<BF16>(P, D);
   int64_t total, ignored;
-  att_totals<ROWS>(P, 0, red, total, ignored);
-  int64_t at = att_first_tile(total, blockIdx.x, gridDim.x);
-  const int64_t end = att_first_tile(total, blockIdx.x + 1ll, gridDim.x);
+  att_totals<ROWS, kAttThreads>(P, 0, red, total, ignored);
+  const AttShares shares(total, gridDim.x);
+  int64_t at = shares.first(blockIdx.x);
+  const int64_t end = shares.first(blockIdx.x + 1ll);
   if (at >= end) return;
 
-  // The sequence that holds the first tile.
+  // The sequence that holds the first tile: 32 at a time, every warp the same.
   int b = 0;
   int64_t rem = at;
-  AttSeq seq = att_seq<ROWS>(P, 0);
-  {
-    // Skip 32 sequences at a time: every warp does the same.
-    for (; b < P.seqs; b += 32) {
-      int64_t w = b + lane < P.seqs ? att_work(P, att_seq<ROWS>(P, b + lane)) : 0;
-      int64_t sum = w;
+  for (; b < P.seqs; b += 32) {
+    const int64_t w = b + lane < P.seqs ? att_work(P, att_seq<ROWS>(P, b + lane)) : 0;
+    int64_t sum = w;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += up;
-      }
-      const uint32_t past = __ballot_sync(0xffffffffu, sum > rem);
-      if (past) {
-        const int k = __ffs(past) - 1;
-        rem -= __shfl_sync(0xffffffffu, sum - w, k);
-        b += k;
-        break;
-      }
-      rem -= __shfl_sync(0xffffffffu, sum, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
     }
-    seq = att_seq<ROWS>(P, b);
+    const uint32_t past = __ballot_sync(0xffffffffu, sum > rem);
+    if (past) {
+      const int k = __ffs(past) - 1;
+      rem -= __shfl_sync(0xffffffffu, sum - w, k);
+      b += k;
+      break;
+    }
+    rem -= __shfl_sync(0xffffffffu, sum, 31);
   }
+  AttSeq seq = att_seq<ROWS>(P, b);
 
+  const int tok_a = g ^ ((g >> 1) & 1);  // key of row g of S^T (row g + 8: 8 further on)
+  const int v_a = (2 * t) ^ (t & 1), v_b = (2 * t + 1) ^ (t & 1);  // keys of the contraction's slots 2t, 2t + 1
   bool first_segment = true;
   while (at < end) {
     while (rem >= att_work(P, seq)) {
@@ -272,37 +279,108 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
     const int row0 = static_cast<int>(unit % seq.row_groups) * ROWS;
     const int n_rows = min(ROWS, seq.queries * P.group - row0);
 
+    // Bounds over the rows of the unit: a query's position grows with its row.
+    const int pos0 = seq.length - seq.queries + row0 / P.group;
+    const int pos1 = seq.length - seq.queries + (row0 + n_rows - 1) / P.group;
+    const int lo_min = P.window > 0 ? max(0, pos0 - P.window + 1) : 0;
+    const int lo_max = P.window > 0 ? max(0, pos1 - P.window + 1) : 0;
+    const int hi_max = P.causal ? max(0, min(pos1 + 1, seq.length)) : seq.length;
+    const int hi_min = P.causal ? max(0, pos0 + 1) : seq.length;  // rows past n_rows are never stored: any mask will do
+
+    // ---- this warp's steps: 32 keys, every fourth of the segment
+    const int key0 = seq.lo + tile0 * kAttTile + warp * kAttKeys;
+    const int key_end = min(seq.lo + tile1 * kAttTile, hi_max);
+    const int skip = lo_min > key0 ? (lo_min - key0) / kAttTile : 0;  // steps that end before the window
+    const int steps = key_end > key0 ? (key_end - key0 + kAttTile - 1) / kAttTile : 0;
+    const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
+    const int page_mask = (1 << P.page_shift) - 1;
+
+    // Pages of a step's halves, -1 past the end: looked up one step before they are needed.
+    int next0 = -1, next1 = -1;
+    auto look_up = [&](int step) {
+      const int key = key0 + step * kAttTile;
+      next0 = key < key_end ? table[key >> P.page_shift] : -1;
+      next1 = key + kAttHalf < key_end ? table[(key + kAttHalf) >> P.page_shift] : -1;
+    };
+    // Copies 16 rows into half a stage; false when the page is not one of the pool's.
+    auto copy_half = [&](uint32_t st, int key, int page) -> uint32_t {
+      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(P.pages)) return 0u;
+      const int64_t row = ((static_cast<int64_t>(page) * 2 * P.kv_heads + head) << P.page_shift) + (key & page_mask);
+      const int64_t value = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows from a key to its value
+      const uint8_t* kc = P.codes + row * (D / 2) + lane * 16;
+      const uint8_t* vc = kc + value * (D / 2);
+#pragma unroll
+      for (int k = 0; k < Shape::kCodes / 512; ++k) {
+        const int c = k * 32 + lane;
+        cp_async<16>(st + c * 16, kc + k * 512, 16);
+        // Value rows four apart would meet in the same banks: swap the halves of every other four rows.
+        const int vd = D == 128 ? (c ^ (((c >> 4) & 1) << 1)) : c;
+        cp_async<16>(st + Shape::kCodes + vd * 16, vc + k * 512, 16);
+      }
+      constexpr int SC = Shape::kScales / 16;
+      if (lane < 2 * SC) {
+        const bool is_v = lane >= SC;
+        const uint8_t* sc = P.scales + (row + (is_v ? value : 0)) * BLOCKS + (lane - (is_v ? SC : 0)) * 16;
+        cp_async<16>(st + 2 * Shape::kCodes + lane * 16, sc, 16);
+      }
+      return 1u;
+    };
+    uint32_t valid = 0;  // two bits per stage
+    auto issue = [&](int step, int stage) {
+      const int page0 = next0, page1 = next1;
+      look_up(step + 1);
+      const int key = key0 + step * kAttTile;
+      const uint32_t st = ring_s + stage * Shape::kStage;
+      uint32_t ok = copy_half(st, key, page0);
+      ok |= copy_half(st + Shape::kHalf, key + kAttHalf, page1) << 1;
+      valid = (valid & ~(3u << (2 * stage))) | (ok << (2 * stage));
+      cp_async_commit();
+    };
+    look_up(skip);
+#pragma unroll
+    for (int k = 0; k < kAttStages - 1; ++k) issue(skip + k, k);
+
     // ---- queries: row n = 8 nt + g of this lane, elements [t D/4, (t + 1) D/4)
     uint32_t q[NT][QREGS];
     float fq[NT][2];        // score factors of rows 2t and 2t + 1
     int key_lo[NT][2], key_hi[NT][2];  // and the keys they see
-    int lo_min = 0x7fffffff, lo_max = 0, hi_min = 0x7fffffff, hi_max = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = 8 * nt + g;
       const bool on = r < n_rows;
       const int i = on ? (row0 + r) / P.group : 0;
-      const int h = head * P.group + (on ? (row0 + r) % P.group : 0);
+      const int h = head * P.group + (on ? (row0 + r) - i * P.group : 0);
       const int64_t base = static_cast<int64_t>(seq.q0 + i) * P.q_token + static_cast<int64_t>(h) * P.q_head + t * (D / 4);
-      float v[D / 4];
-      uint32_t amax = 0;
+      const uint16_t* src = static_cast<const uint16_t*>(P.query) + base;
+      uint16_t raw[D / 4];
+      if (P.q_vec) {
 #pragma unroll
-      for (int k = 0; k < D / 4; ++k) {
-        v[k] = on ? att_load_q<BF16>(P.query, base + k) : 0.0f;
-        amax = max(amax, f32_bits(v[k]) & 0x7fffffffu);
+        for (int k = 0; k < D / 32; ++k)
+          reinterpret_cast<uint4*>(raw)[k] = on ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0, 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int k = 0; k < D / 4; ++k) raw[k] = on ? src[k] : static_cast<uint16_t>(0);
       }
       float f = P.scale_log2;
-      float up = 1.0f;
       if constexpr (BF16) {
+        uint32_t amax = 0;
+#pragma unroll
+        for (int k = 0; k < D / 4; ++k) amax = max(amax, static_cast<uint32_t>(raw[k]) & 0x7fffu);
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         // The row's largest magnitude to [2^14, 2^15): exact in f16 down to 2^-31 of it.
-        const int e = max(static_cast<int>(amax >> 23), 1) - 127 - 14;
-        up = exp2i(min(-e, 127));
-        f = __fmul_rn(f, exp2i(-min(-e, 127)));
-      }
+        const int e = min(127 + 14 - max(static_cast<int>(amax >> 7), 1), 127);
+        const float up = exp2i(e);
+        f = __fmul_rn(f, exp2i(-e));
 #pragma unroll
-      for (int k = 0; k < QREGS; ++k) q[nt][k] = pack_f16x2(__fmul_rn(v[2 * k], up), __fmul_rn(v[2 * k + 1], up));
+        for (int k = 0; k < QREGS; ++k)
+          q[nt][k] = pack_f16x2(__fmul_rn(bits_f32(static_cast<uint32_t>(raw[2 * k]) << 16), up),
+                                __fmul_rn(bits_f32(static_cast<uint32_t>(raw[2 * k + 1]) << 16), up));
+      } else {
+#pragma unroll
+        for (int k = 0; k < QREGS; ++k) q[nt][k] = raw[2 * k] | (static_cast<uint32_t>(raw[2 * k + 1]) << 16);
+      }
+      f = __fmul_rn(f, 1.0f / 8192.0f);  // keys are held times 2^13
       fq[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);      // lane of row 2t
       fq[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);  // lane of row 2t + 1
 #pragma unroll
@@ -312,15 +390,6 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         key_hi[nt][c] = P.causal && rr < n_rows ? max(pos + 1, 0) : seq.length;
         key_lo[nt][c] = P.window > 0 ? max(0, pos - P.window + 1) : 0;
       }
-    }
-    {
-      // Bounds over the rows of the unit: a query's position grows with its row.
-      const int pos0 = seq.length - seq.queries + row0 / P.group;
-      const int pos1 = seq.length - seq.queries + (row0 + n_rows - 1) / P.group;
-      lo_min = P.window > 0 ? max(0, pos0 - P.window + 1) : 0;
-      lo_max = P.window > 0 ? max(0, pos1 - P.window + 1) : 0;
-      hi_max = P.causal ? max(0, min(pos1 + 1, seq.length)) : seq.length;
-      hi_min = P.causal ? max(0, pos0 + 1) : seq.length;  // rows past n_rows are never stored: any mask will do
     }
 
     float o[NT][STEPS][4];
@@ -336,87 +405,25 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
     }
     int ref = 0;  // exponent byte that the values are relative to
 
-    // ---- this warp's steps: tiles of 16 keys, every fourth of the segment
-    const int key0 = seq.lo + tile0 * kAttTile + warp * kAttKeys;
-    const int key_end = min(seq.lo + tile1 * kAttTile, hi_max);
-    int skip = 0;
-    if (lo_min > key0) skip = (lo_min - key0) / kAttTile;  // steps that end before the window
-    const int steps = key_end > key0 ? (key_end - key0 + kAttTile - 1) / kAttTile : 0;
-    const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
-    const int page_mask = (1 << P.page_shift) - 1;
-
-    auto page_of = [&](int step) -> int {
-      const int key = key0 + step * kAttTile;
-      return step < steps ? table[key >> P.page_shift] : -1;
-    };
-    // Copies the 16 rows of a step into its stage; false when its page is not one of the pool's.
-    auto issue = [&](int step, int page) -> bool {
-      const bool ok = step < steps && static_cast<uint32_t>(page) < static_cast<uint64_t>(P.pages);
-      if (ok) {
-        const int key = key0 + step * kAttTile;
-        const int64_t row = ((static_cast<int64_t>(page) * 2 * P.kv_heads + head) << P.page_shift) + (key & page_mask);
-        const int64_t value = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows from a key to its value
-        const uint32_t st = ring_s + (step % kAttStages) * Shape::kStage;
-        const uint8_t* kc = P.codes + row * (D / 2);
-        const uint8_t* vc = kc + value * (D / 2);
-#pragma unroll
-        for (int k = 0; k < Shape::kCodes / 512; ++k) {
-          const int c = k * 32 + lane;
-          cp_async<16>(st + c * 16, kc + c * 16, 16);
-          // Value rows four apart would meet in the same banks: swap the halves of every other four rows.
-          const int vd = D == 128 ? (c ^ (((c >> 4) & 1) << 1)) : c;
-          cp_async<16>(st + Shape::kCodes + vd * 16, vc + c * 16, 16);
-        }
-        constexpr int SC = Shape::kScales / 16;
-        if (lane < 2 * SC) {
-          const bool is_v = lane >= SC;
-          const uint8_t* sc = P.scales + (row + (is_v ? value : 0)) * (D / 32) + (lane - (is_v ? SC : 0)) * 16;
-          cp_async<16>(st + 2 * Shape::kCodes + lane * 16, sc, 16);
-        }
-      }
-      cp_async_commit();
-      return ok;
-    };
-
-    uint32_t valid = 0;  // one bit per stage
-    int next_page = page_of(skip);
-#pragma unroll
-    for (int k = 0; k < kAttStages - 1; ++k) {
-      const int page = next_page;
-      next_page = page_of(skip + k + 1);
-      const bool ok = issue(skip + k, page);
-      const uint32_t bit = 1u << ((skip + k) % kAttStages);
-      valid = ok ? valid | bit : valid & ~bit;
-    }
-
-    const int tok_a = g ^ ((g >> 1) & 1);  // key of row g of S^T (row g + 8: 8 further on)
-    const int v_a = (2 * t) ^ (t & 1), v_b = (2 * t + 1) ^ (t & 1);  // keys of the contraction's slots 2t, 2t + 1
-
+    int stage = 0;
     for (int step = skip; step < steps; ++step) {
-      {
-        const int page = next_page;
-        next_page = page_of(step + kAttStages);
-        const bool ok = issue(step + kAttStages - 1, page);
-        const uint32_t bit = 1u << ((step + kAttStages - 1) % kAttStages);
-        valid = ok ? valid | bit : valid & ~bit;
-      }
+      issue(step + kAttStages - 1, stage == 0 ? kAttStages - 1 : stage - 1);
       cp_async_wait<kAttStages - 1>();
       __syncwarp();
-      const int stage = step % kAttStages;
       const int key = key0 + step * kAttTile;
-      if ((valid >> stage) & 1) {
-        const uint8_t* st = ring + stage * Shape::kStage;
-        const uint8_t* kc = st;
-        const uint8_t* vc = st + Shape::kCodes;
-        const uint8_t* ks = st + 2 * Shape::kCodes;
-        const uint8_t* vs = ks + Shape::kScales;
+      const uint8_t* st = ring + stage * Shape::kStage;
+      const uint32_t held = (valid >> (2 * stage)) & 3u;
 
-        // ---- scores
-        float s[NT][4];
+      // ---- scores
+      float s[2][NT][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t* kc = st + half * Shape::kHalf;
+        const uint8_t* ks = kc + 2 * Shape::kCodes;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s[nt][c] = 0.0f;
+          for (int c = 0; c < 4; ++c) s[half][nt][c] = 0.0f;
         constexpr int KW = D / 32;  // words of a row's quarter
         uint32_t wa[KW], wb[KW];
         if constexpr (D == 128) {
@@ -426,7 +433,6 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(kc + tok_a * 32 + t * 8);
           *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(kc + (tok_a + 8) * 32 + t * 8);
         }
-        constexpr int BLOCKS = D / 32;
         const int sa = ks[tok_a * BLOCKS + t * BLOCKS / 4], sb = ks[(tok_a + 8) * BLOCKS + t * BLOCKS / 4];
         int ra = max(sa, __shfl_xor_sync(0xffffffffu, sa, 1));
         int rb = max(sb, __shfl_xor_sync(0xffffffffu, sb, 1));
@@ -434,82 +440,128 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         rb = max(rb, __shfl_xor_sync(0xffffffffu, rb, 2));
         const uint32_t ma = f16_pow2_13_minus(ra - sa) * 0x10001u, mb = f16_pow2_13_minus(rb - sb) * 0x10001u;
 #pragma unroll
-        for (int w = 0; w < KW; ++w)
+        for (int w = 0; w < KW; ++w) {
+          uint32_t ha[4], hb[4];
+          e2m1x8_to_f16x2(wa[w], ha);
+          e2m1x8_to_f16x2(wb[w], hb);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = hmul2(MXW_PAIR(wa[w], 2 * h), ma), a1 = hmul2(MXW_PAIR(wb[w], 2 * h), mb);
-            const uint32_t a2 = hmul2(MXW_PAIR(wa[w], 2 * h + 1), ma), a3 = hmul2(MXW_PAIR(wb[w], 2 * h + 1), mb);
+            const uint32_t a0 = hmul2(ha[2 * h], ma), a1 = hmul2(hb[2 * h], mb);
+            const uint32_t a2 = hmul2(ha[2 * h + 1], ma), a3 = hmul2(hb[2 * h + 1], mb);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_f16(s[nt], a0, a1, a2, a3, q[nt][4 * w + 2 * h], q[nt][4 * w + 2 * h + 1]);
+              mma_f16(s[half][nt], a0, a1, a2, a3, q[nt][4 * w + 2 * h], q[nt][4 * w + 2 * h + 1]);
           }
-        const float fa = exp2i(ra - 140), fb = exp2i(rb - 140);
-        const int key_a = key + tok_a, key_b = key_a + 8;
-        bool raise = false;
+        }
+        // (A row whose largest scale byte is 0 is held to twice its 2^-127.)
+        const float fa = bits_f32(static_cast<uint32_t>(max(ra, 1)) << 23), fb = bits_f32(static_cast<uint32_t>(max(rb, 1)) << 23);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          s[nt][0] = __fmul_rn(__fmul_rn(s[nt][0], fa), fq[nt][0]);
-          s[nt][1] = __fmul_rn(__fmul_rn(s[nt][1], fa), fq[nt][1]);
-          s[nt][2] = __fmul_rn(__fmul_rn(s[nt][2], fb), fq[nt][0]);
-          s[nt][3] = __fmul_rn(__fmul_rn(s[nt][3], fb), fq[nt][1]);
+          s[half][nt][0] = __fmul_rn(__fmul_rn(s[half][nt][0], fa), fq[nt][0]);
+          s[half][nt][1] = __fmul_rn(__fmul_rn(s[half][nt][1], fa), fq[nt][1]);
+          s[half][nt][2] = __fmul_rn(__fmul_rn(s[half][nt][2], fb), fq[nt][0]);
+          s[half][nt][3] = __fmul_rn(__fmul_rn(s[half][nt][3], fb), fq[nt][1]);
         }
-        const bool edge = key < lo_max || key + kAttKeys > hi_min;
-        if (edge) {
+      }
+      const bool edge = key < lo_max || key + kAttKeys > hi_min || held != 3u;
+      if (edge) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const bool in = (held >> half) & 1u;
+          const int key_a = key + half * kAttHalf + tok_a, key_b = key_a + 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              if (key_a < key_lo[nt][c] || key_a >= key_hi[nt][c]) s[nt][c] = -INFINITY;
-              if (key_b < key_lo[nt][c] || key_b >= key_hi[nt][c]) s[nt][2 + c] = -INFINITY;
+              if (!in || key_a < key_lo[nt][c] || key_a >= key_hi[nt][c]) s[half][nt][c] = -INFINITY;
+              if (!in || key_b < key_lo[nt][c] || key_b >= key_hi[nt][c]) s[half][nt][2 + c] = -INFINITY;
             }
         }
+      }
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          raise |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c])) > __fadd_rn(m[nt][c], kAttSlack);
+      if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) raise |= fmaxf(s[nt][c], s[nt][2 + c]) > __fadd_rn(m[nt][c], kAttSlack);
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float x = fmaxf(s[nt][c], s[nt][2 + c]);
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-              const float up = fmaxf(m[nt][c], x);
-              const float f = m[nt][c] == up ? 1.0f : ex2(__fsub_rn(m[nt][c], up));
-              m[nt][c] = up;
-              l[nt][c] = __fmul_rn(l[nt][c], f);
-#pragma unroll
-              for (int k = 0; k < STEPS; ++k) {
-                o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
-                o[nt][k][2 + c] = __fmul_rn(o[nt][k][2 + c], f);
-              }
-            }
-        }
-
-        // ---- probabilities, transposed into the second product's operand
-        uint32_t p0[NT], p1[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float p[4];
-#pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const float base = __fsub_rn(kAttLift, m[nt][c] == -INFINITY ? 0.0f : m[nt][c]);
-            p[c] = ex2(__fadd_rn(s[nt][c], base));
-            p[2 + c] = ex2(__fadd_rn(s[nt][2 + c], base));
-            l[nt][c] = __fadd_rn(l[nt][c], __fadd_rn(p[c], p[2 + c]));
+            float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float up = fmaxf(m[nt][c], x);
+            const float f = m[nt][c] == up ? 1.0f : ex2(__fsub_rn(m[nt][c], up));
+            m[nt][c] = up;
+            l[nt][c] = __fmul_rn(l[nt][c], f);
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+              o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
+              o[nt][k][2 + c] = __fmul_rn(o[nt][k][2 + c], f);
+            }
           }
-          p0[nt] = transpose8(pack_f16x2(p[0], p[1]));
-          p1[nt] = transpose8(pack_f16x2(p[2], p[3]));
-        }
+      }
 
-        // ---- values
+      // ---- probabilities, transposed into the second product's operand
+      uint32_t p0[2][NT], p1[2][NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float base0 = __fsub_rn(kAttLift, m[nt][0] == -INFINITY ? 0.0f : m[nt][0]);
+        const float base1 = __fsub_rn(kAttLift, m[nt][1] == -INFINITY ? 0.0f : m[nt][1]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float x0 = ex2(__fadd_rn(s[half][nt][0], base0)), x1 = ex2(__fadd_rn(s[half][nt][1], base1));
+          const float x2 = ex2(__fadd_rn(s[half][nt][2], base0)), x3 = ex2(__fadd_rn(s[half][nt][3], base1));
+          l[nt][0] = __fadd_rn(l[nt][0], __fadd_rn(x0, x2));
+          l[nt][1] = __fadd_rn(l[nt][1], __fadd_rn(x1, x3));
+          p0[half][nt] = transpose8(pack_f16x2(x0, x1));
+          p1[half][nt] = transpose8(pack_f16x2(x2, x3));
+        }
+      }
+
+      // ---- values: scales first, for the reference
+      const int blk = g * BLOCKS / 8;
+      int sv[2][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t* vs = st + half * Shape::kHalf + 2 * Shape::kCodes + Shape::kScales + blk;
+        sv[half][0] = vs[v_a * BLOCKS];
+        sv[half][1] = vs[v_b * BLOCKS];
+        sv[half][2] = vs[(v_a + 8) * BLOCKS];
+        sv[half][3] = vs[(v_b + 8) * BLOCKS];
+      }
+      if (edge) {
+        // Keys that no row sees (stale rows of the page) have no say in the reference.
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int k = key + half * kAttHalf + ((c & 1) ? v_b : v_a) + ((c & 2) ? 8 : 0);
+            if (!((held >> half) & 1u) || k < lo_min || k >= hi_max) sv[half][c] = 0;
+          }
+      }
+      const int top = __reduce_max_sync(0xffffffffu, max(max(max(sv[0][0], sv[0][1]), max(sv[0][2], sv[0][3])),
+                                                         max(max(sv[1][0], sv[1][1]), max(sv[1][2], sv[1][3]))));
+      if (top > ref) {
+        const float f = exp2i(max(ref - top, -149));
+        ref = top;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint8_t* vc = st + half * Shape::kHalf + Shape::kCodes;
         constexpr int VW = D / 64;  // words of an eighth of a row
         uint32_t va[VW], vb[VW], vc2[VW], vd[VW];
         if constexpr (D == 128) {
-          const int sw = (t & 2) << 4;  // rows 4..7 and 12..15 of the stage have their halves swapped
-          const int ch = (g * 8) ^ sw;
+          const int ch = (g * 8) ^ ((t & 2) << 4);  // rows 4..7 and 12..15 have their halves swapped
           *reinterpret_cast<uint2*>(va) = *reinterpret_cast<const uint2*>(vc + v_a * 64 + ch);
           *reinterpret_cast<uint2*>(vb) = *reinterpret_cast<const uint2*>(vc + v_b * 64 + ch);
           *reinterpret_cast<uint2*>(vc2) = *reinterpret_cast<const uint2*>(vc + (v_a + 8) * 64 + ch);
@@ -520,45 +572,27 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           vc2[0] = *reinterpret_cast<const uint32_t*>(vc + (v_a + 8) * 32 + g * 4);
           vd[0] = *reinterpret_cast<const uint32_t*>(vc + (v_b + 8) * 32 + g * 4);
         }
-        const int blk = g * BLOCKS / 8;
-        int s0 = vs[v_a * BLOCKS + blk], s1 = vs[v_b * BLOCKS + blk];
-        int s2 = vs[(v_a + 8) * BLOCKS + blk], s3 = vs[(v_b + 8) * BLOCKS + blk];
-        if (edge) {
-          // Keys that no row sees (stale rows of the page) have no say in the reference.
-          if (key + v_a < lo_min || key + v_a >= hi_max) s0 = 0;
-          if (key + v_b < lo_min || key + v_b >= hi_max) s1 = 0;
-          if (key + v_a + 8 < lo_min || key + v_a + 8 >= hi_max) s2 = 0;
-          if (key + v_b + 8 < lo_min || key + v_b + 8 >= hi_max) s3 = 0;
-        }
-        const int top = __reduce_max_sync(0xffffffffu, max(max(s0, s1), max(s2, s3)));
-        if (top > ref) {
-          const float f = exp2i(max(ref - top, -149));
-          ref = top;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
-        }
-        const uint32_t mlo = f16_pow2_13_minus(ref - s0) | (f16_pow2_13_minus(ref - s1) << 16);
-        const uint32_t mhi = f16_pow2_13_minus(ref - s2) | (f16_pow2_13_minus(ref - s3) << 16);
+        const uint32_t mlo = f16_pow2_13_minus(ref - sv[half][0]) | (f16_pow2_13_minus(ref - sv[half][1]) << 16);
+        const uint32_t mhi = f16_pow2_13_minus(ref - sv[half][2]) | (f16_pow2_13_minus(ref - sv[half][3]) << 16);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
-          const uint32_t el = (va[w] & 0x0f0f0f0fu) | ((vb[w] << 4) & 0xf0f0f0f0u);
-          const uint32_t ol = ((va[w] >> 4) & 0x0f0f0f0fu) | (vb[w] & 0xf0f0f0f0u);
-          const uint32_t eh = (vc2[w] & 0x0f0f0f0fu) | ((vd[w] << 4) & 0xf0f0f0f0u);
-          const uint32_t oh = ((vc2[w] >> 4) & 0x0f0f0f0fu) | (vd[w] & 0xf0f0f0f0u);
+          // Bytes of (first key's code, second key's code): even channels, then odd.
+          uint32_t el[4], ol[4], eh[4], oh[4];
+          e2m1x8_to_f16x2((va[w] & 0x0f0f0f0fu) | ((vb[w] << 4) & 0xf0f0f0f0u), el);
+          e2m1x8_to_f16x2(((va[w] >> 4) & 0x0f0f0f0fu) | (vb[w] & 0xf0f0f0f0u), ol);
+          e2m1x8_to_f16x2((vc2[w] & 0x0f0f0f0fu) | ((vd[w] << 4) & 0xf0f0f0f0u), eh);
+          e2m1x8_to_f16x2(((vc2[w] >> 4) & 0x0f0f0f0fu) | (vd[w] & 0xf0f0f0f0u), oh);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t a0 = hmul2(MXW_PAIR(el, k), mlo), a1 = hmul2(MXW_PAIR(ol, k), mlo);
-            const uint32_t a2 = hmul2(MXW_PAIR(eh, k), mhi), a3 = hmul2(MXW_PAIR(oh, k), mhi);
+            const uint32_t a0 = hmul2(el[k], mlo), a1 = hmul2(ol[k], mlo);
+            const uint32_t a2 = hmul2(eh[k], mhi), a3 = hmul2(oh[k], mhi);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + k], a0, a1, a2, a3, p0[nt], p1[nt]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + k], a0, a1, a2, a3, p0[half][nt], p1[half][nt]);
           }
         }
       }
       __syncwarp();
+      stage = stage == kAttStages - 1 ? 0 : stage + 1;
     }
     cp_async_wait<0>();
 
@@ -576,7 +610,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           row_l[warp][8 * nt + 2 * t + c] = x;
         }
       }
-    __syncthreads();
+    __syncthreads();  // (the rings are drained too: `join` takes their place)
     const float back = exp2i(max(ref - 140, -149));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -587,17 +621,15 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 #pragma unroll
         for (int w = 1; w < kAttWarps; ++w) top = fmaxf(top, row_m[w][r]);
         const float f = m[nt][c] == -INFINITY ? 0.0f : ex2(__fsub_rn(m[nt][c], top));
-        float* dst = join + (warp * ROWS + r) * D + g * (D / 8);
+        float2* dst = reinterpret_cast<float2*>(join + (warp * ROWS + r) * D + g * (D / 8));
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
-          dst[2 * k] = __fmul_rn(__fmul_rn(o[nt][k][c], f), back);
-          dst[2 * k + 1] = __fmul_rn(__fmul_rn(o[nt][k][2 + c], f), back);
-        }
+        for (int k = 0; k < STEPS; ++k)
+          dst[k] = make_float2(__fmul_rn(__fmul_rn(o[nt][k][c], f), back), __fmul_rn(__fmul_rn(o[nt][k][2 + c], f), back));
       }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == seq.tiles;
     float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (first_segment ? 0 : 1)) * Shape::kSlot;
-    for (int i = threadIdx.x; i < ROWS * D; i += kAttThreads) {
+    for (int i = threadIdx.x; i < n_rows * D; i += kAttThreads) {
       const int r = i / D, d = i % D;
       float top = row_m[0][r];
 #pragma unroll
@@ -613,71 +645,123 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       const float v = seen ? __fdiv_rn(acc, sum) : 0.0f;
       const float lse2 = seen ? __fadd_rn(top, __fsub_rn(log2f(sum), kAttLift)) : -INFINITY;
       if (whole) {
-        if (r < n_rows) {
-          const int64_t row = static_cast<int64_t>(seq.q0 + (row0 + r) / P.group) * P.heads + head * P.group + (row0 + r) % P.group;
-          att_store<BF16>(P.out, row * D + d, v);
-          if (P.lse && d == 0) P.lse[row] = __fmul_rn(lse2, 0.69314718055994531f);
-        }
+        const int i_q = (row0 + r) / P.group;
+        const int64_t row = static_cast<int64_t>(seq.q0 + i_q) * P.heads + head * P.group + (row0 + r) - i_q * P.group;
+        att_store<BF16>(P.out, row * D + d, v);
+        if (P.lse && d == 0) P.lse[row] = __fmul_rn(lse2, 0.69314718055994531f);
       } else {
         slot[r * D + d] = v;
         if (d == 0) slot[ROWS * D + r] = lse2;
       }
     }
     __syncthreads();
-    const int64_t taken = tile1 - tile0;
-    at += taken;
-    rem += taken;
+    at += tile1 - tile0;
+    rem += tile1 - tile0;
     first_segment = false;
   }
 }
 
 // Adds the partial results of a unit that several blocks shared, in block order.
 template <bool BF16, int D, int NT>
-__global__ void __launch_bounds__(kAttThreads) attention_join_kernel(const AttParams P, int blocks) {
+__global__ void __launch_bounds__(kAttJoinThreads) attention_join_kernel(const AttParams P, int blocks) {
   using Shape = AttShape<D, NT>;
   constexpr int ROWS = Shape::kRows;
-  __shared__ int64_t red[kAttWarps];
+  constexpr int CHUNK = 64;  // partial results whose weights are held at a time
+  constexpr int QUADS = ROWS * D / 4, EACH = (QUADS + kAttJoinThreads - 1) / kAttJoinThreads;
+  __shared__ int64_t red[kAttJoinThreads / 32];
+  __shared__ float weight[CHUNK][ROWS];
+  __shared__ float row_top[ROWS], row_sum[ROWS];
   const int b = blockIdx.y;
   const AttSeq seq = att_seq<ROWS>(P, b);
   const int64_t units = static_cast<int64_t>(seq.row_groups) * P.kv_heads;
   int64_t total = 0, before = 0;
-  if (blockIdx.x < units) att_totals<ROWS>(P, b, red, total, before);
+  if (blockIdx.x < units) att_totals<ROWS, kAttJoinThreads>(P, b, red, total, before);
   // Every block waits, also those without work: what follows this kernel in the
   // stream may then rely on the first kernel's results too.
   grid_dependency_wait();
   // (The grid has a block per unit when the caller's bound on the queries holds.)
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-  const int64_t u0 = before + unit * seq.tiles, u1 = u0 + seq.tiles;  // its tiles
-  // The block whose share holds tile u0.
-  int64_t j = static_cast<int64_t>(static_cast<double>(u0) / static_cast<double>(total) * blocks);
-  j = max(static_cast<int64_t>(0), min(j, static_cast<int64_t>(blocks) - 1));
-  while (j > 0 && att_first_tile(total, j, blocks) > u0) --j;
-  while (j + 1 < blocks && att_first_tile(total, j + 1, blocks) <= u0) ++j;
-  if (att_first_tile(total, j + 1, blocks) >= u1) continue;  // one block had it all
-  const int head = static_cast<int>(unit / seq.row_groups), row0 = static_cast<int>(unit % seq.row_groups) * ROWS;
-  const int n_rows = min(ROWS, seq.queries * P.group - row0);
-  for (int i = threadIdx.x; i < n_rows * D; i += kAttThreads) {
-    const int r = i / D, d = i % D;
-    float top = -INFINITY, sum = 0.0f, acc = 0.0f;
-    for (int64_t k = j; k < blocks; ++k) {
-      const int64_t first = att_first_tile(total, k, blocks);
-      if (first >= u1) break;
-      if (att_first_tile(total, k + 1, blocks) == first) continue;  // a block without work
-      const float* slot = P.partial + (2 * k + (u0 <= first ? 0 : 1)) * Shape::kSlot;
-      const float x = slot[ROWS * D + r];
-      if (x == -INFINITY) continue;
-      const float up = fmaxf(top, x);
-      const float keep = top == up ? 1.0f : ex2(__fsub_rn(top, up));
-      const float w = ex2(__fsub_rn(x, up));
-      sum = __fadd_rn(__fmul_rn(sum, keep), w);
-      acc = __fmaf_rn(slot[r * D + d], w, __fmul_rn(acc, keep));
-      top = up;
+    const AttShares shares(total, blocks);
+    const int64_t u0 = before + unit * seq.tiles, u1 = u0 + seq.tiles;  // its tiles
+    const int64_t j0 = shares.block_of(u0), j1 = shares.block_of(u1 - 1) + 1;  // and the blocks that share them
+    if (j1 - j0 == 1) continue;  // one block had it all
+    // A block's partial result is in its first slot when its share starts with this unit.
+    const float* first = P.partial + (2 * j0 + (u0 <= shares.first(j0) ? 0 : 1)) * Shape::kSlot;
+    auto slot = [&](int64_t j) { return j == j0 ? first : P.partial + 2 * j * Shape::kSlot; };
+    const int n = static_cast<int>(j1 - j0);
+    const int row0 = static_cast<int>(unit % seq.row_groups) * ROWS, head = static_cast<int>(unit / seq.row_groups);
+    const int n_rows = min(ROWS, seq.queries * P.group - row0);
+    // Each row's largest log-sum, by 256 / ROWS threads.
+    __syncthreads();
+    if (threadIdx.x < ROWS * 16) {
+      const int r = threadIdx.x >> 4;
+      float top = -INFINITY;
+      bool bad = false;
+      for (int k = threadIdx.x & 15; k < n; k += 16) {
+        const float x = slot(j0 + k)[ROWS * D + r];
+        bad |= x != x;
+        top = fmaxf(top, x);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        bad |= __shfl_xor_sync(0xffffffffu, static_cast<int>(bad), o) != 0;
+      }
+      if ((threadIdx.x & 15) == 0) {
+        row_top[r] = bad ? NAN : top;
+        row_sum[r] = 0.0f;
+      }
     }
-    const bool seen = !(sum == 0.0f);
-    const int64_t row = static_cast<int64_t>(seq.q0 + (row0 + r) / P.group) * P.heads + head * P.group + (row0 + r) % P.group;
-    att_store<BF16>(P.out, row * D + d, seen ? __fdiv_rn(acc, sum) : 0.0f);
-    if (P.lse && d == 0) P.lse[row] = seen ? __fmul_rn(__fadd_rn(top, log2f(sum)), 0.69314718055994531f) : -INFINITY;
-  }
+    float4 acc[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int c0 = 0; c0 < n; c0 += CHUNK) {
+      const int nc = min(CHUNK, n - c0);
+      __syncthreads();
+      for (int i = threadIdx.x; i < nc * ROWS; i += kAttJoinThreads) {
+        const int k = i / ROWS, r = i % ROWS;
+        const float x = slot(j0 + c0 + k)[ROWS * D + r];
+        weight[k][r] = x == -INFINITY ? 0.0f : ex2(__fsub_rn(x, row_top[r]));
+      }
+      __syncthreads();
+      if (threadIdx.x < ROWS) {
+        float sum = row_sum[threadIdx.x];
+        for (int k = 0; k < nc; ++k) sum = __fadd_rn(sum, weight[k][threadIdx.x]);
+        row_sum[threadIdx.x] = sum;
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = threadIdx.x + e * kAttJoinThreads;
+        const int r = i / (D / 4);
+        if (i < QUADS && r < n_rows) {
+#pragma unroll 8
+          for (int k = 0; k < nc; ++k) {
+            const float4 v = reinterpret_cast<const float4*>(slot(j0 + c0 + k))[i];
+            const float w = weight[k][r];
+            acc[e].x = __fmaf_rn(v.x, w, acc[e].x);
+            acc[e].y = __fmaf_rn(v.y, w, acc[e].y);
+            acc[e].z = __fmaf_rn(v.z, w, acc[e].z);
+            acc[e].w = __fmaf_rn(v.w, w, acc[e].w);
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      const int i = threadIdx.x + e * kAttJoinThreads;
+      const int r = i / (D / 4), d = i % (D / 4) * 4;
+      if (i < QUADS && r < n_rows) {
+        const float sum = row_sum[r];
+        const bool seen = !(sum == 0.0f);
+        const int i_q = (row0 + r) / P.group;
+        const int64_t row = static_cast<int64_t>(seq.q0 + i_q) * P.heads + head * P.group + (row0 + r) - i_q * P.group;
+        const float v[4] = {acc[e].x, acc[e].y, acc[e].z, acc[e].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) att_store<BF16>(P.out, row * D + d + k, seen ? __fdiv_rn(v[k], sum) : 0.0f);
+        if (P.lse && d == 0) P.lse[row] = seen ? __fmul_rn(__fadd_rn(row_top[r], log2f(sum)), 0.69314718055994531f) : -INFINITY;
+      }
+    }
   }
 }
 
@@ -699,7 +783,9 @@ static AttPlan att_plan(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d
   plan.nt = rows <= 8 ? 1 : 2;
   const int64_t unit_rows = 8 * plan.nt;
   plan.units = (rows + unit_rows - 1) / unit_rows * kv_heads;
-  const int64_t tiles = std::max<int64_t>(1, (max_length + kAttTile) / kAttTile) * plan.units * seqs;
+  const int64_t deep = std::max<int64_t>(1, (max_length + kAttTile - 1) / kAttTile), units = plan.units * seqs;
+  // At most 64 blocks per unit: joining more partial results costs what the split saves.
+  const int64_t tiles = std::min<int64_t>(deep, 64) * units;
   plan.blocks = static_cast<unsigned>(std::min<int64_t>(tiles, static_cast<int64_t>(num_sms()) * (plan.nt == 1 ? 4 : 3)));
   plan.bytes = static_cast<size_t>(plan.blocks) * 2 * static_cast<size_t>(unit_rows * dim + unit_rows) * sizeof(float);
   return plan;
@@ -715,7 +801,7 @@ static int launch_attention(const AttParams& P, const AttPlan& plan, cudaStream_
   if (status != MXW_OK) return status;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(plan.units), static_cast<unsigned>(P.seqs));
-  cfg.blockDim = dim3(kAttThreads);
+  cfg.blockDim = dim3(kAttJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -789,6 +875,7 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   P.lengths = lengths;
   P.start = start;
   P.tokens = tokens;
+  P.q_vec = q_token % 8 == 0 && q_head % 8 == 0 && reinterpret_cast<uintptr_t>(query) % 16 == 0;
   P.seqs = static_cast<int>(seqs);
   P.heads = static_cast<int>(heads);
   P.kv_heads = static_cast<int>(kv_heads);
