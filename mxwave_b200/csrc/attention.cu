@@ -13,18 +13,18 @@
 //     S^T = K Q^T (16 keys x 8 query rows) and O^T = V^T P^T (16 channels x 8
 //     rows).  Eight rows is the least a matrix instruction takes; grouped heads
 //     share one, so each code is decoded once per group of up to 8 NT rows.
-//   * The contraction's order is free, so each lane takes the bytes that lie
-//     together in a cached row: for K four lanes share a row (a quarter of it
-//     each), for V eight lanes do, and token pairs are interleaved nibble by
-//     nibble.  Every shared-memory load is 8 or 16 bytes without conflicts.
-//   * A byte of two codes becomes an f16 pair in one conversion, and one f16x2
-//     product applies the scale.  f16 has 11 significant bits where a code has
-//     two; what it lacks is range, so scales are taken relative to a running
-//     reference: the largest of the row's blocks for a key, the largest seen so
-//     far for the values (times 2^13, below f16's maximum).  A block whose scale
-//     is 2^-36 of the reference or more is exact; smaller ones lose bits that
-//     are 2^-37 of the reference.  Queries are exact in the same sense (scaled
-//     by a power of two per row for bf16).
+//   * The contraction's order is free, so lanes take bytes that lie together.
+//     Four lanes share a key row, each a word of eight codes of every block: no
+//     product of 16 elements mixes two scales, and the block's scale is applied
+//     to the fp32 sum.  Eight lanes share a value row, eight bytes each, and
+//     key pairs are interleaved nibble by nibble.  The 16-byte pieces of the
+//     rows are placed so that none of these loads meets a bank conflict.
+//   * A byte of two codes becomes an f16 pair in one conversion.  Codes are
+//     exact in f16; queries are scaled by a power of two per row (bf16) and are
+//     exact down to 2^-31 of the row's largest.  The values' scales run across
+//     the contraction, so they are multiplied into the codes, relative to the
+//     largest scale seen so far (times 2^13, below f16's maximum): exact down to
+//     2^-27 of it, zero below.
 //   * Probabilities are rounded to f16 as 2^(x - m + 7): 11 bits down to 2^-21
 //     of the largest, nothing lost above 2^-31.  Their sum is taken in fp32
 //     before the rounding.  m is raised only when a score passes it by 8
@@ -33,12 +33,14 @@
 //     running maximum and sum, its own ring of asynchronous copies and no
 //     synchronisation with the others until the end of a segment.
 // Work split: the (sequence, head, row group) units are cut into tiles of 128
-// keys, all tiles are laid end to end, and each block takes an equal share of
-// them, whatever the lengths.  A unit that several blocks share leaves partial
+// keys, all tiles are laid end to end (each unit's behind the cost of starting
+// it), and each block takes an equal share, whatever the lengths.  A unit that several blocks share leaves partial
 // results (normalised rows and their log-sum-exp) in the workspace, two slots
 // per block, and attention_join_kernel adds them in block order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "blockscale.cuh"
 #include "common.cuh"
@@ -53,6 +55,11 @@ constexpr int kAttKeys = 2 * kAttHalf;            // keys per warp step
 constexpr int kAttTile = kAttWarps * kAttKeys;    // keys per block step
 constexpr int kAttStages = 3;
 constexpr int kAttJoinThreads = 256;
+// What starting a unit costs a block, in tiles: with units of a tile or two
+// counted by their tiles alone, blocks that got a run of short sequences
+// finished last (393 us against 212 on 32 sequences of 1 to 65,536 keys; 325,
+// 253, 212 and 217 us with 1, 2, 4 and 8 here).
+constexpr int kAttStart = 4;
 constexpr float kAttLift = 7.0f;    // probabilities are held as 2^(x - m + 7)
 constexpr float kAttSlack = 8.0f;   // and x may pass m by 8 before m is raised: at most 2^15
 
@@ -100,7 +107,7 @@ __device__ __forceinline__ AttSeq att_seq(const AttParams& P, int b) {
 }
 
 __device__ __forceinline__ int64_t att_work(const AttParams& P, const AttSeq& s) {
-  return static_cast<int64_t>(s.tiles) * s.row_groups * P.kv_heads;
+  return static_cast<int64_t>(s.tiles + kAttStart) * s.row_groups * P.kv_heads;
 }
 
 // Sum over the block (all threads get it); `red` holds one word per warp.
@@ -176,9 +183,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 2^(13 - n) as f16 bits for n >= 0: normal down to 2^-14, subnormal to 2^-24, then 0.
-__device__ __forceinline__ uint32_t f16_pow2_13_minus(int n) {
-  return n <= 27 ? static_cast<uint32_t>(28 - n) << 10 : 0x400u >> min(n - 27, 31);
+// Two scale bytes, as halfwords, to f16 factors 2^(13 - (ref - byte)): zero from ref - byte = 28 on.
+__device__ __forceinline__ uint32_t f16_factors(uint32_t bytes2, uint32_t lift2) {
+  return __vmaxs2(__vadd2(bytes2, lift2), 0u) << 10;
+}
+// 2^(byte - 127) of byte `b` of a word (0 for a zero byte: 2^-127 is nothing next to a score).
+template <int B>
+__device__ __forceinline__ float scale_of(uint32_t word) {
+  return bits_f32((B == 3 ? word >> 1 : word << (23 - 8 * B)) & 0x7f800000u);
 }
 
 template <int D, int NT>
@@ -266,15 +278,23 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 
   const int tok_a = g ^ ((g >> 1) & 1);  // key of row g of S^T (row g + 8: 8 further on)
   const int v_a = (2 * t) ^ (t & 1), v_b = (2 * t + 1) ^ (t & 1);  // keys of the contraction's slots 2t, 2t + 1
+  const int key_turn = D == 128 ? (tok_a >> 1) & 3 : (tok_a >> 2) & 1;
   bool first_segment = true;
   while (at < end) {
     while (rem >= att_work(P, seq)) {
       rem -= att_work(P, seq);
       seq = att_seq<ROWS>(P, ++b);
     }
-    const int64_t unit = rem / seq.tiles;
-    const int tile0 = static_cast<int>(rem % seq.tiles);
-    const int tile1 = static_cast<int>(min(static_cast<int64_t>(seq.tiles), tile0 + (end - at)));
+    const int cost = seq.tiles + kAttStart;
+    const int64_t unit = rem / cost;
+    const int c0 = static_cast<int>(rem % cost);
+    const int c1 = static_cast<int>(min(static_cast<int64_t>(cost), c0 + (end - at)));
+    const int tile0 = max(0, c0 - kAttStart), tile1 = c1 - kAttStart;
+    const bool opens = first_segment;
+    at += c1 - c0;
+    rem += c1 - c0;
+    first_segment = false;
+    if (tile1 <= tile0) continue;  // the share ends before the unit's first tile
     const int head = static_cast<int>(unit / seq.row_groups);  // key/value head
     const int row0 = static_cast<int>(unit % seq.row_groups) * ROWS;
     const int n_rows = min(ROWS, seq.queries * P.group - row0);
@@ -294,6 +314,14 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
     const int steps = key_end > key0 ? (key_end - key0 + kAttTile - 1) / kAttTile : 0;
     const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
     const int page_mask = (1 << P.page_shift) - 1;
+    // Bytes of a page, of one head's rows in it, and this lane's place in both arrays.
+    const int head_codes = (D / 2) << P.page_shift, head_scales = BLOCKS << P.page_shift;
+    const int64_t page_codes = 2ll * P.kv_heads * head_codes, page_scales = 2ll * P.kv_heads * head_scales;
+    constexpr int SC = Shape::kScales / 16;  // 16-byte pieces of 16 rows' scales
+    const uint8_t* codes = P.codes + static_cast<int64_t>(head) * head_codes + lane * 16;
+    const int64_t to_values = static_cast<int64_t>(P.kv_heads) * head_codes;
+    const uint8_t* scales = P.scales + static_cast<int64_t>(head) * head_scales +
+                            (lane < SC ? lane * 16 : static_cast<int64_t>(P.kv_heads) * head_scales + (lane - SC) * 16);
 
     // Pages of a step's halves, -1 past the end: looked up one step before they are needed.
     int next0 = -1, next1 = -1;
@@ -302,37 +330,31 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       next0 = key < key_end ? table[key >> P.page_shift] : -1;
       next1 = key + kAttHalf < key_end ? table[(key + kAttHalf) >> P.page_shift] : -1;
     };
-    // Copies 16 rows into half a stage; false when the page is not one of the pool's.
-    auto copy_half = [&](uint32_t st, int key, int page) -> uint32_t {
+    // Copies 16 rows into half a stage; 0 when the page is not one of the pool's.
+    auto copy_half = [&](uint32_t st, int offset, int page) -> uint32_t {
       if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(P.pages)) return 0u;
-      const int64_t row = ((static_cast<int64_t>(page) * 2 * P.kv_heads + head) << P.page_shift) + (key & page_mask);
-      const int64_t value = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows from a key to its value
-      const uint8_t* kc = P.codes + row * (D / 2) + lane * 16;
-      const uint8_t* vc = kc + value * (D / 2);
+      const uint8_t* kc = codes + page * page_codes + offset * (D / 2);
+      const uint8_t* vc = kc + to_values;
 #pragma unroll
       for (int k = 0; k < Shape::kCodes / 512; ++k) {
         const int c = k * 32 + lane;
-        cp_async<16>(st + c * 16, kc + k * 512, 16);
-        // Value rows four apart would meet in the same banks: swap the halves of every other four rows.
+        // Pieces of key rows rotate over pairs of rows; value rows four apart have their halves swapped.
+        const int kd = D == 128 ? (c ^ ((c >> 3) & 3)) : (c ^ ((c >> 3) & 1));
+        cp_async<16>(st + kd * 16, kc + k * 512, 16);
         const int vd = D == 128 ? (c ^ (((c >> 4) & 1) << 1)) : c;
         cp_async<16>(st + Shape::kCodes + vd * 16, vc + k * 512, 16);
       }
-      constexpr int SC = Shape::kScales / 16;
-      if (lane < 2 * SC) {
-        const bool is_v = lane >= SC;
-        const uint8_t* sc = P.scales + (row + (is_v ? value : 0)) * BLOCKS + (lane - (is_v ? SC : 0)) * 16;
-        cp_async<16>(st + 2 * Shape::kCodes + lane * 16, sc, 16);
-      }
+      if (lane < 2 * SC) cp_async<16>(st + 2 * Shape::kCodes + lane * 16, scales + page * page_scales + offset * BLOCKS, 16);
       return 1u;
     };
     uint32_t valid = 0;  // two bits per stage
     auto issue = [&](int step, int stage) {
       const int page0 = next0, page1 = next1;
       look_up(step + 1);
-      const int key = key0 + step * kAttTile;
+      const int offset = (key0 + step * kAttTile) & page_mask;
       const uint32_t st = ring_s + stage * Shape::kStage;
-      uint32_t ok = copy_half(st, key, page0);
-      ok |= copy_half(st + Shape::kHalf, key + kAttHalf, page1) << 1;
+      uint32_t ok = copy_half(st, offset, page0);
+      ok |= copy_half(st + Shape::kHalf, (offset + kAttHalf) & page_mask, page1) << 1;
       valid = (valid & ~(3u << (2 * stage))) | (ok << (2 * stage));
       cp_async_commit();
     };
@@ -340,7 +362,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 #pragma unroll
     for (int k = 0; k < kAttStages - 1; ++k) issue(skip + k, k);
 
-    // ---- queries: row n = 8 nt + g of this lane, elements [t D/4, (t + 1) D/4)
+    // ---- queries: row n = 8 nt + g of this lane, elements [8t, 8t + 8) of each block
     uint32_t q[NT][QREGS];
     float fq[NT][2];        // score factors of rows 2t and 2t + 1
     int key_lo[NT][2], key_hi[NT][2];  // and the keys they see
@@ -350,16 +372,16 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       const bool on = r < n_rows;
       const int i = on ? (row0 + r) / P.group : 0;
       const int h = head * P.group + (on ? (row0 + r) - i * P.group : 0);
-      const int64_t base = static_cast<int64_t>(seq.q0 + i) * P.q_token + static_cast<int64_t>(h) * P.q_head + t * (D / 4);
+      const int64_t base = static_cast<int64_t>(seq.q0 + i) * P.q_token + static_cast<int64_t>(h) * P.q_head + t * 8;
       const uint16_t* src = static_cast<const uint16_t*>(P.query) + base;
       uint16_t raw[D / 4];
       if (P.q_vec) {
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k)
-          reinterpret_cast<uint4*>(raw)[k] = on ? reinterpret_cast<const uint4*>(src)[k] : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < BLOCKS; ++k)
+          reinterpret_cast<uint4*>(raw)[k] = on ? reinterpret_cast<const uint4*>(src)[4 * k] : make_uint4(0, 0, 0, 0);
       } else {
 #pragma unroll
-        for (int k = 0; k < D / 4; ++k) raw[k] = on ? src[k] : static_cast<uint16_t>(0);
+        for (int k = 0; k < D / 4; ++k) raw[k] = on ? src[k / 8 * 32 + k % 8] : static_cast<uint16_t>(0);
       }
       float f = P.scale_log2;
       if constexpr (BF16) {
@@ -380,7 +402,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 #pragma unroll
         for (int k = 0; k < QREGS; ++k) q[nt][k] = raw[2 * k] | (static_cast<uint32_t>(raw[2 * k + 1]) << 16);
       }
-      f = __fmul_rn(f, 1.0f / 8192.0f);  // keys are held times 2^13
+      f = fmaxf(f, 1e-37f);  // a masked score times it has to stay -infinity
       fq[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t);      // lane of row 2t
       fq[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t + 4);  // lane of row 2t + 1
 #pragma unroll
@@ -420,47 +442,44 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       for (int half = 0; half < 2; ++half) {
         const uint8_t* kc = st + half * Shape::kHalf;
         const uint8_t* ks = kc + 2 * Shape::kCodes;
+        uint32_t wa[BLOCKS], wb[BLOCKS];  // eight codes of each block, of two keys
+        uint32_t sa, sb;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) s[half][nt][c] = 0.0f;
-        constexpr int KW = D / 32;  // words of a row's quarter
-        uint32_t wa[KW], wb[KW];
+        for (int w = 0; w < BLOCKS; ++w) {
+          // Row r, piece w: rows of D / 2 bytes, the piece's place rotated as it was copied (the same for r + 8).
+          const int place = (w ^ key_turn) * 16 + t * 4;
+          wa[w] = *reinterpret_cast<const uint32_t*>(kc + tok_a * (D / 2) + place);
+          wb[w] = *reinterpret_cast<const uint32_t*>(kc + (tok_a + 8) * (D / 2) + place);
+        }
         if constexpr (D == 128) {
-          *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(kc + tok_a * 64 + t * 16);
-          *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(kc + (tok_a + 8) * 64 + t * 16);
+          sa = *reinterpret_cast<const uint32_t*>(ks + tok_a * 4);
+          sb = *reinterpret_cast<const uint32_t*>(ks + (tok_a + 8) * 4);
         } else {
-          *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(kc + tok_a * 32 + t * 8);
-          *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(kc + (tok_a + 8) * 32 + t * 8);
+          sa = *reinterpret_cast<const uint16_t*>(ks + tok_a * 2);
+          sb = *reinterpret_cast<const uint16_t*>(ks + (tok_a + 8) * 2);
         }
-        const int sa = ks[tok_a * BLOCKS + t * BLOCKS / 4], sb = ks[(tok_a + 8) * BLOCKS + t * BLOCKS / 4];
-        int ra = max(sa, __shfl_xor_sync(0xffffffffu, sa, 1));
-        int rb = max(sb, __shfl_xor_sync(0xffffffffu, sb, 1));
-        ra = max(ra, __shfl_xor_sync(0xffffffffu, ra, 2));
-        rb = max(rb, __shfl_xor_sync(0xffffffffu, rb, 2));
-        const uint32_t ma = f16_pow2_13_minus(ra - sa) * 0x10001u, mb = f16_pow2_13_minus(rb - sb) * 0x10001u;
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
+        auto block = [&](auto which) {
+          constexpr int B = decltype(which)::value;
           uint32_t ha[4], hb[4];
-          e2m1x8_to_f16x2(wa[w], ha);
-          e2m1x8_to_f16x2(wb[w], hb);
+          e2m1x8_to_f16x2(wa[B], ha);
+          e2m1x8_to_f16x2(wb[B], hb);
+          const float fa = scale_of<B>(sa), fb = scale_of<B>(sb);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = hmul2(ha[2 * h], ma), a1 = hmul2(hb[2 * h], mb);
-            const uint32_t a2 = hmul2(ha[2 * h + 1], ma), a3 = hmul2(hb[2 * h + 1], mb);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_f16(s[half][nt], a0, a1, a2, a3, q[nt][4 * w + 2 * h], q[nt][4 * w + 2 * h + 1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_f16(acc, ha[0], hb[0], ha[1], hb[1], q[nt][4 * B], q[nt][4 * B + 1]);
+            mma_f16(acc, ha[2], hb[2], ha[3], hb[3], q[nt][4 * B + 2], q[nt][4 * B + 3]);
+            s[half][nt][0] = B == 0 ? __fmul_rn(acc[0], fa) : __fmaf_rn(acc[0], fa, s[half][nt][0]);
+            s[half][nt][1] = B == 0 ? __fmul_rn(acc[1], fa) : __fmaf_rn(acc[1], fa, s[half][nt][1]);
+            s[half][nt][2] = B == 0 ? __fmul_rn(acc[2], fb) : __fmaf_rn(acc[2], fb, s[half][nt][2]);
+            s[half][nt][3] = B == 0 ? __fmul_rn(acc[3], fb) : __fmaf_rn(acc[3], fb, s[half][nt][3]);
           }
-        }
-        // (A row whose largest scale byte is 0 is held to twice its 2^-127.)
-        const float fa = bits_f32(static_cast<uint32_t>(max(ra, 1)) << 23), fb = bits_f32(static_cast<uint32_t>(max(rb, 1)) << 23);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          s[half][nt][0] = __fmul_rn(__fmul_rn(s[half][nt][0], fa), fq[nt][0]);
-          s[half][nt][1] = __fmul_rn(__fmul_rn(s[half][nt][1], fa), fq[nt][1]);
-          s[half][nt][2] = __fmul_rn(__fmul_rn(s[half][nt][2], fb), fq[nt][0]);
-          s[half][nt][3] = __fmul_rn(__fmul_rn(s[half][nt][3], fb), fq[nt][1]);
+        };
+        block(std::integral_constant<int, 0>{});
+        block(std::integral_constant<int, 1>{});
+        if constexpr (BLOCKS == 4) {
+          block(std::integral_constant<int, 2>{});
+          block(std::integral_constant<int, 3>{});
         }
       }
       const bool edge = key < lo_max || key + kAttKeys > hi_min || held != 3u;
@@ -478,18 +497,22 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
             }
         }
       }
+      // (The factors fq are positive: the largest raw score gives the largest.)
       bool raise = false;
+      float most[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-          raise |= fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c])) > __fadd_rn(m[nt][c], kAttSlack);
+        for (int c = 0; c < 2; ++c) {
+          most[nt][c] = __fmul_rn(fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c])), fq[nt][c]);
+          raise |= most[nt][c] > __fadd_rn(m[nt][c], kAttSlack);
+        }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(fmaxf(s[0][nt][c], s[0][nt][2 + c]), fmaxf(s[1][nt][c], s[1][nt][2 + c]));
+            float x = most[nt][c];
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -513,8 +536,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         const float base1 = __fsub_rn(kAttLift, m[nt][1] == -INFINITY ? 0.0f : m[nt][1]);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const float x0 = ex2(__fadd_rn(s[half][nt][0], base0)), x1 = ex2(__fadd_rn(s[half][nt][1], base1));
-          const float x2 = ex2(__fadd_rn(s[half][nt][2], base0)), x3 = ex2(__fadd_rn(s[half][nt][3], base1));
+          const float x0 = ex2(__fmaf_rn(s[half][nt][0], fq[nt][0], base0)), x1 = ex2(__fmaf_rn(s[half][nt][1], fq[nt][1], base1));
+          const float x2 = ex2(__fmaf_rn(s[half][nt][2], fq[nt][0], base0)), x3 = ex2(__fmaf_rn(s[half][nt][3], fq[nt][1], base1));
           l[nt][0] = __fadd_rn(l[nt][0], __fadd_rn(x0, x2));
           l[nt][1] = __fadd_rn(l[nt][1], __fadd_rn(x1, x3));
           p0[half][nt] = transpose8(pack_f16x2(x0, x1));
@@ -524,27 +547,27 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 
       // ---- values: scales first, for the reference
       const int blk = g * BLOCKS / 8;
-      int sv[2][4];
+      uint32_t sv[2][2];  // halfwords: (v_a, v_b), (v_a + 8, v_b + 8)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint8_t* vs = st + half * Shape::kHalf + 2 * Shape::kCodes + Shape::kScales + blk;
-        sv[half][0] = vs[v_a * BLOCKS];
-        sv[half][1] = vs[v_b * BLOCKS];
-        sv[half][2] = vs[(v_a + 8) * BLOCKS];
-        sv[half][3] = vs[(v_b + 8) * BLOCKS];
+        sv[half][0] = vs[v_a * BLOCKS] | (static_cast<uint32_t>(vs[v_b * BLOCKS]) << 16);
+        sv[half][1] = vs[(v_a + 8) * BLOCKS] | (static_cast<uint32_t>(vs[(v_b + 8) * BLOCKS]) << 16);
       }
       if (edge) {
         // Keys that no row sees (stale rows of the page) have no say in the reference.
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int k = key + half * kAttHalf + ((c & 1) ? v_b : v_a) + ((c & 2) ? 8 : 0);
-            if (!((held >> half) & 1u) || k < lo_min || k >= hi_max) sv[half][c] = 0;
+          for (int c = 0; c < 2; ++c) {
+            const int k = key + half * kAttHalf + 8 * c;
+            const bool in = (held >> half) & 1u;
+            if (!in || k + v_a < lo_min || k + v_a >= hi_max) sv[half][c] &= 0xffff0000u;
+            if (!in || k + v_b < lo_min || k + v_b >= hi_max) sv[half][c] &= 0x0000ffffu;
           }
       }
-      const int top = __reduce_max_sync(0xffffffffu, max(max(max(sv[0][0], sv[0][1]), max(sv[0][2], sv[0][3])),
-                                                         max(max(sv[1][0], sv[1][1]), max(sv[1][2], sv[1][3]))));
+      const uint32_t most2 = __vmaxu2(__vmaxu2(sv[0][0], sv[0][1]), __vmaxu2(sv[1][0], sv[1][1]));
+      const int top = __reduce_max_sync(0xffffffffu, static_cast<int>(max(most2 & 0xffffu, most2 >> 16)));
       if (top > ref) {
         const float f = exp2i(max(ref - top, -149));
         ref = top;
@@ -555,6 +578,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 #pragma unroll
             for (int c = 0; c < 4; ++c) o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
       }
+      const uint32_t lift2 = (static_cast<uint32_t>(28 - ref) & 0xffffu) * 0x10001u;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint8_t* vc = st + half * Shape::kHalf + Shape::kCodes;
@@ -572,8 +596,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           vc2[0] = *reinterpret_cast<const uint32_t*>(vc + (v_a + 8) * 32 + g * 4);
           vd[0] = *reinterpret_cast<const uint32_t*>(vc + (v_b + 8) * 32 + g * 4);
         }
-        const uint32_t mlo = f16_pow2_13_minus(ref - sv[half][0]) | (f16_pow2_13_minus(ref - sv[half][1]) << 16);
-        const uint32_t mhi = f16_pow2_13_minus(ref - sv[half][2]) | (f16_pow2_13_minus(ref - sv[half][3]) << 16);
+        const uint32_t mlo = f16_factors(sv[half][0], lift2), mhi = f16_factors(sv[half][1], lift2);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           // Bytes of (first key's code, second key's code): even channels, then odd.
@@ -628,7 +651,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       }
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == seq.tiles;
-    float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (first_segment ? 0 : 1)) * Shape::kSlot;
+    float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (opens ? 0 : 1)) * Shape::kSlot;
     for (int i = threadIdx.x; i < n_rows * D; i += kAttThreads) {
       const int r = i / D, d = i % D;
       float top = row_m[0][r];
@@ -655,9 +678,6 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       }
     }
     __syncthreads();
-    at += tile1 - tile0;
-    rem += tile1 - tile0;
-    first_segment = false;
   }
 }
 
@@ -682,8 +702,8 @@ __global__ void __launch_bounds__(kAttJoinThreads) attention_join_kernel(const A
   // (The grid has a block per unit when the caller's bound on the queries holds.)
   for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
     const AttShares shares(total, blocks);
-    const int64_t u0 = before + unit * seq.tiles, u1 = u0 + seq.tiles;  // its tiles
-    const int64_t j0 = shares.block_of(u0), j1 = shares.block_of(u1 - 1) + 1;  // and the blocks that share them
+    const int64_t u0 = before + unit * (seq.tiles + kAttStart), u1 = u0 + seq.tiles + kAttStart;
+    const int64_t j0 = shares.block_of(u0 + kAttStart), j1 = shares.block_of(u1 - 1) + 1;  // the blocks that share its tiles
     if (j1 - j0 == 1) continue;  // one block had it all
     // A block's partial result is in its first slot when its share starts with this unit.
     const float* first = P.partial + (2 * j0 + (u0 <= shares.first(j0) ? 0 : 1)) * Shape::kSlot;

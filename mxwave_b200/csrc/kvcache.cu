@@ -27,7 +27,7 @@ struct KvRows {
   uint8_t* scales;
   const int64_t* slots;
   int64_t tokens, n_slots;  // slots of the pool
-  int heads, dim, page;
+  int heads, dim, page_shift;
   int units;      // eight-element pieces of a token: 2 heads dim / 8
   int per_block;  // tokens per block
 };
@@ -45,8 +45,8 @@ __device__ __forceinline__ KvPiece kv_piece(const KvRows& P, int r) {
 
 // The row's index among all rows of the pool.
 __device__ __forceinline__ int64_t kv_row(const KvRows& P, int64_t slot, const KvPiece& p) {
-  const int64_t page = slot / P.page, offset = slot - page * P.page;
-  return ((page * 2 + p.part) * P.heads + p.head) * P.page + offset;
+  const int64_t page = slot >> P.page_shift, offset = slot & ((1 << P.page_shift) - 1);
+  return (((page * 2 + p.part) * P.heads + p.head) << P.page_shift) + offset;
 }
 
 template <int DT>
@@ -263,7 +263,7 @@ static KvRows kv_rows(uint8_t* codes, uint8_t* scales, const int64_t* slots, int
   P.n_slots = pages * page;
   P.heads = static_cast<int>(heads);
   P.dim = static_cast<int>(dim);
-  P.page = static_cast<int>(page);
+  P.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   P.units = static_cast<int>(2 * heads * dim / 8);
   P.per_block = std::max(1, kKvThreads / P.units);
   return P;
