@@ -183,6 +183,48 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with a zero accumulator.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// Shared-memory loads by 32-bit address and a constant offset: the kernel's
+// lanes keep their places and add only the stage.
+template <int OFF>
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1+%2];" : "=r"(v) : "r"(a), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1+%2];" : "=h"(v) : "r"(a), "n"(OFF));
+  return v;
+}
+template <int OFF>
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1+%2];" : "=r"(v) : "r"(a), "n"(OFF));
+  return v;
+}
+// WORDS (1 or 2) consecutive words.
+template <int WORDS, int OFF>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&v)[WORDS]) {
+  if constexpr (WORDS == 2)
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2+%3];" : "=r"(v[0]), "=r"(v[1]) : "r"(a), "n"(OFF));
+  else
+    v[0] = lds32<OFF>(a);
+}
+// The low nibbles of `a` and the high nibbles of `b`: one three-input operation.
+__device__ __forceinline__ uint32_t nibbles(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xCA;" : "=r"(d) : "r"(0x0f0f0f0fu), "r"(a), "r"(b));
+  return d;
+}
 // Two scale bytes, as halfwords, to f16 factors 2^(13 - (ref - byte)): zero from ref - byte = 28 on.
 __device__ __forceinline__ uint32_t f16_factors(uint32_t bytes2, uint32_t lift2) {
   return __vmaxs2(__vadd2(bytes2, lift2), 0u) << 10;
@@ -242,9 +284,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
   grid_dependents_launch();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = att_smem + warp * Shape::kRing;
   float* join = reinterpret_cast<float*>(att_smem);  // [warp][row][D]
-  const uint32_t ring_s = smem_u32(ring);
+  const uint32_t ring_s = smem_u32(att_smem) + warp * Shape::kRing;
 
   att_clear_rest<BF16>(P, D);
   int64_t total, ignored;
@@ -278,7 +319,16 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
 
   const int tok_a = g ^ ((g >> 1) & 1);  // key of row g of S^T (row g + 8: 8 further on)
   const int v_a = (2 * t) ^ (t & 1), v_b = (2 * t + 1) ^ (t & 1);  // keys of the contraction's slots 2t, 2t + 1
-  const int key_turn = D == 128 ? (tok_a >> 1) & 3 : (tok_a >> 2) & 1;
+  // Where this lane's 16-byte pieces of a copy go, and where it reads (bytes of half a stage).  Pieces of
+  // key rows rotate over pairs of rows (D = 128) or fours; value rows four apart have their halves swapped.
+  const uint32_t key_put = 16u * (D == 128 ? lane ^ ((lane >> 3) & 3) : lane ^ ((lane >> 3) & 1));
+  const uint32_t value_put = 16u * (D == 128 ? lane ^ (((lane >> 4) & 1) << 1) : lane);
+  const uint32_t key_get = tok_a * (D / 2) + t * 4 + 16u * (D == 128 ? (tok_a >> 1) & 3 : (tok_a >> 2) & 1);
+  const uint32_t value_a = Shape::kCodes + v_a * (D / 2) + (D == 128 ? (g * 8) ^ ((t & 2) << 4) : g * 4);
+  const uint32_t value_b = value_a + (v_b - v_a) * (D / 2);
+  const uint32_t key_scale = 2 * Shape::kCodes + tok_a * BLOCKS;
+  const uint32_t scale_a = 2 * Shape::kCodes + Shape::kScales + v_a * BLOCKS + g * BLOCKS / 8;
+  const uint32_t scale_b = scale_a + (v_b - v_a) * BLOCKS;
   bool first_segment = true;
   while (at < end) {
     while (rem >= att_work(P, seq)) {
@@ -316,45 +366,54 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
     const int page_mask = (1 << P.page_shift) - 1;
     // Bytes of a page, of one head's rows in it, and this lane's place in both arrays.
     const int head_codes = (D / 2) << P.page_shift, head_scales = BLOCKS << P.page_shift;
-    const int64_t page_codes = 2ll * P.kv_heads * head_codes, page_scales = 2ll * P.kv_heads * head_scales;
+    const uint32_t page_codes = 2u * P.kv_heads * head_codes, page_scales = 2u * P.kv_heads * head_scales;
     constexpr int SC = Shape::kScales / 16;  // 16-byte pieces of 16 rows' scales
     const uint8_t* codes = P.codes + static_cast<int64_t>(head) * head_codes + lane * 16;
     const int64_t to_values = static_cast<int64_t>(P.kv_heads) * head_codes;
     const uint8_t* scales = P.scales + static_cast<int64_t>(head) * head_scales +
                             (lane < SC ? lane * 16 : static_cast<int64_t>(P.kv_heads) * head_scales + (lane - SC) * 16);
 
-    // Pages of a step's halves, -1 past the end: looked up one step before they are needed.
+    // Copies 16 rows, from this lane's first piece on, into half a stage.
+    auto copy_half = [&](uint32_t st, const uint8_t* kc, const uint8_t* sc) {
+      const uint8_t* vc = kc + to_values;
+#pragma unroll
+      for (int k = 0; k < Shape::kCodes / 512; ++k) {
+        cp_async<16>(st + key_put + (k * 512), kc + k * 512, 16);
+        cp_async<16>(st + value_put + (Shape::kCodes + k * 512), vc + k * 512, 16);
+      }
+      if (lane < 2 * SC) cp_async<16>(st + lane * 16 + 2 * Shape::kCodes, sc, 16);
+    };
+    // Pages of a step's halves (-1 past the end, one lookup where a page holds
+    // both), read one step before they are needed.
+    const bool apart = P.page_shift == 4;
     int next0 = -1, next1 = -1;
     auto look_up = [&](int step) {
       const int key = key0 + step * kAttTile;
       next0 = key < key_end ? table[key >> P.page_shift] : -1;
-      next1 = key + kAttHalf < key_end ? table[(key + kAttHalf) >> P.page_shift] : -1;
+      if (apart) next1 = key + kAttHalf < key_end ? table[(key + kAttHalf) >> P.page_shift] : -1;
     };
-    // Copies 16 rows into half a stage; 0 when the page is not one of the pool's.
-    auto copy_half = [&](uint32_t st, int offset, int page) -> uint32_t {
-      if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(P.pages)) return 0u;
-      const uint8_t* kc = codes + page * page_codes + offset * (D / 2);
-      const uint8_t* vc = kc + to_values;
-#pragma unroll
-      for (int k = 0; k < Shape::kCodes / 512; ++k) {
-        const int c = k * 32 + lane;
-        // Pieces of key rows rotate over pairs of rows; value rows four apart have their halves swapped.
-        const int kd = D == 128 ? (c ^ ((c >> 3) & 3)) : (c ^ ((c >> 3) & 1));
-        cp_async<16>(st + kd * 16, kc + k * 512, 16);
-        const int vd = D == 128 ? (c ^ (((c >> 4) & 1) << 1)) : c;
-        cp_async<16>(st + Shape::kCodes + vd * 16, vc + k * 512, 16);
-      }
-      if (lane < 2 * SC) cp_async<16>(st + 2 * Shape::kCodes + lane * 16, scales + page * page_scales + offset * BLOCKS, 16);
-      return 1u;
-    };
-    uint32_t valid = 0;  // two bits per stage
+    uint32_t valid = 0;  // two bits per stage: its halves hold rows of pages of the pool
     auto issue = [&](int step, int stage) {
       const int page0 = next0, page1 = next1;
       look_up(step + 1);
       const int offset = (key0 + step * kAttTile) & page_mask;
       const uint32_t st = ring_s + stage * Shape::kStage;
-      uint32_t ok = copy_half(st, offset, page0);
-      ok |= copy_half(st + Shape::kHalf, (offset + kAttHalf) & page_mask, page1) << 1;
+      uint32_t ok = 0;
+      if (static_cast<uint32_t>(page0) < static_cast<uint32_t>(P.pages)) {
+        const uint8_t* kc = codes + static_cast<uint64_t>(static_cast<uint32_t>(page0)) * page_codes + offset * (D / 2);
+        const uint8_t* sc = scales + static_cast<uint64_t>(static_cast<uint32_t>(page0)) * page_scales + offset * BLOCKS;
+        copy_half(st, kc, sc);
+        ok = 1;
+        if (!apart) {
+          copy_half(st + Shape::kHalf, kc + Shape::kCodes, sc + Shape::kScales);
+          ok = 3;
+        }
+      }
+      if (apart && static_cast<uint32_t>(page1) < static_cast<uint32_t>(P.pages)) {
+        copy_half(st + Shape::kHalf, codes + static_cast<uint64_t>(static_cast<uint32_t>(page1)) * page_codes,
+                  scales + static_cast<uint64_t>(static_cast<uint32_t>(page1)) * page_scales);
+        ok |= 2;
+      }
       valid = (valid & ~(3u << (2 * stage))) | (ok << (2 * stage));
       cp_async_commit();
     };
@@ -433,46 +492,43 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       cp_async_wait<kAttStages - 1>();
       __syncwarp();
       const int key = key0 + step * kAttTile;
-      const uint8_t* st = ring + stage * Shape::kStage;
+      const uint32_t st = ring_s + stage * Shape::kStage;
       const uint32_t held = (valid >> (2 * stage)) & 3u;
 
       // ---- scores
       float s[2][NT][4];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint8_t* kc = st + half * Shape::kHalf;
-        const uint8_t* ks = kc + 2 * Shape::kCodes;
+      auto score_half = [&](auto which) {
+        constexpr int H = decltype(which)::value, OFF = H * Shape::kHalf;
         uint32_t wa[BLOCKS], wb[BLOCKS];  // eight codes of each block, of two keys
-        uint32_t sa, sb;
 #pragma unroll
         for (int w = 0; w < BLOCKS; ++w) {
-          // Row r, piece w: rows of D / 2 bytes, the piece's place rotated as it was copied (the same for r + 8).
-          const int place = (w ^ key_turn) * 16 + t * 4;
-          wa[w] = *reinterpret_cast<const uint32_t*>(kc + tok_a * (D / 2) + place);
-          wb[w] = *reinterpret_cast<const uint32_t*>(kc + (tok_a + 8) * (D / 2) + place);
+          const uint32_t a = st + (key_get ^ (16u * w));
+          wa[w] = lds32<OFF>(a);
+          wb[w] = lds32<OFF + 8 * D / 2>(a);
         }
+        uint32_t sa, sb;
         if constexpr (D == 128) {
-          sa = *reinterpret_cast<const uint32_t*>(ks + tok_a * 4);
-          sb = *reinterpret_cast<const uint32_t*>(ks + (tok_a + 8) * 4);
+          sa = lds32<OFF>(st + key_scale);
+          sb = lds32<OFF + 8 * BLOCKS>(st + key_scale);
         } else {
-          sa = *reinterpret_cast<const uint16_t*>(ks + tok_a * 2);
-          sb = *reinterpret_cast<const uint16_t*>(ks + (tok_a + 8) * 2);
+          sa = lds16<OFF>(st + key_scale);
+          sb = lds16<OFF + 8 * BLOCKS>(st + key_scale);
         }
-        auto block = [&](auto which) {
-          constexpr int B = decltype(which)::value;
+        auto block = [&](auto index) {
+          constexpr int B = decltype(index)::value;
           uint32_t ha[4], hb[4];
           e2m1x8_to_f16x2(wa[B], ha);
           e2m1x8_to_f16x2(wb[B], hb);
           const float fa = scale_of<B>(sa), fb = scale_of<B>(sb);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16(acc, ha[0], hb[0], ha[1], hb[1], q[nt][4 * B], q[nt][4 * B + 1]);
+            float acc[4];
+            mma_f16_first(acc, ha[0], hb[0], ha[1], hb[1], q[nt][4 * B], q[nt][4 * B + 1]);
             mma_f16(acc, ha[2], hb[2], ha[3], hb[3], q[nt][4 * B + 2], q[nt][4 * B + 3]);
-            s[half][nt][0] = B == 0 ? __fmul_rn(acc[0], fa) : __fmaf_rn(acc[0], fa, s[half][nt][0]);
-            s[half][nt][1] = B == 0 ? __fmul_rn(acc[1], fa) : __fmaf_rn(acc[1], fa, s[half][nt][1]);
-            s[half][nt][2] = B == 0 ? __fmul_rn(acc[2], fb) : __fmaf_rn(acc[2], fb, s[half][nt][2]);
-            s[half][nt][3] = B == 0 ? __fmul_rn(acc[3], fb) : __fmaf_rn(acc[3], fb, s[half][nt][3]);
+            s[H][nt][0] = B == 0 ? __fmul_rn(acc[0], fa) : __fmaf_rn(acc[0], fa, s[H][nt][0]);
+            s[H][nt][1] = B == 0 ? __fmul_rn(acc[1], fa) : __fmaf_rn(acc[1], fa, s[H][nt][1]);
+            s[H][nt][2] = B == 0 ? __fmul_rn(acc[2], fb) : __fmaf_rn(acc[2], fb, s[H][nt][2]);
+            s[H][nt][3] = B == 0 ? __fmul_rn(acc[3], fb) : __fmaf_rn(acc[3], fb, s[H][nt][3]);
           }
         };
         block(std::integral_constant<int, 0>{});
@@ -481,7 +537,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           block(std::integral_constant<int, 2>{});
           block(std::integral_constant<int, 3>{});
         }
-      }
+      };
+      score_half(std::integral_constant<int, 0>{});
+      score_half(std::integral_constant<int, 1>{});
       const bool edge = key < lo_max || key + kAttKeys > hi_min || held != 3u;
       if (edge) {
 #pragma unroll
@@ -546,14 +604,11 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       }
 
       // ---- values: scales first, for the reference
-      const int blk = g * BLOCKS / 8;
       uint32_t sv[2][2];  // halfwords: (v_a, v_b), (v_a + 8, v_b + 8)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint8_t* vs = st + half * Shape::kHalf + 2 * Shape::kCodes + Shape::kScales + blk;
-        sv[half][0] = vs[v_a * BLOCKS] | (static_cast<uint32_t>(vs[v_b * BLOCKS]) << 16);
-        sv[half][1] = vs[(v_a + 8) * BLOCKS] | (static_cast<uint32_t>(vs[(v_b + 8) * BLOCKS]) << 16);
-      }
+      sv[0][0] = lds8<0>(st + scale_a) | (lds8<0>(st + scale_b) << 16);
+      sv[0][1] = lds8<8 * BLOCKS>(st + scale_a) | (lds8<8 * BLOCKS>(st + scale_b) << 16);
+      sv[1][0] = lds8<Shape::kHalf>(st + scale_a) | (lds8<Shape::kHalf>(st + scale_b) << 16);
+      sv[1][1] = lds8<Shape::kHalf + 8 * BLOCKS>(st + scale_a) | (lds8<Shape::kHalf + 8 * BLOCKS>(st + scale_b) << 16);
       if (edge) {
         // Keys that no row sees (stale rows of the page) have no say in the reference.
 #pragma unroll
@@ -579,41 +634,34 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
             for (int c = 0; c < 4; ++c) o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
       }
       const uint32_t lift2 = (static_cast<uint32_t>(28 - ref) & 0xffffu) * 0x10001u;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const uint8_t* vc = st + half * Shape::kHalf + Shape::kCodes;
+      auto value_half = [&](auto which) {
+        constexpr int H = decltype(which)::value, OFF = H * Shape::kHalf;
         constexpr int VW = D / 64;  // words of an eighth of a row
-        uint32_t va[VW], vb[VW], vc2[VW], vd[VW];
-        if constexpr (D == 128) {
-          const int ch = (g * 8) ^ ((t & 2) << 4);  // rows 4..7 and 12..15 have their halves swapped
-          *reinterpret_cast<uint2*>(va) = *reinterpret_cast<const uint2*>(vc + v_a * 64 + ch);
-          *reinterpret_cast<uint2*>(vb) = *reinterpret_cast<const uint2*>(vc + v_b * 64 + ch);
-          *reinterpret_cast<uint2*>(vc2) = *reinterpret_cast<const uint2*>(vc + (v_a + 8) * 64 + ch);
-          *reinterpret_cast<uint2*>(vd) = *reinterpret_cast<const uint2*>(vc + (v_b + 8) * 64 + ch);
-        } else {
-          va[0] = *reinterpret_cast<const uint32_t*>(vc + v_a * 32 + g * 4);
-          vb[0] = *reinterpret_cast<const uint32_t*>(vc + v_b * 32 + g * 4);
-          vc2[0] = *reinterpret_cast<const uint32_t*>(vc + (v_a + 8) * 32 + g * 4);
-          vd[0] = *reinterpret_cast<const uint32_t*>(vc + (v_b + 8) * 32 + g * 4);
-        }
-        const uint32_t mlo = f16_factors(sv[half][0], lift2), mhi = f16_factors(sv[half][1], lift2);
+        uint32_t wa[VW], wb[VW], wc[VW], wd[VW];
+        lds_words<VW, OFF>(st + value_a, wa);
+        lds_words<VW, OFF>(st + value_b, wb);
+        lds_words<VW, OFF + 8 * D / 2>(st + value_a, wc);
+        lds_words<VW, OFF + 8 * D / 2>(st + value_b, wd);
+        const uint32_t mlo = f16_factors(sv[H][0], lift2), mhi = f16_factors(sv[H][1], lift2);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           // Bytes of (first key's code, second key's code): even channels, then odd.
           uint32_t el[4], ol[4], eh[4], oh[4];
-          e2m1x8_to_f16x2((va[w] & 0x0f0f0f0fu) | ((vb[w] << 4) & 0xf0f0f0f0u), el);
-          e2m1x8_to_f16x2(((va[w] >> 4) & 0x0f0f0f0fu) | (vb[w] & 0xf0f0f0f0u), ol);
-          e2m1x8_to_f16x2((vc2[w] & 0x0f0f0f0fu) | ((vd[w] << 4) & 0xf0f0f0f0u), eh);
-          e2m1x8_to_f16x2(((vc2[w] >> 4) & 0x0f0f0f0fu) | (vd[w] & 0xf0f0f0f0u), oh);
+          e2m1x8_to_f16x2(nibbles(wa[w], wb[w] << 4), el);
+          e2m1x8_to_f16x2(nibbles(wa[w] >> 4, wb[w]), ol);
+          e2m1x8_to_f16x2(nibbles(wc[w], wd[w] << 4), eh);
+          e2m1x8_to_f16x2(nibbles(wc[w] >> 4, wd[w]), oh);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t a0 = hmul2(el[k], mlo), a1 = hmul2(ol[k], mlo);
             const uint32_t a2 = hmul2(eh[k], mhi), a3 = hmul2(oh[k], mhi);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + k], a0, a1, a2, a3, p0[half][nt], p1[half][nt]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][4 * w + k], a0, a1, a2, a3, p0[H][nt], p1[H][nt]);
           }
         }
-      }
+      };
+      value_half(std::integral_constant<int, 0>{});
+      value_half(std::integral_constant<int, 1>{});
       __syncwarp();
       stage = stage == kAttStages - 1 ? 0 : stage + 1;
     }
