@@ -191,6 +191,12 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
+__device__ __forceinline__ void cp_async16_if(bool on, uint32_t saddr, const void* src, uint32_t src_bytes) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(saddr),
+      "l"(src), "r"(src_bytes), "r"(static_cast<uint32_t>(on))
+      : "memory");
+}
 // Shared-memory loads by 32-bit address and a constant offset: the kernel's
 // lanes keep their places and add only the stage.
 template <int OFF>
@@ -362,58 +368,49 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
     const int key_end = min(seq.lo + tile1 * kAttTile, hi_max);
     const int skip = lo_min > key0 ? (lo_min - key0) / kAttTile : 0;  // steps that end before the window
     const int steps = key_end > key0 ? (key_end - key0 + kAttTile - 1) / kAttTile : 0;
-    const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
-    const int page_mask = (1 << P.page_shift) - 1;
-    // Bytes of a page, of one head's rows in it, and this lane's place in both arrays.
+    // A page's size divides a tile's, so a step's place in its page is that of
+    // the first step.  This lane's places in a page, and the step from page to page:
+    const bool apart = P.page_shift == 4;  // each half of a step has a page of its own
+    const int offset = key0 & ((1 << P.page_shift) - 1);
     const int head_codes = (D / 2) << P.page_shift, head_scales = BLOCKS << P.page_shift;
     const uint32_t page_codes = 2u * P.kv_heads * head_codes, page_scales = 2u * P.kv_heads * head_scales;
-    constexpr int SC = Shape::kScales / 16;  // 16-byte pieces of 16 rows' scales
-    const uint8_t* codes = P.codes + static_cast<int64_t>(head) * head_codes + lane * 16;
+    constexpr int SC = Shape::kScales / 16;  // 16-byte pieces of 16 rows' scales: lanes 0.. keys, SC.. values
+    const uint8_t* codes = P.codes + static_cast<int64_t>(head) * head_codes + offset * (D / 2) + lane * 16;
     const int64_t to_values = static_cast<int64_t>(P.kv_heads) * head_codes;
-    const uint8_t* scales = P.scales + static_cast<int64_t>(head) * head_scales +
+    const uint8_t* scales = P.scales + static_cast<int64_t>(head) * head_scales + offset * BLOCKS +
                             (lane < SC ? lane * 16 : static_cast<int64_t>(P.kv_heads) * head_scales + (lane - SC) * 16);
+    const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld + (key0 >> P.page_shift);
+    const int table_step = kAttTile >> P.page_shift;
 
-    // Copies 16 rows, from this lane's first piece on, into half a stage.
-    auto copy_half = [&](uint32_t st, const uint8_t* kc, const uint8_t* sc) {
+    // Copies 16 rows of a page into half a stage, zeros for a page outside the
+    // pool (no branch, and no read: the copies' source size is zero).
+    auto copy_half = [&](uint32_t st, int page, uint32_t in_page) -> uint32_t {
+      const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(P.pages);
+      const uint32_t at = ok ? page : 0, bytes = ok ? 16u : 0u;
+      const uint8_t* kc = codes + static_cast<uint64_t>(at) * page_codes + in_page * (D / 2);
       const uint8_t* vc = kc + to_values;
+      const uint8_t* sc = scales + static_cast<uint64_t>(at) * page_scales + in_page * BLOCKS;
 #pragma unroll
       for (int k = 0; k < Shape::kCodes / 512; ++k) {
-        cp_async<16>(st + key_put + (k * 512), kc + k * 512, 16);
-        cp_async<16>(st + value_put + (Shape::kCodes + k * 512), vc + k * 512, 16);
+        cp_async<16>(st + key_put + (k * 512), kc + k * 512, bytes);
+        cp_async<16>(st + value_put + (Shape::kCodes + k * 512), vc + k * 512, bytes);
       }
-      if (lane < 2 * SC) cp_async<16>(st + lane * 16 + 2 * Shape::kCodes, sc, 16);
+      cp_async16_if(lane < 2 * SC, st + lane * 16 + 2 * Shape::kCodes, sc, bytes);
+      return ok ? 1u : 0u;
     };
-    // Pages of a step's halves (-1 past the end, one lookup where a page holds
-    // both), read one step before they are needed.
-    const bool apart = P.page_shift == 4;
+    // Pages of a step's halves (-1 past the end), read one step before they are needed.
     int next0 = -1, next1 = -1;
     auto look_up = [&](int step) {
-      const int key = key0 + step * kAttTile;
-      next0 = key < key_end ? table[key >> P.page_shift] : -1;
-      if (apart) next1 = key + kAttHalf < key_end ? table[(key + kAttHalf) >> P.page_shift] : -1;
+      next0 = step < steps ? table[step * table_step] : -1;
+      if (apart) next1 = key0 + step * kAttTile + kAttHalf < key_end ? table[step * table_step + 1] : -1;
     };
     uint32_t valid = 0;  // two bits per stage: its halves hold rows of pages of the pool
     auto issue = [&](int step, int stage) {
-      const int page0 = next0, page1 = next1;
+      const int page0 = next0, page1 = apart ? next1 : next0;
       look_up(step + 1);
-      const int offset = (key0 + step * kAttTile) & page_mask;
       const uint32_t st = ring_s + stage * Shape::kStage;
-      uint32_t ok = 0;
-      if (static_cast<uint32_t>(page0) < static_cast<uint32_t>(P.pages)) {
-        const uint8_t* kc = codes + static_cast<uint64_t>(static_cast<uint32_t>(page0)) * page_codes + offset * (D / 2);
-        const uint8_t* sc = scales + static_cast<uint64_t>(static_cast<uint32_t>(page0)) * page_scales + offset * BLOCKS;
-        copy_half(st, kc, sc);
-        ok = 1;
-        if (!apart) {
-          copy_half(st + Shape::kHalf, kc + Shape::kCodes, sc + Shape::kScales);
-          ok = 3;
-        }
-      }
-      if (apart && static_cast<uint32_t>(page1) < static_cast<uint32_t>(P.pages)) {
-        copy_half(st + Shape::kHalf, codes + static_cast<uint64_t>(static_cast<uint32_t>(page1)) * page_codes,
-                  scales + static_cast<uint64_t>(static_cast<uint32_t>(page1)) * page_scales);
-        ok |= 2;
-      }
+      uint32_t ok = copy_half(st, page0, 0);
+      ok |= copy_half(st + Shape::kHalf, page1, apart ? 0 : kAttHalf) << 1;
       valid = (valid & ~(3u << (2 * stage))) | (ok << (2 * stage));
       cp_async_commit();
     };
@@ -555,8 +552,28 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
             }
         }
       }
+      // ---- scales of the values
+      uint32_t sv[2][2];  // halfwords: (v_a, v_b), (v_a + 8, v_b + 8)
+      sv[0][0] = lds8<0>(st + scale_a) | (lds8<0>(st + scale_b) << 16);
+      sv[0][1] = lds8<8 * BLOCKS>(st + scale_a) | (lds8<8 * BLOCKS>(st + scale_b) << 16);
+      sv[1][0] = lds8<Shape::kHalf>(st + scale_a) | (lds8<Shape::kHalf>(st + scale_b) << 16);
+      sv[1][1] = lds8<Shape::kHalf + 8 * BLOCKS>(st + scale_a) | (lds8<Shape::kHalf + 8 * BLOCKS>(st + scale_b) << 16);
+      if (edge) {
+        // Keys that no row sees (stale rows of the page) have no say in the reference.
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int k = key + half * kAttHalf + 8 * c;
+            const bool in = (held >> half) & 1u;
+            if (!in || k + v_a < lo_min || k + v_a >= hi_max) sv[half][c] &= 0xffff0000u;
+            if (!in || k + v_b < lo_min || k + v_b >= hi_max) sv[half][c] &= 0x0000ffffu;
+          }
+      }
       // (The factors fq are positive: the largest raw score gives the largest.)
-      bool raise = false;
+      const uint32_t most2 = __vmaxu2(__vmaxu2(sv[0][0], sv[0][1]), __vmaxu2(sv[1][0], sv[1][1]));
+      const int lane_top = static_cast<int>(max(most2 & 0xffffu, most2 >> 16));
+      bool raise = lane_top > ref;
       float most[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -584,6 +601,17 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
               o[nt][k][2 + c] = __fmul_rn(o[nt][k][2 + c], f);
             }
           }
+        const int top = __reduce_max_sync(0xffffffffu, lane_top);
+        if (top > ref) {
+          const float f = exp2i(max(ref - top, -149));
+          ref = top;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
+        }
       }
 
       // ---- probabilities, transposed into the second product's operand
@@ -603,36 +631,6 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         }
       }
 
-      // ---- values: scales first, for the reference
-      uint32_t sv[2][2];  // halfwords: (v_a, v_b), (v_a + 8, v_b + 8)
-      sv[0][0] = lds8<0>(st + scale_a) | (lds8<0>(st + scale_b) << 16);
-      sv[0][1] = lds8<8 * BLOCKS>(st + scale_a) | (lds8<8 * BLOCKS>(st + scale_b) << 16);
-      sv[1][0] = lds8<Shape::kHalf>(st + scale_a) | (lds8<Shape::kHalf>(st + scale_b) << 16);
-      sv[1][1] = lds8<Shape::kHalf + 8 * BLOCKS>(st + scale_a) | (lds8<Shape::kHalf + 8 * BLOCKS>(st + scale_b) << 16);
-      if (edge) {
-        // Keys that no row sees (stale rows of the page) have no say in the reference.
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int k = key + half * kAttHalf + 8 * c;
-            const bool in = (held >> half) & 1u;
-            if (!in || k + v_a < lo_min || k + v_a >= hi_max) sv[half][c] &= 0xffff0000u;
-            if (!in || k + v_b < lo_min || k + v_b >= hi_max) sv[half][c] &= 0x0000ffffu;
-          }
-      }
-      const uint32_t most2 = __vmaxu2(__vmaxu2(sv[0][0], sv[0][1]), __vmaxu2(sv[1][0], sv[1][1]));
-      const int top = __reduce_max_sync(0xffffffffu, static_cast<int>(max(most2 & 0xffffu, most2 >> 16)));
-      if (top > ref) {
-        const float f = exp2i(max(ref - top, -149));
-        ref = top;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[nt][k][c] = __fmul_rn(o[nt][k][c], f);
-      }
       const uint32_t lift2 = (static_cast<uint32_t>(28 - ref) & 0xffffu) * 0x10001u;
       auto value_half = [&](auto which) {
         constexpr int H = decltype(which)::value, OFF = H * Shape::kHalf;
