@@ -282,7 +282,7 @@ MXW_API int mxw_finalize_block_hessian(const float* gram, int full, int64_t cols
  *   workspace device memory, 16-byte aligned, of at least
  *             mxw_linear_workspace_size(rows, inner, dtype) bytes; calls that
  *             share one must not overlap on the device
- * inner % 32 == 0; packed 8-byte aligned.  fp32 accumulation; the fixed order
+ * inner % 32 == 0; packed 16-byte aligned.  fp32 accumulation; the fixed order
  * of additions makes results reproducible.  A row of x that holds a NaN or an
  * infinity gives NaN in all its outputs; so does a scale byte 255.
  * flags: MXW_FLAG_TIMEOUT or NULL.

@@ -14,16 +14,14 @@
 // Products and sums are fp32 in TMEM.  A block that holds a NaN or an infinity
 // gets the NaN scale: every output of that row of x is NaN.
 //
-// Two launches:
-//   linear_terms_kernel   x -> terms and scales, as images of the shared-memory
-//                         tiles the product reads (K-major, 128-byte swizzle)
-//   linear_kernel         the product with its epilogue
-// CTA tile: 128 outputs (M, W's rows) x NT rows of x (N).  Four warps copy W's
-// codes with 8-byte cp.async into the 16-byte slots that E2M1 operands take in
-// shared memory (8 bytes of codes, 8 of padding) and its scales into the
-// tensor cores' scale layout; the terms come as bulk copies.  One thread of
-// a fifth warp issues the products.  When there are too few tiles for the SMs
-// the CTAs of a cluster split K and add their fp32 partial tiles over
+// CTA tile: 128 outputs (M, W's rows) x NT rows of x (N), 128 inputs a stage.
+// One thread copies W's packed bytes (TMA) and the terms of x (bulk copies of
+// what linear_terms_kernel laid out) into a ring; four warps spread the codes
+// into the 16-byte slots that E2M1 operands take in shared memory (8 bytes of
+// codes, 8 of padding) and put the scales into the tensor cores' layout; one
+// thread issues the products.  Up to 16 rows of x the four warps make the
+// terms themselves and there is one launch.  When there are too few tiles for
+// the SMs the CTAs of a cluster split K and add their fp32 partial tiles over
 // distributed shared memory in rank order, so results do not change from run
 // to run.
 #include <cuda_bf16.h>
@@ -39,36 +37,44 @@ namespace cg = cooperative_groups;
 
 namespace mxw {
 
-constexpr int kLinM = 128;       // outputs per tile
-constexpr int kLinK = 128;       // inputs per stage
-constexpr int kLinLoaders = 128;  // threads that copy W, and the epilogue's
-constexpr int kLinThreads = kLinLoaders + 32;
-constexpr int kLinWBytes = kLinM * kLinK;  // E2M1 in shared memory: 16 bytes per 16 codes
-constexpr int kLinSfBytes = 512;           // scales of 128 rows x 4 blocks
+constexpr int kLinM = 128;        // outputs per tile
+constexpr int kLinK = 128;        // inputs per stage
+constexpr int kLinSpread = 128;   // threads that spread W's codes, and the epilogue's
+constexpr int kLinThreads = 32 + kLinSpread + 32;  // copies, spreading, products
+constexpr int kLinRawBytes = kLinM * kLinK / 2;    // packed codes of a stage
+constexpr int kLinWBytes = kLinM * kLinK;          // spread: 16 bytes per 16 codes
+constexpr int kLinSfBytes = 512;                   // scales of 128 rows x 4 blocks
 
 template <int NT, int TERMS>
 struct LinearTile {
+  static constexpr bool kFused = NT == 16;  // terms made in the product's kernel
   static constexpr int kTermBytes = NT * kLinK;
   static constexpr int kSfTiles = (NT + 127) / 128;  // 128-row groups of the x scales
   static constexpr int kTermSfBytes = kSfTiles * kLinSfBytes;
-  static constexpr int kXBytes = TERMS * (kTermBytes + kTermSfBytes);  // one chunk of x in the workspace
-  static constexpr int kStageBytes = kLinWBytes + kLinSfBytes + kXBytes;
-  static constexpr int kBudget = NT <= 32 ? 110 * 1024 : 220 * 1024;  // two CTAs per SM for small tiles
-  static constexpr int kStages = kBudget / ((kStageBytes + 1023) / 1024 * 1024) < 8
-                                     ? kBudget / ((kStageBytes + 1023) / 1024 * 1024)
-                                     : 8;
+  static constexpr int kXBytes = TERMS * (kTermBytes + kTermSfBytes);  // one chunk of x: terms, then their scales
+  // A stage of copies: [x terms][x scales][packed W], and a spread buffer:
+  // [W][x terms][x scales][W scales], the x parts where they are made.
+  static constexpr int kStage = (kFused ? 0 : kXBytes) + kLinRawBytes;
+  static constexpr int kStageStride = (kStage + 1023) / 1024 * 1024;
+  static constexpr int kSpread = kLinWBytes + (kFused ? kXBytes : 0) + kLinSfBytes;
+  static constexpr int kSpreadStride = (kSpread + 1023) / 1024 * 1024;
+  static constexpr int kBuffers = 2;
+  static constexpr int kBudget = NT <= 32 ? 111 * 1024 : 222 * 1024;  // two CTAs per SM for small tiles
+  static constexpr int kFit = (kBudget - kBuffers * kSpreadStride) / kStageStride;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
   static_assert(kStages >= 2, "a stage must fit twice");
-  static constexpr int kStageStride = (kStageBytes + 1023) / 1024 * 1024;
-  static constexpr int kSmem = kStages * kStageStride + 1024 + 256;
-  // TMEM: the accumulator, then the scales of two stages.
+  static constexpr int kSmem = kBuffers * kSpreadStride + kStages * kStageStride + 1024 + 256;
+  // TMEM: the accumulator, then the scales of two chunks.
   static constexpr uint32_t kSfCols = 4 * (1 + TERMS * kSfTiles);
   static constexpr uint32_t kCols = NT + 2 * kSfCols;
   static constexpr uint32_t kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
 struct LinearParams {
-  const uint8_t* packed;
   const uint8_t* scales;
+  const void* x;
+  int64_t ldx;
+  int x_vec;  // 16-byte loads of x are aligned
   const uint8_t* terms;  // [token tiles][chunks][kXBytes]
   const void* bias;
   const void* residual;
@@ -95,43 +101,28 @@ __device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t v) {
   return make_float2(__low2float(hh), __high2float(hh));
 }
 
-struct TermsParams {
-  const void* x;
-  int64_t ldx, rows, inner;
-  int chunks;
-  uint8_t* terms;
-};
+// Eight inputs of a row as fp32; zeros outside x.
+template <bool BF16>
+__device__ __forceinline__ void load_x8(const uint16_t* src, bool in, bool vec, float (&v)[8]) {
+  uint16_t raw[8];
+  if (vec) {
+    *reinterpret_cast<uint4*>(raw) = in ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = in ? src[i] : static_cast<uint16_t>(0);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    v[i] = BF16 ? bits_f32(static_cast<uint32_t>(raw[i]) << 16) : __half2float(*reinterpret_cast<__half*>(&raw[i]));
+}
 
-// Sixteen threads take the 128 inputs of one (row, chunk), eight each; four
-// neighbours share a block.  VEC: rows start on 16-byte boundaries.
-template <bool BF16, int NT, bool VEC>
-__global__ void __launch_bounds__(256) linear_terms_kernel(const TermsParams P) {
+// The terms of eight inputs: part `part` (of 16) of row `r` of a tile whose
+// image starts at `terms` and whose scales start at `sf`.  Four neighbouring
+// lanes share a block; all lanes of the warp take part in the shuffles.
+template <bool BF16, int NT>
+__device__ __forceinline__ void split_x8(float (&v)[8], int r, int part, uint8_t* terms, uint8_t* sf, bool store) {
   constexpr int TERMS = BF16 ? 2 : 3;
   using Tile = LinearTile<NT, TERMS>;
-  grid_dependents_launch();
-  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
-  const int part = threadIdx.x & 15;
-  const int64_t padded = (P.rows + NT - 1) / NT * NT;
-  const bool in_grid = unit < padded * P.chunks;  // uniform over the sixteen threads
-  const int64_t row = in_grid ? unit / P.chunks : 0;
-  const int chunk = in_grid ? static_cast<int>(unit % P.chunks) : 0;
-  const int64_t k0 = static_cast<int64_t>(chunk) * kLinK + part * 8;
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-  if (in_grid && row < P.rows && k0 < P.inner) {  // inner % 32 == 0: eight inputs are in or out together
-    const uint16_t* src = static_cast<const uint16_t*>(P.x) + row * P.ldx + k0;
-    uint16_t raw[8];
-    if constexpr (VEC) {
-      *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(src);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) raw[i] = src[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = BF16 ? bits_f32(static_cast<uint32_t>(raw[i]) << 16) : __half2float(*reinterpret_cast<__half*>(&raw[i]));
-  }
   uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
@@ -144,18 +135,16 @@ __global__ void __launch_bounds__(256) linear_terms_kernel(const TermsParams P) 
   const float mult = ebits == 255 ? 0.0f : exp2i(127 - byte);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = ebits == 255 ? 0.0f : __fmul_rn(v[i], mult);
-  if (!in_grid) return;
-  const int r = static_cast<int>(row % NT);
-  uint8_t* base = P.terms + ((row / NT) * P.chunks + chunk) * static_cast<int64_t>(Tile::kXBytes);
+  if (!store) return;
   // 16-byte slot part / 2 of the row's 128 bytes, swizzled over eight rows.
-  uint8_t* dst = base + r * 128 + (((part >> 1) ^ (r & 7)) << 4) + ((part & 1) << 3);
-  uint8_t* sf = base + TERMS * Tile::kTermBytes + (r >> 7) * kLinSfBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (part >> 2);
+  terms += r * 128 + (((part >> 1) ^ (r & 7)) << 4) + ((part & 1) << 3);
+  sf += (r >> 7) * kLinSfBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (part >> 2);
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<uint2*>(dst + t * Tile::kTermBytes) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    *reinterpret_cast<uint2*>(terms + t * Tile::kTermBytes) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
     if ((part & 3) == 0) sf[t * Tile::kTermSfBytes] = static_cast<uint8_t>(byte);
     if (t + 1 < TERMS) {
       const int step = byte == 255 ? 0 : min(byte, 5);  // scales do not go below 2^-127
@@ -169,6 +158,34 @@ __global__ void __launch_bounds__(256) linear_terms_kernel(const TermsParams P) 
       byte -= step;
     }
   }
+}
+
+struct TermsParams {
+  const void* x;
+  int64_t ldx, rows, inner;
+  int chunks;
+  int x_vec;
+  uint8_t* terms;  // [token tiles][chunks][kXBytes]
+};
+
+// Sixteen threads take the 128 inputs of one (row, chunk), eight each.
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(256) linear_terms_kernel(const TermsParams P) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Tile = LinearTile<NT, TERMS>;
+  grid_dependents_launch();
+  const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
+  const int part = threadIdx.x & 15;
+  const int64_t padded = (P.rows + NT - 1) / NT * NT;
+  const bool in_grid = unit < padded * P.chunks;
+  const int64_t row = in_grid ? unit / P.chunks : 0;
+  const int chunk = in_grid ? static_cast<int>(unit % P.chunks) : 0;
+  const int64_t k0 = static_cast<int64_t>(chunk) * kLinK + part * 8;
+  // inner % 32 == 0: eight inputs are in or out together
+  float v[8];
+  load_x8<BF16>(static_cast<const uint16_t*>(P.x) + row * P.ldx + k0, in_grid && row < P.rows && k0 < P.inner, P.x_vec, v);
+  uint8_t* base = P.terms + ((row / NT) * P.chunks + chunk) * static_cast<int64_t>(Tile::kXBytes);
+  split_x8<BF16, NT>(v, static_cast<int>(row % NT), part, base, base + TERMS * Tile::kTermBytes, in_grid);
 }
 
 // ---------------------------------------------------------------- epilogue
@@ -202,123 +219,187 @@ __device__ __forceinline__ void store16(void* p, int64_t i, float v) {
 // ----------------------------------------------------------------- product
 
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(kLinThreads) linear_kernel(const LinearParams P) {
+__global__ void __launch_bounds__(kLinThreads)
+    linear_kernel(const __grid_constant__ CUtensorMap map, const LinearParams P) {
   constexpr int TERMS = BF16 ? 2 : 3;
   using Tile = LinearTile<NT, TERMS>;
-  constexpr int ST = Tile::kStages;
+  constexpr int ST = Tile::kStages, WB = Tile::kBuffers;
+  constexpr bool FUSED = Tile::kFused;
+  constexpr int kXPart = FUSED ? 0 : Tile::kXBytes;  // x's part of a stage of copies
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * Tile::kStageStride);
-  uint64_t* empty = full + ST;
-  uint64_t* done = empty + ST;
+  uint8_t* ring = smem + WB * Tile::kSpreadStride;
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(ring + ST * Tile::kStageStride);
+  uint64_t* raw_empty = raw_full + ST;
+  uint64_t* w_full = raw_empty + ST;
+  uint64_t* w_empty = w_full + WB;
+  uint64_t* done = w_empty + WB;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   int* fail = reinterpret_cast<int*>(tmem_slot + 1);
 
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kLinM;
   const int64_t tile = blockIdx.z;
   const int c_begin = static_cast<int>(static_cast<int64_t>(P.chunks) * rank / ranks);
   const int n_chunks = static_cast<int>(static_cast<int64_t>(P.chunks) * (rank + 1) / ranks) - c_begin;
 
-  if (tid == 0) {
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map);
     for (int s = 0; s < ST; ++s) {
-      mbar_init(&full[s], kLinLoaders + 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], FUSED ? 4 : 1);  // freed by the spreading warps, or by the products that read x there
+    }
+    for (int b = 0; b < WB; ++b) {
+      mbar_init(&w_full[b], 4);
+      mbar_init(&w_empty[b], 1);
     }
     mbar_init(done, 1);
     *fail = 0;
     fence_mbar_init();
   }
-  if (warp == 4) tmem_alloc(tmem_slot, Tile::kTmemCols);
+  if (warp == 5) tmem_alloc(tmem_slot, Tile::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp < 4) {
+  if (warp == 0) {
     // --------------------------------------------------------------- copies
-    bool ok = true;
-    bool waited = false;  // for the terms of x, which the launch before this one writes
-    const uint8_t* xsrc = P.terms + (tile * P.chunks + c_begin) * static_cast<int64_t>(Tile::kXBytes);
-    int issued = 0;
-    for (int i = 0; i < n_chunks + ST - 2; ++i) {
-      if (i < n_chunks && ok) {
+    if (lane == 0) {
+      bool ok = true;
+      const uint8_t* xsrc = P.terms + (tile * P.chunks + c_begin) * static_cast<int64_t>(Tile::kXBytes);
+      // W does not depend on the launch that makes the terms: its first stages go ahead.
+      const int ahead = n_chunks < ST ? n_chunks : ST;
+      auto copy_w = [&](int i) {
         const int s = i % ST;
-        if (i >= ST && !mbar_wait(&empty[s], static_cast<uint32_t>((i / ST - 1) & 1))) ok = false;
-        if (ok) {
-          uint8_t* st = smem + s * Tile::kStageStride;  // [W codes][x terms][x scales][W scales]
-          const uint32_t sw = smem_u32(st);
-          const int64_t kbyte = static_cast<int64_t>(c_begin + i) * (kLinK / 2);
-          // 8 pieces of 16 codes per row, 4 rows per warp and step.
+        mbar_arrive_expect_tx(&raw_full[s], kXPart + kLinRawBytes);
+        tma_load_2d(ring + s * Tile::kStageStride + kXPart, &map, &raw_full[s], (c_begin + i) * (kLinK / 2),
+                    static_cast<int32_t>(n0));
+      };
+      auto copy_x = [&](int i) {
+        const int s = i % ST;
+        bulk_load(ring + s * Tile::kStageStride, xsrc + static_cast<int64_t>(i) * Tile::kXBytes, Tile::kXBytes, &raw_full[s]);
+      };
+      for (int i = 0; i < ahead; ++i) copy_w(i);
+      if constexpr (!FUSED) {
+        grid_dependency_wait();
+        for (int i = 0; i < ahead; ++i) copy_x(i);
+      }
+      int i = ahead;
+      for (; i < n_chunks; ++i) {
+        if (!mbar_wait(&raw_empty[i % ST], static_cast<uint32_t>((i / ST - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        copy_w(i);
+        if constexpr (!FUSED) copy_x(i);
+      }
+      // Copies in flight have to land before the CTA may end.
+      for (int j = i > ST ? i - ST : 0; j < i; ++j)
+        if (!mbar_wait(&raw_full[j % ST], static_cast<uint32_t>((j / ST) & 1))) ok = false;
+      if (!ok) atomicOr(fail, 1);
+    }
+  } else if (warp < 5) {
+    // ------------------------------------------------------------ spreading
+    const int e = threadIdx.x - 32;  // and the row of W whose scales this thread brings
+    const int64_t nb = P.inner / 32;
+    const bool row_in = n0 + e < P.outs;
+    const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0) + static_cast<int64_t>(c_begin) * 4;
+    // Scales of four chunks at a time (one 32-byte sector feeds eight), loaded a group ahead.
+    uint32_t sf[4], sf_next[4];
+    auto load_scales = [&](int i, uint32_t (&w)[4]) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int r = 16 * j + (tid >> 3), p = tid & 7;
-            const bool in = n0 + r < P.outs && kbyte + 8 * p < P.inner / 2;
-            const uint8_t* src = P.packed + (in ? (n0 + r) * (P.inner / 2) + kbyte + 8 * p : 0);
-            cp_async<8>(sw + r * 128 + ((p ^ (r & 7)) << 4), src, in ? 8u : 0u);
-          }
-          {
-            const int r = tid;
-            const int64_t b0 = static_cast<int64_t>(c_begin + i) * (kLinK / 32);
-            const int64_t nb = P.inner / 32;
-            uint8_t* dst = st + kLinWBytes + Tile::kXBytes + (r & 31) * 16 + (r >> 5) * 4;
-            const bool in = n0 + r < P.outs;
-            const uint8_t* src = P.scales + (in ? (n0 + r) * nb + b0 : 0);
-            if (P.words) {
-              cp_async<4>(smem_u32(dst), src, in ? 4u : 0u);
-            } else {
-              uint32_t w = 0;
+      for (int q = 0; q < 4; ++q) {
+        w[q] = 0;
+        if (row_in && i + q < n_chunks) {
+          if (P.words) {
+            w[q] = *reinterpret_cast<const uint32_t*>(srow + 4 * (i + q));
+          } else {
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (in && b0 + q < nb) w |= static_cast<uint32_t>(src[q]) << (8 * q);
-              *reinterpret_cast<uint32_t*>(dst) = w;
-            }
+            for (int k = 0; k < 4; ++k)
+              if (static_cast<int64_t>(c_begin + i + q) * 4 + k < nb)
+                w[q] |= static_cast<uint32_t>(srow[4 * (i + q) + k]) << (8 * k);
           }
-          if (tid == 0) {
-            if (!waited) grid_dependency_wait();
-            waited = true;
-            mbar_arrive_expect_tx(&full[s], Tile::kXBytes);
-            bulk_load(st + kLinWBytes, xsrc, Tile::kXBytes, &full[s]);
-            xsrc += Tile::kXBytes;
-          }
-          ++issued;
         }
       }
-      cp_async_commit();
-      cp_async_wait<ST - 2>();
-      const int ready = i - (ST - 2);
-      if (ready >= 0 && ready < issued) {
-        fence_proxy_async_smem();
-        mbar_arrive(&full[ready % ST]);
+    };
+    // Rows e / 16 (and 8 further) of x, eight inputs each, loaded a chunk ahead.
+    const int part = e & 15;
+    const int64_t row_a = tile * NT + (e >> 4), row_b = row_a + 8;
+    const uint16_t* xa = static_cast<const uint16_t*>(P.x) + (row_a < P.rows ? row_a : 0) * P.ldx;
+    const uint16_t* xb = static_cast<const uint16_t*>(P.x) + (row_b < P.rows ? row_b : 0) * P.ldx;
+    const bool two = FUSED && tile * NT + 8 < P.rows;
+    float va[8], vb[8];
+    auto load_rows = [&](int i) {
+      const int64_t k = static_cast<int64_t>(c_begin + i) * kLinK + part * 8;
+      const bool in = i < n_chunks && k < P.inner;
+      load_x8<BF16>(xa + (in ? k : 0), in && row_a < P.rows, P.x_vec, va);
+      if (two) load_x8<BF16>(xb + (in ? k : 0), in && row_b < P.rows, P.x_vec, vb);
+    };
+    load_scales(0, sf_next);
+    if constexpr (FUSED) load_rows(0);
+    bool ok = true;
+    for (int i = 0; i < n_chunks; ++i) {
+      const int s = i % ST, b = i % WB;
+      if ((i & 3) == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sf[q] = sf_next[q];
+        load_scales(i + 4, sf_next);
       }
+      uint8_t* w = smem + b * Tile::kSpreadStride;
+      if (i >= WB && !__all_sync(0xffffffffu, mbar_wait(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
+      if (ok) {
+        const uint32_t word = (i & 2) ? ((i & 1) ? sf[3] : sf[2]) : ((i & 1) ? sf[1] : sf[0]);
+        *reinterpret_cast<uint32_t*>(w + Tile::kSpread - kLinSfBytes + (e & 31) * 16 + (e >> 5) * 4) = word;
+        if constexpr (FUSED) {
+          uint8_t* xt = w + kLinWBytes;
+          split_x8<BF16, NT>(va, e >> 4, part, xt, xt + TERMS * Tile::kTermBytes, true);
+          if (two) split_x8<BF16, NT>(vb, 8 + (e >> 4), part, xt, xt + TERMS * Tile::kTermBytes, true);
+          load_rows(i + 1);
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
+      }
+      if (!ok) break;
+      const uint8_t* raw = ring + s * Tile::kStageStride + kXPart;
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = reinterpret_cast<const uint4*>(raw)[e + j * kLinSpread];
+      if constexpr (FUSED) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[s]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // 32 codes of row r: slots 2p and 2p + 1 of its 128 bytes, swizzled over eight rows.
+        const int u = e + j * kLinSpread, r = u >> 2, p = u & 3;
+        uint8_t* row = w + r * 128;
+        *reinterpret_cast<uint2*>(row + (((2 * p) ^ (r & 7)) << 4)) = make_uint2(v[j].x, v[j].y);
+        *reinterpret_cast<uint2*>(row + (((2 * p + 1) ^ (r & 7)) << 4)) = make_uint2(v[j].z, v[j].w);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_full[b]);
     }
-    if (!ok) {
-      // Stages never filled: the issuer's own wait gives up.  Copies in flight
-      // have to land before the CTA may end.
-      cp_async_wait<0>();
-      if (tid == 0)
-        for (int j = issued > ST ? issued - ST : 0; j < issued; ++j)
-          mbar_wait(&full[j % ST], static_cast<uint32_t>((j / ST) & 1));
-      atomicOr(fail, 1);
-    }
+    if (!ok) atomicOr(fail, 1);
   } else if (lane == 0) {
     // ------------------------------------------------------------- products
     constexpr uint32_t idesc = make_idesc_e2m1_e4m3(kLinM, NT);
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
-      const int s = i % ST;
-      if (!mbar_wait(&full[s], static_cast<uint32_t>((i / ST) & 1))) {
+      const int s = i % ST, b = i % WB;
+      if (!mbar_wait(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) ||
+          (!FUSED && !mbar_wait(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t sw = smem_u32(smem + s * Tile::kStageStride);
-      const uint32_t sx = sw + kLinWBytes;
+      const uint32_t sw = smem_u32(smem + b * Tile::kSpreadStride);
+      const uint32_t sx = FUSED ? sw + kLinWBytes : smem_u32(ring + s * Tile::kStageStride);
       const uint32_t sfa = tmem + NT + (i & 1) * Tile::kSfCols;
       const uint32_t sfb = sfa + 4;
-      tmem_cp_scales(sfa, sx + Tile::kXBytes);
+      tmem_cp_scales(sfa, sw + Tile::kSpread - kLinSfBytes);
 #pragma unroll
       for (int t = 0; t < TERMS * Tile::kSfTiles; ++t)
         tmem_cp_scales(sfb + 4 * t, sx + TERMS * Tile::kTermBytes + t * kLinSfBytes);
@@ -332,7 +413,8 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const LinearParams 
           mma_mxf8f6f4(tmem, ad, bd, mx_idesc_scale_byte(idesc, kk), sfa, sfb + 4 * t * Tile::kSfTiles,
                        (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
         }
-      mma_commit(&empty[s]);
+      mma_commit(&w_empty[b]);
+      if constexpr (!FUSED) mma_commit(&raw_empty[s]);
     }
     mma_commit(done);
     if (!ok) atomicOr(fail, 1);
@@ -340,19 +422,21 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const LinearParams 
 
   // ---------------------------------------------------------------- epilogue
   __syncwarp();
-  if (warp < 4 && !__all_sync(0xffffffffu, mbar_wait(done, 0))) atomicOr(fail, 1);
+  const bool epilogue = warp >= 1 && warp < 5;
+  const int quarter = warp & 3, tid = 32 * quarter + lane;  // a warp reads its own quarter of the TMEM lanes
+  if (epilogue && !__all_sync(0xffffffffu, mbar_wait(done, 0))) atomicOr(fail, 1);
   tc_fence_after();
-  const int64_t n = n0 + tid;  // this thread's output (warps 0..3)
+  const int64_t n = n0 + tid;  // this thread's output
   const int64_t t0 = tile * NT;
   float bias = 0.0f;
-  if (warp < 4 && P.bias && n < P.outs) bias = load16<BF16>(P.bias, n);
+  if (epilogue && P.bias && n < P.outs) bias = load16<BF16>(P.bias, n);
   if (ranks == 1) {
-    if (warp < 4) {
+    if (epilogue) {
 #pragma unroll 1
       for (int c = 0; c < NT; c += 16) {
         if (t0 + c >= P.rows) break;
         float v[16];
-        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + c, v);
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
         if (n < P.outs) {
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
@@ -368,17 +452,17 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const LinearParams 
     }
   } else {
     float* part = reinterpret_cast<float*>(smem);  // [NT][128], in the drained stages
-    if (warp < 4) {
+    if (epilogue) {
 #pragma unroll 1
       for (int c = 0; c < NT; c += 16) {
         float v[16];
-        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + c, v);
+        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
 #pragma unroll
         for (int u = 0; u < 16; ++u) part[(c + u) * 128 + tid] = v[u];
       }
     }
     cluster_sync_all();
-    if (warp < 4 && n < P.outs) {
+    if (epilogue && n < P.outs) {
       for (int c = rank; c < NT && t0 + c < P.rows; c += ranks) {
         float v = 0.0f;
         for (int k = 0; k < ranks; ++k) v = __fadd_rn(v, cluster.map_shared_rank(part, k)[c * 128 + tid]);
@@ -392,11 +476,11 @@ __global__ void __launch_bounds__(kLinThreads) linear_kernel(const LinearParams 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, Tile::kTmemCols);
   }
-  if (tid == 0 && *fail && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
+  if (threadIdx.x == 0 && *fail && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
 }
 
 // -------------------------------------------------------------------- host
@@ -411,19 +495,20 @@ static int linear_tile(int64_t rows, int dtype) {
 }
 
 template <bool BF16, int NT>
-static int launch_linear(const TermsParams& T, LinearParams P, cudaStream_t s) {
+static int launch_linear(const TermsParams& T, const uint8_t* packed, const LinearParams& P, cudaStream_t s) {
   constexpr int TERMS = BF16 ? 2 : 3;
   using Tile = LinearTile<NT, TERMS>;
   const int64_t tiles = (P.rows + NT - 1) / NT;
-  const int64_t units = tiles * NT * P.chunks;
-  const bool vec = T.ldx % 8 == 0 && reinterpret_cast<uintptr_t>(T.x) % 16 == 0;
-  const unsigned grid = static_cast<unsigned>((units * 16 + 255) / 256);
-  if (vec)
-    linear_terms_kernel<BF16, NT, true><<<grid, 256, 0, s>>>(T);
-  else
-    linear_terms_kernel<BF16, NT, false><<<grid, 256, 0, s>>>(T);
-  int status = check_launch();
+  CUtensorMap map;
+  int status = make_tensor_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, packed, P.inner / 2, P.outs, P.inner / 2, kLinK / 2, kLinM,
+                                  CU_TENSOR_MAP_SWIZZLE_NONE);
   if (status != MXW_OK) return status;
+  if constexpr (!Tile::kFused) {
+    const int64_t units = tiles * NT * P.chunks;
+    linear_terms_kernel<BF16, NT><<<static_cast<unsigned>((units * 16 + 255) / 256), 256, 0, s>>>(T);
+    status = check_launch();
+    if (status != MXW_OK) return status;
+  }
 
   auto kernel = linear_kernel<BF16, NT>;
   status = set_max_smem(reinterpret_cast<const void*>(kernel), Tile::kSmem);
@@ -442,24 +527,24 @@ static int launch_linear(const TermsParams& T, LinearParams P, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, P);
+  cfg.numAttrs = Tile::kFused ? 1 : 2;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, map, P);
   return err == cudaSuccess ? MXW_OK : record_cuda_error(err);
 }
 
 template <bool BF16>
-static int launch_linear_rows(const TermsParams& T, const LinearParams& P, cudaStream_t s) {
+static int launch_linear_rows(const TermsParams& T, const uint8_t* packed, const LinearParams& P, cudaStream_t s) {
   switch (linear_tile(P.rows, BF16 ? MXW_BF16 : MXW_F16)) {
     case 16:
-      return launch_linear<BF16, 16>(T, P, s);
+      return launch_linear<BF16, 16>(T, packed, P, s);
     case 32:
-      return launch_linear<BF16, 32>(T, P, s);
+      return launch_linear<BF16, 32>(T, packed, P, s);
     case 64:
-      return launch_linear<BF16, 64>(T, P, s);
+      return launch_linear<BF16, 64>(T, packed, P, s);
     case 128:
-      return launch_linear<BF16, 128>(T, P, s);
+      return launch_linear<BF16, 128>(T, packed, P, s);
     default:
-      if constexpr (BF16) return launch_linear<BF16, 256>(T, P, s);
+      if constexpr (BF16) return launch_linear<BF16, 256>(T, packed, P, s);
       return MXW_EUNSUPPORTED;
   }
 }
@@ -471,6 +556,7 @@ using namespace mxw;
 extern "C" size_t mxw_linear_workspace_size(int64_t rows, int64_t inner, int dtype) {
   if (rows <= 0 || inner <= 0 || (dtype != MXW_BF16 && dtype != MXW_F16)) return 0;
   const int64_t nt = linear_tile(rows, dtype);
+  if (nt == 16) return 16;  // the terms stay in shared memory
   const int64_t per_chunk = (dtype == MXW_BF16 ? 2 : 3) * (nt * kLinK + (nt + 127) / 128 * kLinSfBytes);
   return static_cast<size_t>((rows + nt - 1) / nt * ((inner + kLinK - 1) / kLinK) * per_chunk);
 }
@@ -485,7 +571,7 @@ extern "C" int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t 
   if (residual && ldr < outs) return MXW_EINVAL;
   if (rows == 0 || outs == 0) return MXW_OK;
   if (!x || !packed || !scales || !y || !workspace) return MXW_EINVAL;
-  if (reinterpret_cast<uintptr_t>(packed) % 8 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return MXW_EINVAL;
+  if (reinterpret_cast<uintptr_t>(packed) % 16 != 0 || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return MXW_EINVAL;
   if (workspace_bytes < mxw_linear_workspace_size(rows, inner, dtype)) return MXW_EINVAL;
   // Grid limits: 65535 tiles of 128 outputs and of 128 rows; 2^31 blocks of terms.
   if (outs > 65535ll * kLinM || rows > 65535ll * 128 || inner > (1ll << 30)) return MXW_EUNSUPPORTED;
@@ -496,10 +582,13 @@ extern "C" int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t 
   T.rows = rows;
   T.inner = inner;
   T.chunks = static_cast<int>((inner + kLinK - 1) / kLinK);
+  T.x_vec = ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
   T.terms = static_cast<uint8_t*>(workspace);
   LinearParams P{};
-  P.packed = packed;
   P.scales = scales;
+  P.x = x;
+  P.ldx = ldx;
+  P.x_vec = T.x_vec;
   P.terms = T.terms;
   P.bias = bias;
   P.residual = residual;
@@ -513,5 +602,5 @@ extern "C" int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t 
   P.words = inner % 128 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
   P.flags = flags;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == MXW_BF16 ? launch_linear_rows<true>(T, P, s) : launch_linear_rows<false>(T, P, s);
+  return dtype == MXW_BF16 ? launch_linear_rows<true>(T, packed, P, s) : launch_linear_rows<false>(T, packed, P, s);
 }

@@ -68,7 +68,7 @@ def linear_mxfp4(
 
     rows = _rows(x, inner)
     packed = packed.contiguous()
-    if packed.data_ptr() % 8 != 0:
+    if packed.data_ptr() % 16 != 0:
         packed = packed.clone()
     args = (rows, packed, scales.contiguous(), None if bias is None else bias.contiguous(),
             None if residual is None else _rows(residual, outs), ACTIVATIONS[activation])
