@@ -21,6 +21,19 @@ __host__ __device__ constexpr uint32_t make_idesc_e2m1_e4m3(int m, int n) {
          | (static_cast<uint32_t>(m >> 4) << 24);    // M / 16
 }
 
+// The same with A = E4M3 and B = E2M1.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3_e2m1(int m, int n) {
+  return (0u << 7) | (5u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// A K-major 128-byte-swizzled operand: the descriptor's upper half, and the
+// lower for a 1024-byte aligned address (advance by 2 per 32 bytes of K).
+constexpr uint32_t kDescKSw128Hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_sw128_lo(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint64_t desc_of(uint32_t hi, uint32_t lo) {
+  return (static_cast<uint64_t>(hi) << 32) | lo;
+}
+
 __device__ __forceinline__ uint32_t mx_idesc_scale_byte(uint32_t idesc, uint32_t byte) {
   return idesc | (byte << 4) | (byte << 29);
 }
@@ -40,6 +53,18 @@ __device__ __forceinline__ void mma_mxf8f6f4(uint32_t d_tmem, uint64_t a_desc, u
 __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
   const uint64_t desc = make_smem_desc_k_noswz(saddr, 0, 128);
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// mbar_wait with its limit counted in SM cycles (2 s at 2 GHz).  Reading the
+// global timer takes about a microsecond, which a pipeline that waits for every
+// stage pays at each of them; the cycle counter is read in a few tens of cycles.
+__device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  while (!mbar_try_wait(bar, parity)) {
+    if (clock64() - start > 4000000000ll) return false;
+  }
+  return true;
 }
 
 // Untiled asynchronous copies into shared memory.

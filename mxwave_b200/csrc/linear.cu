@@ -84,6 +84,7 @@ struct LinearParams {
   int chunks;
   int act;
   int words;  // the scales of a row start on a 4-byte boundary
+  int pairs;  // rows of y and of the residual start on 4-byte boundaries
   uint32_t* flags;
 };
 
@@ -216,6 +217,21 @@ __device__ __forceinline__ void store16(void* p, int64_t i, float v) {
     static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// Two neighbours at an even index of 4-byte aligned memory.
+template <bool BF16>
+__device__ __forceinline__ float2 load16x2(const void* p, int64_t i) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+  if constexpr (BF16) return make_float2(bits_f32(w << 16), bits_f32(w & 0xffff0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF16>
+__device__ __forceinline__ void store16x2(void* p, int64_t i, float a, float b) {
+  if constexpr (BF16)
+    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p) + i) = __floats2bfloat162_rn(a, b);
+  else
+    *reinterpret_cast<__half2*>(static_cast<__half*>(p) + i) = __floats2half2_rn(a, b);
+}
+
 // ----------------------------------------------------------------- product
 
 template <bool BF16, int NT>
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(kLinThreads)
       }
       int i = ahead;
       for (; i < n_chunks; ++i) {
-        if (!mbar_wait(&raw_empty[i % ST], static_cast<uint32_t>((i / ST - 1) & 1))) {
+        if (!mbar_wait_cycles(&raw_empty[i % ST], static_cast<uint32_t>((i / ST - 1) & 1))) {
           ok = false;
           break;
         }
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(kLinThreads)
       }
       // Copies in flight have to land before the CTA may end.
       for (int j = i > ST ? i - ST : 0; j < i; ++j)
-        if (!mbar_wait(&raw_full[j % ST], static_cast<uint32_t>((j / ST) & 1))) ok = false;
+        if (!mbar_wait_cycles(&raw_full[j % ST], static_cast<uint32_t>((j / ST) & 1))) ok = false;
       if (!ok) atomicOr(fail, 1);
     }
   } else if (warp < 5) {
@@ -349,7 +365,7 @@ __global__ void __launch_bounds__(kLinThreads)
         load_scales(i + 4, sf_next);
       }
       uint8_t* w = smem + b * Tile::kSpreadStride;
-      if (i >= WB && !__all_sync(0xffffffffu, mbar_wait(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
+      if (i >= WB && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
       if (ok) {
         const uint32_t word = (i & 2) ? ((i & 1) ? sf[3] : sf[2]) : ((i & 1) ? sf[1] : sf[0]);
         *reinterpret_cast<uint32_t*>(w + Tile::kSpread - kLinSfBytes + (e & 31) * 16 + (e >> 5) * 4) = word;
@@ -359,7 +375,7 @@ __global__ void __launch_bounds__(kLinThreads)
           if (two) split_x8<BF16, NT>(vb, 8 + (e >> 4), part, xt, xt + TERMS * Tile::kTermBytes, true);
           load_rows(i + 1);
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
+        if (!__all_sync(0xffffffffu, mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
       }
       if (!ok) break;
       const uint8_t* raw = ring + s * Tile::kStageStride + kXPart;
@@ -389,8 +405,8 @@ __global__ void __launch_bounds__(kLinThreads)
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int s = i % ST, b = i % WB;
-      if (!mbar_wait(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) ||
-          (!FUSED && !mbar_wait(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) {
+      if (!mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) ||
+          (!FUSED && !mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) {
         ok = false;
         break;
       }
@@ -403,16 +419,13 @@ __global__ void __launch_bounds__(kLinThreads)
 #pragma unroll
       for (int t = 0; t < TERMS * Tile::kSfTiles; ++t)
         tmem_cp_scales(sfb + 4 * t, sx + TERMS * Tile::kTermBytes + t * kLinSfBytes);
+      const uint32_t a_lo = desc_k_sw128_lo(sw), b_lo = desc_k_sw128_lo(sx);
 #pragma unroll
       for (int t = 0; t < TERMS; ++t)
 #pragma unroll
-        for (int kk = 0; kk < kLinK / 32; ++kk) {
-          // 32 inputs are 32 bytes of a swizzled 128-byte row.
-          const uint64_t ad = make_smem_desc_mn_sw128(sw + kk * 32, 16, 1024);
-          const uint64_t bd = make_smem_desc_mn_sw128(sx + t * Tile::kTermBytes + kk * 32, 16, 1024);
-          mma_mxf8f6f4(tmem, ad, bd, mx_idesc_scale_byte(idesc, kk), sfa, sfb + 4 * t * Tile::kSfTiles,
-                       (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < kLinK / 32; ++kk)  // 32 inputs are 32 bytes of a swizzled 128-byte row
+          mma_mxf8f6f4(tmem, desc_of(kDescKSw128Hi, a_lo + 2 * kk), desc_of(kDescKSw128Hi, b_lo + t * (Tile::kTermBytes >> 4) + 2 * kk),
+                       mx_idesc_scale_byte(idesc, kk), sfa, sfb + 4 * t * Tile::kSfTiles, (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
       mma_commit(&w_empty[b]);
       if constexpr (!FUSED) mma_commit(&raw_empty[s]);
     }
@@ -424,7 +437,7 @@ __global__ void __launch_bounds__(kLinThreads)
   __syncwarp();
   const bool epilogue = warp >= 1 && warp < 5;
   const int quarter = warp & 3, tid = 32 * quarter + lane;  // a warp reads its own quarter of the TMEM lanes
-  if (epilogue && !__all_sync(0xffffffffu, mbar_wait(done, 0))) atomicOr(fail, 1);
+  if (epilogue && !__all_sync(0xffffffffu, mbar_wait_cycles(done, 0))) atomicOr(fail, 1);
   tc_fence_after();
   const int64_t n = n0 + tid;  // this thread's output
   const int64_t t0 = tile * NT;
@@ -483,15 +496,302 @@ __global__ void __launch_bounds__(kLinThreads)
   if (threadIdx.x == 0 && *fail && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
 }
 
+// ---------------------------------------------------- product of many rows
+//
+// Tiles of 128 rows of x (M) x 256 outputs (N) for prompts: the terms of x are
+// the A operand, W's codes the B operand.  A chunk of 128 inputs brings 33 KB
+// of terms and 17 KB of W for 1024 cycles of products (the orientation above
+// would bring 75 KB), so three stages of copies cover their latency.  What
+// bounds it is shared memory: the products read 96 bytes a cycle of it, copies
+// and spreading write 64 more.
+
+constexpr int kWideN = 256;
+constexpr int kWideSpread = 256;  // spreading threads: eight warps, the epilogue's too
+constexpr int kWideThreads = 32 + kWideSpread + 32;
+
+template <int TERMS>
+struct WideTile {
+  using X = LinearTile<128, TERMS>;  // the terms' images are those of 128-row tiles
+  static constexpr int kRawBytes = kWideN * kLinK / 2;
+  static constexpr int kStageStride = (X::kXBytes + kRawBytes + 1023) / 1024 * 1024;  // [x terms][x scales][packed W]
+  static constexpr int kSpreadStride = kWideN * kLinK + 2 * kLinSfBytes;              // [W][W scales]
+  static constexpr int kBuffers = 2;
+  static constexpr int kStages = (222 * 1024 - kBuffers * kSpreadStride) / kStageStride;
+  static_assert(kStages >= 2, "a stage must fit twice");
+  static constexpr int kSmem = kBuffers * kSpreadStride + kStages * kStageStride + 1024 + 256;
+  static constexpr uint32_t kSfCols = 4 * TERMS + 8;
+  static constexpr uint32_t kTmemCols = 512;  // 256 + 2 kSfCols, rounded up
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    linear_wide_kernel(const __grid_constant__ CUtensorMap map, const LinearParams P) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Tile = WideTile<TERMS>;
+  using X = typename Tile::X;
+  constexpr int ST = Tile::kStages, WB = Tile::kBuffers;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint8_t* ring = smem + WB * Tile::kSpreadStride;
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(ring + ST * Tile::kStageStride);
+  uint64_t* raw_empty = raw_full + ST;
+  uint64_t* w_full = raw_empty + ST;
+  uint64_t* w_empty = w_full + WB;
+  uint64_t* done = w_empty + WB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  int* fail = reinterpret_cast<int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kWideN;
+  const int64_t tile = blockIdx.y;
+  const int n_chunks = P.chunks;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&raw_full[s], 1);
+      mbar_init(&raw_empty[s], 1);
+    }
+    for (int b = 0; b < WB; ++b) {
+      mbar_init(&w_full[b], kWideSpread / 32);
+      mbar_init(&w_empty[b], 1);
+    }
+    mbar_init(done, 1);
+    *fail = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, Tile::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // --------------------------------------------------------------- copies
+    if (lane == 0) {
+      bool ok = true;
+      const uint8_t* xsrc = P.terms + tile * P.chunks * static_cast<int64_t>(X::kXBytes);
+      grid_dependency_wait();
+      int i = 0;
+      for (; i < n_chunks; ++i) {
+        const int s = i % ST;
+        if (i >= ST && !mbar_wait_cycles(&raw_empty[s], static_cast<uint32_t>((i / ST - 1) & 1))) {
+          ok = false;
+          break;
+        }
+        uint8_t* st = ring + s * Tile::kStageStride;
+        mbar_arrive_expect_tx(&raw_full[s], X::kXBytes + Tile::kRawBytes);
+        tma_load_2d(st + X::kXBytes, &map, &raw_full[s], i * (kLinK / 2), static_cast<int32_t>(n0));
+        bulk_load(st, xsrc + static_cast<int64_t>(i) * X::kXBytes, X::kXBytes, &raw_full[s]);
+      }
+      // Copies in flight have to land before the CTA may end.
+      for (int j = i > ST ? i - ST : 0; j < i; ++j)
+        if (!mbar_wait_cycles(&raw_full[j % ST], static_cast<uint32_t>((j / ST) & 1))) ok = false;
+      if (!ok) atomicOr(fail, 1);
+    }
+  } else if (warp < 9) {
+    // ------------------------------------------------------------ spreading
+    const int e = threadIdx.x - 32;  // and the row of W whose scales this thread brings
+    const int64_t nb = P.inner / 32;
+    const bool row_in = n0 + e < P.outs;
+    const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0);
+    uint32_t sf[4], sf_next[4];
+    auto load_scales = [&](int i, uint32_t (&w)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        w[q] = 0;
+        if (row_in && i + q < n_chunks) {
+          if (P.words) {
+            w[q] = *reinterpret_cast<const uint32_t*>(srow + 4 * (i + q));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (static_cast<int64_t>(i + q) * 4 + k < nb) w[q] |= static_cast<uint32_t>(srow[4 * (i + q) + k]) << (8 * k);
+          }
+        }
+      }
+    };
+    load_scales(0, sf_next);
+    bool ok = true;
+    for (int i = 0; i < n_chunks; ++i) {
+      const int s = i % ST, b = i % WB;
+      if ((i & 3) == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sf[q] = sf_next[q];
+        load_scales(i + 4, sf_next);
+      }
+      uint8_t* w = smem + b * Tile::kSpreadStride;
+      if (i >= WB && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
+      if (ok) {
+        const uint32_t word = (i & 2) ? ((i & 1) ? sf[3] : sf[2]) : ((i & 1) ? sf[1] : sf[0]);
+        *reinterpret_cast<uint32_t*>(w + kWideN * kLinK + (e >> 7) * kLinSfBytes + (e & 31) * 16 + ((e >> 5) & 3) * 4) = word;
+        if (!__all_sync(0xffffffffu, mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
+      }
+      if (!ok) break;
+      const uint8_t* raw = ring + s * Tile::kStageStride + X::kXBytes;
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = reinterpret_cast<const uint4*>(raw)[e + j * kWideSpread];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int u = e + j * kWideSpread, r = u >> 2, p = u & 3;
+        uint8_t* row = w + r * 128;
+        *reinterpret_cast<uint2*>(row + (((2 * p) ^ (r & 7)) << 4)) = make_uint2(v[j].x, v[j].y);
+        *reinterpret_cast<uint2*>(row + (((2 * p + 1) ^ (r & 7)) << 4)) = make_uint2(v[j].z, v[j].w);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_full[b]);
+    }
+    if (!ok) atomicOr(fail, 1);
+  } else if (lane == 0) {
+    // ------------------------------------------------------------- products
+    constexpr uint32_t idesc = make_idesc_e4m3_e2m1(128, kWideN);
+    bool ok = true;
+    for (int i = 0; i < n_chunks; ++i) {
+      const int s = i % ST, b = i % WB;
+      if (!mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) ||
+          !mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t sw = smem_u32(smem + b * Tile::kSpreadStride);
+      const uint32_t sx = smem_u32(ring + s * Tile::kStageStride);
+      const uint32_t sfa = tmem + kWideN + (i & 1) * Tile::kSfCols;
+      const uint32_t sfb = sfa + 4 * TERMS;
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t) tmem_cp_scales(sfa + 4 * t, sx + TERMS * X::kTermBytes + t * kLinSfBytes);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) tmem_cp_scales(sfb + 4 * h, sw + kWideN * kLinK + h * kLinSfBytes);
+      const uint32_t a_lo = desc_k_sw128_lo(sx), b_lo = desc_k_sw128_lo(sw);
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int kk = 0; kk < kLinK / 32; ++kk)
+          mma_mxf8f6f4(tmem, desc_of(kDescKSw128Hi, a_lo + t * (X::kTermBytes >> 4) + 2 * kk), desc_of(kDescKSw128Hi, b_lo + 2 * kk),
+                       mx_idesc_scale_byte(idesc, kk), sfa + 4 * t, sfb, (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
+      mma_commit(&w_empty[b]);
+      mma_commit(&raw_empty[s]);
+    }
+    mma_commit(done);
+    if (!ok) atomicOr(fail, 1);
+  }
+
+  // ---------------------------------------------------------------- epilogue
+  // A warp reads its quarter of the rows and half of the columns, 64 at a
+  // time, and turns them over in shared memory so that a row's 64 outputs are
+  // read (residual) and written together.
+  __syncwarp();
+  if (warp >= 1 && warp < 9) {
+    if (!__all_sync(0xffffffffu, mbar_wait_cycles(done, 0))) atomicOr(fail, 1);
+    tc_fence_after();
+    const int quarter = warp & 3, half = (warp - 1) >> 2;
+    float* turn = reinterpret_cast<float*>(smem) + (warp - 1) * (32 * 66);  // [32 rows][64 + 2]
+    const int64_t t0 = tile * 128 + 32 * quarter;
+    const int rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), P.rows - t0)));
+    const bool pairs = P.pairs;  // two outputs per load and store
+#pragma unroll 1
+    for (int c = 128 * half; c < 128 * half + 128; c += 64) {
+      if (n0 + c >= P.outs || rows == 0) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c + 32 * h, v);
+#pragma unroll
+        for (int u = 0; u < 16; ++u) *reinterpret_cast<float2*>(turn + lane * 66 + 32 * h + 2 * u) = make_float2(v[2 * u], v[2 * u + 1]);
+      }
+      __syncwarp();
+      const int64_t n = n0 + c + 2 * lane;
+      const bool in0 = n < P.outs, in1 = n + 1 < P.outs;
+      const float bias0 = P.bias && in0 ? load16<BF16>(P.bias, n) : 0.0f;
+      const float bias1 = P.bias && in1 ? load16<BF16>(P.bias, n + 1) : 0.0f;
+#pragma unroll 1
+      for (int r0 = 0; r0 < rows; r0 += 8) {
+        float2 res[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          res[r] = make_float2(0.0f, 0.0f);
+          if (P.residual && r0 + r < rows) {
+            const int64_t at = (t0 + r0 + r) * P.ldr + n;
+            if (pairs && in1)
+              res[r] = load16x2<BF16>(P.residual, at);
+            else if (in0)
+              res[r] = make_float2(load16<BF16>(P.residual, at), in1 ? load16<BF16>(P.residual, at + 1) : 0.0f);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          if (r0 + r >= rows) break;
+          const float2 v = *reinterpret_cast<const float2*>(turn + (r0 + r) * 66 + 2 * lane);
+          float o0 = activate(__fadd_rn(v.x, bias0), P.act), o1 = activate(__fadd_rn(v.y, bias1), P.act);
+          if (P.residual) {
+            o0 = __fadd_rn(o0, res[r].x);
+            o1 = __fadd_rn(o1, res[r].y);
+          }
+          const int64_t at = (t0 + r0 + r) * P.outs + n;
+          if (pairs && in1) {
+            store16x2<BF16>(P.y, at, o0, o1);
+          } else {
+            if (in0) store16<BF16>(P.y, at, o0);
+            if (in1) store16<BF16>(P.y, at + 1, o1);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Tile::kTmemCols);
+  }
+  if (threadIdx.x == 0 && *fail && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
+}
+
 // -------------------------------------------------------------------- host
 
-// Rows of x per tile: the smallest tile that takes them all, so that W is read
-// once, up to what two stages of shared memory hold.
-static int linear_tile(int64_t rows, int dtype) {
-  if (rows <= 16) return 16;
-  if (rows <= 32) return 32;
-  if (rows <= 64) return 64;
-  return rows <= 128 || dtype == MXW_F16 ? 128 : 256;
+// Rows of x per tile: the smallest tile that takes them all, so that W is read once.
+static int linear_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+// Whether the wide tiles fill most of the SMs; below that the narrow kernel,
+// whose clusters split K, ends sooner.
+static bool linear_wide(int64_t rows, int64_t outs) {
+  return rows > 128 && (rows + 127) / 128 * ((outs + kWideN - 1) / kWideN) >= num_sms() / 2;
+}
+
+template <bool BF16, int NT>
+static int launch_terms(const TermsParams& T, cudaStream_t s) {
+  const int64_t units = (T.rows + NT - 1) / NT * NT * T.chunks;
+  linear_terms_kernel<BF16, NT><<<static_cast<unsigned>((units * 16 + 255) / 256), 256, 0, s>>>(T);
+  return check_launch();
+}
+
+template <bool BF16>
+static int launch_wide(const TermsParams& T, const uint8_t* packed, const LinearParams& P, cudaStream_t s) {
+  using Tile = WideTile<BF16 ? 2 : 3>;
+  CUtensorMap map;
+  int status = make_tensor_map_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, packed, P.inner / 2, P.outs, P.inner / 2, kLinK / 2, kWideN,
+                                  CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (status != MXW_OK) return status;
+  status = launch_terms<BF16, 128>(T, s);
+  if (status != MXW_OK) return status;
+  auto kernel = linear_wide_kernel<BF16>;
+  status = set_max_smem(reinterpret_cast<const void*>(kernel), Tile::kSmem);
+  if (status != MXW_OK) return status;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((P.outs + kWideN - 1) / kWideN), static_cast<unsigned>((P.rows + 127) / 128));
+  cfg.blockDim = dim3(kWideThreads);
+  cfg.dynamicSmemBytes = Tile::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, map, P);
+  return err == cudaSuccess ? MXW_OK : record_cuda_error(err);
 }
 
 template <bool BF16, int NT>
@@ -504,9 +804,7 @@ static int launch_linear(const TermsParams& T, const uint8_t* packed, const Line
                                   CU_TENSOR_MAP_SWIZZLE_NONE);
   if (status != MXW_OK) return status;
   if constexpr (!Tile::kFused) {
-    const int64_t units = tiles * NT * P.chunks;
-    linear_terms_kernel<BF16, NT><<<static_cast<unsigned>((units * 16 + 255) / 256), 256, 0, s>>>(T);
-    status = check_launch();
+    status = launch_terms<BF16, NT>(T, s);
     if (status != MXW_OK) return status;
   }
 
@@ -534,18 +832,16 @@ static int launch_linear(const TermsParams& T, const uint8_t* packed, const Line
 
 template <bool BF16>
 static int launch_linear_rows(const TermsParams& T, const uint8_t* packed, const LinearParams& P, cudaStream_t s) {
-  switch (linear_tile(P.rows, BF16 ? MXW_BF16 : MXW_F16)) {
+  if (linear_wide(P.rows, P.outs)) return launch_wide<BF16>(T, packed, P, s);
+  switch (linear_tile(P.rows)) {
     case 16:
       return launch_linear<BF16, 16>(T, packed, P, s);
     case 32:
       return launch_linear<BF16, 32>(T, packed, P, s);
     case 64:
       return launch_linear<BF16, 64>(T, packed, P, s);
-    case 128:
-      return launch_linear<BF16, 128>(T, packed, P, s);
     default:
-      if constexpr (BF16) return launch_linear<BF16, 256>(T, packed, P, s);
-      return MXW_EUNSUPPORTED;
+      return launch_linear<BF16, 128>(T, packed, P, s);
   }
 }
 
@@ -555,7 +851,7 @@ using namespace mxw;
 
 extern "C" size_t mxw_linear_workspace_size(int64_t rows, int64_t inner, int dtype) {
   if (rows <= 0 || inner <= 0 || (dtype != MXW_BF16 && dtype != MXW_F16)) return 0;
-  const int64_t nt = linear_tile(rows, dtype);
+  const int64_t nt = linear_tile(rows);
   if (nt == 16) return 16;  // the terms stay in shared memory
   const int64_t per_chunk = (dtype == MXW_BF16 ? 2 : 3) * (nt * kLinK + (nt + 127) / 128 * kLinSfBytes);
   return static_cast<size_t>((rows + nt - 1) / nt * ((inner + kLinK - 1) / kLinK) * per_chunk);
@@ -600,6 +896,8 @@ extern "C" int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t 
   P.chunks = T.chunks;
   P.act = act;
   P.words = inner % 128 == 0 && reinterpret_cast<uintptr_t>(scales) % 4 == 0;
+  P.pairs = outs % 2 == 0 && reinterpret_cast<uintptr_t>(y) % 4 == 0 &&
+            (!residual || (ldr % 2 == 0 && reinterpret_cast<uintptr_t>(residual) % 4 == 0));
   P.flags = flags;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == MXW_BF16 ? launch_linear_rows<true>(T, packed, P, s) : launch_linear_rows<false>(T, packed, P, s);
