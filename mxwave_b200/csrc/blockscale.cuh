@@ -55,6 +55,16 @@ __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint32_t saddr) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
+// One lane of a converged warp.  The issuing warp runs its loop whole and lets
+// this lane issue: its addresses and descriptors then stay in uniform
+// registers, where a single-lane branch moves each operand there anew (some 65
+// cycles per instruction).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on != 0;
+}
+
 // mbar_wait with its limit counted in SM cycles (2 s at 2 GHz).  Reading the
 // global timer takes about a microsecond, which a pipeline that waits for every
 // stage pays at each of them; the cycle counter is read in a few tens of cycles.

@@ -40,7 +40,7 @@ namespace mxw {
 constexpr int kLinM = 128;        // outputs per tile
 constexpr int kLinK = 128;        // inputs per stage
 constexpr int kLinSpread = 128;   // threads that spread W's codes, and the epilogue's
-constexpr int kLinThreads = 32 + kLinSpread + 32;  // copies, spreading, products
+constexpr int kLinThreads = 32 + kLinSpread + 32;  // copies, spreading, products (and four warps that make terms)
 constexpr int kLinRawBytes = kLinM * kLinK / 2;    // packed codes of a stage
 constexpr int kLinWBytes = kLinM * kLinK;          // spread: 16 bytes per 16 codes
 constexpr int kLinSfBytes = 512;                   // scales of 128 rows x 4 blocks
@@ -48,25 +48,37 @@ constexpr int kLinSfBytes = 512;                   // scales of 128 rows x 4 blo
 template <int NT, int TERMS>
 struct LinearTile {
   static constexpr bool kFused = NT == 16;  // terms made in the product's kernel
+  // Small tiles take the terms as rows of one operand (and add up their columns
+  // at the end): a quarter of the instructions, which one thread issues at some
+  // 65 cycles each.
+  static constexpr bool kMerged = NT < 128;
   static constexpr int kTermBytes = NT * kLinK;
-  static constexpr int kSfTiles = (NT + 127) / 128;  // 128-row groups of the x scales
-  static constexpr int kTermSfBytes = kSfTiles * kLinSfBytes;
-  static constexpr int kXBytes = TERMS * (kTermBytes + kTermSfBytes);  // one chunk of x: terms, then their scales
-  // A stage of copies: [x terms][x scales][packed W], and a spread buffer:
-  // [W][x terms][x scales][W scales], the x parts where they are made.
+  static constexpr int kN = kMerged ? TERMS * NT : NT;               // columns of the accumulator
+  static constexpr int kOperands = kMerged ? 1 : TERMS;
+  static constexpr int kSfTiles = (kMerged ? (TERMS * NT + 127) / 128 : TERMS * ((NT + 127) / 128));
+  static constexpr int kXBytes = TERMS * kTermBytes + kSfTiles * kLinSfBytes;  // one chunk of x: terms, then their scales
+  // Where the scale of term t of row r lies: 128 operand rows to 512 bytes, [row % 32][row / 32][block].
+  __host__ __device__ static constexpr int sf_place(int t, int r) {
+    const int n = kMerged ? t * NT + r : r;
+    return (kMerged ? 0 : t * kLinSfBytes) + (n >> 7) * kLinSfBytes + (n & 31) * 16 + ((n >> 5) & 3) * 4;
+  }
+  // A stage of copies: [x terms][x scales][packed W]; a spread buffer: [W][W
+  // scales]; and where the terms are made, a ring of those.
   static constexpr int kStage = (kFused ? 0 : kXBytes) + kLinRawBytes;
   static constexpr int kStageStride = (kStage + 1023) / 1024 * 1024;
-  static constexpr int kSpread = kLinWBytes + (kFused ? kXBytes : 0) + kLinSfBytes;
-  static constexpr int kSpreadStride = (kSpread + 1023) / 1024 * 1024;
+  static constexpr int kSpreadStride = (kLinWBytes + kLinSfBytes + 1023) / 1024 * 1024;
+  static constexpr int kXStages = kFused ? 4 : 0;
+  static constexpr int kXStride = (kXBytes + 1023) / 1024 * 1024;
+  static constexpr int kThreads = kLinThreads + 32 * kXStages;
   static constexpr int kBuffers = 2;
   static constexpr int kBudget = NT <= 32 ? 111 * 1024 : 222 * 1024;  // two CTAs per SM for small tiles
-  static constexpr int kFit = (kBudget - kBuffers * kSpreadStride) / kStageStride;
+  static constexpr int kFit = (kBudget - kBuffers * kSpreadStride - kXStages * kXStride) / kStageStride;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
   static_assert(kStages >= 2, "a stage must fit twice");
-  static constexpr int kSmem = kBuffers * kSpreadStride + kStages * kStageStride + 1024 + 256;
+  static constexpr int kSmem = kBuffers * kSpreadStride + kXStages * kXStride + kStages * kStageStride + 1024 + 256;
   // TMEM: the accumulator, then the scales of two chunks.
-  static constexpr uint32_t kSfCols = 4 * (1 + TERMS * kSfTiles);
-  static constexpr uint32_t kCols = NT + 2 * kSfCols;
+  static constexpr uint32_t kSfCols = 4 * (1 + kSfTiles);
+  static constexpr uint32_t kCols = kN + 2 * kSfCols;
   static constexpr uint32_t kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
@@ -102,28 +114,36 @@ __device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t v) {
   return make_float2(__low2float(hh), __high2float(hh));
 }
 
-// Eight inputs of a row as fp32; zeros outside x.
-template <bool BF16>
-__device__ __forceinline__ void load_x8(const uint16_t* src, bool in, bool vec, float (&v)[8]) {
-  uint16_t raw[8];
-  if (vec) {
-    *reinterpret_cast<uint4*>(raw) = in ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-  } else {
+// Eight inputs of a row; zeros outside x.
+__device__ __forceinline__ uint4 load_x8(const uint16_t* src, bool in, bool vec) {
+  if (!in) return make_uint4(0, 0, 0, 0);
+  if (vec) return *reinterpret_cast<const uint4*>(src);
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = in ? src[i] : static_cast<uint16_t>(0);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    v[i] = BF16 ? bits_f32(static_cast<uint32_t>(raw[i]) << 16) : __half2float(*reinterpret_cast<__half*>(&raw[i]));
+  for (int i = 0; i < 4; ++i) w[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // The terms of eight inputs: part `part` (of 16) of row `r` of a tile whose
 // image starts at `terms` and whose scales start at `sf`.  Four neighbouring
 // lanes share a block; all lanes of the warp take part in the shuffles.
 template <bool BF16, int NT>
-__device__ __forceinline__ void split_x8(float (&v)[8], int r, int part, uint8_t* terms, uint8_t* sf, bool store) {
+__device__ __forceinline__ void split_x8(const uint4& raw, int r, int part, uint8_t* terms, uint8_t* sf, bool store) {
   constexpr int TERMS = BF16 ? 2 : 3;
   using Tile = LinearTile<NT, TERMS>;
+  float v[8];
+  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      v[2 * i] = bits_f32(words[i] << 16);
+      v[2 * i + 1] = bits_f32(words[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
   uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
 #pragma unroll
   for (int i = 0; i < 8; ++i) amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
@@ -139,14 +159,13 @@ __device__ __forceinline__ void split_x8(float (&v)[8], int r, int part, uint8_t
   if (!store) return;
   // 16-byte slot part / 2 of the row's 128 bytes, swizzled over eight rows.
   terms += r * 128 + (((part >> 1) ^ (r & 7)) << 4) + ((part & 1) << 3);
-  sf += (r >> 7) * kLinSfBytes + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (part >> 2);
 #pragma unroll
   for (int t = 0; t < TERMS; ++t) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[2 * i], v[2 * i + 1]);
     *reinterpret_cast<uint2*>(terms + t * Tile::kTermBytes) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-    if ((part & 3) == 0) sf[t * Tile::kTermSfBytes] = static_cast<uint8_t>(byte);
+    if ((part & 3) == 0) sf[Tile::sf_place(t, r) + (part >> 2)] = static_cast<uint8_t>(byte);
     if (t + 1 < TERMS) {
       const int step = byte == 255 ? 0 : min(byte, 5);  // scales do not go below 2^-127
       const float up = static_cast<float>(1 << step);
@@ -183,8 +202,7 @@ __global__ void __launch_bounds__(256) linear_terms_kernel(const TermsParams P) 
   const int chunk = in_grid ? static_cast<int>(unit % P.chunks) : 0;
   const int64_t k0 = static_cast<int64_t>(chunk) * kLinK + part * 8;
   // inner % 32 == 0: eight inputs are in or out together
-  float v[8];
-  load_x8<BF16>(static_cast<const uint16_t*>(P.x) + row * P.ldx + k0, in_grid && row < P.rows && k0 < P.inner, P.x_vec, v);
+  const uint4 v = load_x8(static_cast<const uint16_t*>(P.x) + row * P.ldx + k0, in_grid && row < P.rows && k0 < P.inner, P.x_vec);
   uint8_t* base = P.terms + ((row / NT) * P.chunks + chunk) * static_cast<int64_t>(Tile::kXBytes);
   split_x8<BF16, NT>(v, static_cast<int>(row % NT), part, base, base + TERMS * Tile::kTermBytes, in_grid);
 }
@@ -217,6 +235,21 @@ __device__ __forceinline__ void store16(void* p, int64_t i, float v) {
     static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// Sixteen columns of the accumulator, the terms' columns added up.
+template <int NT, int TERMS>
+__device__ __forceinline__ void load_sums(uint32_t taddr, float (&v)[16]) {
+  tmem_ld_32x32b_x16(taddr, v);
+  if constexpr (LinearTile<NT, TERMS>::kMerged) {
+#pragma unroll
+    for (int t = 1; t < TERMS; ++t) {
+      float w[16];
+      tmem_ld_32x32b_x16(taddr + t * NT, w);
+#pragma unroll
+      for (int u = 0; u < 16; ++u) v[u] = __fadd_rn(v[u], w[u]);
+    }
+  }
+}
+
 // Two neighbours at an even index of 4-byte aligned memory.
 template <bool BF16>
 __device__ __forceinline__ float2 load16x2(const void* p, int64_t i) {
@@ -235,7 +268,7 @@ __device__ __forceinline__ void store16x2(void* p, int64_t i, float a, float b) 
 // ----------------------------------------------------------------- product
 
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(kLinThreads)
+__global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     linear_kernel(const __grid_constant__ CUtensorMap map, const LinearParams P) {
   constexpr int TERMS = BF16 ? 2 : 3;
   using Tile = LinearTile<NT, TERMS>;
@@ -244,12 +277,16 @@ __global__ void __launch_bounds__(kLinThreads)
   constexpr int kXPart = FUSED ? 0 : Tile::kXBytes;  // x's part of a stage of copies
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
-  uint8_t* ring = smem + WB * Tile::kSpreadStride;
+  constexpr int XS = FUSED ? Tile::kXStages : 1;
+  uint8_t* xring = smem + WB * Tile::kSpreadStride;
+  uint8_t* ring = xring + Tile::kXStages * Tile::kXStride;
   uint64_t* raw_full = reinterpret_cast<uint64_t*>(ring + ST * Tile::kStageStride);
   uint64_t* raw_empty = raw_full + ST;
   uint64_t* w_full = raw_empty + ST;
   uint64_t* w_empty = w_full + WB;
-  uint64_t* done = w_empty + WB;
+  uint64_t* x_full = w_empty + WB;
+  uint64_t* x_empty = x_full + XS;
+  uint64_t* done = x_empty + XS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   int* fail = reinterpret_cast<int*>(tmem_slot + 1);
 
@@ -270,6 +307,10 @@ __global__ void __launch_bounds__(kLinThreads)
     for (int b = 0; b < WB; ++b) {
       mbar_init(&w_full[b], 4);
       mbar_init(&w_empty[b], 1);
+    }
+    for (int x = 0; x < XS; ++x) {
+      mbar_init(&x_full[x], 1);
+      mbar_init(&x_empty[x], 1);
     }
     mbar_init(done, 1);
     *fail = 0;
@@ -341,21 +382,7 @@ __global__ void __launch_bounds__(kLinThreads)
         }
       }
     };
-    // Rows e / 16 (and 8 further) of x, eight inputs each, loaded a chunk ahead.
-    const int part = e & 15;
-    const int64_t row_a = tile * NT + (e >> 4), row_b = row_a + 8;
-    const uint16_t* xa = static_cast<const uint16_t*>(P.x) + (row_a < P.rows ? row_a : 0) * P.ldx;
-    const uint16_t* xb = static_cast<const uint16_t*>(P.x) + (row_b < P.rows ? row_b : 0) * P.ldx;
-    const bool two = FUSED && tile * NT + 8 < P.rows;
-    float va[8], vb[8];
-    auto load_rows = [&](int i) {
-      const int64_t k = static_cast<int64_t>(c_begin + i) * kLinK + part * 8;
-      const bool in = i < n_chunks && k < P.inner;
-      load_x8<BF16>(xa + (in ? k : 0), in && row_a < P.rows, P.x_vec, va);
-      if (two) load_x8<BF16>(xb + (in ? k : 0), in && row_b < P.rows, P.x_vec, vb);
-    };
     load_scales(0, sf_next);
-    if constexpr (FUSED) load_rows(0);
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int s = i % ST, b = i % WB;
@@ -368,13 +395,7 @@ __global__ void __launch_bounds__(kLinThreads)
       if (i >= WB && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
       if (ok) {
         const uint32_t word = (i & 2) ? ((i & 1) ? sf[3] : sf[2]) : ((i & 1) ? sf[1] : sf[0]);
-        *reinterpret_cast<uint32_t*>(w + Tile::kSpread - kLinSfBytes + (e & 31) * 16 + (e >> 5) * 4) = word;
-        if constexpr (FUSED) {
-          uint8_t* xt = w + kLinWBytes;
-          split_x8<BF16, NT>(va, e >> 4, part, xt, xt + TERMS * Tile::kTermBytes, true);
-          if (two) split_x8<BF16, NT>(vb, 8 + (e >> 4), part, xt, xt + TERMS * Tile::kTermBytes, true);
-          load_rows(i + 1);
-        }
+        *reinterpret_cast<uint32_t*>(w + kLinWBytes + (e & 31) * 16 + (e >> 5) * 4) = word;
         if (!__all_sync(0xffffffffu, mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
       }
       if (!ok) break;
@@ -399,37 +420,72 @@ __global__ void __launch_bounds__(kLinThreads)
       if (lane == 0) mbar_arrive(&w_full[b]);
     }
     if (!ok) atomicOr(fail, 1);
-  } else if (lane == 0) {
+  } else if (warp == 5) {
     // ------------------------------------------------------------- products
-    constexpr uint32_t idesc = make_idesc_e2m1_e4m3(kLinM, NT);
+    constexpr uint32_t idesc = make_idesc_e2m1_e4m3(kLinM, Tile::kN);
+    const bool leader = elect_one();
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
-      const int s = i % ST, b = i % WB;
-      if (!mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) ||
-          (!FUSED && !mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) {
+      const int s = i % ST, b = i % WB, xs = i % XS;
+      ok = mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) &&
+           (FUSED ? mbar_wait_cycles(&x_full[xs], static_cast<uint32_t>((i / XS) & 1))
+                  : mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)));
+      if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t sw = smem_u32(smem + b * Tile::kSpreadStride);
-      const uint32_t sx = FUSED ? sw + kLinWBytes : smem_u32(ring + s * Tile::kStageStride);
-      const uint32_t sfa = tmem + NT + (i & 1) * Tile::kSfCols;
+      const uint32_t sw = smem_u32(smem) + b * Tile::kSpreadStride;
+      const uint32_t sx = FUSED ? smem_u32(xring) + xs * Tile::kXStride : smem_u32(ring) + s * Tile::kStageStride;
+      const uint32_t sfa = tmem + Tile::kN + (i & 1) * Tile::kSfCols;
       const uint32_t sfb = sfa + 4;
-      tmem_cp_scales(sfa, sw + Tile::kSpread - kLinSfBytes);
-#pragma unroll
-      for (int t = 0; t < TERMS * Tile::kSfTiles; ++t)
-        tmem_cp_scales(sfb + 4 * t, sx + TERMS * Tile::kTermBytes + t * kLinSfBytes);
       const uint32_t a_lo = desc_k_sw128_lo(sw), b_lo = desc_k_sw128_lo(sx);
+      if (leader) {
+        tmem_cp_scales(sfa, sw + kLinWBytes);
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
+        for (int t = 0; t < Tile::kSfTiles; ++t) tmem_cp_scales(sfb + 4 * t, sx + TERMS * Tile::kTermBytes + t * kLinSfBytes);
 #pragma unroll
-        for (int kk = 0; kk < kLinK / 32; ++kk)  // 32 inputs are 32 bytes of a swizzled 128-byte row
-          mma_mxf8f6f4(tmem, desc_of(kDescKSw128Hi, a_lo + 2 * kk), desc_of(kDescKSw128Hi, b_lo + t * (Tile::kTermBytes >> 4) + 2 * kk),
-                       mx_idesc_scale_byte(idesc, kk), sfa, sfb + 4 * t * Tile::kSfTiles, (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
-      mma_commit(&w_empty[b]);
-      if constexpr (!FUSED) mma_commit(&raw_empty[s]);
+        for (int t = 0; t < Tile::kOperands; ++t)
+#pragma unroll
+          for (int kk = 0; kk < kLinK / 32; ++kk)  // 32 inputs are 32 bytes of a swizzled 128-byte row
+            mma_mxf8f6f4(tmem, desc_of(kDescKSw128Hi, a_lo + 2 * kk), desc_of(kDescKSw128Hi, b_lo + t * (Tile::kTermBytes >> 4) + 2 * kk),
+                         mx_idesc_scale_byte(idesc, kk), sfa, sfb + 4 * t, (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&w_empty[b]);
+        mma_commit(FUSED ? &x_empty[xs] : &raw_empty[s]);
+      }
+      __syncwarp();
     }
-    mma_commit(done);
+    if (leader) {
+      mma_commit(done);
+      if (!ok) atomicOr(fail, 1);
+    }
+  } else if constexpr (FUSED) {
+    // --------------------------------------------------------- terms of x
+    // A warp takes a chunk whole, every fourth chunk: two rows at a time, 16 lanes each.
+    const int part = lane & 15, sub = lane >> 4;
+    const int n_rows = static_cast<int>(min(static_cast<int64_t>(NT), P.rows - tile * NT));
+    const uint16_t* x = static_cast<const uint16_t*>(P.x) + tile * NT * P.ldx + part * 8;
+    const int in_left = static_cast<int>(min(P.inner - static_cast<int64_t>(c_begin) * kLinK, static_cast<int64_t>(n_chunks) * kLinK)) - part * 8;
+    bool ok = true;
+    for (int i = warp - 6; i < n_chunks; i += XS) {
+      const int xs = i % XS;
+      uint8_t* xt = xring + xs * Tile::kXStride;
+      const uint16_t* src = x + (static_cast<int64_t>(c_begin) + i) * kLinK;
+      const bool in = i * kLinK < in_left;  // inner % 32 == 0: eight inputs are in or out together
+      uint4 v = load_x8(src + sub * P.ldx, in && sub < n_rows, P.x_vec);
+      if (i >= XS && !__all_sync(0xffffffffu, mbar_wait_cycles(&x_empty[xs], static_cast<uint32_t>((i / XS - 1) & 1)))) {
+        ok = false;
+        break;
+      }
+      for (int r = 0; r < n_rows; r += 2) {
+        const uint4 now = v;
+        v = load_x8(src + (r + 2 + sub) * P.ldx, in && r + 2 + sub < n_rows, P.x_vec);
+        split_x8<BF16, NT>(now, r + sub, part, xt, xt + TERMS * Tile::kTermBytes, true);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&x_full[xs]);
+    }
     if (!ok) atomicOr(fail, 1);
   }
 
@@ -449,14 +505,18 @@ __global__ void __launch_bounds__(kLinThreads)
       for (int c = 0; c < NT; c += 16) {
         if (t0 + c >= P.rows) break;
         float v[16];
-        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
+        load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
         if (n < P.outs) {
+          float res[16];
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+            res[u] = P.residual && t0 + c + u < P.rows ? load16<BF16>(P.residual, (t0 + c + u) * P.ldr + n) : 0.0f;
 #pragma unroll
           for (int u = 0; u < 16; ++u) {
             const int64_t t = t0 + c + u;
             if (t < P.rows) {
               float o = activate(__fadd_rn(v[u], bias), P.act);
-              if (P.residual) o = __fadd_rn(o, load16<BF16>(P.residual, t * P.ldr + n));
+              if (P.residual) o = __fadd_rn(o, res[u]);
               store16<BF16>(P.y, t * P.outs + n, o);
             }
           }
@@ -467,22 +527,38 @@ __global__ void __launch_bounds__(kLinThreads)
     float* part = reinterpret_cast<float*>(smem);  // [NT][128], in the drained stages
     if (epilogue) {
 #pragma unroll 1
-      for (int c = 0; c < NT; c += 16) {
+      for (int c = 0; c < NT && t0 + c < P.rows; c += 16) {
         float v[16];
-        tmem_ld_32x32b_x16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
+        load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
 #pragma unroll
         for (int u = 0; u < 16; ++u) part[(c + u) * 128 + tid] = v[u];
       }
     }
     cluster_sync_all();
     if (epilogue && n < P.outs) {
-      for (int c = rank; c < NT && t0 + c < P.rows; c += ranks) {
-        float v = 0.0f;
-        for (int k = 0; k < ranks; ++k) v = __fadd_rn(v, cluster.map_shared_rank(part, k)[c * 128 + tid]);
-        float o = activate(__fadd_rn(v, bias), P.act);
-        const int64_t t = t0 + c;
-        if (P.residual) o = __fadd_rn(o, load16<BF16>(P.residual, t * P.ldr + n));
-        store16<BF16>(P.y, t * P.outs + n, o);
+      // Columns rank, rank + ranks, ...: two at a time, all ranks' parts in flight, added in rank order.
+      for (int c = rank; c < NT && t0 + c < P.rows; c += 2 * ranks) {
+        float v[2][8], res[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = c + h * ranks;
+          const bool in = col < NT && t0 + col < P.rows;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[h][k] = in && k < ranks ? cluster.map_shared_rank(part, k)[col * 128 + tid] : 0.0f;
+          res[h] = in && P.residual ? load16<BF16>(P.residual, (t0 + col) * P.ldr + n) : 0.0f;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t t = t0 + c + h * ranks;
+          if (c + h * ranks >= NT || t >= P.rows) break;
+          float sum = v[h][0];
+#pragma unroll
+          for (int k = 1; k < 8; ++k)
+            if (k < ranks) sum = __fadd_rn(sum, v[h][k]);
+          float o = activate(__fadd_rn(sum, bias), P.act);
+          if (P.residual) o = __fadd_rn(o, res[h]);
+          store16<BF16>(P.y, t * P.outs + n, o);
+        }
       }
     }
     cluster_sync_all();
@@ -644,38 +720,45 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       if (lane == 0) mbar_arrive(&w_full[b]);
     }
     if (!ok) atomicOr(fail, 1);
-  } else if (lane == 0) {
+  } else {
     // ------------------------------------------------------------- products
     constexpr uint32_t idesc = make_idesc_e4m3_e2m1(128, kWideN);
+    const bool leader = elect_one();
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int s = i % ST, b = i % WB;
-      if (!mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) ||
-          !mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1))) {
+      ok = mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) &&
+           mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1));
+      if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t sw = smem_u32(smem + b * Tile::kSpreadStride);
-      const uint32_t sx = smem_u32(ring + s * Tile::kStageStride);
+      const uint32_t sw = smem_u32(smem) + b * Tile::kSpreadStride;
+      const uint32_t sx = smem_u32(ring) + s * Tile::kStageStride;
       const uint32_t sfa = tmem + kWideN + (i & 1) * Tile::kSfCols;
       const uint32_t sfb = sfa + 4 * TERMS;
-#pragma unroll
-      for (int t = 0; t < TERMS; ++t) tmem_cp_scales(sfa + 4 * t, sx + TERMS * X::kTermBytes + t * kLinSfBytes);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) tmem_cp_scales(sfb + 4 * h, sw + kWideN * kLinK + h * kLinSfBytes);
       const uint32_t a_lo = desc_k_sw128_lo(sx), b_lo = desc_k_sw128_lo(sw);
+      if (leader) {
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
+        for (int t = 0; t < TERMS; ++t) tmem_cp_scales(sfa + 4 * t, sx + TERMS * X::kTermBytes + t * kLinSfBytes);
 #pragma unroll
-        for (int kk = 0; kk < kLinK / 32; ++kk)
-          mma_mxf8f6f4(tmem, desc_of(kDescKSw128Hi, a_lo + t * (X::kTermBytes >> 4) + 2 * kk), desc_of(kDescKSw128Hi, b_lo + 2 * kk),
-                       mx_idesc_scale_byte(idesc, kk), sfa + 4 * t, sfb, (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
-      mma_commit(&w_empty[b]);
-      mma_commit(&raw_empty[s]);
+        for (int h = 0; h < 2; ++h) tmem_cp_scales(sfb + 4 * h, sw + kWideN * kLinK + h * kLinSfBytes);
+#pragma unroll
+        for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+          for (int kk = 0; kk < kLinK / 32; ++kk)
+            mma_mxf8f6f4(tmem, desc_of(kDescKSw128Hi, a_lo + t * (X::kTermBytes >> 4) + 2 * kk), desc_of(kDescKSw128Hi, b_lo + 2 * kk),
+                         mx_idesc_scale_byte(idesc, kk), sfa + 4 * t, sfb, (i > 0 || t > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&w_empty[b]);
+        mma_commit(&raw_empty[s]);
+      }
+      __syncwarp();
     }
-    mma_commit(done);
-    if (!ok) atomicOr(fail, 1);
+    if (leader) {
+      mma_commit(done);
+      if (!ok) atomicOr(fail, 1);
+    }
   }
 
   // ---------------------------------------------------------------- epilogue
@@ -816,7 +899,7 @@ static int launch_linear(const TermsParams& T, const uint8_t* packed, const Line
   while (split < 8 && row_tiles * tiles * split * 2 <= 2 * num_sms() && split * 4 <= P.chunks) split *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(row_tiles), static_cast<unsigned>(tiles));
-  cfg.blockDim = dim3(kLinThreads);
+  cfg.blockDim = dim3(Tile::kThreads);
   cfg.dynamicSmemBytes = Tile::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -851,9 +934,10 @@ using namespace mxw;
 
 extern "C" size_t mxw_linear_workspace_size(int64_t rows, int64_t inner, int dtype) {
   if (rows <= 0 || inner <= 0 || (dtype != MXW_BF16 && dtype != MXW_F16)) return 0;
-  const int64_t nt = linear_tile(rows);
+  const int64_t nt = linear_tile(rows), terms = dtype == MXW_BF16 ? 2 : 3;
   if (nt == 16) return 16;  // the terms stay in shared memory
-  const int64_t per_chunk = (dtype == MXW_BF16 ? 2 : 3) * (nt * kLinK + (nt + 127) / 128 * kLinSfBytes);
+  const int64_t sf_tiles = nt < 128 ? (terms * nt + 127) / 128 : terms;
+  const int64_t per_chunk = terms * nt * kLinK + sf_tiles * kLinSfBytes;
   return static_cast<size_t>((rows + nt - 1) / nt * ((inner + kLinK - 1) / kLinK) * per_chunk);
 }
 
