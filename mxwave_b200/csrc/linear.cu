@@ -39,8 +39,10 @@ namespace mxw {
 
 constexpr int kLinM = 128;        // outputs per tile
 constexpr int kLinK = 128;        // inputs per stage
-constexpr int kLinSpread = 128;   // threads that spread W's codes, and the epilogue's
-constexpr int kLinThreads = 32 + kLinSpread + 32;  // copies, spreading, products (and four warps that make terms)
+constexpr int kLinSpread = 128;   // threads that spread a stage of W
+constexpr int kLinGroups = 2;     // groups of them, which take every other stage
+constexpr int kLinSpreadWarps = kLinGroups * kLinSpread / 32;  // the epilogue's warps too
+constexpr int kLinThreads = 64 + 32 * kLinSpreadWarps;  // copies, products, spreading (and four warps that make terms)
 constexpr int kLinRawBytes = kLinM * kLinK / 2;    // packed codes of a stage
 constexpr int kLinWBytes = kLinM * kLinK;          // spread: 16 bytes per 16 codes
 constexpr int kLinSfBytes = 512;                   // scales of 128 rows x 4 blocks
@@ -70,7 +72,7 @@ struct LinearTile {
   static constexpr int kXStages = kFused ? 4 : 0;
   static constexpr int kXStride = (kXBytes + 1023) / 1024 * 1024;
   static constexpr int kThreads = kLinThreads + 32 * kXStages;
-  static constexpr int kBuffers = 2;
+  static constexpr int kBuffers = kLinGroups;  // one spread buffer per group
   static constexpr int kBudget = NT <= 32 ? 111 * 1024 : 222 * 1024;  // two CTAs per SM for small tiles
   static constexpr int kFit = (kBudget - kBuffers * kSpreadStride - kXStages * kXStride) / kStageStride;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
@@ -298,6 +300,14 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
   const int c_begin = static_cast<int>(static_cast<int64_t>(P.chunks) * rank / ranks);
   const int n_chunks = static_cast<int>(static_cast<int64_t>(P.chunks) * (rank + 1) / ranks) - c_begin;
 
+  // The copying thread makes the barriers and sends off the first stages of W
+  // before the others are ready to take them.
+  auto copy_w = [&](int i) {
+    const int s = i % ST;
+    mbar_arrive_expect_tx(&raw_full[s], kXPart + kLinRawBytes);
+    tma_load_2d(ring + s * Tile::kStageStride + kXPart, &map, &raw_full[s], (c_begin + i) * (kLinK / 2), static_cast<int32_t>(n0));
+  };
+  const int ahead = n_chunks < ST ? n_chunks : ST;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map);
     for (int s = 0; s < ST; ++s) {
@@ -315,8 +325,9 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     mbar_init(done, 1);
     *fail = 0;
     fence_mbar_init();
+    for (int i = 0; i < ahead; ++i) copy_w(i);
   }
-  if (warp == 5) tmem_alloc(tmem_slot, Tile::kTmemCols);
+  if (warp == 1) tmem_alloc(tmem_slot, Tile::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -327,21 +338,12 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     if (lane == 0) {
       bool ok = true;
       const uint8_t* xsrc = P.terms + (tile * P.chunks + c_begin) * static_cast<int64_t>(Tile::kXBytes);
-      // W does not depend on the launch that makes the terms: its first stages go ahead.
-      const int ahead = n_chunks < ST ? n_chunks : ST;
-      auto copy_w = [&](int i) {
-        const int s = i % ST;
-        mbar_arrive_expect_tx(&raw_full[s], kXPart + kLinRawBytes);
-        tma_load_2d(ring + s * Tile::kStageStride + kXPart, &map, &raw_full[s], (c_begin + i) * (kLinK / 2),
-                    static_cast<int32_t>(n0));
-      };
       auto copy_x = [&](int i) {
         const int s = i % ST;
         bulk_load(ring + s * Tile::kStageStride, xsrc + static_cast<int64_t>(i) * Tile::kXBytes, Tile::kXBytes, &raw_full[s]);
       };
-      for (int i = 0; i < ahead; ++i) copy_w(i);
       if constexpr (!FUSED) {
-        grid_dependency_wait();
+        grid_dependency_wait();  // W does not depend on the launch that makes the terms: its first stages went ahead
         for (int i = 0; i < ahead; ++i) copy_x(i);
       }
       int i = ahead;
@@ -358,43 +360,44 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
         if (!mbar_wait_cycles(&raw_full[j % ST], static_cast<uint32_t>((j / ST) & 1))) ok = false;
       if (!ok) atomicOr(fail, 1);
     }
-  } else if (warp < 5) {
+  } else if (warp >= 2 && warp < 2 + kLinSpreadWarps) {
     // ------------------------------------------------------------ spreading
-    const int e = threadIdx.x - 32;  // and the row of W whose scales this thread brings
+    const int group = (warp - 2) / (kLinSpread / 32);
+    const int e = (threadIdx.x - 64) % kLinSpread;  // and the row of W whose scales this thread brings
     const int64_t nb = P.inner / 32;
     const bool row_in = n0 + e < P.outs;
     const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0) + static_cast<int64_t>(c_begin) * 4;
-    // Scales of four chunks at a time (one 32-byte sector feeds eight), loaded a group ahead.
+    // Scales of four of the group's chunks at a time, loaded that far ahead.
     uint32_t sf[4], sf_next[4];
     auto load_scales = [&](int i, uint32_t (&w)[4]) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
+        const int c = i + kLinGroups * q;
         w[q] = 0;
-        if (row_in && i + q < n_chunks) {
+        if (row_in && c < n_chunks) {
           if (P.words) {
-            w[q] = *reinterpret_cast<const uint32_t*>(srow + 4 * (i + q));
+            w[q] = *reinterpret_cast<const uint32_t*>(srow + 4 * c);
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (static_cast<int64_t>(c_begin + i + q) * 4 + k < nb)
-                w[q] |= static_cast<uint32_t>(srow[4 * (i + q) + k]) << (8 * k);
+              if (static_cast<int64_t>(c_begin + c) * 4 + k < nb) w[q] |= static_cast<uint32_t>(srow[4 * c + k]) << (8 * k);
           }
         }
       }
     };
-    load_scales(0, sf_next);
+    load_scales(group, sf_next);
     bool ok = true;
-    for (int i = 0; i < n_chunks; ++i) {
-      const int s = i % ST, b = i % WB;
-      if ((i & 3) == 0) {
+    uint8_t* w = smem + group * Tile::kSpreadStride;
+    for (int i = group, turn = 0; i < n_chunks; i += kLinGroups, ++turn) {
+      const int s = i % ST;
+      if ((turn & 3) == 0) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) sf[q] = sf_next[q];
-        load_scales(i + 4, sf_next);
+        load_scales(i + 4 * kLinGroups, sf_next);
       }
-      uint8_t* w = smem + b * Tile::kSpreadStride;
-      if (i >= WB && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
+      if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[group], static_cast<uint32_t>((turn - 1) & 1)))) ok = false;
       if (ok) {
-        const uint32_t word = (i & 2) ? ((i & 1) ? sf[3] : sf[2]) : ((i & 1) ? sf[1] : sf[0]);
+        const uint32_t word = (turn & 2) ? ((turn & 1) ? sf[3] : sf[2]) : ((turn & 1) ? sf[1] : sf[0]);
         *reinterpret_cast<uint32_t*>(w + kLinWBytes + (e & 31) * 16 + (e >> 5) * 4) = word;
         if (!__all_sync(0xffffffffu, mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
       }
@@ -417,10 +420,10 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&w_full[b]);
+      if (lane == 0) mbar_arrive(&w_full[group]);
     }
     if (!ok) atomicOr(fail, 1);
-  } else if (warp == 5) {
+  } else if (warp == 1) {
     // ------------------------------------------------------------- products
     constexpr uint32_t idesc = make_idesc_e2m1_e4m3(kLinM, Tile::kN);
     const bool leader = elect_one();
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     const uint16_t* x = static_cast<const uint16_t*>(P.x) + tile * NT * P.ldx + part * 8;
     const int in_left = static_cast<int>(min(P.inner - static_cast<int64_t>(c_begin) * kLinK, static_cast<int64_t>(n_chunks) * kLinK)) - part * 8;
     bool ok = true;
-    for (int i = warp - 6; i < n_chunks; i += XS) {
+    for (int i = warp - 2 - kLinSpreadWarps; i < n_chunks; i += XS) {
       const int xs = i % XS;
       uint8_t* xt = xring + xs * Tile::kXStride;
       const uint16_t* src = x + (static_cast<int64_t>(c_begin) + i) * kLinK;
@@ -491,7 +494,8 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
 
   // ---------------------------------------------------------------- epilogue
   __syncwarp();
-  const bool epilogue = warp >= 1 && warp < 5;
+  const bool epilogue = warp >= 2 && warp < 2 + kLinSpreadWarps;
+  const int half = (warp - 2) >> 2;  // and every other group of columns
   const int quarter = warp & 3, tid = 32 * quarter + lane;  // a warp reads its own quarter of the TMEM lanes
   if (epilogue && !__all_sync(0xffffffffu, mbar_wait_cycles(done, 0))) atomicOr(fail, 1);
   tc_fence_after();
@@ -502,7 +506,7 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
   if (ranks == 1) {
     if (epilogue) {
 #pragma unroll 1
-      for (int c = 0; c < NT; c += 16) {
+      for (int c = 16 * half; c < NT; c += 32) {
         if (t0 + c >= P.rows) break;
         float v[16];
         load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
@@ -527,7 +531,7 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     float* part = reinterpret_cast<float*>(smem);  // [NT][128], in the drained stages
     if (epilogue) {
 #pragma unroll 1
-      for (int c = 0; c < NT && t0 + c < P.rows; c += 16) {
+      for (int c = 16 * half; c < NT && t0 + c < P.rows; c += 32) {
         float v[16];
         load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
 #pragma unroll
@@ -536,12 +540,13 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     }
     cluster_sync_all();
     if (epilogue && n < P.outs) {
-      // Columns rank, rank + ranks, ...: two at a time, all ranks' parts in flight, added in rank order.
-      for (int c = rank; c < NT && t0 + c < P.rows; c += 2 * ranks) {
+      // Columns rank, rank + ranks, ..., every other one: two at a time, all
+      // ranks' parts in flight, added in rank order.
+      for (int c = rank + half * ranks; c < NT && t0 + c < P.rows; c += 4 * ranks) {
         float v[2][8], res[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int col = c + h * ranks;
+          const int col = c + 2 * h * ranks;
           const bool in = col < NT && t0 + col < P.rows;
 #pragma unroll
           for (int k = 0; k < 8; ++k) v[h][k] = in && k < ranks ? cluster.map_shared_rank(part, k)[col * 128 + tid] : 0.0f;
@@ -549,8 +554,8 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int64_t t = t0 + c + h * ranks;
-          if (c + h * ranks >= NT || t >= P.rows) break;
+          const int64_t t = t0 + c + 2 * h * ranks;
+          if (c + 2 * h * ranks >= NT || t >= P.rows) break;
           float sum = v[h][0];
 #pragma unroll
           for (int k = 1; k < 8; ++k)
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Tile::kTmemCols);
   }
@@ -582,8 +587,10 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
 // and spreading write 64 more.
 
 constexpr int kWideN = 256;
-constexpr int kWideSpread = 256;  // spreading threads: eight warps, the epilogue's too
-constexpr int kWideThreads = 32 + kWideSpread + 32;
+constexpr int kWideSpread = 256;  // threads that spread a stage of W
+constexpr int kWideGroups = 2;    // groups of them, which take every other stage
+constexpr int kWideSpreadWarps = kWideGroups * kWideSpread / 32;  // the epilogue's warps too
+constexpr int kWideThreads = 64 + 32 * kWideSpreadWarps;
 
 template <int TERMS>
 struct WideTile {
@@ -591,7 +598,7 @@ struct WideTile {
   static constexpr int kRawBytes = kWideN * kLinK / 2;
   static constexpr int kStageStride = (X::kXBytes + kRawBytes + 1023) / 1024 * 1024;  // [x terms][x scales][packed W]
   static constexpr int kSpreadStride = kWideN * kLinK + 2 * kLinSfBytes;              // [W][W scales]
-  static constexpr int kBuffers = 2;
+  static constexpr int kBuffers = kWideGroups;
   static constexpr int kStages = (222 * 1024 - kBuffers * kSpreadStride) / kStageStride;
   static_assert(kStages >= 2, "a stage must fit twice");
   static constexpr int kSmem = kBuffers * kSpreadStride + kStages * kStageStride + 1024 + 256;
@@ -636,7 +643,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     *fail = 0;
     fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc(tmem_slot, Tile::kTmemCols);
+  if (warp == 1) tmem_alloc(tmem_slot, Tile::kTmemCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -665,62 +672,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         if (!mbar_wait_cycles(&raw_full[j % ST], static_cast<uint32_t>((j / ST) & 1))) ok = false;
       if (!ok) atomicOr(fail, 1);
     }
-  } else if (warp < 9) {
-    // ------------------------------------------------------------ spreading
-    const int e = threadIdx.x - 32;  // and the row of W whose scales this thread brings
-    const int64_t nb = P.inner / 32;
-    const bool row_in = n0 + e < P.outs;
-    const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0);
-    uint32_t sf[4], sf_next[4];
-    auto load_scales = [&](int i, uint32_t (&w)[4]) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        w[q] = 0;
-        if (row_in && i + q < n_chunks) {
-          if (P.words) {
-            w[q] = *reinterpret_cast<const uint32_t*>(srow + 4 * (i + q));
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (static_cast<int64_t>(i + q) * 4 + k < nb) w[q] |= static_cast<uint32_t>(srow[4 * (i + q) + k]) << (8 * k);
-          }
-        }
-      }
-    };
-    load_scales(0, sf_next);
-    bool ok = true;
-    for (int i = 0; i < n_chunks; ++i) {
-      const int s = i % ST, b = i % WB;
-      if ((i & 3) == 0) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sf[q] = sf_next[q];
-        load_scales(i + 4, sf_next);
-      }
-      uint8_t* w = smem + b * Tile::kSpreadStride;
-      if (i >= WB && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[b], static_cast<uint32_t>((i / WB - 1) & 1)))) ok = false;
-      if (ok) {
-        const uint32_t word = (i & 2) ? ((i & 1) ? sf[3] : sf[2]) : ((i & 1) ? sf[1] : sf[0]);
-        *reinterpret_cast<uint32_t*>(w + kWideN * kLinK + (e >> 7) * kLinSfBytes + (e & 31) * 16 + ((e >> 5) & 3) * 4) = word;
-        if (!__all_sync(0xffffffffu, mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
-      }
-      if (!ok) break;
-      const uint8_t* raw = ring + s * Tile::kStageStride + X::kXBytes;
-      uint4 v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = reinterpret_cast<const uint4*>(raw)[e + j * kWideSpread];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int u = e + j * kWideSpread, r = u >> 2, p = u & 3;
-        uint8_t* row = w + r * 128;
-        *reinterpret_cast<uint2*>(row + (((2 * p) ^ (r & 7)) << 4)) = make_uint2(v[j].x, v[j].y);
-        *reinterpret_cast<uint2*>(row + (((2 * p + 1) ^ (r & 7)) << 4)) = make_uint2(v[j].z, v[j].w);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w_full[b]);
-    }
-    if (!ok) atomicOr(fail, 1);
-  } else {
+  } else if (warp == 1) {
     // ------------------------------------------------------------- products
     constexpr uint32_t idesc = make_idesc_e4m3_e2m1(128, kWideN);
     const bool leader = elect_one();
@@ -759,24 +711,78 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       mma_commit(done);
       if (!ok) atomicOr(fail, 1);
     }
+  } else {
+    // ------------------------------------------------------------ spreading
+    const int group = (warp - 2) / (kWideSpread / 32);
+    const int e = (threadIdx.x - 64) % kWideSpread;  // and the row of W whose scales this thread brings
+    const int64_t nb = P.inner / 32;
+    const bool row_in = n0 + e < P.outs;
+    const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0);
+    uint32_t sf[4], sf_next[4];
+    auto load_scales = [&](int i, uint32_t (&w)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = i + kWideGroups * q;
+        w[q] = 0;
+        if (row_in && c < n_chunks) {
+          if (P.words) {
+            w[q] = *reinterpret_cast<const uint32_t*>(srow + 4 * c);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (static_cast<int64_t>(c) * 4 + k < nb) w[q] |= static_cast<uint32_t>(srow[4 * c + k]) << (8 * k);
+          }
+        }
+      }
+    };
+    load_scales(group, sf_next);
+    bool ok = true;
+    uint8_t* w = smem + group * Tile::kSpreadStride;
+    for (int i = group, turn = 0; i < n_chunks; i += kWideGroups, ++turn) {
+      const int s = i % ST;
+      if ((turn & 3) == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sf[q] = sf_next[q];
+        load_scales(i + 4 * kWideGroups, sf_next);
+      }
+      if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&w_empty[group], static_cast<uint32_t>((turn - 1) & 1)))) ok = false;
+      if (ok) {
+        const uint32_t word = (turn & 2) ? ((turn & 1) ? sf[3] : sf[2]) : ((turn & 1) ? sf[1] : sf[0]);
+        *reinterpret_cast<uint32_t*>(w + kWideN * kLinK + (e >> 7) * kLinSfBytes + (e & 31) * 16 + ((e >> 5) & 3) * 4) = word;
+        if (!__all_sync(0xffffffffu, mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)))) ok = false;
+      }
+      if (!ok) break;
+      const uint8_t* raw = ring + s * Tile::kStageStride + X::kXBytes;
+      uint4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = reinterpret_cast<const uint4*>(raw)[e + j * kWideSpread];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int u = e + j * kWideSpread, r = u >> 2, p = u & 3;
+        uint8_t* row = w + r * 128;
+        *reinterpret_cast<uint2*>(row + (((2 * p) ^ (r & 7)) << 4)) = make_uint2(v[j].x, v[j].y);
+        *reinterpret_cast<uint2*>(row + (((2 * p + 1) ^ (r & 7)) << 4)) = make_uint2(v[j].z, v[j].w);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_full[group]);
+    }
+    if (!ok) atomicOr(fail, 1);
   }
 
   // ---------------------------------------------------------------- epilogue
-  // A warp reads its quarter of the rows and half of the columns, 64 at a
-  // time, and turns them over in shared memory so that a row's 64 outputs are
+  // A warp reads its quarter of the rows and 64 of the columns and turns them over in shared memory so that a row's 64 outputs are
   // read (residual) and written together.
   __syncwarp();
-  if (warp >= 1 && warp < 9) {
+  if (warp >= 2) {
     if (!__all_sync(0xffffffffu, mbar_wait_cycles(done, 0))) atomicOr(fail, 1);
     tc_fence_after();
-    const int quarter = warp & 3, half = (warp - 1) >> 2;
-    float* turn = reinterpret_cast<float*>(smem) + (warp - 1) * (32 * 66);  // [32 rows][64 + 2]
+    const int quarter = warp & 3, c = 64 * ((warp - 2) >> 2);
+    float* turn = reinterpret_cast<float*>(smem) + (warp - 2) * (32 * 66);  // [32 rows][64 + 2]
     const int64_t t0 = tile * 128 + 32 * quarter;
     const int rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), P.rows - t0)));
     const bool pairs = P.pairs;  // two outputs per load and store
-#pragma unroll 1
-    for (int c = 128 * half; c < 128 * half + 128; c += 64) {
-      if (n0 + c >= P.outs || rows == 0) break;
+    if (n0 + c < P.outs && rows > 0) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
@@ -821,12 +827,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           }
         }
       }
-      __syncwarp();
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Tile::kTmemCols);
   }
