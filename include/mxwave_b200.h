@@ -348,7 +348,7 @@ MXW_API int mxw_copy_pages(uint8_t* codes, uint8_t* scales, int64_t layers, int6
  * workspace: device memory, 16-byte aligned, of at least
  * mxw_paged_attention_workspace_size bytes for the same arguments; calls that
  * share one must not overlap on the device.
- * fp32 statistics and sums in a fixed order.
+ * fp32 statistics and sums in a fixed order.  flags: MXW_FLAG_TIMEOUT or NULL.
  */
 MXW_API size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,
                                                   int64_t max_length, int64_t max_queries);
@@ -358,7 +358,7 @@ MXW_API int mxw_paged_attention(const void* query, int dtype, int64_t tokens, in
                                 int64_t table_ld, int64_t table_width, const int32_t* lengths, const int32_t* start,
                                 int64_t seqs, int64_t max_length, int64_t max_queries, double softmax_scale,
                                 int causal, int64_t window, void* out, float* lse, void* workspace,
-                                size_t workspace_bytes, void* stream);
+                                size_t workspace_bytes, uint32_t* flags, void* stream);
 
 #ifdef __cplusplus
 }

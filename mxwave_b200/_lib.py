@@ -81,7 +81,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mxw_paged_attention_workspace_size": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "mxw_paged_attention": (_int, [_vp, _int, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64,
                                    _i64, _vp, _vp, _i64, _i64, _i64, ctypes.c_double, _int, _i64, _vp, _vp, _vp,
-                                   ctypes.c_size_t, _vp]),
+                                   ctypes.c_size_t, _vp, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None

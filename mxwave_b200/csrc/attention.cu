@@ -42,6 +42,7 @@
 
 #include <type_traits>
 
+#include "attention.cuh"
 #include "blockscale.cuh"
 #include "common.cuh"
 #include "runtime.h"
@@ -60,28 +61,7 @@ constexpr int kAttJoinThreads = 256;
 // finished last (393 us against 212 on 32 sequences of 1 to 65,536 keys; 325,
 // 253, 212 and 217 us with 1, 2, 4 and 8 here).
 constexpr int kAttStart = 4;
-constexpr float kAttLift = 7.0f;    // probabilities are held as 2^(x - m + 7)
-constexpr float kAttSlack = 8.0f;   // and x may pass m by 8 before m is raised: at most 2^15
 
-struct AttParams {
-  const void* query;
-  int64_t q_token, q_head;  // strides in elements
-  const uint8_t* codes;
-  const uint8_t* scales;
-  int64_t pages;
-  const int32_t* table;
-  int64_t table_ld, table_width;
-  const int32_t* lengths;
-  const int32_t* start;
-  int64_t tokens;
-  int q_vec;  // 16-byte loads of the queries are aligned
-  int seqs, heads, kv_heads, group, page_shift;
-  float scale_log2;  // softmax scale times log2(e)
-  int causal, window;
-  void* out;   // [tokens][heads][dim]
-  float* lse;  // [tokens][heads] or null
-  float* partial;
-};
 
 // One sequence's share of the work.
 struct AttSeq {
@@ -148,29 +128,6 @@ struct AttShares {
   }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// The f16 pairs of a word's four bytes.
-__device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t word, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(word));
-}
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -255,28 +212,6 @@ struct AttShape {
   static constexpr int kSlot = kRows * D + kRows;  // floats of a partial result
 };
 
-template <bool BF16>
-__device__ __forceinline__ void att_store(void* p, int64_t i, float v) {
-  if constexpr (BF16)
-    static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else
-    static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
-
-// Rows of `out` that no sequence covers: zeros.
-template <bool BF16>
-__device__ __forceinline__ void att_clear_rest(const AttParams& P, int dim) {
-  const int64_t first = max(static_cast<int64_t>(0), min(static_cast<int64_t>(P.start[0]), P.tokens));
-  const int64_t last = max(first, min(static_cast<int64_t>(P.start[P.seqs]), P.tokens));
-  const int64_t width = static_cast<int64_t>(P.heads) * dim, rest = P.tokens - (last - first);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kAttThreads;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kAttThreads + threadIdx.x; i < rest * width; i += step) {
-    const int64_t r = i / width, token = r < first ? r : last + r - first;
-    att_store<BF16>(P.out, token * width + i % width, 0.0f);
-    if (P.lse && i % width < P.heads) P.lse[token * P.heads + i % width] = -INFINITY;
-  }
-}
-
 template <bool BF16, int D, int NT>
 __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attention_kernel(const AttParams P) {
   using Shape = AttShape<D, NT>;
@@ -293,7 +228,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
   float* join = reinterpret_cast<float*>(att_smem);  // [warp][row][D]
   const uint32_t ring_s = smem_u32(att_smem) + warp * Shape::kRing;
 
-  att_clear_rest<BF16>(P, D);
+  att_clear_rest<BF16>(P, D, blockIdx.x, gridDim.x);
   int64_t total, ignored;
   att_totals<ROWS, kAttThreads>(P, 0, red, total, ignored);
   const AttShares shares(total, gridDim.x);
@@ -897,6 +832,7 @@ using namespace mxw;
 extern "C" size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,
                                                      int64_t max_length, int64_t max_queries) {
   if (!att_shape_ok(seqs, heads, kv_heads, dim, max_length, max_queries) || seqs == 0 || max_queries == 0) return 0;
+  if (attention_prompt_fits(seqs, heads, kv_heads, max_queries)) return 16;  // nothing is shared between blocks
   return att_plan(seqs, heads, kv_heads, dim, max_length, max_queries).bytes;
 }
 
@@ -906,7 +842,7 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
                                    int64_t table_ld, int64_t table_width, const int32_t* lengths, const int32_t* start,
                                    int64_t seqs, int64_t max_length, int64_t max_queries, double softmax_scale,
                                    int causal, int64_t window, void* out, float* lse, void* workspace,
-                                   size_t workspace_bytes, void* stream) {
+                                   size_t workspace_bytes, uint32_t* flags, void* stream) {
   if (!att_shape_ok(seqs, heads, kv_heads, dim, max_length, max_queries) || tokens < 0) return MXW_EINVAL;
   if (dtype != MXW_BF16 && dtype != MXW_F16) return MXW_EINVAL;
   if (page_tokens != 16 && page_tokens != 32 && page_tokens != 64 && page_tokens != 128) return MXW_EINVAL;
@@ -926,7 +862,8 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   if (!codes || !scales || !lengths || !start || (table_width > 0 && !table)) return MXW_EINVAL;
   if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0) return MXW_EINVAL;
   const AttPlan plan = att_plan(seqs, heads, kv_heads, dim, max_length, max_queries);
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < plan.bytes) return MXW_EINVAL;
+  const bool prompt = attention_prompt_fits(seqs, heads, kv_heads, max_queries);
+  if (!prompt && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < plan.bytes)) return MXW_EINVAL;
   if (seqs > 65535 || plan.units > 0x7fffffff || tokens > 0x7fffffff) return MXW_EUNSUPPORTED;
   AttParams P{};
   P.query = query;
@@ -947,12 +884,14 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   P.kv_heads = static_cast<int>(kv_heads);
   P.group = static_cast<int>(heads / kv_heads);
   P.page_shift = page_tokens == 16 ? 4 : page_tokens == 32 ? 5 : page_tokens == 64 ? 6 : 7;
-  P.scale_log2 = static_cast<float>(softmax_scale * 1.4426950408889634);
+  P.scale_log2 = std::max(static_cast<float>(softmax_scale * 1.4426950408889634), 1e-37f);  // positive: it meets -infinity
   P.causal = causal ? 1 : 0;
   P.window = static_cast<int>(std::min<int64_t>(window, 0x3fffffff));
   P.out = out;
   P.lse = lse;
   P.partial = static_cast<float*>(workspace);
+  P.flags = flags;
+  if (prompt) return launch_attention_prompt(P, dtype == MXW_BF16, static_cast<int>(dim), max_queries, s);
   if (dtype == MXW_BF16)
     return dim == 128 ? launch_attention_rows<true, 128>(P, plan, s) : launch_attention_rows<true, 64>(P, plan, s);
   return dim == 128 ? launch_attention_rows<false, 128>(P, plan, s) : launch_attention_rows<false, 64>(P, plan, s);

@@ -1,0 +1,577 @@
+// K11: attention over the MXFP4 cache for prompts, on the tcgen05 tensor cores.
+//
+// The same function as K10 where a sequence brings many query rows and the time
+// is that of the products.  A block owns 256 rows (two tiles of 128; a row is
+// one query of one of the heads that share a key/value head) and walks the keys
+// in tiles of 64:
+//   S = Q K^T   kind::mxf8f6f4: K's codes and scales go to the tensor cores as
+//               they are cached; Q is split into E4M3 terms once (terms.cuh)
+//   O += P V    kind::f16: P from TMEM, V decoded to f16 in shared memory.  V's
+//               scales run across the contraction, so they are multiplied into
+//               the codes relative to the tile's largest (times 2^13), and that
+//               one is folded into P: exact down to 2^-27 of the tile's largest.
+// Warps 0-3 and 4-7 are the softmax of the two row tiles, a thread a row: no
+// exchange between threads.  P = 2^(x - m + 7) is rounded to f16 (11 bits; the
+// sum is taken in fp32 before); m is raised only when a score passes it by 8, so
+// the accumulator, which lives in TMEM, is seldom rescaled.  Warps 8-11 bring
+// keys and values (cp.async a row piece at a time: pages may end anywhere in a
+// tile), spread K's codes and decode V; warp 12 issues the products.  While one
+// row tile is in its softmax the products of the other run.
+// What bounds it: per 64 keys 1024 cycles of products against the issue slots of
+// 16,384 exponentials and the maxima, sums, conversions around them.
+#include "attention.cuh"
+#include "blockscale.cuh"
+#include "common.cuh"
+#include "runtime.h"
+#include "terms.cuh"
+
+namespace mxw {
+
+constexpr int kPromptKeys = 64;
+constexpr int kPromptRows = 128;  // rows of a tile
+constexpr int kPromptThreads = 13 * 32;
+constexpr int kPromptRaw = 3;     // stages of copies
+
+template <int D, int TERMS>
+struct PromptShape {
+  static constexpr int kBlocks = D / 32;
+  static constexpr int kQTerm = kPromptRows * 128;             // a term of a row tile: rows of 128 bytes
+  static constexpr int kQ = TERMS * (kQTerm + kLinSfBytes);    // terms, then their scales
+  static constexpr int kK = kPromptKeys * 128 + kLinSfBytes;   // spread codes, then scales
+  static constexpr int kV = kPromptKeys * D * 2;
+  static constexpr int kKStride = (kK + 1023) / 1024 * 1024;
+  static constexpr int kRawCodes = kPromptKeys * D / 2, kRawScales = kPromptKeys * kBlocks;
+  static constexpr int kRawStage = 2 * (kRawCodes + kRawScales);  // [K codes][V codes][K scales][V scales]
+  static constexpr int kQStride = (kQ + 1023) / 1024 * 1024;
+  static constexpr int kSmem = 2 * kQStride + 2 * kKStride + 2 * kV + kPromptRaw * kRawStage + 1024 + 512;
+  // TMEM columns: S and O and P of both row tiles, the scales of Q, of two key tiles.
+  static constexpr int kS = 0, kO = 2 * kPromptKeys, kP = kO + 2 * D, kSfQ = kP + kPromptKeys, kSfK = kSfQ + 8 * TERMS;
+  static_assert(kSfK + 8 <= 512, "TMEM has 512 columns");
+};
+
+// D[128 x N] (+)= A B with A [128 x 16] f16 in TMEM.
+__device__ __forceinline__ void mma_f16_tmem(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 32 columns of TMEM, without the wait; and the store.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Barrier 1 over 128 threads; true when all of them bring true.
+__device__ __forceinline__ bool named_barrier_and(bool on) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred.aligned q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(on))
+      : "memory");
+  return all != 0;
+}
+
+// The block's rows and keys: the same for every role.
+struct PromptUnit {
+  int q0, queries, length;
+  int rows;    // of this block's 256 (0: none)
+  int row0;    // first, among the sequence's queries x group
+  int lo, hi;  // keys that some row sees
+  int tiles;
+};
+
+__device__ __forceinline__ PromptUnit prompt_unit(const AttParams& P, int b, int row0) {
+  PromptUnit u;
+  const int64_t first = P.start[b], last = P.start[b + 1];
+  u.q0 = static_cast<int>(max(static_cast<int64_t>(0), min(first, P.tokens)));
+  u.queries = static_cast<int>(max(static_cast<int64_t>(0), min(last, P.tokens) - u.q0));
+  const int64_t held = P.table_width << P.page_shift;
+  u.length = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(P.lengths[b]), held)));
+  u.row0 = row0;
+  u.rows = max(0, min(2 * kPromptRows, u.queries * P.group - row0));
+  const int pos0 = u.length - u.queries + row0 / P.group;
+  const int pos1 = u.length - u.queries + (row0 + max(u.rows, 1) - 1) / P.group;
+  u.lo = P.window > 0 ? max(0, pos0 - P.window + 1) / 16 * 16 : 0;
+  u.hi = P.causal ? max(0, min(pos1 + 1, u.length)) : u.length;
+  u.tiles = max(0, (u.hi - u.lo + kPromptKeys - 1) / kPromptKeys);
+  return u;
+}
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(const AttParams P) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Shape = PromptShape<D, TERMS>;
+  constexpr int BLOCKS = Shape::kBlocks;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint8_t* q_smem = smem;                                  // [2 row tiles]
+  uint8_t* k_smem = q_smem + 2 * Shape::kQStride;          // [2]
+  uint8_t* v_smem = k_smem + 2 * Shape::kKStride;          // [2]
+  uint8_t* raw_smem = v_smem + 2 * Shape::kV;              // [3]
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(raw_smem + kPromptRaw * Shape::kRawStage);  // [2]
+  uint64_t* kv_full = q_full + 2;    // [2]
+  uint64_t* kv_empty = kv_full + 2;  // [2]
+  uint64_t* s_full = kv_empty + 2;   // [2 row tiles]
+  uint64_t* s_free = s_full + 2;
+  uint64_t* p_full = s_free + 2;
+  uint64_t* o_done = p_full + 2;
+  int* tile_ref = reinterpret_cast<int*>(o_done + 2);  // [2] largest scale byte of the values
+  uint32_t* tile_in = reinterpret_cast<uint32_t*>(tile_ref + 2);  // [2][2] keys whose page is one of the pool's, as bits
+  int* warp_ref = reinterpret_cast<int*>(tile_in + 4);           // [2][4]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(warp_ref + 8);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int head = blockIdx.x, b = blockIdx.y;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&kv_full[i], 4);
+      mbar_init(&kv_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 12) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  att_clear_rest<BF16>(P, D, (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x,
+                       static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z);
+
+  // Row tiles from the last on: under a causal mask those see the most keys.
+  // (A block takes one when the caller's bound on the queries holds.)
+  const int n_units = (prompt_unit(P, b, 0).queries * P.group + 2 * kPromptRows - 1) / (2 * kPromptRows);
+  bool ok = true;
+  int kv = 0;     // key tiles so far (all roles count alike)
+  int count[2] = {0, 0};  // key tiles so far of each row tile
+  int made[2] = {0, 0};   // and its sets of queries
+  for (int z = n_units - 1 - static_cast<int>(blockIdx.z); z >= 0 && ok; z -= static_cast<int>(gridDim.z)) {
+    const PromptUnit u = prompt_unit(P, b, z * 2 * kPromptRows);
+    if (u.rows == 0) continue;
+    const bool second = u.rows > kPromptRows;
+
+    if (warp < 8) {
+      // ------------------------------------------------------------ softmax
+      const int x = warp >> 2, quarter = warp & 3;
+      const int r = 32 * quarter + lane;  // this thread's row of the tile
+      const int row = x * kPromptRows + r;
+      if (x == 1 && !second) {
+        ;
+      } else {
+        // The tile's queries as terms: 16 (D = 128) or 8 lanes a row, eight elements each.
+        if (u.tiles > 0) {
+          constexpr int PARTS = D / 8, PER = 32 / PARTS;
+          const int part = lane % PARTS;
+          uint8_t* qt = q_smem + x * Shape::kQStride;
+#pragma unroll 4
+          for (int k = 0; k < 32; k += PER) {
+            const int rr = 32 * quarter + k + lane / PARTS, at = u.row0 + x * kPromptRows + rr;
+            const bool in = x * kPromptRows + rr < u.rows;
+            const int i = in ? at / P.group : 0, h = in ? at - i * P.group : 0;
+            const uint16_t* src = static_cast<const uint16_t*>(P.query) + static_cast<int64_t>(u.q0 + i) * P.q_token +
+                                  static_cast<int64_t>(head * P.group + h) * P.q_head + part * 8;
+            const uint4 v = load_x8(src, in, P.q_vec);
+            split_x8<BF16, 128>(v, rr, part, qt, qt + TERMS * Shape::kQTerm, true);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[x]);
+        }
+        const bool live = row < u.rows;
+        const int at = u.row0 + (live ? row : 0), i_q = at / P.group;
+        const int pos = u.length - u.queries + i_q;
+        const int key_hi = P.causal ? max(0, pos + 1) : u.length;
+        const int key_lo = P.window > 0 ? max(0, pos - P.window + 1) : 0;
+        // Key tiles between these bounds need no mask for any row of the warp.
+        const int warp_last = min(x * kPromptRows + 32 * quarter + 31, u.rows - 1), warp_first = min(x * kPromptRows + 32 * quarter, u.rows - 1);
+        const int pos_first = u.length - u.queries + (u.row0 + warp_first) / P.group;
+        const int pos_last = u.length - u.queries + (u.row0 + warp_last) / P.group;
+        const int open_hi = P.causal ? max(0, pos_first + 1) : u.length;
+        const int open_lo = P.window > 0 ? max(0, pos_last - P.window + 1) : 0;
+        const uint32_t lanes = static_cast<uint32_t>(32 * quarter) << 16;
+        const uint32_t s_t = tmem + lanes + Shape::kS + x * kPromptKeys, o_t = tmem + lanes + Shape::kO + x * D;
+        const uint32_t p_t = tmem + lanes + Shape::kP + x * (kPromptKeys / 2);
+        float m = -INFINITY, l = 0.0f;
+        int ref = 0;  // scale byte that the accumulator is relative to
+        for (int t = 0; t < u.tiles; ++t) {
+          const int n = count[x] + t;
+          if (!__all_sync(0xffffffffu, mbar_wait_cycles(&s_full[x], n & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint32_t s0[32], s1[32];
+          tmem_load32(s_t, s0);
+          tmem_load32(s_t + 32, s1);
+          // (kv_full completed before the products were issued: this wait only orders the two reads.)
+          const int buf = (kv + t) & 1;
+          if (!__all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], ((kv + t) >> 1) & 1))) {
+            ok = false;
+            break;
+          }
+          const int ref_t = *reinterpret_cast<volatile int*>(&tile_ref[buf]);
+          const uint32_t in0 = *reinterpret_cast<volatile uint32_t*>(&tile_in[2 * buf]);
+          const uint32_t in1 = *reinterpret_cast<volatile uint32_t*>(&tile_in[2 * buf + 1]);
+          tmem_wait_load();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[x]);
+          const int key = u.lo + t * kPromptKeys;
+          if (key < open_lo || key + kPromptKeys > open_hi) {
+            const int from = key_lo - key, to = key_hi - key;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (j < from || j >= to) s0[j] = 0xff800000u;
+              if (j + 32 < from || j + 32 >= to) s1[j] = 0xff800000u;
+            }
+          }
+          if ((in0 & in1) != 0xffffffffu) {
+            // Keys whose page is not one of the pool's.
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (!((in0 >> j) & 1u)) s0[j] = 0xff800000u;
+              if (!((in1 >> j) & 1u)) s1[j] = 0xff800000u;
+            }
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) top = fmaxf(top, fmaxf(bits_f32(s0[j]), bits_f32(s1[j])));
+          top = __fmul_rn(top, P.scale_log2);
+          // The accumulator and P belong to the last tile's product until that is done.
+          if (t > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (n - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          const bool raise = top > __fadd_rn(m, kAttSlack);
+          if (__any_sync(0xffffffffu, raise) || ref_t > ref) {
+            const float up = raise ? fmaxf(m, top) : m;
+            const float fm = m == up ? 1.0f : ex2(__fsub_rn(m, up));
+            m = up;
+            l = __fmul_rn(l, fm);
+            const float f = __fmul_rn(fm, ref_t > ref ? exp2i(max(ref - ref_t, -149)) : 1.0f);
+            ref = max(ref, ref_t);
+            if (t > 0) {
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D; c += 16) {
+                float o[16];
+                uint32_t w[16];
+                tmem_ld_32x32b_x16(o_t + c, o);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = f32_bits(__fmul_rn(o[j], f));
+                tmem_store16(o_t + c, w);
+              }
+            }
+          }
+          const float base = __fsub_rn(kAttLift, m == -INFINITY ? 0.0f : m);
+          // P is relative to the accumulator's reference; its sum is not.
+          const float fold = exp2i(max(ref_t - ref, -149));
+          float sum0 = 0.0f, sum1 = 0.0f;
+          auto probabilities = [&](const uint32_t (&s)[32], uint32_t taddr) {
+            uint32_t p[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float a = ex2(__fmaf_rn(bits_f32(s[2 * j]), P.scale_log2, base));
+              const float c = ex2(__fmaf_rn(bits_f32(s[2 * j + 1]), P.scale_log2, base));
+              sum0 = __fadd_rn(sum0, a);
+              sum1 = __fadd_rn(sum1, c);
+              p[j] = pack_f16x2(__fmul_rn(a, fold), __fmul_rn(c, fold));
+            }
+            tmem_store16(taddr, p);
+          };
+          probabilities(s0, p_t);
+          probabilities(s1, p_t + 16);
+          l = __fadd_rn(l, __fadd_rn(sum0, sum1));
+          tmem_wait_store();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[x]);
+        }
+        if (u.tiles > 0 && ok) {
+          if (!__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (count[x] + u.tiles - 1) & 1))) ok = false;
+          tc_fence_after();
+        }
+        const bool seen = !(l == 0.0f);  // NaN counts as seen
+        const float inv = seen ? __fdiv_rn(1.0f, l) : 0.0f;
+        const float back = exp2i(max(ref - 140, -149));
+        const int64_t out_row = static_cast<int64_t>(u.q0 + i_q) * P.heads + head * P.group + (at - i_q * P.group);
+        uint16_t* out = static_cast<uint16_t*>(P.out) + out_row * D;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (u.tiles > 0) {
+            tmem_load32(o_t + c, o);
+            tmem_wait_load();
+          }
+          if (live && ok) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float a = seen ? __fmul_rn(__fmul_rn(bits_f32(o[j + 2 * k]), inv), back) : 0.0f;
+                const float e = seen ? __fmul_rn(__fmul_rn(bits_f32(o[j + 2 * k + 1]), inv), back) : 0.0f;
+                if constexpr (BF16) {
+                  const __nv_bfloat162 h2 = __floats2bfloat162_rn(a, e);
+                  w[k] = *reinterpret_cast<const uint32_t*>(&h2);
+                } else {
+                  w[k] = pack_f16x2(a, e);
+                }
+              }
+              *reinterpret_cast<uint4*>(out + c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (live && ok && P.lse) P.lse[out_row] = seen ? __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(l), kAttLift)), 0.69314718055994531f) : -INFINITY;
+        tc_fence_before();
+      }
+    } else if (warp < 12) {
+      // -------------------------------------------------- keys and values in
+      const int e = threadIdx.x - 256;
+      const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
+      const int page_mask = (1 << P.page_shift) - 1;
+      const int64_t page_rows = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows of a page's keys
+      // Key `j` of tile t: the page that holds it, -1 past the last key, -2 when it is not one of the pool's.
+      auto page_of = [&](int t, int j) -> int {
+        const int key = u.lo + t * kPromptKeys + j;
+        if (t >= u.tiles || key >= u.hi) return -1;
+        const int page = table[key >> P.page_shift];
+        return static_cast<uint32_t>(page) < static_cast<uint32_t>(P.pages) ? page : -2;
+      };
+      // Pieces of 16 bytes: D / 32 per row.  A thread's pieces lie 128 / BLOCKS rows apart.
+      constexpr int PIECES = kPromptKeys * BLOCKS / 128;  // per thread: 2 or 1
+      constexpr int SCALES = Shape::kRawScales / 16;      // pieces of a tensor's scales: 16 / BLOCKS keys each
+      // Pages of this thread's next copies, read a tile ahead.  16 bytes of
+      // scales are 16 / BLOCKS neighbouring keys: of one page, as tiles start
+      // at multiples of 16.
+      const int scale_piece = e % SCALES, scale_key = scale_piece * (16 / BLOCKS);
+      int next[PIECES], next_scale = -1;
+      auto look_up = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) next[j] = page_of(t, (e + 128 * j) / BLOCKS);
+        if (e < 2 * SCALES) next_scale = page_of(t, scale_key);
+      };
+      auto row_of = [&](int page, int key) -> int64_t {
+        return ((static_cast<int64_t>(max(page, 0)) * 2 * P.kv_heads + head) << P.page_shift) + (key & page_mask);
+      };
+      auto issue = [&](int t) {
+        const uint32_t st = smem_u32(raw_smem) + ((kv + t) % kPromptRaw) * Shape::kRawStage;
+        const int key0 = u.lo + t * kPromptKeys;
+        if (t < u.tiles) {
+#pragma unroll
+          for (int j = 0; j < PIECES; ++j) {
+            const int unit = e + 128 * j;
+            const uint32_t bytes = next[j] >= 0 ? 16u : 0u;
+            const uint8_t* kc = next[j] >= 0 ? P.codes + row_of(next[j], key0 + unit / BLOCKS) * (D / 2) + unit % BLOCKS * 16 : P.codes;
+            cp_async<16>(st + unit * 16, kc, bytes);
+            cp_async<16>(st + Shape::kRawCodes + unit * 16, next[j] >= 0 ? kc + page_rows * (D / 2) : P.codes, bytes);
+          }
+          if (e < 2 * SCALES) {
+            const int64_t line = row_of(next_scale, key0 + scale_key) + (e >= SCALES ? page_rows : 0);
+            cp_async<16>(st + 2 * Shape::kRawCodes + e * 16, next_scale >= 0 ? P.scales + line * BLOCKS : P.scales, next_scale >= 0 ? 16u : 0u);
+          }
+          look_up(t + 1);
+        }
+        cp_async_commit();
+      };
+      look_up(0);
+      issue(0);
+      issue(1);
+      for (int t = 0; t < u.tiles; ++t) {
+        const int n = kv + t, buf = n & 1;
+        cp_async_wait<1>();
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the tile is here, and all are done with the stage refilled below
+        issue(t + 2);
+        const uint8_t* raw = raw_smem + (n % kPromptRaw) * Shape::kRawStage;
+        const uint8_t* ks = raw + 2 * Shape::kRawCodes;
+        const uint8_t* vs = ks + Shape::kRawScales;
+        // Scale bytes of this thread's pieces of values; keys that no row sees have none.
+        int sv[PIECES];
+        int top = 0;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int unit = e + 128 * j, key = u.lo + t * kPromptKeys + unit / BLOCKS;
+          sv[j] = key < u.hi ? vs[unit] : 0;
+          top = max(top, sv[j]);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) warp_ref[buf * 4 + warp - 8] = top;
+        const bool in_pool = e < kPromptKeys ? page_of(t, e) != -2 : true;
+        if (n >= 2) ok = mbar_wait_cycles(&kv_empty[buf], ((n >> 1) - 1) & 1);
+        ok = named_barrier_and(ok);  // (all four warps go on, or none)
+        if (!ok) break;
+        top = max(max(warp_ref[buf * 4], warp_ref[buf * 4 + 1]), max(warp_ref[buf * 4 + 2], warp_ref[buf * 4 + 3]));
+        if (e == 0) tile_ref[buf] = top;
+        const uint32_t in = __ballot_sync(0xffffffffu, in_pool);
+        if (e < kPromptKeys && lane == 0) tile_in[2 * buf + (e >> 5)] = in;
+        uint8_t* kd = k_smem + buf * Shape::kKStride;
+        uint8_t* vd = v_smem + buf * Shape::kV;
+        if (e < kPromptKeys) {
+          const uint32_t word = D == 128 ? reinterpret_cast<const uint32_t*>(ks)[e] : reinterpret_cast<const uint16_t*>(ks)[e];
+          *reinterpret_cast<uint32_t*>(kd + kPromptKeys * 128 + (e & 31) * 16 + (e >> 5) * 4) = word;
+        }
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const int unit = e + 128 * j, key = unit / BLOCKS, p = unit % BLOCKS;
+          // Keys: 32 codes to slots 2p and 2p + 1 of the row's 128 bytes, swizzled over eight rows.
+          const uint4 kw = reinterpret_cast<const uint4*>(raw)[unit];
+          uint8_t* row = kd + key * 128;
+          *reinterpret_cast<uint2*>(row + (((2 * p) ^ (key & 7)) << 4)) = make_uint2(kw.x, kw.y);
+          *reinterpret_cast<uint2*>(row + (((2 * p + 1) ^ (key & 7)) << 4)) = make_uint2(kw.z, kw.w);
+          // Values: 32 channels to four 16-byte slots of the key's row in a box of 64 channels.
+          const uint4 vw = reinterpret_cast<const uint4*>(raw + Shape::kRawCodes)[unit];
+          const int drop = top - sv[j];
+          const uint32_t factor = drop < 28 ? static_cast<uint32_t>(28 - drop) << 10 : 0u;  // f16 2^(13 - drop)
+          const uint32_t f2 = factor * 0x10001u;
+          uint8_t* box = vd + (p >> 1) * (kPromptKeys * 128) + key * 128;
+          const uint32_t words[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t h[4];
+            e2m1x8_to_f16x2(words[w], h);
+            *reinterpret_cast<uint4*>(box + ((((p & 1) * 4 + w) ^ (key & 7)) << 4)) =
+                make_uint4(hmul2(h[0], f2), hmul2(h[1], f2), hmul2(h[2], f2), hmul2(h[3], f2));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&kv_full[buf]);
+      }
+      cp_async_wait<0>();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    } else {
+      // ----------------------------------------------------------- products
+      constexpr uint32_t idesc_s = make_idesc_e4m3_e2m1(128, kPromptKeys);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);  // f16, B MN-major
+      const bool leader = elect_one();
+      const int tiles_x = second ? 2 : 1;
+      const uint32_t qs = smem_u32(q_smem), ksm = smem_u32(k_smem), vsm = smem_u32(v_smem);
+      // O of row tile x += P V of key tile t (whose count over the kernel is n).
+      auto values = [&](int x, int t) {
+        const int buf = (kv + t) & 1;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_cycles(&p_full[x], (count[x] + t) & 1));
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t vb = vsm + buf * Shape::kV;
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < kPromptKeys / 16; ++kk)
+            mma_f16_tmem(tmem + Shape::kO + x * D, tmem + Shape::kP + x * (kPromptKeys / 2) + 8 * kk,
+                         make_smem_desc_mn_sw128(vb + kk * 2048, kPromptKeys * 128, 1024), idesc_o, (t > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(&o_done[x]);
+        }
+        __syncwarp();
+      };
+      for (int t = 0; t <= u.tiles && ok; ++t) {
+        if (t < u.tiles) {
+          const int n = kv + t, buf = n & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], (n >> 1) & 1));
+          for (int x = 0; x < tiles_x && ok; ++x) {
+            if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&q_full[x], made[x] & 1));
+            // S is free once the softmax has read the last tile's.
+            if (ok && count[x] + t > 0) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&s_free[x], (count[x] + t - 1) & 1));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t qb = qs + x * Shape::kQStride, kb = ksm + buf * Shape::kKStride;
+            const uint32_t sfq = tmem + Shape::kSfQ + x * 4 * TERMS, sfk = tmem + Shape::kSfK + 4 * buf;
+            const uint32_t a_lo = desc_k_sw128_lo(qb), b_lo = desc_k_sw128_lo(kb);
+            if (leader) {
+              if (t == 0) {
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) tmem_cp_scales(sfq + 4 * k, qb + TERMS * Shape::kQTerm + k * kLinSfBytes);
+              }
+              if (x == 0) tmem_cp_scales(sfk, kb + kPromptKeys * 128);
+#pragma unroll
+              for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+                for (int kk = 0; kk < BLOCKS; ++kk)
+                  mma_mxf8f6f4(tmem + Shape::kS + x * kPromptKeys, desc_of(kDescKSw128Hi, a_lo + k * (Shape::kQTerm >> 4) + 2 * kk),
+                               desc_of(kDescKSw128Hi, b_lo + 2 * kk), mx_idesc_scale_byte(idesc_s, kk), sfq + 4 * k, sfk,
+                               (k > 0 || kk > 0) ? 1u : 0u);
+              mma_commit(&s_full[x]);
+            }
+            __syncwarp();
+          }
+        }
+        if (t > 0 && ok) {
+          for (int x = 0; x < tiles_x; ++x) values(x, t - 1);
+          if (ok && leader) mma_commit(&kv_empty[(kv + t - 1) & 1]);
+          __syncwarp();
+        }
+      }
+    }
+    if (u.tiles > 0) {
+      kv += u.tiles;
+      count[0] += u.tiles;
+      ++made[0];
+      if (second) {
+        count[1] += u.tiles;
+        ++made[1];
+      }
+    }
+  }
+  if (!ok && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool BF16, int D>
+static int launch_prompt(const AttParams& P, int64_t row_tiles, cudaStream_t s) {
+  using Shape = PromptShape<D, BF16 ? 2 : 3>;
+  auto kernel = attention_prompt_kernel<BF16, D>;
+  const int status = set_max_smem(reinterpret_cast<const void*>(kernel), Shape::kSmem);
+  if (status != MXW_OK) return status;
+  const dim3 grid(static_cast<unsigned>(P.kv_heads), static_cast<unsigned>(P.seqs), static_cast<unsigned>(row_tiles));
+  kernel<<<grid, kPromptThreads, Shape::kSmem, s>>>(P);
+  return check_launch();
+}
+
+static int64_t prompt_tiles(int64_t group, int64_t max_queries) {
+  return std::max<int64_t>(1, std::min<int64_t>((max_queries * group + 2 * kPromptRows - 1) / (2 * kPromptRows), 65535));
+}
+
+// One block holds an SM and takes a sequence's keys whole, where the decoding
+// kernel spreads them over the GPU: it needs enough blocks, and rows to fill
+// its tiles.
+bool attention_prompt_fits(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t max_queries) {
+  const int64_t group = heads / kv_heads;
+  return max_queries * group > kPromptRows / 2 && seqs * kv_heads * prompt_tiles(group, max_queries) >= num_sms() / 5;
+}
+
+int launch_attention_prompt(const AttParams& P, int bf16, int dim, int64_t max_queries, cudaStream_t s) {
+  const int64_t tiles = prompt_tiles(P.group, max_queries);
+  if (bf16) return dim == 128 ? launch_prompt<true, 128>(P, tiles, s) : launch_prompt<true, 64>(P, tiles, s);
+  return dim == 128 ? launch_prompt<false, 128>(P, tiles, s) : launch_prompt<false, 64>(P, tiles, s);
+}
+
+}  // namespace mxw

@@ -1,0 +1,142 @@
+// bf16 and f16 rows as sums of E4M3 terms with E8M0 block scales: the operand
+// that meets MXFP4 in a block-scaled product.  E4M3 carries 4 significant bits,
+// so two terms hold bf16's 8 and three hold f16's 11:
+//   s = 2^(floor(log2 amax) - 7) of the block of 32,  t0 = e4m3(x / s),
+//   t1 = e4m3((x / s - t0) 2^5),  t2 = e4m3(((x / s - t0) 2^5 - t1) 2^5)
+// with scales s, s 2^-5, s 2^-10.  Every remainder is exact in fp32.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "blockscale.cuh"
+#include "common.cuh"
+
+namespace mxw {
+
+constexpr int kLinM = 128;        // outputs per tile
+constexpr int kLinK = 128;        // inputs per stage
+constexpr int kLinSpread = 128;   // threads that spread a stage of W
+constexpr int kLinGroups = 2;     // groups of them, which take every other stage
+constexpr int kLinSpreadWarps = kLinGroups * kLinSpread / 32;  // the epilogue's warps too
+constexpr int kLinThreads = 64 + 32 * kLinSpreadWarps;  // copies, products, spreading (and four warps that make terms)
+constexpr int kLinRawBytes = kLinM * kLinK / 2;    // packed codes of a stage
+constexpr int kLinWBytes = kLinM * kLinK;          // spread: 16 bytes per 16 codes
+constexpr int kLinSfBytes = 512;                   // scales of 128 rows x 4 blocks
+
+template <int NT, int TERMS>
+struct LinearTile {
+  static constexpr bool kFused = NT == 16;  // terms made in the product's kernel
+  // Small tiles take the terms as rows of one operand (and add up their columns
+  // at the end): a quarter of the instructions, which one thread issues at some
+  // 65 cycles each.
+  static constexpr bool kMerged = NT < 128;
+  static constexpr int kTermBytes = NT * kLinK;
+  static constexpr int kN = kMerged ? TERMS * NT : NT;               // columns of the accumulator
+  static constexpr int kOperands = kMerged ? 1 : TERMS;
+  static constexpr int kSfTiles = (kMerged ? (TERMS * NT + 127) / 128 : TERMS * ((NT + 127) / 128));
+  static constexpr int kXBytes = TERMS * kTermBytes + kSfTiles * kLinSfBytes;  // one chunk of x: terms, then their scales
+  // Where the scale of term t of row r lies: 128 operand rows to 512 bytes, [row % 32][row / 32][block].
+  __host__ __device__ static constexpr int sf_place(int t, int r) {
+    const int n = kMerged ? t * NT + r : r;
+    return (kMerged ? 0 : t * kLinSfBytes) + (n >> 7) * kLinSfBytes + (n & 31) * 16 + ((n >> 5) & 3) * 4;
+  }
+  // A stage of copies: [x terms][x scales][packed W]; a spread buffer: [W][W
+  // scales]; and where the terms are made, a ring of those.
+  static constexpr int kStage = (kFused ? 0 : kXBytes) + kLinRawBytes;
+  static constexpr int kStageStride = (kStage + 1023) / 1024 * 1024;
+  static constexpr int kSpreadStride = (kLinWBytes + kLinSfBytes + 1023) / 1024 * 1024;
+  static constexpr int kXStages = kFused ? 4 : 0;
+  static constexpr int kXStride = (kXBytes + 1023) / 1024 * 1024;
+  static constexpr int kThreads = kLinThreads + 32 * kXStages;
+  static constexpr int kBuffers = kLinGroups;  // one spread buffer per group
+  static constexpr int kBudget = NT <= 32 ? 111 * 1024 : 222 * 1024;  // two CTAs per SM for small tiles
+  static constexpr int kFit = (kBudget - kBuffers * kSpreadStride - kXStages * kXStride) / kStageStride;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static_assert(kStages >= 2, "a stage must fit twice");
+  static constexpr int kSmem = kBuffers * kSpreadStride + kXStages * kXStride + kStages * kStageStride + 1024 + 256;
+  // TMEM: the accumulator, then the scales of two chunks.
+  static constexpr uint32_t kSfCols = 4 * (1 + kSfTiles);
+  static constexpr uint32_t kCols = kN + 2 * kSfCols;
+  static constexpr uint32_t kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+};
+
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
+  const __half2 hh = *reinterpret_cast<__half2*>(&h);
+  return make_float2(__low2float(hh), __high2float(hh));
+}
+
+// Eight inputs of a row; zeros outside x.
+__device__ __forceinline__ uint4 load_x8(const uint16_t* src, bool in, bool vec) {
+  if (!in) return make_uint4(0, 0, 0, 0);
+  if (vec) return *reinterpret_cast<const uint4*>(src);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = src[2 * i] | (static_cast<uint32_t>(src[2 * i + 1]) << 16);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The terms of eight inputs: part `part` (of 16) of row `r` of a tile whose
+// image starts at `terms` and whose scales start at `sf`.  Four neighbouring
+// lanes share a block; all lanes of the warp take part in the shuffles.
+template <bool BF16, int NT>
+__device__ __forceinline__ void split_x8(const uint4& raw, int r, int part, uint8_t* terms, uint8_t* sf, bool store) {
+  constexpr int TERMS = BF16 ? 2 : 3;
+  using Tile = LinearTile<NT, TERMS>;
+  float v[8];
+  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      v[2 * i] = bits_f32(words[i] << 16);
+      v[2 * i + 1] = bits_f32(words[i] & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  // byte = 127 + floor(log2 amax) - 7, at least 0; 255 (NaN) for a non-finite block.
+  const int ebits = static_cast<int>(amax >> 23);
+  int byte = max(ebits - 7, 0);
+  if (ebits == 255) byte = 255;
+  const float mult = ebits == 255 ? 0.0f : exp2i(127 - byte);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = ebits == 255 ? 0.0f : __fmul_rn(v[i], mult);
+  if (!store) return;
+  // 16-byte slot part / 2 of the row's 128 bytes, swizzled over eight rows.
+  terms += r * 128 + (((part >> 1) ^ (r & 7)) << 4) + ((part & 1) << 3);
+#pragma unroll
+  for (int t = 0; t < TERMS; ++t) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<uint2*>(terms + t * Tile::kTermBytes) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    if ((part & 3) == 0) sf[Tile::sf_place(t, r) + (part >> 2)] = static_cast<uint8_t>(byte);
+    if (t + 1 < TERMS) {
+      const int step = byte == 255 ? 0 : min(byte, 5);  // scales do not go below 2^-127
+      const float up = static_cast<float>(1 << step);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 q = e4m3x2_to_f32x2(w[i]);
+        v[2 * i] = __fmul_rn(__fsub_rn(v[2 * i], q.x), up);
+        v[2 * i + 1] = __fmul_rn(__fsub_rn(v[2 * i + 1], q.y), up);
+      }
+      byte -= step;
+    }
+  }
+}
+
+}  // namespace mxw

@@ -403,7 +403,7 @@ def _paged_attention_mxfp4(query: Tensor, codes: Tensor, scales: Tensor, table: 
             codes.data_ptr(), scales.data_ptr(), pages, kv_heads, page, dim, table.data_ptr(), table.stride(0), width,
             lengths.data_ptr(), query_start.data_ptr(), seqs, max_length, max_queries, softmax_scale, causal, window,
             out.data_ptr(), lse.data_ptr() if want_lse else None, workspace.data_ptr(), nbytes,
-            _raw_stream(query.device),
+            None, _raw_stream(query.device),
         )
     _lib.check(status, "mxw_paged_attention")
     return out, lse
