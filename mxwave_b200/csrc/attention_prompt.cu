@@ -30,7 +30,8 @@ namespace mxw {
 constexpr int kPromptKeys = 64;
 constexpr int kPromptRows = 128;  // rows of a tile
 constexpr int kPromptThreads = 13 * 32;
-constexpr int kPromptRaw = 3;     // stages of copies
+constexpr int kPromptRaw = 4;     // stages of copies
+constexpr int kPromptKv = 3;      // decoded tiles: one in the scores' product, one in the values', one being made
 
 template <int D, int TERMS>
 struct PromptShape {
@@ -43,7 +44,7 @@ struct PromptShape {
   static constexpr int kRawCodes = kPromptKeys * D / 2, kRawScales = kPromptKeys * kBlocks;
   static constexpr int kRawStage = 2 * (kRawCodes + kRawScales);  // [K codes][V codes][K scales][V scales]
   static constexpr int kQStride = (kQ + 1023) / 1024 * 1024;
-  static constexpr int kSmem = 2 * kQStride + 2 * kKStride + 2 * kV + kPromptRaw * kRawStage + 1024 + 512;
+  static constexpr int kSmem = 2 * kQStride + kPromptKv * (kKStride + kV) + kPromptRaw * kRawStage + 1024 + 512;
   // TMEM columns: S and O and P of both row tiles, the scales of Q, of two key tiles.
   static constexpr int kS = 0, kO = 2 * kPromptKeys, kP = kO + 2 * D, kSfQ = kP + kPromptKeys, kSfK = kSfQ + 8 * TERMS;
   static_assert(kSfK + 8 <= 512, "TMEM has 512 columns");
@@ -126,28 +127,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
   uint8_t* q_smem = smem;                                  // [2 row tiles]
-  uint8_t* k_smem = q_smem + 2 * Shape::kQStride;          // [2]
-  uint8_t* v_smem = k_smem + 2 * Shape::kKStride;          // [2]
-  uint8_t* raw_smem = v_smem + 2 * Shape::kV;              // [3]
+  uint8_t* k_smem = q_smem + 2 * Shape::kQStride;          // [3]
+  uint8_t* v_smem = k_smem + kPromptKv * Shape::kKStride;  // [3]
+  uint8_t* raw_smem = v_smem + kPromptKv * Shape::kV;      // [4]
   uint64_t* q_full = reinterpret_cast<uint64_t*>(raw_smem + kPromptRaw * Shape::kRawStage);  // [2]
-  uint64_t* kv_full = q_full + 2;    // [2]
-  uint64_t* kv_empty = kv_full + 2;  // [2]
-  uint64_t* s_full = kv_empty + 2;   // [2 row tiles]
+  uint64_t* kv_full = q_full + 2;             // [3]
+  uint64_t* kv_empty = kv_full + kPromptKv;   // [3]
+  uint64_t* s_full = kv_empty + kPromptKv;    // [2 row tiles]
   uint64_t* s_free = s_full + 2;
   uint64_t* p_full = s_free + 2;
   uint64_t* o_done = p_full + 2;
-  int* tile_ref = reinterpret_cast<int*>(o_done + 2);  // [2] largest scale byte of the values
-  uint32_t* tile_in = reinterpret_cast<uint32_t*>(tile_ref + 2);  // [2][2] keys whose page is one of the pool's, as bits
-  int* warp_ref = reinterpret_cast<int*>(tile_in + 4);           // [2][4]
+  int* tile_ref = reinterpret_cast<int*>(o_done + 2);  // [3] largest scale byte of the values
+  uint32_t* tile_in = reinterpret_cast<uint32_t*>(tile_ref + kPromptKv);  // [3][2] keys whose page is one of the pool's, as bits
+  int* warp_ref = reinterpret_cast<int*>(tile_in + 2 * kPromptKv);           // [2][4]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(warp_ref + 8);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x, b = blockIdx.y;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 4);
+    for (int i = 0; i < kPromptKv; ++i) {
       mbar_init(&kv_full[i], 4);
       mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
@@ -229,8 +232,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
           tmem_load32(s_t, s0);
           tmem_load32(s_t + 32, s1);
           // (kv_full completed before the products were issued: this wait only orders the two reads.)
-          const int buf = (kv + t) & 1;
-          if (!__all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], ((kv + t) >> 1) & 1))) {
+          const int buf = (kv + t) % kPromptKv;
+          if (!__all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], (kv + t) / kPromptKv & 1))) {
             ok = false;
             break;
           }
@@ -258,9 +261,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
               if (!((in1 >> j) & 1u)) s1[j] = 0xff800000u;
             }
           }
-          float top = -INFINITY;
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) top = fmaxf(top, fmaxf(bits_f32(s0[j]), bits_f32(s1[j])));
+          for (int j = 0; j < 32; j += 4)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(bits_f32(s0[j + k]), bits_f32(s1[j + k])));
+          float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           top = __fmul_rn(top, P.scale_log2);
           // The accumulator and P belong to the last tile's product until that is done.
           if (t > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (n - 1) & 1))) {
@@ -288,25 +294,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
               }
             }
           }
-          const float base = __fsub_rn(kAttLift, m == -INFINITY ? 0.0f : m);
-          // P is relative to the accumulator's reference; its sum is not.
-          const float fold = exp2i(max(ref_t - ref, -149));
-          float sum0 = 0.0f, sum1 = 0.0f;
+          // P is relative to the accumulator's reference (in the exponent); its
+          // sum is not.  Values 2^-40 of the reference are as good as nothing.
+          const int drop = min(ref - ref_t, 40);
+          const float base = __fsub_rn(kAttLift - static_cast<float>(drop), m == -INFINITY ? 0.0f : m);
+          const unsigned long long f2 = pack2(P.scale_log2, P.scale_log2), b2 = pack2(base, base);
+          unsigned long long sum2 = 0ull, sum3 = 0ull;
           auto probabilities = [&](const uint32_t (&s)[32], uint32_t taddr) {
             uint32_t p[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              const float a = ex2(__fmaf_rn(bits_f32(s[2 * j]), P.scale_log2, base));
-              const float c = ex2(__fmaf_rn(bits_f32(s[2 * j + 1]), P.scale_log2, base));
-              sum0 = __fadd_rn(sum0, a);
-              sum1 = __fadd_rn(sum1, c);
-              p[j] = pack_f16x2(__fmul_rn(a, fold), __fmul_rn(c, fold));
+              const struct f2 x2 = unpack2(fma2(pack2(bits_f32(s[2 * j]), bits_f32(s[2 * j + 1])), f2, b2));
+              const float a = ex2(x2.x), c = ex2(x2.y);
+              if (j & 1)
+                sum2 = add2(sum2, pack2(a, c));
+              else
+                sum3 = add2(sum3, pack2(a, c));
+              p[j] = pack_f16x2(a, c);
             }
             tmem_store16(taddr, p);
           };
           probabilities(s0, p_t);
           probabilities(s1, p_t + 16);
-          l = __fadd_rn(l, __fadd_rn(sum0, sum1));
+          const struct f2 sums = unpack2(add2(sum2, sum3));
+          l = __fmaf_rn(__fadd_rn(sums.x, sums.y), exp2i(drop), l);
           tmem_wait_store();
           tc_fence_before();
           __syncwarp();
@@ -355,80 +366,107 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
       const int e = threadIdx.x - 256;
       const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
       const int page_mask = (1 << P.page_shift) - 1;
-      const int64_t page_rows = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows of a page's keys
-      // Key `j` of tile t: the page that holds it, -1 past the last key, -2 when it is not one of the pool's.
-      auto page_of = [&](int t, int j) -> int {
-        const int key = u.lo + t * kPromptKeys + j;
-        if (t >= u.tiles || key >= u.hi) return -1;
-        const int page = table[key >> P.page_shift];
-        return static_cast<uint32_t>(page) < static_cast<uint32_t>(P.pages) ? page : -2;
-      };
+      // Bytes of a page, from a key to its value, and this thread's places in a page (rows apart).
+      const uint32_t page_codes = 2u * P.kv_heads * (D / 2) << P.page_shift, page_scales = 2u * P.kv_heads * BLOCKS << P.page_shift;
+      const int64_t to_values = static_cast<int64_t>(P.kv_heads) * (D / 2) << P.page_shift;
       // Pieces of 16 bytes: D / 32 per row.  A thread's pieces lie 128 / BLOCKS rows apart.
       constexpr int PIECES = kPromptKeys * BLOCKS / 128;  // per thread: 2 or 1
-      constexpr int SCALES = Shape::kRawScales / 16;      // pieces of a tensor's scales: 16 / BLOCKS keys each
-      // Pages of this thread's next copies, read a tile ahead.  16 bytes of
-      // scales are 16 / BLOCKS neighbouring keys: of one page, as tiles start
-      // at multiples of 16.
-      const int scale_piece = e % SCALES, scale_key = scale_piece * (16 / BLOCKS);
+      constexpr int SCALES = Shape::kRawScales / 16;      // pieces of a tensor's scales: 16 / BLOCKS keys each, of one
+      const int key_e = e / BLOCKS;                       // page, as tiles start at multiples of 16
+      const int scale_key = e % SCALES * (16 / BLOCKS);
+      const uint8_t* codes = P.codes + (static_cast<int64_t>(head) * (D / 2) << P.page_shift) + e % BLOCKS * 16;
+      const uint8_t* scales = P.scales + (static_cast<int64_t>(head) * BLOCKS << P.page_shift) +
+                              (e >= SCALES ? static_cast<int64_t>(P.kv_heads) * BLOCKS << P.page_shift : 0);
+      // Pages of this thread's next copies, read a tile ahead: -1 past the last key.
       int next[PIECES], next_scale = -1;
       auto look_up = [&](int t) {
+        const int key = u.lo + t * kPromptKeys;
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) next[j] = page_of(t, (e + 128 * j) / BLOCKS);
-        if (e < 2 * SCALES) next_scale = page_of(t, scale_key);
+        for (int j = 0; j < PIECES; ++j) {
+          const int k = key + key_e + 128 / BLOCKS * j;
+          next[j] = k < u.hi ? table[k >> P.page_shift] : -1;
+          if (k < u.hi && next[j] < 0) next[j] = 0x7fffffff;
+        }
+        if (e < 2 * SCALES) next_scale = key + scale_key < u.hi ? table[(key + scale_key) >> P.page_shift] : -1;
       };
-      auto row_of = [&](int page, int key) -> int64_t {
-        return ((static_cast<int64_t>(max(page, 0)) * 2 * P.kv_heads + head) << P.page_shift) + (key & page_mask);
-      };
+      uint32_t strays = 0;  // tiles (mod 4) where this thread met a page that is not one of the pool's
       auto issue = [&](int t) {
-        const uint32_t st = smem_u32(raw_smem) + ((kv + t) % kPromptRaw) * Shape::kRawStage;
-        const int key0 = u.lo + t * kPromptKeys;
         if (t < u.tiles) {
+          const int n = kv + t;
+          const uint32_t st = smem_u32(raw_smem) + (n % kPromptRaw) * Shape::kRawStage;
+          const int key = u.lo + t * kPromptKeys;
+          uint32_t stray = 0;
 #pragma unroll
           for (int j = 0; j < PIECES; ++j) {
-            const int unit = e + 128 * j;
-            const uint32_t bytes = next[j] >= 0 ? 16u : 0u;
-            const uint8_t* kc = next[j] >= 0 ? P.codes + row_of(next[j], key0 + unit / BLOCKS) * (D / 2) + unit % BLOCKS * 16 : P.codes;
-            cp_async<16>(st + unit * 16, kc, bytes);
-            cp_async<16>(st + Shape::kRawCodes + unit * 16, next[j] >= 0 ? kc + page_rows * (D / 2) : P.codes, bytes);
+            const bool in = static_cast<uint32_t>(next[j]) < static_cast<uint32_t>(P.pages);
+            stray |= !in && next[j] >= 0 ? 1u : 0u;
+            const int offset = (key + key_e + 128 / BLOCKS * j) & page_mask;
+            const uint8_t* kc = codes + static_cast<uint64_t>(in ? static_cast<uint32_t>(next[j]) : 0u) * page_codes + offset * (D / 2);
+            const uint32_t bytes = in ? 16u : 0u;
+            cp_async<16>(st + (e + 128 * j) * 16, kc, bytes);
+            cp_async<16>(st + Shape::kRawCodes + (e + 128 * j) * 16, kc + to_values, bytes);
           }
           if (e < 2 * SCALES) {
-            const int64_t line = row_of(next_scale, key0 + scale_key) + (e >= SCALES ? page_rows : 0);
-            cp_async<16>(st + 2 * Shape::kRawCodes + e * 16, next_scale >= 0 ? P.scales + line * BLOCKS : P.scales, next_scale >= 0 ? 16u : 0u);
+            const bool in = static_cast<uint32_t>(next_scale) < static_cast<uint32_t>(P.pages);
+            const uint8_t* sc = scales + static_cast<uint64_t>(in ? static_cast<uint32_t>(next_scale) : 0u) * page_scales + ((key + scale_key) & page_mask) * BLOCKS;
+            cp_async<16>(st + 2 * Shape::kRawCodes + e * 16, sc, in ? 16u : 0u);
           }
+          strays = (strays & ~(1u << (n & 3))) | (stray << (n & 3));
           look_up(t + 1);
         }
         cp_async_commit();
       };
-      look_up(0);
-      issue(0);
-      issue(1);
-      for (int t = 0; t < u.tiles; ++t) {
-        const int n = kv + t, buf = n & 1;
-        cp_async_wait<1>();
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the tile is here, and all are done with the stage refilled below
-        issue(t + 2);
-        const uint8_t* raw = raw_smem + (n % kPromptRaw) * Shape::kRawStage;
-        const uint8_t* ks = raw + 2 * Shape::kRawCodes;
-        const uint8_t* vs = ks + Shape::kRawScales;
-        // Scale bytes of this thread's pieces of values; keys that no row sees have none.
-        int sv[PIECES];
+      // The largest scale byte of a tile's values, by warps, a tile ahead; bit
+      // 8: a stray page.  Keys that no row sees have no say.
+      int sv[PIECES], sv_next[PIECES];
+      auto find_top = [&](int t) {
+        if (t >= u.tiles) return;
+        const int n = kv + t;
+        const uint8_t* vs = raw_smem + (n % kPromptRaw) * Shape::kRawStage + 2 * Shape::kRawCodes + Shape::kRawScales;
         int top = 0;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-          const int unit = e + 128 * j, key = u.lo + t * kPromptKeys + unit / BLOCKS;
-          sv[j] = key < u.hi ? vs[unit] : 0;
-          top = max(top, sv[j]);
+          sv_next[j] = u.lo + t * kPromptKeys + key_e + 128 / BLOCKS * j < u.hi ? vs[e + 128 * j] : 0;
+          top = max(top, sv_next[j]);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) warp_ref[buf * 4 + warp - 8] = top;
-        const bool in_pool = e < kPromptKeys ? page_of(t, e) != -2 : true;
-        if (n >= 2) ok = mbar_wait_cycles(&kv_empty[buf], ((n >> 1) - 1) & 1);
-        ok = named_barrier_and(ok);  // (all four warps go on, or none)
+        top = __reduce_max_sync(0xffffffffu, top | static_cast<int>((strays >> (n & 3)) & 1u) << 8);
+        if (lane == 0) warp_ref[(n & 1) * 4 + warp - 8] = top;
+      };
+      look_up(0);
+      issue(0);
+      issue(1);
+      issue(2);
+      cp_async_wait<2>();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      find_top(0);
+      for (int t = 0; t < u.tiles; ++t) {
+        const int n = kv + t, buf = n % kPromptKv;
+        cp_async_wait<1>();  // the next tile is here
+        // All warps' copies and findings, and all are done with the stage
+        // refilled below.  All four warps go on, or none.
+        ok = named_barrier_and(ok);
         if (!ok) break;
-        top = max(max(warp_ref[buf * 4], warp_ref[buf * 4 + 1]), max(warp_ref[buf * 4 + 2], warp_ref[buf * 4 + 3]));
+        issue(t + 3);
+        const int* found = warp_ref + (n & 1) * 4;
+        int top = max(max(found[0], found[1]), max(found[2], found[3]));
+        const bool stray = top >= 256;
+        if (stray) top = max(max(found[0] & 255, found[1] & 255), max(found[2] & 255, found[3] & 255));
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) sv[j] = sv_next[j];
+        find_top(t + 1);
+        const uint8_t* raw = raw_smem + (n % kPromptRaw) * Shape::kRawStage;
+        const uint8_t* ks = raw + 2 * Shape::kRawCodes;
+        if (n >= kPromptKv) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&kv_empty[buf], (n / kPromptKv - 1) & 1));
+        if (!ok) continue;  // to the barrier, where the other warps learn of it
         if (e == 0) tile_ref[buf] = top;
-        const uint32_t in = __ballot_sync(0xffffffffu, in_pool);
-        if (e < kPromptKeys && lane == 0) tile_in[2 * buf + (e >> 5)] = in;
+        if (e < kPromptKeys) {
+          uint32_t bits = 0xffffffffu;
+          if (stray) {
+            const int k = u.lo + t * kPromptKeys + e;
+            bits = __ballot_sync(0xffffffffu, k >= u.hi || static_cast<uint32_t>(table[k >> P.page_shift]) < static_cast<uint32_t>(P.pages));
+          }
+          if (lane == 0) tile_in[2 * buf + (e >> 5)] = bits;
+        }
         uint8_t* kd = k_smem + buf * Shape::kKStride;
         uint8_t* vd = v_smem + buf * Shape::kV;
         if (e < kPromptKeys) {
@@ -463,7 +501,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         if (lane == 0) mbar_arrive(&kv_full[buf]);
       }
       cp_async_wait<0>();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      ok = named_barrier_and(ok);  // before the next rows' copies, or the end of all four
     } else {
       // ----------------------------------------------------------- products
       constexpr uint32_t idesc_s = make_idesc_e4m3_e2m1(128, kPromptKeys);
@@ -473,7 +511,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
       const uint32_t qs = smem_u32(q_smem), ksm = smem_u32(k_smem), vsm = smem_u32(v_smem);
       // O of row tile x += P V of key tile t (whose count over the kernel is n).
       auto values = [&](int x, int t) {
-        const int buf = (kv + t) & 1;
+        const int buf = (kv + t) % kPromptKv;
         ok = ok && __all_sync(0xffffffffu, mbar_wait_cycles(&p_full[x], (count[x] + t) & 1));
         if (!ok) return;
         tc_fence_after();
@@ -489,8 +527,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
       };
       for (int t = 0; t <= u.tiles && ok; ++t) {
         if (t < u.tiles) {
-          const int n = kv + t, buf = n & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], (n >> 1) & 1));
+          const int n = kv + t, buf = n % kPromptKv;
+          ok = __all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], n / kPromptKv & 1));
           for (int x = 0; x < tiles_x && ok; ++x) {
             if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&q_full[x], made[x] & 1));
             // S is free once the softmax has read the last tile's.
@@ -498,7 +536,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             if (!ok) break;
             tc_fence_after();
             const uint32_t qb = qs + x * Shape::kQStride, kb = ksm + buf * Shape::kKStride;
-            const uint32_t sfq = tmem + Shape::kSfQ + x * 4 * TERMS, sfk = tmem + Shape::kSfK + 4 * buf;
+            const uint32_t sfq = tmem + Shape::kSfQ + x * 4 * TERMS, sfk = tmem + Shape::kSfK + 4 * (n & 1);
             const uint32_t a_lo = desc_k_sw128_lo(qb), b_lo = desc_k_sw128_lo(kb);
             if (leader) {
               if (t == 0) {
@@ -520,7 +558,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         }
         if (t > 0 && ok) {
           for (int x = 0; x < tiles_x; ++x) values(x, t - 1);
-          if (ok && leader) mma_commit(&kv_empty[(kv + t - 1) & 1]);
+          if (ok && leader) mma_commit(&kv_empty[(kv + t - 1) % kPromptKv]);
           __syncwarp();
         }
       }
