@@ -15,8 +15,8 @@
 // sum is taken in fp32 before); m is raised only when a score passes it by 8, so
 // the accumulator, which lives in TMEM, is seldom rescaled.  Warps 8-11 bring
 // keys and values (cp.async a row piece at a time: pages may end anywhere in a
-// tile), spread K's codes and decode V; warp 12 issues the products.  While one
-// row tile is in its softmax the products of the other run.
+// tile), spread K's codes and decode V; warps 12 and 13 issue the products of a
+// row tile each, so that one's waits are covered by the other's products.
 // What bounds it: per 64 keys 1024 cycles of products against the issue slots of
 // 16,384 exponentials and the maxima, sums, conversions around them.
 #include "attention.cuh"
@@ -29,7 +29,7 @@ namespace mxw {
 
 constexpr int kPromptKeys = 64;
 constexpr int kPromptRows = 128;  // rows of a tile
-constexpr int kPromptThreads = 13 * 32;
+constexpr int kPromptThreads = 14 * 32;
 constexpr int kPromptRaw = 4;     // stages of copies
 constexpr int kPromptKv = 3;      // decoded tiles: one in the scores' product, one in the values', one being made
 
@@ -45,9 +45,9 @@ struct PromptShape {
   static constexpr int kRawStage = 2 * (kRawCodes + kRawScales);  // [K codes][V codes][K scales][V scales]
   static constexpr int kQStride = (kQ + 1023) / 1024 * 1024;
   static constexpr int kSmem = 2 * kQStride + kPromptKv * (kKStride + kV) + kPromptRaw * kRawStage + 1024 + 512;
-  // TMEM columns: S and O and P of both row tiles, the scales of Q, of two key tiles.
+  // TMEM columns: S and O and P of both row tiles, the scales of Q and of two key tiles.
   static constexpr int kS = 0, kO = 2 * kPromptKeys, kP = kO + 2 * D, kSfQ = kP + kPromptKeys, kSfK = kSfQ + 8 * TERMS;
-  static_assert(kSfK + 8 <= 512, "TMEM has 512 columns");
+  static_assert(kSfK + 16 <= 512, "TMEM has 512 columns");
 };
 
 // D[128 x N] (+)= A B with A [128 x 16] f16 in TMEM.
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
   if (threadIdx.x == 0) {
     for (int i = 0; i < kPromptKv; ++i) {
       mbar_init(&kv_full[i], 4);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
@@ -503,47 +503,40 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
       cp_async_wait<0>();
       ok = named_barrier_and(ok);  // before the next rows' copies, or the end of all four
     } else {
-      // ----------------------------------------------------------- products
+      // ------------------------------------- products of row tile warp - 12
       constexpr uint32_t idesc_s = make_idesc_e4m3_e2m1(128, kPromptKeys);
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (8u << 24);  // f16, B MN-major
+      const int x = warp - 12;
       const bool leader = elect_one();
-      const int tiles_x = second ? 2 : 1;
-      const uint32_t qs = smem_u32(q_smem), ksm = smem_u32(k_smem), vsm = smem_u32(v_smem);
-      // O of row tile x += P V of key tile t (whose count over the kernel is n).
-      auto values = [&](int x, int t) {
-        const int buf = (kv + t) % kPromptKv;
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_cycles(&p_full[x], (count[x] + t) & 1));
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t vb = vsm + buf * Shape::kV;
-        if (leader) {
-#pragma unroll
-          for (int kk = 0; kk < kPromptKeys / 16; ++kk)
-            mma_f16_tmem(tmem + Shape::kO + x * D, tmem + Shape::kP + x * (kPromptKeys / 2) + 8 * kk,
-                         make_smem_desc_mn_sw128(vb + kk * 2048, kPromptKeys * 128, 1024), idesc_o, (t > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&o_done[x]);
-        }
-        __syncwarp();
-      };
-      for (int t = 0; t <= u.tiles && ok; ++t) {
-        if (t < u.tiles) {
+      const uint32_t qb = smem_u32(q_smem) + x * Shape::kQStride, ksm = smem_u32(k_smem), vsm = smem_u32(v_smem);
+      const uint32_t sfq = tmem + Shape::kSfQ + x * 4 * TERMS;
+      auto reached = [&](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait_cycles(bar, phase & 1)) != 0; };
+      if (x == 1 && !second) {
+        // No rows: the tiles' buffers still count this warp's word.
+        for (int t = 0; t < u.tiles && ok; ++t) {
           const int n = kv + t, buf = n % kPromptKv;
-          ok = __all_sync(0xffffffffu, mbar_wait_cycles(&kv_full[buf], n / kPromptKv & 1));
-          for (int x = 0; x < tiles_x && ok; ++x) {
-            if (t == 0) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&q_full[x], made[x] & 1));
-            // S is free once the softmax has read the last tile's.
-            if (ok && count[x] + t > 0) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&s_free[x], (count[x] + t - 1) & 1));
+          ok = reached(&kv_full[buf], n / kPromptKv);
+          if (ok && leader) mbar_arrive(&kv_empty[buf]);
+          __syncwarp();
+        }
+      } else if (u.tiles > 0) {
+        ok = reached(&q_full[x], made[x]);
+        for (int t = 0; t <= u.tiles && ok; ++t) {
+          if (t < u.tiles) {
+            // S = Q K^T, once the softmax has read the last tile's.
+            const int n = kv + t, buf = n % kPromptKv;
+            ok = reached(&kv_full[buf], n / kPromptKv) && (count[x] + t == 0 || reached(&s_free[x], count[x] + t - 1));
             if (!ok) break;
             tc_fence_after();
-            const uint32_t qb = qs + x * Shape::kQStride, kb = ksm + buf * Shape::kKStride;
-            const uint32_t sfq = tmem + Shape::kSfQ + x * 4 * TERMS, sfk = tmem + Shape::kSfK + 4 * (n & 1);
+            const uint32_t kb = ksm + buf * Shape::kKStride;
+            const uint32_t sfk = tmem + Shape::kSfK + 8 * x + 4 * (n & 1);
             const uint32_t a_lo = desc_k_sw128_lo(qb), b_lo = desc_k_sw128_lo(kb);
             if (leader) {
               if (t == 0) {
 #pragma unroll
                 for (int k = 0; k < TERMS; ++k) tmem_cp_scales(sfq + 4 * k, qb + TERMS * Shape::kQTerm + k * kLinSfBytes);
               }
-              if (x == 0) tmem_cp_scales(sfk, kb + kPromptKeys * 128);
+              tmem_cp_scales(sfk, kb + kPromptKeys * 128);
 #pragma unroll
               for (int k = 0; k < TERMS; ++k)
 #pragma unroll
@@ -555,11 +548,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             }
             __syncwarp();
           }
-        }
-        if (t > 0 && ok) {
-          for (int x = 0; x < tiles_x; ++x) values(x, t - 1);
-          if (ok && leader) mma_commit(&kv_empty[(kv + t - 1) % kPromptKv]);
-          __syncwarp();
+          if (t > 0) {
+            // O += P V of the tile before.
+            const int n = kv + t - 1, buf = n % kPromptKv;
+            ok = reached(&p_full[x], count[x] + t - 1);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t vb = vsm + buf * Shape::kV;
+            if (leader) {
+#pragma unroll
+              for (int kk = 0; kk < kPromptKeys / 16; ++kk)
+                mma_f16_tmem(tmem + Shape::kO + x * D, tmem + Shape::kP + x * (kPromptKeys / 2) + 8 * kk,
+                             make_smem_desc_mn_sw128(vb + kk * 2048, kPromptKeys * 128, 1024), idesc_o, (t > 1 || kk > 0) ? 1u : 0u);
+              mma_commit(&o_done[x]);
+              mma_commit(&kv_empty[buf]);
+            }
+            __syncwarp();
+          }
         }
       }
     }

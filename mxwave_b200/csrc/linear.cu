@@ -306,9 +306,9 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int s = i % ST, b = i % WB, xs = i % XS;
+      // (The spreading warps have seen the copies' barrier: theirs covers x too.)
       ok = mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) &&
-           (FUSED ? mbar_wait_cycles(&x_full[xs], static_cast<uint32_t>((i / XS) & 1))
-                  : mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1)));
+           (!FUSED || mbar_wait_cycles(&x_full[xs], static_cast<uint32_t>((i / XS) & 1)));
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
@@ -555,8 +555,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     bool ok = true;
     for (int i = 0; i < n_chunks; ++i) {
       const int s = i % ST, b = i % WB;
-      ok = mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1)) &&
-           mbar_wait_cycles(&raw_full[s], static_cast<uint32_t>((i / ST) & 1));
+      // (The spreading warps have seen the copies' barrier: theirs covers x too.)
+      ok = mbar_wait_cycles(&w_full[b], static_cast<uint32_t>((i / WB) & 1));
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
         break;
