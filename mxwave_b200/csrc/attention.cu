@@ -67,7 +67,7 @@ constexpr int kAttStart = 4;
 struct AttSeq {
   int q0, queries;  // its rows of the packed queries
   int length;       // cached tokens
-  int lo;           // first key that some query sees, rounded down to 16
+  int lo;           // first key that some query sees, rounded down to 32 (a step stays in a page)
   int tiles;        // tiles of 128 keys from lo on, at least one
   int row_groups;   // groups of 8 NT rows per key/value head
 };
@@ -80,7 +80,7 @@ __device__ __forceinline__ AttSeq att_seq(const AttParams& P, int b) {
   s.queries = static_cast<int>(max(static_cast<int64_t>(0), min(last, P.tokens) - s.q0));
   const int64_t held = P.table_width << P.page_shift;
   s.length = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(P.lengths[b]), held)));
-  s.lo = P.window > 0 ? max(0, s.length - s.queries - P.window + 1) / kAttHalf * kAttHalf : 0;
+  s.lo = P.window > 0 ? max(0, s.length - s.queries - P.window + 1) / kAttKeys * kAttKeys : 0;
   s.tiles = max(1, (s.length - s.lo + kAttTile - 1) / kAttTile);
   s.row_groups = (s.queries * P.group + ROWS - 1) / ROWS;
   return s;

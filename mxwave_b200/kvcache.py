@@ -16,8 +16,9 @@ no counterpart.
 
 from __future__ import annotations
 
-from collections.abc import Sequence
-
+import heapq
+from collections.abc import Iterable, Sequence
+from dataclasses import dataclass, field
 
 import torch
 
@@ -50,7 +51,7 @@ def _check_pool(codes: torch.Tensor, scales: torch.Tensor, layers: bool = False)
         raise ValueError(f"scales is on {scales.device}, codes on {codes.device}")
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError("codes and scales must be contiguous")
-    if codes.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0:
+    if _ops().plain_eager(codes) and (codes.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0):
         raise ValueError("codes and scales must be 16-byte aligned")
 
 
@@ -196,4 +197,259 @@ def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
-__all__ = ["HEAD_DIMS", "PAGE_TOKENS", "append_mxfp4_", "copy_pages_", "gather_mxfp4", "paged_attention_mxfp4"]
+@dataclass
+class _Held:
+    """One sequence: its pages in order, and how many tokens of them it has."""
+
+    pages: list[int] = field(default_factory=list)
+    length: int = 0
+
+
+class PageBooks:
+    """Which pages are free, which sequences hold which, and what has to be copied.
+
+    Host bookkeeping without tensors.  Pages are shared by reference; a page
+    that more than one sequence holds is never written: the writer gets a copy
+    first (``grow`` names the copies).
+    """
+
+    def __init__(self, pages: int, page_tokens: int) -> None:
+        if pages <= 0 or page_tokens <= 0:
+            raise ValueError("pages and page_tokens must be positive")
+        self.pages = pages
+        self.page_tokens = page_tokens
+        self._holders = [0] * pages
+        self._free = list(range(pages))  # a heap: low pages first keeps the pool compact
+        self._held: dict[int, _Held] = {}
+        self._next_id = 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    @property
+    def sequences(self) -> list[int]:
+        return list(self._held)
+
+    def _get(self, seq: int) -> _Held:
+        try:
+            return self._held[seq]
+        except KeyError:
+            raise KeyError(f"no sequence {seq}") from None
+
+    def length(self, seq: int) -> int:
+        return self._get(seq).length
+
+    def pages_of(self, seq: int) -> list[int]:
+        return list(self._get(seq).pages)
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        seq = self._next_id
+        self._next_id += 1
+        self._held[seq] = _Held()
+        return seq
+
+    def fork(self, seq: int) -> int:
+        """A new sequence with the same tokens: it shares every page."""
+        held = self._get(seq)
+        new = self.add()
+        self._held[new] = _Held(list(held.pages), held.length)
+        for page in held.pages:
+            self._holders[page] += 1
+        return new
+
+    def free(self, seq: int) -> None:
+        """Drop a sequence; pages that nobody else holds are free again."""
+        for page in self._get(seq).pages:
+            self._drop(page)
+        del self._held[seq]
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Drop the tokens from `length` on."""
+        held = self._get(seq)
+        if not 0 <= length <= held.length:
+            raise ValueError(f"length must be in [0, {held.length}], got {length}")
+        keep = -(-length // self.page_tokens)
+        for page in held.pages[keep:]:
+            self._drop(page)
+        del held.pages[keep:]
+        held.length = length
+
+    def grow(self, seqs: Sequence[int], tokens: Sequence[int]) -> list[tuple[int, int]]:
+        """Room for tokens[i] more tokens of each sequence; returns the (source, target) page copies due first.
+
+        Raises, and changes nothing, when the free pages do not suffice.
+        """
+        if len(seqs) != len(tokens):
+            raise ValueError(f"{len(seqs)} sequences, {len(tokens)} token counts")
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence is named twice")
+        if any(n < 1 for n in tokens):
+            raise ValueError("every sequence needs at least one new token")
+        held = [self._get(seq) for seq in seqs]
+        need = 0
+        holders = {}  # of shared last pages, as the copies below will leave them
+        for h, n in zip(held, tokens):
+            need += -(-(h.length + n) // self.page_tokens) - len(h.pages)
+            if h.length % self.page_tokens and holders.setdefault(h.pages[-1], self._holders[h.pages[-1]]) > 1:
+                holders[h.pages[-1]] -= 1
+                need += 1
+        if need > len(self._free):
+            raise RuntimeError(f"the cache is full: {need} pages needed, {len(self._free)} of {self.pages} free")
+        copies = []
+        for h, n in zip(held, tokens):
+            if h.length % self.page_tokens and self._holders[h.pages[-1]] > 1:
+                source = h.pages[-1]
+                h.pages[-1] = self._take()
+                self._holders[source] -= 1
+                copies.append((source, h.pages[-1]))
+            h.length += n
+            while len(h.pages) * self.page_tokens < h.length:
+                h.pages.append(self._take())
+        return copies
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Move every held page to the front of the pool; returns the (source, target) page copies due."""
+        live = self.pages - len(self._free)
+        holes = [page for page in range(live) if not self._holders[page]]
+        moves = dict(zip((page for page in range(live, self.pages) if self._holders[page]), holes))
+        for h in self._held.values():
+            h.pages = [moves.get(page, page) for page in h.pages]
+        for source, target in moves.items():
+            self._holders[target], self._holders[source] = self._holders[source], 0
+        self._free = list(range(live, self.pages))
+        return list(moves.items())
+
+    def _take(self) -> int:
+        page = heapq.heappop(self._free)
+        self._holders[page] = 1
+        return page
+
+    def _drop(self, page: int) -> None:
+        self._holders[page] -= 1
+        if self._holders[page] == 0:
+            heapq.heappush(self._free, page)
+
+
+@dataclass(frozen=True)
+class KVBatch:
+    """The device-side description of one step: what ``PagedKVCache.plan`` returns."""
+
+    slots: torch.Tensor        # int64 [tokens]: where the new tokens go
+    table: torch.Tensor        # int32 [seqs, width]: pages
+    lengths: torch.Tensor      # int32 [seqs]: tokens, the new ones included
+    query_start: torch.Tensor  # int32 [seqs + 1]: rows of the new tokens
+    max_length: int
+    max_queries: int
+    epoch: int
+
+
+class PagedKVCache:
+    """Keys and values of many sequences and layers in MXFP4 pages.
+
+    One step of a decoder: ``batch = cache.plan(seqs, new_tokens)``, then in
+    each layer ``cache.append(layer, k, v, batch)`` and ``cache.attend(layer, q,
+    batch)``.  ``fork`` shares pages (the first sequence that writes to a shared
+    page gets a copy of it, in all layers), ``truncate`` and ``free`` give them
+    back, ``compact`` moves what is held to the front of the pool.  All work is
+    ordered on the current stream.  A batch ends with the next plan, fork, free,
+    truncate or compact: using it later raises.
+    """
+
+    def __init__(self, pages: int, *, kv_heads: int, head_dim: int, layers: int = 1, page_tokens: int = 64,
+                 device: torch.device | str = "cuda") -> None:
+        if page_tokens not in PAGE_TOKENS or head_dim not in HEAD_DIMS:
+            raise ValueError(f"page_tokens must be one of {PAGE_TOKENS} and head_dim one of {HEAD_DIMS}, got {page_tokens} and {head_dim}")
+        if kv_heads <= 0 or layers <= 0:
+            raise ValueError("kv_heads and layers must be positive")
+        self.books = PageBooks(pages, page_tokens)
+        shape = (layers, pages, 2, kv_heads, page_tokens)
+        self.codes = torch.zeros((*shape, head_dim // 2), dtype=torch.uint8, device=device)
+        self.scales = torch.zeros((*shape, head_dim // BLOCK_SIZE), dtype=torch.uint8, device=device)
+        self.epoch = 0
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        return self.books.add()
+
+    def fork(self, seq: int) -> int:
+        """A new sequence with the same tokens; pages are shared until one of the two writes."""
+        new = self.books.fork(seq)
+        self.epoch += 1
+        return new
+
+    def free(self, seq: int) -> None:
+        """Drop a sequence."""
+        self.books.free(seq)
+        self.epoch += 1
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Drop a sequence's tokens from `length` on (rejected drafts)."""
+        self.books.truncate(seq, length)
+        self.epoch += 1
+
+    def compact(self) -> int:
+        """Move the held pages to the front of the pool; returns how many moved."""
+        self.epoch += 1
+        return self._copy(self.books.compact())
+
+    def plan(self, seqs: Iterable[int], new_tokens: Iterable[int]) -> KVBatch:
+        """Make room for each sequence's new tokens and describe the step to the device.
+
+        Raises RuntimeError, and changes nothing, when the pool is full.
+        """
+        seqs, new_tokens = list(seqs), [int(n) for n in new_tokens]
+        if not seqs:
+            raise ValueError("a step needs at least one sequence")
+        copies = self.books.grow(seqs, new_tokens)
+        self.epoch += 1
+        self._copy(copies)
+        page = self.books.page_tokens
+        held = [self.books.pages_of(seq) for seq in seqs]
+        lengths = [self.books.length(seq) for seq in seqs]
+        width = max(map(len, held))
+        table = torch.zeros((len(seqs), width), dtype=torch.int32)
+        slots = []
+        for i, (pages, length, n) in enumerate(zip(held, lengths, new_tokens)):
+            row = torch.tensor(pages, dtype=torch.int32)
+            table[i, : len(pages)] = row
+            token = torch.arange(length - n, length)
+            slots.append(row[token // page].long() * page + token % page)
+        start = torch.zeros(len(seqs) + 1, dtype=torch.int32)
+        start[1:] = torch.tensor(new_tokens, dtype=torch.int32).cumsum(0)
+        device = self.codes.device
+        return KVBatch(torch.cat(slots).to(device), table.to(device), torch.tensor(lengths, dtype=torch.int32).to(device), start.to(device),
+                       max(lengths), max(new_tokens), self.epoch)
+
+    def append(self, layer: int, key: torch.Tensor, value: torch.Tensor, batch: KVBatch) -> None:
+        """Write the new tokens' keys and values [tokens, kv_heads, head_dim] of one layer."""
+        self._check(batch)
+        append_mxfp4_(self.codes[layer], self.scales[layer], key, value, batch.slots)
+
+    def attend(self, layer: int, query: torch.Tensor, batch: KVBatch, *, softmax_scale: float | None = None, window: int = 0) -> torch.Tensor:
+        """Causal attention of the new tokens' queries [tokens, heads, head_dim] over one layer."""
+        self._check(batch)
+        return paged_attention_mxfp4(query, self.codes[layer], self.scales[layer], batch.table, batch.lengths, batch.query_start,
+                                     max_length=batch.max_length, max_queries=batch.max_queries, softmax_scale=softmax_scale, window=window)
+
+    def gather(self, layer: int, seq: int, dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """A sequence's keys and values of one layer, each [length, kv_heads, head_dim] of `dtype`."""
+        page = self.books.page_tokens
+        token = torch.arange(self.books.length(seq))
+        slots = torch.tensor(self.books.pages_of(seq), dtype=torch.int64)[token // page] * page + token % page
+        return gather_mxfp4(self.codes[layer], self.scales[layer], slots.to(self.codes.device), dtype)
+
+    def _check(self, batch: KVBatch) -> None:
+        if batch.epoch != self.epoch:
+            raise ValueError("this batch was planned before another plan, fork, free, truncate or compact: plan the step again")
+
+    def _copy(self, copies: list[tuple[int, int]]) -> int:
+        if copies:
+            # A page may go to several targets, and no target is a source: see grow and compact.
+            copy_pages_(self.codes, self.scales, [s for s, _ in copies], [t for _, t in copies])
+        return len(copies)
+
+
+__all__ = ["HEAD_DIMS", "PAGE_TOKENS", "KVBatch", "PageBooks", "PagedKVCache", "append_mxfp4_", "copy_pages_", "gather_mxfp4",
+           "paged_attention_mxfp4"]

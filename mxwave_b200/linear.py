@@ -67,10 +67,7 @@ def linear_mxfp4(
     from . import ops
 
     rows = _rows(x, inner)
-    packed = packed.contiguous()
-    if packed.data_ptr() % 16 != 0:
-        packed = packed.clone()
-    args = (rows, packed, scales.contiguous(), None if bias is None else bias.contiguous(),
+    args = (rows, packed.contiguous(), scales.contiguous(), None if bias is None else bias.contiguous(),
             None if residual is None else _rows(residual, outs), ACTIVATIONS[activation])
     y = ops._linear_mxfp4(*args) if ops.plain_eager(x) else torch.ops.mxwave_b200.linear_mxfp4(*args)
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], outs)

@@ -292,6 +292,8 @@ def _linear_mxfp4(x: Tensor, packed: Tensor, scales: Tensor, bias: Tensor | None
     y = torch.empty((rows, outs), dtype=x.dtype, device=x.device)
     if rows == 0 or outs == 0:
         return y
+    if packed.data_ptr() % 16 != 0:  # a slice that starts inside a 16-byte line
+        packed = packed.clone()
     lib = _lib.load()
     code = _DTYPE_CODES[x.dtype]
     nbytes = lib.mxw_linear_workspace_size(rows, inner, code)
