@@ -795,7 +795,8 @@ static AttPlan att_plan(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t d
 template <bool BF16, int D, int NT>
 static int launch_attention(const AttParams& P, const AttPlan& plan, cudaStream_t s) {
   auto kernel = attention_kernel<BF16, D, NT>;
-  int status = set_max_smem(reinterpret_cast<const void*>(kernel), AttShape<D, NT>::kSmem);
+  static std::atomic<uint64_t> done{0};
+  int status = set_max_smem_once(reinterpret_cast<const void*>(kernel), AttShape<D, NT>::kSmem, done);
   if (status != MXW_OK) return status;
   kernel<<<plan.blocks, kAttThreads, AttShape<D, NT>::kSmem, s>>>(P);
   status = check_launch();

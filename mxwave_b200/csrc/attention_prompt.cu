@@ -592,7 +592,8 @@ template <bool BF16, int D>
 static int launch_prompt(const AttParams& P, int64_t row_tiles, cudaStream_t s) {
   using Shape = PromptShape<D, BF16 ? 2 : 3>;
   auto kernel = attention_prompt_kernel<BF16, D>;
-  const int status = set_max_smem(reinterpret_cast<const void*>(kernel), Shape::kSmem);
+  static std::atomic<uint64_t> done{0};
+  const int status = set_max_smem_once(reinterpret_cast<const void*>(kernel), Shape::kSmem, done);
   if (status != MXW_OK) return status;
   const dim3 grid(static_cast<unsigned>(P.kv_heads), static_cast<unsigned>(P.seqs), static_cast<unsigned>(row_tiles));
   kernel<<<grid, kPromptThreads, Shape::kSmem, s>>>(P);

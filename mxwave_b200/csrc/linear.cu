@@ -742,7 +742,8 @@ static int launch_wide(const TermsParams& T, const uint8_t* packed, const Linear
   status = launch_terms<BF16, 128>(T, s);
   if (status != MXW_OK) return status;
   auto kernel = linear_wide_kernel<BF16>;
-  status = set_max_smem(reinterpret_cast<const void*>(kernel), Tile::kSmem);
+  static std::atomic<uint64_t> done{0};
+  status = set_max_smem_once(reinterpret_cast<const void*>(kernel), Tile::kSmem, done);
   if (status != MXW_OK) return status;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>((P.outs + kWideN - 1) / kWideN), static_cast<unsigned>((P.rows + 127) / 128));
@@ -773,7 +774,8 @@ static int launch_linear(const TermsParams& T, const uint8_t* packed, const Line
   }
 
   auto kernel = linear_kernel<BF16, NT>;
-  status = set_max_smem(reinterpret_cast<const void*>(kernel), Tile::kSmem);
+  static std::atomic<uint64_t> done{0};
+  status = set_max_smem_once(reinterpret_cast<const void*>(kernel), Tile::kSmem, done);
   if (status != MXW_OK) return status;
   const int64_t row_tiles = (P.outs + kLinM - 1) / kLinM;
   int split = 1;

@@ -44,6 +44,17 @@ int set_max_smem(const void* kernel, size_t bytes) {
   return err == cudaSuccess ? MXW_OK : record_cuda_error(err);
 }
 
+int set_max_smem_once(const void* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  const cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return record_cuda_error(err);
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return MXW_OK;
+  const int status = set_max_smem(kernel, bytes);
+  if (status == MXW_OK) done.fetch_or(bit, std::memory_order_relaxed);
+  return status;
+}
+
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "../../include/mxwave_b200.h"
@@ -23,6 +24,10 @@ int num_sms();
 
 // Raise a kernel's dynamic shared-memory limit (idempotent per kernel+device).
 int set_max_smem(const void* kernel, size_t bytes);
+
+// The same once per kernel and device: `done` is the caller's, one bit per
+// device (devices past 63 are set every time).
+int set_max_smem_once(const void* kernel, size_t bytes, std::atomic<uint64_t>& done);
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point.  2-D tensor
 // [rows, cols] with a row stride of `row_bytes`, box [box_rows, box_cols].

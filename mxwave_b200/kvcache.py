@@ -22,6 +22,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from . import ops
 from .core import BLOCK_SIZE
 
 PAGE_TOKENS = (16, 32, 64, 128)
@@ -29,29 +30,25 @@ HEAD_DIMS = (64, 128)
 _ROW_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _ops():
-    from . import ops
-
-    return ops
-
-
 def _check_pool(codes: torch.Tensor, scales: torch.Tensor, layers: bool = False) -> None:
     """Codes and scales of one layer, or of several with a leading dimension."""
-    lead = 1 if layers else 0
-    if codes.ndim != 5 + lead or scales.ndim != 5 + lead or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise ValueError(f"codes and scales must be {5 + lead}-D uint8 tensors")
-    two, _heads, page, half = codes.shape[1 + lead :]
-    if two != 2 or page not in PAGE_TOKENS or 2 * half not in HEAD_DIMS:
-        raise ValueError(f"codes must be [.., pages, 2, kv_heads, page in {PAGE_TOKENS}, head_dim/2 of {HEAD_DIMS}], got {tuple(codes.shape)}")
-    if scales.shape != (*codes.shape[:-1], half * 2 // BLOCK_SIZE):
-        raise ValueError(f"scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}")
-    if codes.device.type != "cuda":
-        raise RuntimeError(f"mxwave_b200 runs on CUDA devices only; codes is on {codes.device} (no CPU fallback)")
-    if scales.device != codes.device:
-        raise ValueError(f"scales is on {scales.device}, codes on {codes.device}")
+    shape, blocks = codes.shape, scales.shape
+    ndim = 6 if layers else 5
+    if len(shape) != ndim or len(blocks) != ndim or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"codes and scales must be {ndim}-D uint8 tensors")
+    half = shape[-1]
+    if shape[-4] != 2 or shape[-2] not in PAGE_TOKENS or 2 * half not in HEAD_DIMS:
+        raise ValueError(f"codes must be [.., pages, 2, kv_heads, page in {PAGE_TOKENS}, head_dim/2 of {HEAD_DIMS}], got {tuple(shape)}")
+    if blocks[:-1] != shape[:-1] or blocks[-1] * BLOCK_SIZE != 2 * half:
+        raise ValueError(f"scales {tuple(blocks)} do not match codes {tuple(shape)}")
+    device = codes.device
+    if device.type != "cuda":
+        raise RuntimeError(f"mxwave_b200 runs on CUDA devices only; codes is on {device} (no CPU fallback)")
+    if scales.device != device:
+        raise ValueError(f"scales is on {scales.device}, codes on {device}")
     if not codes.is_contiguous() or not scales.is_contiguous():
         raise ValueError("codes and scales must be contiguous")
-    if _ops().plain_eager(codes) and (codes.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0):
+    if ops.plain_eager(codes) and (codes.data_ptr() % 16 != 0 or scales.data_ptr() % 16 != 0):
         raise ValueError("codes and scales must be 16-byte aligned")
 
 
@@ -78,7 +75,6 @@ def append_mxfp4_(codes: torch.Tensor, scales: torch.Tensor, key: torch.Tensor, 
     _check_index("slots", slots, torch.int64, 1, codes.device)
     if slots.shape[0] != key.shape[0]:
         raise ValueError(f"slots holds {slots.shape[0]} entries for {key.shape[0]} rows")
-    ops = _ops()
     args = (codes, scales, _unit_rows(key.detach()), _unit_rows(value.detach()), slots.contiguous())
     if ops.plain_eager(codes):
         ops._kv_append_mxfp4_(*args)
@@ -98,7 +94,6 @@ def gather_mxfp4(
     if dtype not in _ROW_TYPES:
         raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     _check_index("slots", slots, torch.int64, 1, codes.device)
-    ops = _ops()
     args = (codes, scales, slots.contiguous(), dtype)
     return ops._kv_gather_mxfp4(*args) if ops.plain_eager(codes) else torch.ops.mxwave_b200.kv_gather_mxfp4(*args)
 
@@ -113,13 +108,17 @@ def copy_pages_(
     one call run in no order.
     """
     _check_pool(codes, scales, layers=True)
-    source = torch.as_tensor(source, dtype=torch.int64)
-    target = torch.as_tensor(target, dtype=torch.int64)
+    if not isinstance(source, torch.Tensor):
+        source = torch.tensor(source, dtype=torch.int64)
+    if not isinstance(target, torch.Tensor):
+        target = torch.tensor(target, dtype=torch.int64)
+    if source.dtype.is_floating_point or target.dtype.is_floating_point:
+        raise ValueError("source and target must hold whole numbers")
+    source, target = source.to(torch.int64), target.to(torch.int64)
     if source.device.type != "cpu" or target.device.type != "cpu":
         raise ValueError("source and target are page numbers on the host")
     if source.ndim != 1 or source.shape != target.shape:
         raise ValueError(f"source and target must be vectors of one length, got {tuple(source.shape)} and {tuple(target.shape)}")
-    ops = _ops()
     args = (codes, scales, source.contiguous(), target.contiguous())
     if ops.plain_eager(codes):
         ops._copy_pages_(*args)
@@ -182,13 +181,15 @@ def paged_attention_mxfp4(
         raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
     if torch.is_grad_enabled() and query.requires_grad:
         raise RuntimeError("paged_attention_mxfp4 has no gradient: call it under torch.no_grad()")
-    ops = _ops()
     if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
         table = table.contiguous()
     args = (_unit_rows(query), codes, scales, table, lengths.contiguous(), query_start.contiguous(), int(max_length), int(max_queries),
-            scale, bool(causal), int(window), bool(return_lse))
-    fn = ops._paged_attention_mxfp4 if ops.plain_eager(query) else torch.ops.mxwave_b200.paged_attention_mxfp4
-    out, lse = fn(*args)
+            scale, bool(causal), int(window))
+    if ops.plain_eager(query):
+        lse = ops._new_lse(query, True) if return_lse else None
+        out = ops._paged_attention_mxfp4(*args, lse)
+    else:
+        out, lse = torch.ops.mxwave_b200.paged_attention_mxfp4(*args, bool(return_lse))
     return (out, lse) if return_lse else out
 
 

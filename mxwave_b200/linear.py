@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from .core import BLOCK_SIZE
 
 ACTIVATIONS = {
@@ -40,43 +40,51 @@ def linear_mxfp4(
     calls give equal bits.  A row of x that holds a NaN or an infinity gives
     NaN in all its outputs.  There is no gradient.
     """
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"Unknown activation: {activation}")
-    if x.ndim < 1 or packed.ndim != 2 or scales.ndim != 2:
-        raise ValueError("x must have a last dimension, packed and scales must be matrices")
-    inner, outs = x.shape[-1], packed.shape[0]
-    if inner == 0 or inner % BLOCK_SIZE != 0:
-        raise ValueError(f"Last dim {inner} not divisible by BLOCK_SIZE={BLOCK_SIZE}")
-    if packed.shape[1] != inner // 2 or scales.shape != (outs, inner // BLOCK_SIZE):
-        raise ValueError(f"packed {tuple(packed.shape)} and scales {tuple(scales.shape)} do not hold [out, {inner}] weights")
-    if packed.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise ValueError("packed and scales must be uint8")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"x must be bfloat16 or float16, got {x.dtype}")
-    if x.device.type != "cuda":
-        raise RuntimeError(f"mxwave_b200 runs on CUDA devices only; x is on {x.device} (no CPU fallback)")
-    for name, t, shape in (("bias", bias, (outs,)), ("residual", residual, (*x.shape[:-1], outs))):
-        if t is not None and (t.shape != shape or t.dtype != x.dtype):
-            raise ValueError(f"{name} must be a {x.dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    for name, t in (("packed", packed), ("scales", scales), ("bias", bias), ("residual", residual)):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, bias, residual)):
-        raise RuntimeError("linear_mxfp4 has no gradient: call it under torch.no_grad()")
-
-    from . import ops
-
-    rows = _rows(x, inner)
-    args = (rows, packed.contiguous(), scales.contiguous(), None if bias is None else bias.contiguous(),
-            None if residual is None else _rows(residual, outs), ACTIVATIONS[activation])
+    _check(x, packed, scales, bias, residual)
+    outs = packed.shape[0]
+    args = (_rows(x), packed.contiguous(), scales.contiguous(), None if bias is None else bias.contiguous(),
+            None if residual is None else _rows(residual), act)
     y = ops._linear_mxfp4(*args) if ops.plain_eager(x) else torch.ops.mxwave_b200.linear_mxfp4(*args)
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], outs)
 
 
-def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+def _check(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None) -> None:
+    shape, held, blocks = x.shape, packed.shape, scales.shape
+    if len(shape) < 1 or len(held) != 2 or len(blocks) != 2:
+        raise ValueError("x must have a last dimension, packed and scales must be matrices")
+    inner, outs = shape[-1], held[0]
+    if inner == 0 or inner % BLOCK_SIZE != 0:
+        raise ValueError(f"Last dim {inner} not divisible by BLOCK_SIZE={BLOCK_SIZE}")
+    if held[1] != inner // 2 or blocks[0] != outs or blocks[1] != inner // BLOCK_SIZE:
+        raise ValueError(f"packed {tuple(held)} and scales {tuple(blocks)} do not hold [out, {inner}] weights")
+    if packed.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError("packed and scales must be uint8")
+    dtype, device = x.dtype, x.device
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f"x must be bfloat16 or float16, got {dtype}")
+    if device.type != "cuda":
+        raise RuntimeError(f"mxwave_b200 runs on CUDA devices only; x is on {device} (no CPU fallback)")
+    if bias is not None and (bias.shape != (outs,) or bias.dtype != dtype):
+        raise ValueError(f"bias must be a {dtype} tensor of shape {(outs,)}, got {bias.dtype} {tuple(bias.shape)}")
+    if residual is not None and (residual.shape != (*shape[:-1], outs) or residual.dtype != dtype):
+        raise ValueError(f"residual must be a {dtype} tensor of shape {(*shape[:-1], outs)}, got {residual.dtype} {tuple(residual.shape)}")
+    for t in (packed, scales, bias, residual):
+        if t is not None and t.device != device:
+            raise ValueError(f"x is on {device}, another argument is on {t.device}")
+    if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad or residual is not None and residual.requires_grad):
+        raise RuntimeError("linear_mxfp4 has no gradient: call it under torch.no_grad()")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
     """`t` as a matrix whose rows are contiguous and do not overlap."""
-    m = t if t.ndim == 2 else t.reshape(-1, width)
-    if width > 1 and m.stride(1) != 1 or m.shape[0] > 1 and m.stride(0) < width:
+    m = t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
+    if m.is_contiguous():
+        return m
+    rows, width = m.shape
+    if width > 1 and m.stride(1) != 1 or rows > 1 and m.stride(0) < width:
         m = m.contiguous()
     return m
 

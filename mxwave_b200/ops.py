@@ -263,33 +263,26 @@ def plain_eager(t: Tensor) -> bool:
     return type(t) is Tensor and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
 
 
-class _on_device:
-    """``torch.cuda.device(d)`` that does nothing when `d` is current already."""
-
-    __slots__ = ("index", "previous")
-
-    def __init__(self, device: torch.device) -> None:
-        self.index = device.index
-
-    def __enter__(self) -> None:
-        self.previous = torch._C._cuda_getDevice()
-        if self.previous != self.index:
-            torch._C._cuda_setDevice(self.index)
-
-    def __exit__(self, *exc: object) -> None:
-        if self.previous != self.index:
-            torch._C._cuda_setDevice(self.previous)
-
-
-def _raw_stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _call(fn, index: int, args: tuple, what: str) -> None:
+    """One call of the C ABI on device `index`, with its current stream as the last argument."""
+    current = torch._C._cuda_getDevice()
+    if current == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        torch._C._cuda_setDevice(index)
+        try:
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        finally:
+            torch._C._cuda_setDevice(current)
+    if status != _lib.MXW_OK:
+        _lib.check(status, what)
 
 
 def _linear_mxfp4(x: Tensor, packed: Tensor, scales: Tensor, bias: Tensor | None, residual: Tensor | None,
                   act: int) -> Tensor:
     rows, inner = x.shape
     outs = packed.shape[0]
-    y = torch.empty((rows, outs), dtype=x.dtype, device=x.device)
+    y = x.new_empty((rows, outs))
     if rows == 0 or outs == 0:
         return y
     if packed.data_ptr() % 16 != 0:  # a slice that starts inside a 16-byte line
@@ -297,14 +290,13 @@ def _linear_mxfp4(x: Tensor, packed: Tensor, scales: Tensor, bias: Tensor | None
     lib = _lib.load()
     code = _DTYPE_CODES[x.dtype]
     nbytes = lib.mxw_linear_workspace_size(rows, inner, code)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    with _on_device(x.device):
-        status = lib.mxw_linear_mxfp4(
-            x.data_ptr(), code, rows, inner, x.stride(0) if rows > 1 else inner, packed.data_ptr(), scales.data_ptr(),
-            outs, _ptr(bias), act, _ptr(residual), residual.stride(0) if residual is not None and rows > 1 else outs,
-            y.data_ptr(), workspace.data_ptr(), nbytes, None, _raw_stream(x.device),
-        )
-    _lib.check(status, "mxw_linear_mxfp4")
+    # Up to 16 rows the kernel needs none: any address will do.
+    workspace = packed if nbytes <= 16 else packed.new_empty(nbytes)
+    _call(lib.mxw_linear_mxfp4, x.device.index, (
+        x.data_ptr(), code, rows, inner, x.stride(0) if rows > 1 else inner, packed.data_ptr(), scales.data_ptr(), outs,
+        None if bias is None else bias.data_ptr(), act, None if residual is None else residual.data_ptr(),
+        residual.stride(0) if residual is not None and rows > 1 else outs, y.data_ptr(), workspace.data_ptr(), nbytes, None,
+    ), "mxw_linear_mxfp4")
     return y
 
 
@@ -317,18 +309,16 @@ def _(x, packed, scales, bias, residual, act):
 
 
 def _kv_append_mxfp4_(codes: Tensor, scales: Tensor, key: Tensor, value: Tensor, slots: Tensor) -> None:
-    tokens = key.shape[0]
-    if tokens == 0 or codes.shape[0] == 0:
-        return
-    lib = _lib.load()
     pages, _two, heads, page, half = codes.shape
-    with _on_device(codes.device):
-        status = lib.mxw_kv_append(
-            codes.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, key.data_ptr(), value.data_ptr(),
-            _DTYPE_CODES[key.dtype], key.stride(0), key.stride(1), value.stride(0), value.stride(1), slots.data_ptr(),
-            tokens, _raw_stream(codes.device),
-        )
-    _lib.check(status, "mxw_kv_append")
+    tokens = slots.shape[0]
+    if tokens == 0 or pages == 0:
+        return
+    key_token, key_head, _one = key.stride()
+    value_token, value_head, _one = value.stride()
+    _call(_lib.load().mxw_kv_append, codes.device.index, (
+        codes.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, key.data_ptr(), value.data_ptr(), _DTYPE_CODES[key.dtype],
+        key_token, key_head, value_token, value_head, slots.data_ptr(), tokens,
+    ), "mxw_kv_append")
 
 
 kv_append_mxfp4_ = torch.library.custom_op("mxwave_b200::kv_append_mxfp4_", _kv_append_mxfp4_,
@@ -343,16 +333,14 @@ def _(codes, scales, key, value, slots):
 def _kv_gather_mxfp4(codes: Tensor, scales: Tensor, slots: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
     pages, _two, heads, page, half = codes.shape
     tokens = slots.shape[0]
-    key = torch.empty((tokens, heads, 2 * half), dtype=dtype, device=codes.device)
+    key = codes.new_empty((tokens, heads, 2 * half), dtype=dtype)
     value = torch.empty_like(key)
     if tokens == 0:
         return key, value
-    lib = _lib.load()
-    with _on_device(codes.device):
-        status = lib.mxw_kv_gather(codes.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, slots.data_ptr(),
-                                   tokens, _DTYPE_CODES[dtype], key.data_ptr(), value.data_ptr(),
-                                   _raw_stream(codes.device))
-    _lib.check(status, "mxw_kv_gather")
+    _call(_lib.load().mxw_kv_gather, codes.device.index, (
+        codes.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, slots.data_ptr(), tokens, _DTYPE_CODES[dtype], key.data_ptr(),
+        value.data_ptr(),
+    ), "mxw_kv_gather")
     return key, value
 
 
@@ -366,16 +354,14 @@ def _(codes, scales, slots, dtype):
 
 
 def _copy_pages_(codes: Tensor, scales: Tensor, source: Tensor, target: Tensor) -> None:
-    layers, pages = codes.shape[:2]
+    layers, pages, two, heads, page, half = codes.shape
     n = source.shape[0]
     if n == 0 or layers == 0:
         return
-    lib = _lib.load()
-    with _on_device(codes.device):
-        status = lib.mxw_copy_pages(codes.data_ptr(), scales.data_ptr(), layers, pages, codes[0, 0].numel(),
-                                    scales[0, 0].numel(), source.data_ptr(), target.data_ptr(), n,
-                                    _raw_stream(codes.device))
-    _lib.check(status, "mxw_copy_pages")
+    rows = two * heads * page
+    _call(_lib.load().mxw_copy_pages, codes.device.index, (
+        codes.data_ptr(), scales.data_ptr(), layers, pages, rows * half, rows * scales.shape[5], source.data_ptr(), target.data_ptr(), n,
+    ), "mxw_copy_pages")
 
 
 copy_pages_ = torch.library.custom_op("mxwave_b200::copy_pages_", _copy_pages_, mutates_args=("codes", "scales"))
@@ -386,41 +372,47 @@ def _(codes, scales, source, target):
     return None
 
 
-def _paged_attention_mxfp4(query: Tensor, codes: Tensor, scales: Tensor, table: Tensor, lengths: Tensor,
-                           query_start: Tensor, max_length: int, max_queries: int, softmax_scale: float, causal: bool,
-                           window: int, want_lse: bool) -> tuple[Tensor, Tensor]:
+def _paged_attention_mxfp4(query: Tensor, codes: Tensor, scales: Tensor, table: Tensor, lengths: Tensor, query_start: Tensor,
+                           max_length: int, max_queries: int, softmax_scale: float, causal: bool, window: int,
+                           lse: Tensor | None) -> Tensor:
     tokens, heads, dim = query.shape
     pages, _two, kv_heads, page, _half = codes.shape
     seqs, width = table.shape
-    lse = torch.empty((tokens, heads) if want_lse else (0,), dtype=torch.float32, device=query.device)
     if tokens == 0 or seqs == 0 or max_queries == 0:
-        return torch.zeros((tokens, heads, dim), dtype=query.dtype, device=query.device), lse.fill_(float("-inf"))
-    out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=query.device)
+        if lse is not None:
+            lse.fill_(float("-inf"))
+        return query.new_zeros((tokens, heads, dim))
+    out = query.new_empty((tokens, heads, dim))
     lib = _lib.load()
-    with _on_device(query.device):
-        nbytes = lib.mxw_paged_attention_workspace_size(seqs, heads, kv_heads, dim, max_length, max_queries)
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
-        status = lib.mxw_paged_attention(
-            query.data_ptr(), _DTYPE_CODES[query.dtype], tokens, heads, query.stride(0), query.stride(1),
-            codes.data_ptr(), scales.data_ptr(), pages, kv_heads, page, dim, table.data_ptr(), table.stride(0), width,
-            lengths.data_ptr(), query_start.data_ptr(), seqs, max_length, max_queries, softmax_scale, causal, window,
-            out.data_ptr(), lse.data_ptr() if want_lse else None, workspace.data_ptr(), nbytes,
-            None, _raw_stream(query.device),
-        )
-    _lib.check(status, "mxw_paged_attention")
+    nbytes = lib.mxw_paged_attention_workspace_size(seqs, heads, kv_heads, dim, max_length, max_queries)
+    workspace = codes if nbytes <= 16 else codes.new_empty(nbytes)  # (prompts need none: any address will do)
+    q_token, q_head, _one = query.stride()
+    _call(lib.mxw_paged_attention, query.device.index, (
+        query.data_ptr(), _DTYPE_CODES[query.dtype], tokens, heads, q_token, q_head, codes.data_ptr(), scales.data_ptr(), pages, kv_heads,
+        page, dim, table.data_ptr(), table.stride(0), width, lengths.data_ptr(), query_start.data_ptr(), seqs, max_length, max_queries,
+        softmax_scale, causal, window, out.data_ptr(), None if lse is None else lse.data_ptr(), workspace.data_ptr(), nbytes, None,
+    ), "mxw_paged_attention")
+    return out
+
+
+def _new_lse(query: Tensor, want: bool) -> Tensor:
+    return query.new_empty(query.shape[:2] if want else (0,), dtype=torch.float32)
+
+
+@torch.library.custom_op("mxwave_b200::paged_attention_mxfp4", mutates_args=())
+def paged_attention_mxfp4(query: Tensor, codes: Tensor, scales: Tensor, table: Tensor, lengths: Tensor, query_start: Tensor,
+                          max_length: int, max_queries: int, softmax_scale: float, causal: bool, window: int,
+                          want_lse: bool) -> tuple[Tensor, Tensor]:
+    lse = _new_lse(query, want_lse)
+    out = _paged_attention_mxfp4(query, codes, scales, table, lengths, query_start, max_length, max_queries, softmax_scale, causal, window,
+                                 lse if want_lse else None)
     return out, lse
-
-
-paged_attention_mxfp4 = torch.library.custom_op("mxwave_b200::paged_attention_mxfp4", _paged_attention_mxfp4,
-                                                mutates_args=())
 
 
 @paged_attention_mxfp4.register_fake
 def _(query, codes, scales, table, lengths, query_start, max_length, max_queries, softmax_scale, causal, window,
       want_lse):
-    tokens, heads, _dim = query.shape
-    return (query.new_empty(query.shape),
-            query.new_empty((tokens, heads) if want_lse else (0,), dtype=torch.float32))
+    return query.new_empty(query.shape), _new_lse(query, want_lse)
 
 
 OPS = (
