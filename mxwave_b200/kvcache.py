@@ -64,6 +64,8 @@ def append_mxfp4_(codes: torch.Tensor, scales: torch.Tensor, key: torch.Tensor, 
     projection need no copy).  slots: int64 [tokens], distinct; a slot outside
     the pool (-1) skips its row.  Nothing but the named rows is written.
     """
+    if ops.binding is not None and not torch.compiler.is_compiling() and ops.binding.append(codes, scales, key, value, slots):
+        return
     _check_pool(codes, scales)
     heads, dim = codes.shape[2], 2 * codes.shape[4]
     if key.ndim != 3 or key.shape[1:] != (heads, dim) or value.shape != key.shape:
@@ -78,6 +80,7 @@ def append_mxfp4_(codes: torch.Tensor, scales: torch.Tensor, key: torch.Tensor, 
     args = (codes, scales, _unit_rows(key.detach()), _unit_rows(value.detach()), slots.contiguous())
     if ops.plain_eager(codes):
         ops._kv_append_mxfp4_(*args)
+        _written(codes, scales)
     else:
         torch.ops.mxwave_b200.kv_append_mxfp4_(*args)
 
@@ -90,6 +93,10 @@ def gather_mxfp4(
     bf16 and fp32 hold every MXFP4 value exactly; f16 rounds.  A slot outside
     the pool gives zeros.
     """
+    if ops.binding is not None and not torch.compiler.is_compiling():
+        rows = ops.binding.gather(codes, scales, slots, dtype)
+        if rows is not None:
+            return rows
     _check_pool(codes, scales)
     if dtype not in _ROW_TYPES:
         raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
@@ -107,6 +114,8 @@ def copy_pages_(
     the call.  No target may also be a source or appear twice: the copies of
     one call run in no order.
     """
+    if ops.binding is not None and not torch.compiler.is_compiling() and ops.binding.copy_pages(codes, scales, source, target):
+        return
     _check_pool(codes, scales, layers=True)
     if not isinstance(source, torch.Tensor):
         source = torch.tensor(source, dtype=torch.int64)
@@ -122,6 +131,7 @@ def copy_pages_(
     args = (codes, scales, source.contiguous(), target.contiguous())
     if ops.plain_eager(codes):
         ops._copy_pages_(*args)
+        _written(codes, scales)
     else:
         torch.ops.mxwave_b200.copy_pages_(*args)
 
@@ -158,6 +168,11 @@ def paged_attention_mxfp4(
     reaches, and a row of `query` behind the last sequence, gives zeros (and
     -inf).  Equal calls give equal bits.  There is no gradient.
     """
+    if ops.binding is not None and not torch.compiler.is_compiling():
+        got = ops.binding.attention(query, codes, scales, table, lengths, query_start, max_length, max_queries, softmax_scale, causal, window,
+                                    return_lse)
+        if got is not None:
+            return got
     _check_pool(codes, scales)
     kv_heads, dim = codes.shape[2], 2 * codes.shape[4]
     if query.ndim != 3 or query.shape[2] != dim or query.shape[1] == 0 or query.shape[1] % kv_heads != 0:
@@ -191,6 +206,13 @@ def paged_attention_mxfp4(
     else:
         out, lse = torch.ops.mxwave_b200.paged_attention_mxfp4(*args, bool(return_lse))
     return (out, lse) if return_lse else out
+
+
+def _written(*tensors: torch.Tensor) -> None:
+    """What an in-place operator does to its tensors' version counters (inference tensors have none)."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:

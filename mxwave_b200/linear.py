@@ -43,6 +43,10 @@ def linear_mxfp4(
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"Unknown activation: {activation}")
+    if ops.binding is not None and not torch.compiler.is_compiling():
+        y = ops.binding.linear(x, packed, scales, bias, residual, act)
+        if y is not None:
+            return y
     _check(x, packed, scales, bias, residual)
     outs = packed.shape[0]
     args = (_rows(x), packed.contiguous(), scales.contiguous(), None if bias is None else bias.contiguous(),

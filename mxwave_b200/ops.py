@@ -38,10 +38,11 @@ and ``mxwave_b200.kvcache`` hold their public functions and argument checks):
   max_length, max_queries, softmax_scale, causal, window, want_lse) -> (out,
   lse)``; lse is empty unless wanted.
 
-These have an implementation function of the same name with a leading
-underscore, which the public functions call directly for plain eager CUDA
-tensors: dispatching a custom operator costs more host time than their
-smallest calls take on the device.
+Dispatching a custom operator costs more host time than their smallest calls
+take on the device, so the public functions have two shorter ways for eager
+calls on plain CUDA tensors: ``binding`` (csrc/binding.cpp) takes the ordinary
+ones whole, and the functions here with a leading underscore, which the
+operators wrap, take the rest.
 """
 
 from __future__ import annotations
@@ -255,6 +256,11 @@ def _(gram, full, count, damp, mode):
 
 
 # ----------------------------------------------------------------- serving
+
+try:
+    from ._native import _binding as binding  # built with the library; without it calls only take longer
+except ImportError:
+    binding = None
 
 
 def plain_eager(t: Tensor) -> bool:

@@ -23,7 +23,7 @@ import math
 import pytest
 import torch
 
-from mxwave_b200 import kvcache
+from mxwave_b200 import kvcache, ops
 from mxwave_b200.core import dequant_mxfp4, quantize_mxfp4
 from mxwave_b200.linear import linear_mxfp4
 
@@ -498,6 +498,32 @@ def test_opcheck() -> None:
                           (case.query, case.codes, case.scales, case.table, case.lengths, case.start, 20, 1, 0.125, True, 0, True))
     layers = case.codes[None].clone(), case.scales[None].clone()
     torch.library.opcheck(op.copy_pages_.default, (*layers, torch.tensor([0]), torch.tensor([1])))
+
+
+def test_the_two_eager_ways_agree(monkeypatch) -> None:
+    """The host binding and the general path: the same results, the same side effects."""
+    assert ops.binding is not None
+    g = gen(20)
+    packed, scales = quantize_mxfp4(randn(g, 200, 128), method="rtn")
+    case = Case(21, [300, 20], [2, 2], 8, 2, 32, 64, BF)
+    x, bias, residual = randn(g, 5, 128).to(BF), randn(g, 200).to(BF), randn(g, 5, 200).to(BF)
+    rows, slots = randn(g, 4, 2, 64).to(BF), torch.tensor([1, 3, -1, 40], device="cuda")
+    layers = case.codes[None].repeat(2, 1, 1, 1, 1, 1), case.scales[None].repeat(2, 1, 1, 1, 1, 1)
+
+    def run():
+        codes, sc = case.codes.clone(), case.scales.clone()
+        versions = codes._version, sc._version
+        kvcache.append_mxfp4_(codes, sc, rows, rows, slots)
+        assert codes._version > versions[0] and sc._version > versions[1]
+        pair = layers[0].clone(), layers[1].clone()
+        kvcache.copy_pages_(*pair, torch.tensor([0, 2]), torch.tensor([1, 3]))
+        return [linear_mxfp4(x, packed, scales, bias, activation="gelu", residual=residual), linear_mxfp4(x[None], packed, scales), codes, sc, *pair,
+                *kvcache.gather_mxfp4(codes, sc, slots, HF), *case.run(window=50), case.run(return_lse=False)]
+
+    first = run()
+    monkeypatch.setattr(ops, "binding", None)
+    for a, b in zip(first, run()):
+        assert a.shape == b.shape and torch.equal(a, b)
 
 
 def test_captured_steps_replay_with_new_inputs() -> None:
