@@ -49,30 +49,36 @@ __device__ __forceinline__ int64_t kv_row(const KvRows& P, int64_t slot, const K
   return (((page * 2 + p.part) * P.heads + p.head) << P.page_shift) + offset;
 }
 
-template <int DT>
-__device__ __forceinline__ float kv_load(const void* p, int64_t i) {
-  if constexpr (DT == MXW_BF16) return bits_f32(static_cast<uint32_t>(static_cast<const uint16_t*>(p)[i]) << 16);
-  if constexpr (DT == MXW_F16) return __half2float(static_cast<const __half*>(p)[i]);
-  return static_cast<const float*>(p)[i];
-}
-
-// Eight elements of one row; VEC: 16-byte aligned.
+// Eight elements of one row, as they are; VEC: 16-byte aligned.
 template <int DT, bool VEC>
-__device__ __forceinline__ void kv_load8(const void* p, int64_t i, float (&v)[8]) {
-  if constexpr (VEC && DT == MXW_F32) {
-    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else if constexpr (VEC) {
-    uint16_t raw[8];
-    *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+struct KvRaw {
+  static constexpr int kWords = DT == MXW_F32 ? 8 : 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void* p, int64_t i) {
+    if constexpr (VEC) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * (DT == MXW_F32 ? 4 : 2));
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = kv_load<DT>(raw, k);
-  } else {
+      for (int k = 0; k < kWords / 4; ++k) reinterpret_cast<uint4*>(w)[k] = src[k];
+    } else if constexpr (DT == MXW_F32) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = kv_load<DT>(p, i + k);
+      for (int k = 0; k < 8; ++k) w[k] = static_cast<const uint32_t*>(p)[i + k];
+    } else {
+      const uint16_t* src = static_cast<const uint16_t*>(p) + i;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = src[2 * k] | (static_cast<uint32_t>(src[2 * k + 1]) << 16);
+    }
   }
-}
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) w[k] = 0;
+  }
+  __device__ __forceinline__ float value(int k) const {
+    if constexpr (DT == MXW_F32) return bits_f32(w[k]);
+    if constexpr (DT == MXW_BF16) return bits_f32((k & 1) ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+    const uint16_t h = static_cast<uint16_t>((k & 1) ? w[k / 2] >> 16 : w[k / 2]);
+    return __half2float(*reinterpret_cast<const __half*>(&h));
+  }
+};
 
 struct KvSource {
   const void *key, *value;
@@ -81,56 +87,71 @@ struct KvSource {
 
 // Eight elements per thread, a block of 32 per four neighbours: the largest
 // magnitude over two shuffles, one 4-byte store of codes each, and the first
-// of them stores the scale.
-template <int DT, bool VEC>
+// of them stores the scale.  TOK tokens per thread, loads first: with one, a
+// block's life is one chain of dependent loads and HBM waits (append of 16,384
+// tokens of 8 heads: 39 us with one, see kKvAhead).
+template <int DT, bool VEC, int TOK>
 __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvRows P, const KvSource S) {
-  const int sub = static_cast<int>(threadIdx.x) / P.units;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * P.per_block + sub;
-  const int first = P.per_block == 1 ? static_cast<int>(threadIdx.x) : static_cast<int>(threadIdx.x) - sub * P.units;
-  const bool mine = (P.per_block == 1 || sub < P.per_block) && token < P.tokens;
-  const int64_t slot = mine ? P.slots[P.per_block == 1 ? blockIdx.x : token] : -1;
-  const bool kept = slot >= 0 && slot < P.n_slots;
+  const int sub = P.per_block == 1 ? 0 : static_cast<int>(threadIdx.x) / P.units;
+  const int first = static_cast<int>(threadIdx.x) - sub * P.units;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * P.per_block * TOK + sub;
   // The loop count is the block's, so that the shuffles see whole warps.
   for (int r0 = 0; r0 < P.units; r0 += P.per_block == 1 ? kKvThreads : P.units) {
     const int r = first + r0;
-    const bool on = kept && r < P.units;
+    const bool on = sub < P.per_block && r < P.units;
     const KvPiece p = kv_piece(P, on ? r : 0);
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (on) {
-      const int64_t at = p.part ? token * S.value_token + p.head * S.value_head + p.d
-                                : token * S.key_token + p.head * S.key_head + p.d;
-      kv_load8<DT, VEC>(p.part ? S.value : S.key, at, v);
-    }
-    uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
+    const void* src = p.part ? S.value : S.key;
+    const int64_t step = p.part ? S.value_token : S.key_token;
+    const int64_t at = p.head * (p.part ? S.value_head : S.key_head) + p.d;
+    KvRaw<DT, VEC> raw[TOK];
+    int64_t slot[TOK];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) amax = max(amax, f32_bits(v[k]) & 0x7fffffffu);
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // Exponent of the block (the quantizer's rtn rule, its non-finite cases
-    // included: -127 for a NaN or zero maximum, 127 for an infinite one).
-    int e;
-    if (amax > 0x7f800000u || amax == 0u) {
-      e = -127;
-    } else if (amax == 0x7f800000u) {
-      e = 127;
-    } else {
-      const uint32_t safe = max(amax, 0x00800000u);
-      e = static_cast<int>(safe >> 23) - 129 + ((safe & 0x7fffffu) >= 0x600000u ? 1 : 0);
-      e = max(e, -127);
+    for (int k = 0; k < TOK; ++k) {
+      const int64_t token = token0 + static_cast<int64_t>(k) * P.per_block;
+      const bool in = on && token < P.tokens;
+      slot[k] = in ? P.slots[token] : -1;
+      if (in)
+        raw[k].load(src, token * step + at);
+      else
+        raw[k].clear();
     }
-    if (on) {
-      const float inv = exp2i(-e);
-      uint32_t word = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a = __fadd_rn(__fmul_rn(v[2 * k], inv), 0.0f), b = __fadd_rn(__fmul_rn(v[2 * k + 1], inv), 0.0f);
-        if (a != a) a = 6.0f;  // a NaN takes the last code, without a sign
-        if (b != b) b = 6.0f;
-        word |= e2m1x2(a, b) << (8 * k);
+    for (int k = 0; k < TOK; ++k) {
+      float v[8];
+      uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = raw[k].value(i);
+        amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
       }
-      const int64_t row = kv_row(P, slot, p);
-      *reinterpret_cast<uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2) = word;
-      if ((r & 3) == 0) P.scales[row * (P.dim / 32) + p.d / 32] = static_cast<uint8_t>(e + 127);
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      // Exponent of the block (the quantizer's rtn rule, its non-finite cases
+      // included: -127 for a NaN or zero maximum, 127 for an infinite one).
+      int e;
+      if (amax > 0x7f800000u || amax == 0u) {
+        e = -127;
+      } else if (amax == 0x7f800000u) {
+        e = 127;
+      } else {
+        const uint32_t safe = max(amax, 0x00800000u);
+        e = static_cast<int>(safe >> 23) - 129 + ((safe & 0x7fffffu) >= 0x600000u ? 1 : 0);
+        e = max(e, -127);
+      }
+      if (slot[k] >= 0 && slot[k] < P.n_slots) {
+        const float inv = exp2i(-e);
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float a = __fadd_rn(__fmul_rn(v[2 * i], inv), 0.0f), b = __fadd_rn(__fmul_rn(v[2 * i + 1], inv), 0.0f);
+          if (a != a) a = 6.0f;  // a NaN takes the last code, without a sign
+          if (b != b) b = 6.0f;
+          word |= e2m1x2(a, b) << (8 * i);
+        }
+        const int64_t row = kv_row(P, slot[k], p);
+        *reinterpret_cast<uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2) = word;
+        if ((r & 3) == 0) P.scales[row * (P.dim / 32) + p.d / 32] = static_cast<uint8_t>(e + 127);
+      }
     }
   }
 }
@@ -154,29 +175,44 @@ __device__ __forceinline__ void kv_store8(__half* p, const float (&v)[8]) {
 
 // Rows read back as values, [tokens][heads][dim] each; zeros for a slot that
 // lies outside the pool.
-template <typename OUT>
+template <typename OUT, int TOK>
 __global__ void __launch_bounds__(kKvThreads) kv_gather_kernel(const KvRows P, OUT* key, OUT* value) {
-  const int sub = static_cast<int>(threadIdx.x) / P.units;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * P.per_block + (P.per_block == 1 ? 0 : sub);
-  if (token >= P.tokens || (P.per_block > 1 && sub >= P.per_block)) return;
-  const int64_t slot = P.slots[token];
-  const bool kept = slot >= 0 && slot < P.n_slots;
-  const int first = static_cast<int>(threadIdx.x) - (P.per_block == 1 ? 0 : sub * P.units);
-  for (int r = first; r < P.units; r += P.per_block == 1 ? kKvThreads : P.units) {
-    const KvPiece p = kv_piece(P, r);
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    if (kept) {
-      const int64_t row = kv_row(P, slot, p);
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2);
-      const float sc = exp2i(static_cast<int>(P.scales[row * (P.dim / 32) + p.d / 32]) - 127);
+  const int sub = P.per_block == 1 ? 0 : static_cast<int>(threadIdx.x) / P.units;
+  if (sub >= P.per_block) return;
+  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * P.per_block * TOK + sub;
+  int64_t slot[TOK];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f2 q = unpack2(e2m1x2_to_f32x2((word >> (8 * k)) & 0xffu));
-        v[2 * k] = __fmul_rn(q.x, sc);
-        v[2 * k + 1] = __fmul_rn(q.y, sc);
+  for (int k = 0; k < TOK; ++k) {
+    const int64_t token = token0 + static_cast<int64_t>(k) * P.per_block;
+    slot[k] = token < P.tokens ? P.slots[token] : -1;
+    if (slot[k] >= P.n_slots) slot[k] = -1;
+  }
+  for (int r = static_cast<int>(threadIdx.x) - sub * P.units; r < P.units; r += P.per_block == 1 ? kKvThreads : P.units) {
+    const KvPiece p = kv_piece(P, r);
+    uint32_t word[TOK], byte[TOK];
+#pragma unroll
+    for (int k = 0; k < TOK; ++k) {
+      word[k] = byte[k] = 0;  // reads as zeros
+      if (slot[k] >= 0) {
+        const int64_t row = kv_row(P, slot[k], p);
+        word[k] = *reinterpret_cast<const uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2);
+        byte[k] = P.scales[row * (P.dim / 32) + p.d / 32];
       }
     }
-    kv_store8((p.part ? value : key) + (token * P.heads + p.head) * P.dim + p.d, v);
+#pragma unroll
+    for (int k = 0; k < TOK; ++k) {
+      const int64_t token = token0 + static_cast<int64_t>(k) * P.per_block;
+      if (token >= P.tokens) break;
+      const float sc = exp2i(static_cast<int>(byte[k]) - 127);
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f2 q = unpack2(e2m1x2_to_f32x2((word[k] >> (8 * i)) & 0xffu));
+        v[2 * i] = __fmul_rn(q.x, sc);
+        v[2 * i + 1] = __fmul_rn(q.y, sc);
+      }
+      kv_store8((p.part ? value : key) + (token * P.heads + p.head) * P.dim + p.d, v);
+    }
   }
 }
 
@@ -269,13 +305,39 @@ static KvRows kv_rows(uint8_t* codes, uint8_t* scales, const int64_t* slots, int
   return P;
 }
 
+// Tokens per thread: kKvAhead once every SM has a few blocks of them, one below.
+constexpr int kKvAhead = 4;
+static int kv_tokens_per_thread(const KvRows& P) {
+  return P.tokens >= static_cast<int64_t>(P.per_block) * kKvAhead * num_sms() * 4 ? kKvAhead : 1;
+}
+static unsigned kv_grid(const KvRows& P, int tok) {
+  const int64_t each = static_cast<int64_t>(P.per_block) * tok;
+  return static_cast<unsigned>((P.tokens + each - 1) / each);
+}
+
+template <int DT, bool VEC>
+static void launch_append(const KvRows& P, const KvSource& S, cudaStream_t s) {
+  const int tok = kv_tokens_per_thread(P);
+  if (tok == 1)
+    kv_append_kernel<DT, VEC, 1><<<kv_grid(P, tok), kKvThreads, 0, s>>>(P, S);
+  else
+    kv_append_kernel<DT, VEC, kKvAhead><<<kv_grid(P, tok), kKvThreads, 0, s>>>(P, S);
+}
 template <int DT>
 static void launch_append(const KvRows& P, const KvSource& S, bool vec, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((P.tokens + P.per_block - 1) / P.per_block);
   if (vec)
-    kv_append_kernel<DT, true><<<grid, kKvThreads, 0, s>>>(P, S);
+    launch_append<DT, true>(P, S, s);
   else
-    kv_append_kernel<DT, false><<<grid, kKvThreads, 0, s>>>(P, S);
+    launch_append<DT, false>(P, S, s);
+}
+
+template <typename OUT>
+static void launch_gather(const KvRows& P, void* key, void* value, cudaStream_t s) {
+  const int tok = kv_tokens_per_thread(P);
+  if (tok == 1)
+    kv_gather_kernel<OUT, 1><<<kv_grid(P, tok), kKvThreads, 0, s>>>(P, static_cast<OUT*>(key), static_cast<OUT*>(value));
+  else
+    kv_gather_kernel<OUT, kKvAhead><<<kv_grid(P, tok), kKvThreads, 0, s>>>(P, static_cast<OUT*>(key), static_cast<OUT*>(value));
 }
 
 }  // namespace mxw
@@ -320,14 +382,13 @@ extern "C" int mxw_kv_gather(const uint8_t* codes, const uint8_t* scales, int64_
   if (tokens > 0x7fffffff) return MXW_EUNSUPPORTED;
   const KvRows P = kv_rows(const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales), slots, tokens, pages, heads,
                            page_tokens, dim);
-  const unsigned grid = static_cast<unsigned>((tokens + P.per_block - 1) / P.per_block);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == MXW_BF16)
-    kv_gather_kernel<<<grid, kKvThreads, 0, s>>>(P, static_cast<__nv_bfloat16*>(key), static_cast<__nv_bfloat16*>(value));
+    launch_gather<__nv_bfloat16>(P, key, value, s);
   else if (dtype == MXW_F16)
-    kv_gather_kernel<<<grid, kKvThreads, 0, s>>>(P, static_cast<__half*>(key), static_cast<__half*>(value));
+    launch_gather<__half>(P, key, value, s);
   else
-    kv_gather_kernel<<<grid, kKvThreads, 0, s>>>(P, static_cast<float*>(key), static_cast<float*>(value));
+    launch_gather<float>(P, key, value, s);
   return check_launch();
 }
 
