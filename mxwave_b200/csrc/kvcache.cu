@@ -15,6 +15,7 @@
 #include <cuda_fp16.h>
 #include <stdlib.h>
 
+#include "attention.cuh"
 #include "common.cuh"
 #include "runtime.h"
 
@@ -30,6 +31,7 @@ struct KvRows {
   int heads, dim, page_shift;
   int units;      // eight-element pieces of a token: 2 heads dim / 8
   int per_block;  // tokens per block
+  float zero, negzero;  // 0 and -0 that the compiler does not know (mul2_rounded)
 };
 
 // Where piece `r` of a token lies: part (0 key, 1 value), head, first element.
@@ -72,11 +74,30 @@ struct KvRaw {
 #pragma unroll
     for (int k = 0; k < kWords; ++k) w[k] = 0;
   }
-  __device__ __forceinline__ float value(int k) const {
-    if constexpr (DT == MXW_F32) return bits_f32(w[k]);
-    if constexpr (DT == MXW_BF16) return bits_f32((k & 1) ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
-    const uint16_t h = static_cast<uint16_t>((k & 1) ? w[k / 2] >> 16 : w[k / 2]);
-    return __half2float(*reinterpret_cast<const __half*>(&h));
+  // Elements 2k and 2k + 1.
+  __device__ __forceinline__ f2 pair(int k) const {
+    if constexpr (DT == MXW_F32) return {bits_f32(w[2 * k]), bits_f32(w[2 * k + 1])};
+    if constexpr (DT == MXW_BF16) return {bits_f32(w[k] << 16), bits_f32(w[k] & 0xffff0000u)};
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+    return {f.x, f.y};
+  }
+  // The largest magnitude as bits of the type: ordered, NaN above infinity.
+  __device__ __forceinline__ uint32_t largest() const {
+    if constexpr (DT == MXW_F32) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = max(m, w[k] & 0x7fffffffu);
+      return m;
+    }
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+  }
+  // And those bits as fp32 bits.
+  static __device__ __forceinline__ uint32_t to_f32_bits(uint32_t m) {
+    if constexpr (DT == MXW_F32) return m;
+    if constexpr (DT == MXW_BF16) return m << 16;
+    const uint16_t h = static_cast<uint16_t>(m);
+    return f32_bits(__half2float(*reinterpret_cast<const __half*>(&h)));
   }
 };
 
@@ -117,15 +138,10 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvRows P, c
     }
 #pragma unroll
     for (int k = 0; k < TOK; ++k) {
-      float v[8];
-      uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = raw[k].value(i);
-        amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
-      }
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      uint32_t top = raw[k].largest();
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t amax = KvRaw<DT, VEC>::to_f32_bits(top);
       // Exponent of the block (the quantizer's rtn rule, its non-finite cases
       // included: -127 for a NaN or zero maximum, 127 for an infinite one).
       int e;
@@ -140,14 +156,19 @@ __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvRows P, c
       }
       if (slot[k] >= 0 && slot[k] < P.n_slots) {
         const float inv = exp2i(-e);
-        uint32_t word = 0;
+        const unsigned long long inv2 = pack2(inv, inv), nz2 = pack2(P.negzero, P.negzero), z2 = pack2(P.zero, P.zero);
+        uint32_t bytes[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float a = __fadd_rn(__fmul_rn(v[2 * i], inv), 0.0f), b = __fadd_rn(__fmul_rn(v[2 * i + 1], inv), 0.0f);
-          if (a != a) a = 6.0f;  // a NaN takes the last code, without a sign
-          if (b != b) b = 6.0f;
-          word |= e2m1x2(a, b) << (8 * i);
+          const f2 v = raw[k].pair(i);
+          f2 x = unpack2(add2(mul2_rounded(pack2(v.x, v.y), inv2, nz2), z2));  // -0 + 0 = 0: code 0
+          if (amax > 0x7f800000u) {  // a NaN takes the last code, without a sign
+            if (x.x != x.x) x.x = 6.0f;
+            if (x.y != x.y) x.y = 6.0f;
+          }
+          bytes[i] = e2m1x2(x.x, x.y);
         }
+        const uint32_t word = __byte_perm(__byte_perm(bytes[0], bytes[1], 0x0040), __byte_perm(bytes[2], bytes[3], 0x0040), 0x5410);
         const int64_t row = kv_row(P, slot[k], p);
         *reinterpret_cast<uint32_t*>(P.codes + row * (P.dim / 2) + p.d / 2) = word;
         if ((r & 3) == 0) P.scales[row * (P.dim / 32) + p.d / 32] = static_cast<uint8_t>(e + 127);
@@ -204,10 +225,12 @@ __global__ void __launch_bounds__(kKvThreads) kv_gather_kernel(const KvRows P, O
       const int64_t token = token0 + static_cast<int64_t>(k) * P.per_block;
       if (token >= P.tokens) break;
       const float sc = exp2i(static_cast<int>(byte[k]) - 127);
+      uint32_t h[4];
+      e2m1x8_to_f16x2(word[k], h);
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f2 q = unpack2(e2m1x2_to_f32x2((word[k] >> (8 * i)) & 0xffu));
+        const float2 q = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
         v[2 * i] = __fmul_rn(q.x, sc);
         v[2 * i + 1] = __fmul_rn(q.y, sc);
       }
@@ -302,6 +325,8 @@ static KvRows kv_rows(uint8_t* codes, uint8_t* scales, const int64_t* slots, int
   P.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   P.units = static_cast<int>(2 * heads * dim / 8);
   P.per_block = std::max(1, kKvThreads / P.units);
+  P.zero = 0.0f;
+  P.negzero = -0.0f;
   return P;
 }
 
