@@ -133,21 +133,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// The same with a zero accumulator.
-__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                              uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
-}
 __device__ __forceinline__ void cp_async16_if(bool on, uint32_t saddr, const void* src, uint32_t src_bytes) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n\t}" ::"r"(saddr),
@@ -187,10 +172,6 @@ __device__ __forceinline__ uint32_t nibbles(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("lop3.b32 %0, %1, %2, %3, 0xCA;" : "=r"(d) : "r"(0x0f0f0f0fu), "r"(a), "r"(b));
   return d;
-}
-// Two scale bytes, as halfwords, to f16 factors 2^(13 - (ref - byte)): zero from ref - byte = 28 on.
-__device__ __forceinline__ uint32_t f16_factors(uint32_t bytes2, uint32_t lift2) {
-  return __vmaxs2(__vadd2(bytes2, lift2), 0u) << 10;
 }
 // 2^(byte - 127) of byte `b` of a word (0 for a zero byte: 2^-127 is nothing next to a score).
 template <int B>

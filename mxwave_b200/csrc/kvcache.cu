@@ -15,8 +15,8 @@
 #include <cuda_fp16.h>
 #include <stdlib.h>
 
-#include "attention.cuh"
 #include "common.cuh"
+#include "f16mma.cuh"
 #include "runtime.h"
 
 namespace mxw {

@@ -93,6 +93,18 @@ def test_linear_matches_64_bits(rows: int, outs: int, inner: int, dtype: torch.d
         check_linear(x, packed, scales, b, act, r, linear_mxfp4(x, packed, scales, b, activation=act, residual=r))
 
 
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 24, 100, 300])
+@pytest.mark.parametrize("outs, inner", [(9472, 5120), (2048, 17408)])
+def test_linear_over_long_rows(rows: int, outs: int, inner: int) -> None:
+    """Rows of many stages, more blocks than SMs, weights not in the caches: every ring of stages wraps while loads are slow."""
+    g = gen(rows)
+    x = randn(g, rows, inner).to(BF)
+    weights = [quantize_mxfp4(randn(g, outs, inner) * 0.02, method="rtn") for _ in range(4)]
+    got = [linear_mxfp4(x, p, s) for p, s in weights]
+    for (p, s), y in zip(weights, got):
+        check_linear(x, p, s, None, "none", None, y)
+
+
 @pytest.mark.parametrize("rows", [3, 40, 300])
 def test_linear_takes_strides_slices_and_leading_dims(rows: int) -> None:
     g = gen(rows)
