@@ -19,8 +19,8 @@
 // what linear_terms_kernel laid out) into a ring; four warps spread the codes
 // into the 16-byte slots that E2M1 operands take in shared memory (8 bytes of
 // codes, 8 of padding) and put the scales into the tensor cores' layout; one
-// thread issues the products.  Up to 16 rows of x the four warps make the
-// terms themselves and there is one launch.  When there are too few tiles for
+// warp issues the products.  Up to four rows of x four more warps make the
+// terms in the same launch.  When there are too few tiles for
 // the SMs the CTAs of a cluster split K and add their fp32 partial tiles over
 // distributed shared memory in rank order, so results do not change from run
 // to run.
@@ -31,7 +31,6 @@
 
 #include "blockscale.cuh"
 #include "common.cuh"
-#include "f16mma.cuh"
 #include "runtime.h"
 #include "terms.cuh"
 
@@ -717,217 +716,43 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   if (threadIdx.x == 0 && *fail && P.flags) atomicOr(P.flags, MXW_FLAG_TIMEOUT);
 }
 
-// ---------------------------------------------------- product of a few rows
-//
-// Up to eight rows of x the time is that of reading W, and the tensor cores'
-// shared-memory operands are in the way: W would pass through shared memory
-// three times (copied, spread, read), which holds it to some 4.5 TB/s.  Here W
-// goes from global memory to registers: lane (g, t) takes 16 bytes (one block of
-// 32 codes) of output row g, so a warp's load covers 64 bytes of eight rows, and
-// the order of the contraction, which is free, is that of the bytes.  The
-// matrix instructions take W as the 16-row operand and x as the 8-column one.
-// Codes times their scale are f16, relative to the largest scale of the row's
-// 128 inputs (times 2^13; zero below 2^-27 of it); x is f16 scaled by a power of
-// two per row and 128 inputs, exact down to 2^-31 of their largest.  The eight
-// warps of a block take 128 inputs in turn and add up at the end, in order.
-
-constexpr int kFewWarps = 8;
-constexpr int kFewRows = 8;
-constexpr int kFewXBytes = 96 * 1024;  // of x in shared memory, as f16
-
-// 16-byte piece p of block b of row r: spread so that eight lanes' reads meet eight different banks.
-__device__ __forceinline__ int few_piece(int r, int b, int p) { return b * 64 + ((p ^ (b & 3) ^ (r & 1)) << 4); }
-
-template <bool BF16, int MT>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) linear_few_kernel(const LinearParams P) {
-  constexpr int PF = MT == 1 ? 4 : 3;  // chunks of W in flight per warp
-  extern __shared__ __align__(16) uint8_t few_smem[];
-  __shared__ float part[kFewWarps][MT * 16 * kFewRows];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int rows = static_cast<int>(P.rows);
-  const int x_row = P.chunks * 256;  // bytes of a row of x in shared memory
-  float* x_scale = reinterpret_cast<float*>(few_smem + rows * x_row);  // [chunk][8]
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (MT * 16);
-  const int blocks = static_cast<int>(P.inner / 32);
-
-  // ---- W: 16 bytes and a scale of each of this lane's rows, some chunks ahead
-  const uint8_t* codes[2 * MT];
-  const uint8_t* scales[2 * MT];
-#pragma unroll
-  for (int m = 0; m < 2 * MT; ++m) {
-    const int64_t n = min(n0 + 8 * m + g, P.outs - 1);  // rows past the last are not stored
-    codes[m] = P.packed + n * (P.inner / 2) + t * 16;
-    scales[m] = P.scales + n * blocks + t;
-  }
-  uint4 w[PF][2 * MT];
-  int ws[PF][2 * MT];
-  auto load = [&](int s, int chunk) {
-    const bool in = chunk * 4 + t < blocks;
-#pragma unroll
-    for (int m = 0; m < 2 * MT; ++m) {
-      w[s][m] = in ? __ldcs(reinterpret_cast<const uint4*>(codes[m] + static_cast<int64_t>(chunk) * 64)) : make_uint4(0, 0, 0, 0);
-      ws[s][m] = in ? scales[m][chunk * 4] : 0;
-    }
-  };
-#pragma unroll
-  for (int s = 0; s < PF; ++s) load(s, warp + s * kFewWarps);
-
-  // ---- x to shared memory as f16: sixteen lanes a row and chunk, eight inputs each
-  {
-    const int part16 = lane & 15;
-    const int units = rows * P.chunks;
-    for (int u = warp * 2 + (lane >> 4); u - (lane >> 4) < units; u += kFewWarps * 2) {
-      const bool on = u < units;
-      const int r = on ? u % rows : 0, c = on ? u / rows : 0;
-      const int k0 = c * kLinK + part16 * 8;
-      const uint4 raw = load_x8(static_cast<const uint16_t*>(P.x) + r * P.ldx + k0, on && k0 < P.inner, P.x_vec);
-      const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-      uint32_t top = __vmaxu2(__vmaxu2(words[0] & 0x7fff7fffu, words[1] & 0x7fff7fffu), __vmaxu2(words[2] & 0x7fff7fffu, words[3] & 0x7fff7fffu));
-      top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      uint32_t h[4];
-      float down = 1.0f;
-      bool finite;
-      if constexpr (BF16) {
-        finite = top < 0x7f80u;
-        // The largest magnitude to [2^14, 2^15).
-        const int e = min(127 + 14 - max(static_cast<int>(top >> 7), 1), 127);
-        const float up = exp2i(e);
-        down = exp2i(-e);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          h[i] = pack_f16x2(__fmul_rn(bits_f32(words[i] << 16), up), __fmul_rn(bits_f32(words[i] & 0xffff0000u), up));
-      } else {
-        finite = top < 0x7c00u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = words[i];
-      }
-      if (on) {
-        uint4 v = make_uint4(h[0], h[1], h[2], h[3]);
-        if (!finite) v = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);  // NaN in every output
-        *reinterpret_cast<uint4*>(few_smem + r * x_row + few_piece(r, c * 4 + (part16 >> 2), part16 & 3)) = v;
-        if (part16 == 0) x_scale[c * kFewRows + r] = down;
-      }
-    }
-    for (int i = threadIdx.x; i < P.chunks * kFewRows; i += kFewWarps * 32)
-      if (i % kFewRows >= rows) x_scale[i] = 0.0f;
-  }
-  __syncthreads();
-
-  // ---- products
-  float total[MT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) total[m][c] = 0.0f;
-  const uint8_t* x = few_smem + g * x_row;
-  const bool live = g < rows;
-  auto multiply = [&](int s, int chunk) {
-    uint4 xv[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p)
-      xv[p] = live ? *reinterpret_cast<const uint4*>(x + few_piece(g, chunk * 4 + t, p)) : make_uint4(0, 0, 0, 0);
-    const float2 down = *reinterpret_cast<const float2*>(x_scale + chunk * kFewRows + 2 * t);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int sa = ws[s][2 * m], sb = ws[s][2 * m + 1];
-      uint32_t top = sa | (sb << 16);  // halfwords: rows g and g + 8
-      const uint32_t own = top;
-      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t f = f16_factors(own, __vsub2(28u * 0x10001u, top));
-      const uint32_t fa = __byte_perm(f, 0u, 0x1010), fb = __byte_perm(f, 0u, 0x3232);
-      const uint32_t wa[4] = {w[s][2 * m].x, w[s][2 * m].y, w[s][2 * m].z, w[s][2 * m].w};
-      const uint32_t wb[4] = {w[s][2 * m + 1].x, w[s][2 * m + 1].y, w[s][2 * m + 1].z, w[s][2 * m + 1].w};
-      float acc[4];
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        // Word p: inputs 8p .. 8p + 7 of this lane's block, piece p of x.
-        uint32_t ha[4], hb[4];
-        e2m1x8_to_f16x2(wa[p], ha);
-        e2m1x8_to_f16x2(wb[p], hb);
-        const uint32_t a0 = hmul2(ha[0], fa), b0 = hmul2(hb[0], fb), a1 = hmul2(ha[1], fa), b1 = hmul2(hb[1], fb);
-        if (p == 0)
-          mma_f16_first(acc, a0, b0, a1, b1, xv[p].x, xv[p].y);
-        else
-          mma_f16(acc, a0, b0, a1, b1, xv[p].x, xv[p].y);
-        mma_f16(acc, hmul2(ha[2], fa), hmul2(hb[2], fb), hmul2(ha[3], fa), hmul2(hb[3], fb), xv[p].z, xv[p].w);
-      }
-      const float ra = exp2i(static_cast<int>(top & 0xffffu) - 140), rb = exp2i(static_cast<int>(top >> 16) - 140);
-      total[m][0] = __fmaf_rn(__fmul_rn(acc[0], down.x), ra, total[m][0]);
-      total[m][1] = __fmaf_rn(__fmul_rn(acc[1], down.y), ra, total[m][1]);
-      total[m][2] = __fmaf_rn(__fmul_rn(acc[2], down.x), rb, total[m][2]);
-      total[m][3] = __fmaf_rn(__fmul_rn(acc[3], down.y), rb, total[m][3]);
-    }
-  };
-  for (int c0 = warp; c0 < P.chunks; c0 += PF * kFewWarps) {
-#pragma unroll
-    for (int s = 0; s < PF; ++s) {
-      const int chunk = c0 + s * kFewWarps;
-      if (chunk < P.chunks) {
-        multiply(s, chunk);
-        load(s, chunk + PF * kFewWarps);
-      }
-    }
-  }
-
-  // ---- the warps' sums in order, and the epilogue
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    // Rows g and g + 8 of the tile, columns 2t and 2t + 1: [column][output].
-    float* dst = &part[warp][m * 16 + g];
-    dst[(2 * t) * MT * 16] = total[m][0];
-    dst[(2 * t + 1) * MT * 16] = total[m][1];
-    dst[(2 * t) * MT * 16 + 8] = total[m][2];
-    dst[(2 * t + 1) * MT * 16 + 8] = total[m][3];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * MT * 16; i += kFewWarps * 32) {
-    const int64_t r = i / (MT * 16), n = n0 + i % (MT * 16);
-    if (n >= P.outs) continue;
-    float v = part[0][i];
-#pragma unroll
-    for (int k = 1; k < kFewWarps; ++k) v = __fadd_rn(v, part[k][i]);
-    if (P.bias) v = __fadd_rn(v, load16<BF16>(P.bias, n));
-    v = activate(v, P.act);
-    if (P.residual) v = __fadd_rn(v, load16<BF16>(P.residual, r * P.ldr + n));
-    store16<BF16>(P.y, r * P.outs + n, v);
-  }
-}
-
 // -------------------------------------------------------------------- host
 
-// Rows of x per tile: the smallest tile that takes them all, so that W is read once.
-static int linear_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Rows of x per tile: the smallest tile that takes them all, so that W is read
+// once.  Up to four rows the terms are made in the product's kernel (tiles of
+// 16), which saves a launch; its four warps do not keep up with more rows
+// (5120 x 5120 bf16 in clusters of four, one launch against two: 11.0 and 11.6
+// us with one row, 11.6 and 11.8 with four, 13.9 and 12.0 with eight, 17.7 and
+// 12.4 with sixteen).
+static int linear_tile(int64_t rows) { return rows <= 4 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+// CTAs of a cluster that split K between them.  An SM's time is that of its
+// CTAs' chunks and of starting them (some 2.3 chunks); two CTAs on an SM hide
+// one another's waits (0.87 of the time).  A cluster lies within a group of 16
+// SMs or a few more, so sizes that leave part of 16 x CTAs per SM empty fit
+// fewer at a time.  One row, 5120 x 5120, split 1 to 8: 18.6, 11.8, 10.0, 11.2,
+// 10.3, 9.9, 14.1, 13.5 us (6 is taken); 17408 x 5120: 20.9, 19.0 (taken), 24.9,
+// 24.6, 27.6, 32.2, 33.1, 36.1 us.
+static int linear_split(int64_t tiles, int chunks, int per_sm) {
+  int best = 1;
+  int64_t best_cost = 0;
+  for (int s = 1; s <= 8 && (s == 1 || 2 * s <= chunks); ++s) {
+    const int64_t group = 16 * per_sm, slots = num_sms() * (group / s * s) / 16;  // per_sm x SMs, less what stays empty
+    const int64_t turns = (tiles * s * per_sm + slots - 1) / slots;               // of one CTA per SM
+    const int64_t weight = turns > 1 && per_sm > 1 ? 87 * turns : 100 * turns;
+    const int64_t cost = weight * (10 * ((chunks + s - 1) / s) + 23);
+    if (s == 1 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
 
 // Whether the wide tiles fill most of the SMs; below that the narrow kernel,
 // whose clusters split K, ends sooner.
 static bool linear_wide(int64_t rows, int64_t outs) {
   return rows > 128 && (rows + 127) / 128 * ((outs + kWideN - 1) / kWideN) >= num_sms() / 2;
-}
-
-// Whether the kernel for a few rows takes the call: x has to fit shared memory.
-static bool linear_few(int64_t rows, int64_t inner) {
-  return rows <= kFewRows && rows * ((inner + kLinK - 1) / kLinK) * (2 * kLinK) <= kFewXBytes;
-}
-
-template <bool BF16, int MT>
-static int launch_few_tiles(const LinearParams& P, cudaStream_t s) {
-  auto kernel = linear_few_kernel<BF16, MT>;
-  static std::atomic<uint64_t> done{0};
-  const int most = kFewXBytes + kFewXBytes / (2 * kLinK) * kFewRows * 4;
-  const int status = set_max_smem_once(reinterpret_cast<const void*>(kernel), most, done);
-  if (status != MXW_OK) return status;
-  const size_t smem = static_cast<size_t>(P.rows * P.chunks * (2 * kLinK)) + static_cast<size_t>(P.chunks) * kFewRows * 4;
-  kernel<<<static_cast<unsigned>((P.outs + MT * 16 - 1) / (MT * 16)), kFewWarps * 32, smem, s>>>(P);
-  return check_launch();
-}
-
-// 32 outputs per block, 16 where that would leave SMs without one.
-template <bool BF16>
-static int launch_few(const LinearParams& P, cudaStream_t s) {
-  return P.outs > 32ll * num_sms() ? launch_few_tiles<BF16, 2>(P, s) : launch_few_tiles<BF16, 1>(P, s);
 }
 
 template <bool BF16, int NT>
@@ -983,8 +808,7 @@ static int launch_linear(const TermsParams& T, const uint8_t* packed, const Line
   status = set_max_smem_once(reinterpret_cast<const void*>(kernel), Tile::kSmem, done);
   if (status != MXW_OK) return status;
   const int64_t row_tiles = (P.outs + kLinM - 1) / kLinM;
-  int split = 1;
-  while (split < 8 && row_tiles * tiles * split * 2 <= 2 * num_sms() && split * 4 <= P.chunks) split *= 2;
+  const int split = linear_split(row_tiles * tiles, P.chunks, NT <= 32 ? 2 : 1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(split), static_cast<unsigned>(row_tiles), static_cast<unsigned>(tiles));
   cfg.blockDim = dim3(Tile::kThreads);
@@ -1003,7 +827,6 @@ static int launch_linear(const TermsParams& T, const uint8_t* packed, const Line
 
 template <bool BF16>
 static int launch_linear_rows(const TermsParams& T, const uint8_t* packed, const LinearParams& P, cudaStream_t s) {
-  if (linear_few(P.rows, P.inner)) return launch_few<BF16>(P, s);
   if (linear_wide(P.rows, P.outs)) return launch_wide<BF16>(T, packed, P, s);
   switch (linear_tile(P.rows)) {
     case 16:
