@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             const uint16_t* src = static_cast<const uint16_t*>(P.query) + static_cast<int64_t>(u.q0 + i) * P.q_token +
                                   static_cast<int64_t>(head * P.group + h) * P.q_head + part * 8;
             const uint4 v = load_x8(src, in, P.q_vec);
-            split_x8<BF16, 128>(v, rr, part, qt, qt + TERMS * Shape::kQTerm, true);
+            split_x8<BF16, 128, PARTS>(v, rr, part, qt, qt + TERMS * Shape::kQTerm, true);
           }
           fence_proxy_async_smem();
           __syncwarp();

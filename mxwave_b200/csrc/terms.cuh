@@ -3,14 +3,19 @@
 // so two terms hold bf16's 8 and three hold f16's 11:
 //   s = 2^(floor(log2 amax) - 7) of the block of 32,  t0 = e4m3(x / s),
 //   t1 = e4m3((x / s - t0) 2^5),  t2 = e4m3(((x / s - t0) 2^5 - t1) 2^5)
-// with scales s, s 2^-5, s 2^-10.  Every remainder is exact in fp32.
+// with scales s, s 2^-5, s 2^-10.  x / s and the remainders are held in f16: below
+// 2^8 their last place is at least as fine as the last term's (2^-14, 2^-19),
+// and f16's own steps (2^-24) only touch inputs under 2^-24 (bf16) or 2^-20
+// (f16) of the block's largest.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
 
 #include "blockscale.cuh"
 #include "common.cuh"
+#include "f16mma.cuh"
 
 namespace mxw {
 
@@ -61,16 +66,15 @@ struct LinearTile {
   static constexpr uint32_t kTmemCols = kCols <= 32 ? 32 : kCols <= 64 ? 64 : kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+__device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t v) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float2 e4m3x2_to_f32x2(uint32_t v) {
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) {
   uint32_t h;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(static_cast<uint16_t>(v)));
-  const __half2 hh = *reinterpret_cast<__half2*>(&h);
-  return make_float2(__low2float(hh), __high2float(hh));
+  return h;
 }
 
 // Eight inputs of a row; zeros outside x.
@@ -83,38 +87,45 @@ __device__ __forceinline__ uint4 load_x8(const uint16_t* src, bool in, bool vec)
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The terms of eight inputs: part `part` (of 16) of row `r` of a tile whose
+// The terms of eight inputs: part `part` (of PARTS) of row `r` of a tile whose
 // image starts at `terms` and whose scales start at `sf`.  Four neighbouring
 // lanes share a block; all lanes of the warp take part in the shuffles.
-template <bool BF16, int NT>
+template <bool BF16, int NT, int PARTS = 16>
 __device__ __forceinline__ void split_x8(const uint4& raw, int r, int part, uint8_t* terms, uint8_t* sf, bool store) {
   constexpr int TERMS = BF16 ? 2 : 3;
   using Tile = LinearTile<NT, TERMS>;
-  float v[8];
-  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t v[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t pair = 0;  // magnitudes as bits: ordered, NaN above infinity
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pair = __vmaxu2(pair, v[i] & 0x7fff7fffu);
+  pair = __vmaxu2(pair, __shfl_xor_sync(0xffffffffu, pair, 1));
+  pair = __vmaxu2(pair, __shfl_xor_sync(0xffffffffu, pair, 2));
+  const uint32_t amax = max(pair & 0xffffu, pair >> 16);
+  // byte = 127 + floor(log2 amax) - 7, at least 0; 255 (NaN) for a non-finite block.
+  const int ebits = static_cast<int>(BF16 ? amax >> 7 : f32_bits(__half2float(__ushort_as_half(static_cast<unsigned short>(amax)))) >> 23);
+  int byte = max(ebits - 7, 0);
+  if (ebits == 255) byte = 255;
+  // x / s in f16.
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if constexpr (BF16) {
-      v[2 * i] = bits_f32(words[i] << 16);
-      v[2 * i + 1] = bits_f32(words[i] & 0xffff0000u);
+      const uint32_t mult = static_cast<uint32_t>(254 - byte) << 7;  // 2^(127 - byte)
+      const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&v[i]);
+      const __nv_bfloat16 f = __ushort_as_bfloat16(static_cast<unsigned short>(mult));
+      const __nv_bfloat162 scaled = __hmul2(m, __halves2bfloat162(f, f));
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(&scaled);
+      v[i] = pack_f16x2(bits_f32(w << 16), bits_f32(w & 0xffff0000u));
     } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
+      const float mult = exp2i(127 - min(byte, 254));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      v[i] = pack_f16x2(__fmul_rn(f.x, mult), __fmul_rn(f.y, mult));
     }
+    if (ebits == 255) v[i] = 0;
   }
-  uint32_t amax = 0;  // magnitudes as bits: ordered, NaN above infinity
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = max(amax, f32_bits(v[i]) & 0x7fffffffu);
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  // byte = 127 + floor(log2 amax) - 7, at least 0; 255 (NaN) for a non-finite block.
-  const int ebits = static_cast<int>(amax >> 23);
-  int byte = max(ebits - 7, 0);
-  if (ebits == 255) byte = 255;
-  const float mult = ebits == 255 ? 0.0f : exp2i(127 - byte);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = ebits == 255 ? 0.0f : __fmul_rn(v[i], mult);
+  // The row's scales, one per block of its 8 PARTS inputs, as a word.
+  uint32_t word = static_cast<uint32_t>(byte) << (8 * (part >> 2));
+  word |= __shfl_xor_sync(0xffffffffu, word, 4);
+  if constexpr (PARTS == 16) word |= __shfl_xor_sync(0xffffffffu, word, 8);
   if (!store) return;
   // 16-byte slot part / 2 of the row's 128 bytes, swizzled over eight rows.
   terms += r * 128 + (((part >> 1) ^ (r & 7)) << 4) + ((part & 1) << 3);
@@ -122,19 +133,21 @@ __device__ __forceinline__ void split_x8(const uint4& raw, int r, int part, uint
   for (int t = 0; t < TERMS; ++t) {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = e4m3x2(v[2 * i], v[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) w[i] = f16x2_to_e4m3x2(v[i]);
     *reinterpret_cast<uint2*>(terms + t * Tile::kTermBytes) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-    if ((part & 3) == 0) sf[Tile::sf_place(t, r) + (part >> 2)] = static_cast<uint8_t>(byte);
+    if (part == 0) *reinterpret_cast<uint32_t*>(sf + Tile::sf_place(t, r)) = word;
     if (t + 1 < TERMS) {
       const int step = byte == 255 ? 0 : min(byte, 5);  // scales do not go below 2^-127
-      const float up = static_cast<float>(1 << step);
+      const __half2 up = __float2half2_rn(static_cast<float>(1 << step));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 q = e4m3x2_to_f32x2(w[i]);
-        v[2 * i] = __fmul_rn(__fsub_rn(v[2 * i], q.x), up);
-        v[2 * i + 1] = __fmul_rn(__fsub_rn(v[2 * i + 1], q.y), up);
+        const uint32_t q = e4m3x2_to_f16x2(w[i]);
+        const __half2 rest = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v[i]), *reinterpret_cast<const __half2*>(&q)), up);
+        v[i] = *reinterpret_cast<const uint32_t*>(&rest);
       }
       byte -= step;
+      const uint32_t nan = __vcmpeq4(word, 0xffffffffu);
+      word = (__vsubus4(word, 0x05050505u) & ~nan) | (word & nan);
     }
   }
 }
