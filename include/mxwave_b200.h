@@ -285,7 +285,7 @@ MXW_API int mxw_finalize_block_hessian(const float* gram, int full, int64_t cols
  * inner % 32 == 0; packed 16-byte aligned.  fp32 accumulation; the fixed order
  * of additions makes results reproducible.  A row of x that holds a NaN or an
  * infinity gives NaN in all its outputs; so does a scale byte 255.
- * flags: MXW_FLAG_TIMEOUT or NULL.
+ * flags: MXW_FLAG_TIMEOUT or NULL; outputs whose wait gave up are NaN.
  */
 MXW_API size_t mxw_linear_workspace_size(int64_t rows, int64_t inner, int dtype);
 MXW_API int mxw_linear_mxfp4(const void* x, int dtype, int64_t rows, int64_t inner, int64_t ldx,
@@ -343,12 +343,13 @@ MXW_API int mxw_copy_pages(uint8_t* codes, uint8_t* scales, int64_t layers, int6
  * speed does not).  Pages outside [0, pages) are not read: their keys are left
  * out.  A query without a key gives zeros and -infinity; so do rows of `out`
  * that no sequence covers.
- *   out [tokens][heads][dim] of `dtype`; lse [tokens][heads] fp32 (natural log
+ *   out [tokens][heads][dim] of `dtype`, 16-byte aligned; lse [tokens][heads] fp32 (natural log
  *   of the sum of exponentials) or NULL.
  * workspace: device memory, 16-byte aligned, of at least
  * mxw_paged_attention_workspace_size bytes for the same arguments; calls that
  * share one must not overlap on the device.
- * fp32 statistics and sums in a fixed order.  flags: MXW_FLAG_TIMEOUT or NULL.
+ * fp32 statistics and sums in a fixed order.  flags: MXW_FLAG_TIMEOUT or NULL;
+ * outputs whose wait gave up are NaN.
  */
 MXW_API size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,
                                                   int64_t max_length, int64_t max_queries);

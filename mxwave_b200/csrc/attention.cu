@@ -832,7 +832,7 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   if (q_token < 0 || q_head < 0 || window < 0 || (window > 0 && !causal)) return MXW_EINVAL;
   if (!(softmax_scale > 0.0) || !std::isfinite(softmax_scale)) return MXW_EINVAL;
   if (tokens == 0) return MXW_OK;
-  if (!query || !out) return MXW_EINVAL;
+  if (!query || !out || reinterpret_cast<uintptr_t>(out) % 16 != 0) return MXW_EINVAL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (seqs == 0 || max_queries == 0) {
     // No sequence has a query: every row is one that no key reaches.

@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
           if (!__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (count[x] + u.tiles - 1) & 1))) ok = false;
           tc_fence_after();
         }
+        if (!ok) l = NAN;  // a wait gave up: NaN, whether or not anybody reads the flags
         const bool seen = !(l == 0.0f);  // NaN counts as seen
         const float inv = seen ? __fdiv_rn(1.0f, l) : 0.0f;
         const float back = exp2i(max(ref - 140, -149));
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             tmem_load32(o_t + c, o);
             tmem_wait_load();
           }
-          if (live && ok) {
+          if (live) {
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
               uint32_t w[4];
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             }
           }
         }
-        if (live && ok && P.lse) P.lse[out_row] = seen ? __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(l), kAttLift)), 0.69314718055994531f) : -INFINITY;
+        if (live && P.lse) P.lse[out_row] = seen ? __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(l), kAttLift)), 0.69314718055994531f) : -INFINITY;
         tc_fence_before();
       }
     } else if (warp < 12) {

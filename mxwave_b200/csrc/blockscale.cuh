@@ -65,9 +65,8 @@ __device__ __forceinline__ bool elect_one() {
   return on != 0;
 }
 
-// mbar_wait with its limit counted in SM cycles (2 s at 2 GHz).  Reading the
-// global timer takes about a microsecond, which a pipeline that waits for every
-// stage pays at each of them; the cycle counter is read in a few tens of cycles.
+// mbar_wait with its limit counted in SM cycles (2 s at 2 GHz), and no timer
+// read by a wait that is over at once.
 __device__ __forceinline__ bool mbar_wait_cycles(uint64_t* bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;
   const long long start = clock64();

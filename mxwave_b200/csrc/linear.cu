@@ -126,9 +126,9 @@ __device__ __forceinline__ void store16(void* p, int64_t i, float v) {
     static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
-// Sixteen columns of the accumulator, the terms' columns added up.
+// Sixteen columns of the accumulator, the terms' columns added up; NaN for a `bad` one.
 template <int NT, int TERMS>
-__device__ __forceinline__ void load_sums(uint32_t taddr, float (&v)[16]) {
+__device__ __forceinline__ void load_sums(uint32_t taddr, bool bad, float (&v)[16]) {
   tmem_ld_32x32b_x16(taddr, v);
   if constexpr (LinearTile<NT, TERMS>::kMerged) {
 #pragma unroll
@@ -139,6 +139,8 @@ __device__ __forceinline__ void load_sums(uint32_t taddr, float (&v)[16]) {
       for (int u = 0; u < 16; ++u) v[u] = __fadd_rn(v[u], w[u]);
     }
   }
+#pragma unroll
+  for (int u = 0; u < 16; ++u) v[u] = bad ? NAN : v[u];
 }
 
 // Two neighbours at an even index of 4-byte aligned memory.
@@ -349,8 +351,8 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
       __syncwarp();
     }
     if (leader) {
-      mma_commit(done);
       if (!ok) atomicOr(fail, 1);
+      mma_commit(done);
     }
   } else if constexpr (FUSED) {
     // --------------------------------------------------------- terms of x
@@ -387,7 +389,12 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
   const bool epilogue = warp >= 2 && warp < 2 + kLinSpreadWarps;
   const int half = (warp - 2) >> 2;  // and every other group of columns
   const int quarter = warp & 3, tid = 32 * quarter + lane;  // a warp reads its own quarter of the TMEM lanes
-  if (epilogue && !__all_sync(0xffffffffu, mbar_wait_cycles(done, 0))) atomicOr(fail, 1);
+  bool bad = false;  // a wait gave up: NaN, whether or not anybody reads the flags
+  if (epilogue) {
+    bad = !__all_sync(0xffffffffu, mbar_wait_cycles(done, 0));
+    if (bad) atomicOr(fail, 1);
+    bad |= *static_cast<volatile int*>(fail) != 0;
+  }
   tc_fence_after();
   const int64_t n = n0 + tid;  // this thread's output
   const int64_t t0 = tile * NT;
@@ -399,7 +406,7 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
       for (int c = 16 * half; c < NT; c += 32) {
         if (t0 + c >= P.rows) break;
         float v[16];
-        load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
+        load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, bad, v);
         if (n < P.outs) {
           float res[16];
 #pragma unroll
@@ -423,7 +430,7 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
 #pragma unroll 1
       for (int c = 16 * half; c < NT && t0 + c < P.rows; c += 32) {
         float v[16];
-        load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
+        load_sums<NT, TERMS>(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, bad, v);
 #pragma unroll
         for (int u = 0; u < 16; ++u) part[(c + u) * 128 + tid] = v[u];
       }
@@ -598,8 +605,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       __syncwarp();
     }
     if (leader) {
-      mma_commit(done);
       if (!ok) atomicOr(fail, 1);
+      mma_commit(done);
     }
   } else {
     // ------------------------------------------------------------ spreading
@@ -665,7 +672,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   // read (residual) and written together.
   __syncwarp();
   if (warp >= 2) {
-    if (!__all_sync(0xffffffffu, mbar_wait_cycles(done, 0))) atomicOr(fail, 1);
+    bool bad = !__all_sync(0xffffffffu, mbar_wait_cycles(done, 0));
+    if (bad) atomicOr(fail, 1);
+    bad |= *static_cast<volatile int*>(fail) != 0;  // a wait gave up: NaN, whether or not anybody reads the flags
     tc_fence_after();
     const int quarter = warp & 3, c = 64 * ((warp - 2) >> 2);
     float* turn = reinterpret_cast<float*>(smem) + (warp - 2) * (32 * 66);  // [32 rows][64 + 2]
@@ -678,7 +687,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         float v[32];
         tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c + 32 * h, v);
 #pragma unroll
-        for (int u = 0; u < 16; ++u) *reinterpret_cast<float2*>(turn + lane * 66 + 32 * h + 2 * u) = make_float2(v[2 * u], v[2 * u + 1]);
+        for (int u = 0; u < 16; ++u) *reinterpret_cast<float2*>(turn + lane * 66 + 32 * h + 2 * u) = make_float2(bad ? NAN : v[2 * u], bad ? NAN : v[2 * u + 1]);
       }
       __syncwarp();
       const int64_t n = n0 + c + 2 * lane;

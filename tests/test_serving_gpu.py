@@ -105,6 +105,18 @@ def test_linear_over_long_rows(rows: int, outs: int, inner: int) -> None:
         check_linear(x, p, s, None, "none", None, y)
 
 
+@pytest.mark.parametrize("rows", [4, 20, 50, 200])
+@pytest.mark.parametrize("outs, inner", [(100, 96), (100, 640), (4780, 1184), (2310, 1184), (3480, 1184), (100, 1184), (100, 2080), (100, 4064)])
+def test_linear_shares_of_the_inputs(rows: int, outs: int, inner: int) -> None:
+    """Clusters of one to eight blocks, with shares of the inputs that are not equal and end in the middle of a chunk."""
+    g = gen(rows + outs + inner)
+    packed, scales = quantize_mxfp4(randn(g, outs, inner) * 0.02, method="rtn")
+    x, bias, residual = randn(g, rows, inner).to(HF), randn(g, outs).to(HF), randn(g, rows, outs).to(HF)
+    y = linear_mxfp4(x, packed, scales, bias, activation="silu", residual=residual)
+    check_linear(x, packed, scales, bias, "silu", residual, y)
+    assert torch.equal(y, linear_mxfp4(x, packed, scales, bias, activation="silu", residual=residual))
+
+
 @pytest.mark.parametrize("rows", [3, 40, 300])
 def test_linear_takes_strides_slices_and_leading_dims(rows: int) -> None:
     g = gen(rows)
@@ -467,6 +479,34 @@ def test_equal_calls_give_equal_bits_on_any_stream(lens, queries, heads, kv, pag
             got += [case.run() for _ in range(3)]  # three streams at once, each with its own workspaces
     torch.cuda.synchronize()
     assert all(torch.equal(o, out) and torch.equal(le, lse) for o, le in got)
+
+
+@pytest.mark.parametrize("queries", [1, 600])
+def test_pages_past_32_bits(queries: int) -> None:
+    """A layer of more than 2^32 bytes: what lies at its end is as good as what lies at its start."""
+    g = gen(20)
+    kv, page, dim, pages, held = 8, 128, 128, 33000, 5
+    big = [torch.zeros(pages, 2, kv, page, n, dtype=torch.uint8, device="cuda") for n in (dim // 2, dim // 32)]
+    small = [torch.zeros(held, 2, kv, page, n, dtype=torch.uint8, device="cuda") for n in (dim // 2, dim // 32)]
+    assert big[0].numel() > 2**32
+    tokens = held * page - 7
+    key, value, query = randn(g, tokens, kv, dim), randn(g, tokens, kv, dim), randn(g, queries, 4 * kv, dim).to(BF)
+    slots = torch.arange(tokens, device="cuda")
+    far = pages - held
+    start = torch.tensor([0, queries], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([tokens], dtype=torch.int32, device="cuda")
+    got = []
+    for pool, first in ((small, 0), (big, far)):
+        kvcache.append_mxfp4_(*pool, key, value, slots + first * page)
+        table = torch.arange(first, first + held, dtype=torch.int32, device="cuda")[None]
+        got.append((*kvcache.gather_mxfp4(*pool, slots + first * page),
+                    *kvcache.paged_attention_mxfp4(query, *pool, table, lengths, start, max_length=tokens, max_queries=queries, return_lse=True)))
+    assert got[0][0].abs().sum() > 0 and got[0][2].abs().sum() > 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    kvcache.copy_pages_(big[0][None], big[1][None], [far + 1, far + 2], [2, far - 1])
+    for part, pool in enumerate(big):
+        assert torch.equal(pool[2], small[part][1]) and torch.equal(pool[far - 1], small[part][2])
+        assert not pool[0].any() and not pool[far - 2].any()
 
 
 def test_no_sequences_and_no_queries() -> None:
