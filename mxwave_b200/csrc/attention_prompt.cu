@@ -268,13 +268,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(bits_f32(s0[j + k]), bits_f32(s1[j + k])));
           float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
           top = __fmul_rn(top, P.scale_log2);
-          // The accumulator and P belong to the last tile's product until that is done.
-          if (t > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (n - 1) & 1))) {
-            ok = false;
-            break;
-          }
+          // The accumulator and P belong to the last tile's product until that
+          // is done: seldom waited for here, else when the exponentials are.
           const bool raise = top > __fadd_rn(m, kAttSlack);
-          if (__any_sync(0xffffffffu, raise) || ref_t > ref) {
+          const bool rescale = __any_sync(0xffffffffu, raise) || ref_t > ref;
+          if (rescale) {
+            if (t > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (n - 1) & 1))) {
+              ok = false;
+              break;
+            }
             const float up = raise ? fmaxf(m, top) : m;
             const float fm = m == up ? 1.0f : ex2(__fsub_rn(m, up));
             m = up;
@@ -300,8 +302,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
           const float base = __fsub_rn(kAttLift - static_cast<float>(drop), m == -INFINITY ? 0.0f : m);
           const unsigned long long f2 = pack2(P.scale_log2, P.scale_log2), b2 = pack2(base, base);
           unsigned long long sum2 = 0ull, sum3 = 0ull;
-          auto probabilities = [&](const uint32_t (&s)[32], uint32_t taddr) {
-            uint32_t p[16];
+          uint32_t p0[16], p1[16];
+          auto probabilities = [&](const uint32_t (&s)[32], uint32_t (&p)[16]) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const struct f2 x2 = unpack2(fma2(pack2(bits_f32(s[2 * j]), bits_f32(s[2 * j + 1])), f2, b2));
@@ -312,10 +314,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
                 sum3 = add2(sum3, pack2(a, c));
               p[j] = pack_f16x2(a, c);
             }
-            tmem_store16(taddr, p);
           };
-          probabilities(s0, p_t);
-          probabilities(s1, p_t + 16);
+          probabilities(s0, p0);
+          probabilities(s1, p1);
+          if (!rescale && t > 0 && !__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (n - 1) & 1))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          tmem_store16(p_t, p0);
+          tmem_store16(p_t + 16, p1);
           const struct f2 sums = unpack2(add2(sum2, sum3));
           l = __fmaf_rn(__fadd_rn(sums.x, sums.y), exp2i(drop), l);
           tmem_wait_store();
