@@ -143,12 +143,19 @@ __device__ __forceinline__ void load_sums(uint32_t taddr, bool bad, float (&v)[1
   for (int u = 0; u < 16; ++u) v[u] = bad ? NAN : v[u];
 }
 
-// Two neighbours at an even index of 4-byte aligned memory.
+// Two neighbours from a word.
 template <bool BF16>
-__device__ __forceinline__ float2 load16x2(const void* p, int64_t i) {
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+__device__ __forceinline__ float2 pair_values(uint32_t w) {
   if constexpr (BF16) return make_float2(bits_f32(w << 16), bits_f32(w & 0xffff0000u));
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// Brings 128 bytes of a row of the residual towards the epilogue that reads them when the products are done.
+__device__ __forceinline__ void prefetch_residual(const LinearParams& P, int64_t row, int64_t n) {
+  if (row >= P.rows || n >= P.outs) return;
+  const uint16_t* at = static_cast<const uint16_t*>(P.residual) + row * P.ldr + n;
+  prefetch_l2(at);
+  prefetch_l2(at + min(static_cast<int64_t>(63), P.outs - 1 - n));
 }
 template <bool BF16>
 __device__ __forceinline__ void store16x2(void* p, int64_t i, float a, float b) {
@@ -258,6 +265,9 @@ __global__ void __launch_bounds__((LinearTile<NT, BF16 ? 2 : 3>::kThreads))
     const int64_t nb = P.inner / 32;
     const bool row_in = n0 + e < P.outs;
     const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0) + static_cast<int64_t>(c_begin) * 4;
+    if (P.residual)
+      for (int i = threadIdx.x - 64; i < 2 * NT; i += 32 * kLinSpreadWarps)
+        if ((i >> 1) % ranks == rank) prefetch_residual(P, tile * NT + (i >> 1), n0 + 64 * (i & 1));
     // Scales of four of the group's chunks at a time, loaded that far ahead.
     uint32_t sf[4], sf_next[4];
     auto load_scales = [&](int i, uint32_t (&w)[4]) {
@@ -615,6 +625,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const int64_t nb = P.inner / 32;
     const bool row_in = n0 + e < P.outs;
     const uint8_t* srow = P.scales + (row_in ? (n0 + e) * nb : 0);
+    if (P.residual) prefetch_residual(P, tile * 128 + 32 * (warp & 3) + lane, n0 + 64 * ((warp - 2) >> 2));
     uint32_t sf[4], sf_next[4];
     auto load_scales = [&](int i, uint32_t (&w)[4]) {
 #pragma unroll
@@ -668,19 +679,45 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   }
 
   // ---------------------------------------------------------------- epilogue
-  // A warp reads its quarter of the rows and 64 of the columns and turns them over in shared memory so that a row's 64 outputs are
-  // read (residual) and written together.
+  // A warp reads its quarter of the rows and 64 of the columns and turns them
+  // over in shared memory so that a row's 64 outputs are read (residual) and
+  // written together.  The residual's first 16 rows are read before the products
+  // are waited for, the others before the first are written.
   __syncwarp();
   if (warp >= 2) {
+    const int quarter = warp & 3, c = 64 * ((warp - 2) >> 2);
+    const int64_t t0 = tile * 128 + 32 * quarter, n = n0 + c + 2 * lane;
+    const int rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), P.rows - t0)));
+    const bool pairs = P.pairs;  // two outputs per load and store
+    const bool in0 = n < P.outs, in1 = n + 1 < P.outs;
+    uint32_t res[2][16];
+    auto load_residual = [&](int half, uint32_t (&w)[16]) {
+      const int live = P.residual && in0 ? rows - 16 * half : 0;
+      const uint16_t* at = static_cast<const uint16_t*>(P.residual) + (t0 + 16 * half) * P.ldr + n;
+      if (pairs) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          w[r] = 0;
+          if (r < live) w[r] = in1 ? *reinterpret_cast<const uint32_t*>(at + r * P.ldr) : at[r * P.ldr];
+        }
+      } else {
+        uint16_t lo[16], hi[16];  // put together when all are on their way
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          lo[r] = hi[r] = 0;
+          if (r < live) lo[r] = at[r * P.ldr];
+          if (r < live && in1) hi[r] = at[r * P.ldr + 1];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] = lo[r] | (static_cast<uint32_t>(hi[r]) << 16);
+      }
+    };
+    load_residual(0, res[0]);
     bool bad = !__all_sync(0xffffffffu, mbar_wait_cycles(done, 0));
     if (bad) atomicOr(fail, 1);
     bad |= *static_cast<volatile int*>(fail) != 0;  // a wait gave up: NaN, whether or not anybody reads the flags
     tc_fence_after();
-    const int quarter = warp & 3, c = 64 * ((warp - 2) >> 2);
     float* turn = reinterpret_cast<float*>(smem) + (warp - 2) * (32 * 66);  // [32 rows][64 + 2]
-    const int64_t t0 = tile * 128 + 32 * quarter;
-    const int rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(32), P.rows - t0)));
-    const bool pairs = P.pairs;  // two outputs per load and store
     if (n0 + c < P.outs && rows > 0) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -690,34 +727,23 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         for (int u = 0; u < 16; ++u) *reinterpret_cast<float2*>(turn + lane * 66 + 32 * h + 2 * u) = make_float2(bad ? NAN : v[2 * u], bad ? NAN : v[2 * u + 1]);
       }
       __syncwarp();
-      const int64_t n = n0 + c + 2 * lane;
-      const bool in0 = n < P.outs, in1 = n + 1 < P.outs;
+      load_residual(1, res[1]);
       const float bias0 = P.bias && in0 ? load16<BF16>(P.bias, n) : 0.0f;
       const float bias1 = P.bias && in1 ? load16<BF16>(P.bias, n + 1) : 0.0f;
-#pragma unroll 1
-      for (int r0 = 0; r0 < rows; r0 += 8) {
-        float2 res[8];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          res[r] = make_float2(0.0f, 0.0f);
-          if (P.residual && r0 + r < rows) {
-            const int64_t at = (t0 + r0 + r) * P.ldr + n;
-            if (pairs && in1)
-              res[r] = load16x2<BF16>(P.residual, at);
-            else if (in0)
-              res[r] = make_float2(load16<BF16>(P.residual, at), in1 ? load16<BF16>(P.residual, at + 1) : 0.0f);
-          }
-        }
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          if (r0 + r >= rows) break;
-          const float2 v = *reinterpret_cast<const float2*>(turn + (r0 + r) * 66 + 2 * lane);
+        for (int r = 0; r < 16; ++r) {
+          const int row = 16 * half + r;
+          if (row >= rows) break;
+          const float2 v = *reinterpret_cast<const float2*>(turn + row * 66 + 2 * lane);
           float o0 = activate(__fadd_rn(v.x, bias0), P.act), o1 = activate(__fadd_rn(v.y, bias1), P.act);
           if (P.residual) {
-            o0 = __fadd_rn(o0, res[r].x);
-            o1 = __fadd_rn(o1, res[r].y);
+            const float2 add = pair_values<BF16>(res[half][r]);
+            o0 = __fadd_rn(o0, add.x);
+            o1 = __fadd_rn(o1, add.y);
           }
-          const int64_t at = (t0 + r0 + r) * P.outs + n;
+          const int64_t at = (t0 + row) * P.outs + n;
           if (pairs && in1) {
             store16x2<BF16>(P.y, at, o0, o1);
           } else {
