@@ -109,8 +109,8 @@ struct KvSource {
 // Eight elements per thread, a block of 32 per four neighbours: the largest
 // magnitude over two shuffles, one 4-byte store of codes each, and the first
 // of them stores the scale.  TOK tokens per thread, loads first: with one, a
-// block's life is one chain of dependent loads and HBM waits (append of 16,384
-// tokens of 8 heads: 39 us with one, see kKvAhead).
+// block's life is one chain of dependent loads and HBM waits (kKvAhead has
+// the times).
 template <int DT, bool VEC, int TOK>
 __global__ void __launch_bounds__(kKvThreads) kv_append_kernel(const KvRows P, const KvSource S) {
   const int sub = P.per_block == 1 ? 0 : static_cast<int>(threadIdx.x) / P.units;
@@ -330,10 +330,12 @@ static KvRows kv_rows(uint8_t* codes, uint8_t* scales, const int64_t* slots, int
   return P;
 }
 
-// Tokens per thread: kKvAhead once every SM has a few blocks of them, one below.
+// Tokens per thread: kKvAhead once every SM has a block of them, one below
+// (append of 64, 592, 1184, 2368, 16,384 bf16 tokens of 8 heads of 128: 3.9,
+// 5.2, 7.2, 11.3, 60.7 us with one, 5.1, 5.0, 6.2, 8.7, 44 us with four).
 constexpr int kKvAhead = 4;
 static int kv_tokens_per_thread(const KvRows& P) {
-  return P.tokens >= static_cast<int64_t>(P.per_block) * kKvAhead * num_sms() * 4 ? kKvAhead : 1;
+  return P.tokens >= static_cast<int64_t>(P.per_block) * kKvAhead * num_sms() ? kKvAhead : 1;
 }
 static unsigned kv_grid(const KvRows& P, int tok) {
   const int64_t each = static_cast<int64_t>(P.per_block) * tok;
