@@ -17,8 +17,11 @@
 // keys and values (cp.async a row piece at a time: pages may end anywhere in a
 // tile), spread K's codes and decode V; warps 12 and 13 issue the products of a
 // row tile each, so that one's waits are covered by the other's products.
-// What bounds it: per 64 keys 1024 cycles of products against the issue slots of
-// 16,384 exponentials and the maxima, sums, conversions around them.
+// What bounds it: the chain of a row tile from scores to probabilities to the
+// next scores, some 2700 cycles per 64 keys, in which the products take 1300
+// (the scores' narrow ones are held back by their operands' shared-memory reads)
+// and the 16,384 exponentials 1024.  Four prompts of up to 3001 new tokens over
+// up to 1000 cached ones, 40 heads over 8 of 128, bf16: 598 us, 500 TFLOP/s.
 #include "attention.cuh"
 #include "blockscale.cuh"
 #include "common.cuh"

@@ -9,8 +9,11 @@
 //   e = floor(log2 amax) - 2, plus 1 when amax >= 1.75 2^floor(log2 amax)
 // clamped to [-127, 127].  Token `slot` lives in page slot / page_tokens.
 //
-// All three kernels move bytes once and are bound by HBM; a row's 4.25 bits per
-// element leave too little arithmetic to matter.
+// All three kernels move bytes once.  Page copies run at HBM's rate (400
+// pages of 16 layers, 0.9 GB read and written, in 135 us: 6.6 TB/s); appending and
+// reading back are bound by the encoding's instructions in large calls (16,384
+// bf16 tokens of 8 heads of 128 written and read back: 44 us where their bytes
+// take 26) and by the launches in small ones (4.5 us for both).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdlib.h>
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_gather_kernel(const KvRows P, O
 //
 // The pairs travel as a kernel argument: no copy to the device, nothing to
 // keep alive until the launch runs, and the call can be captured in a graph.
-// Two sizes: 16 KB of arguments cost a launch more than 512 bytes do.
+// Two sizes: 16 KB of arguments cost the host 6.8 us a call, 512 bytes 3.8.
 template <int N>
 struct PagePairs {
   int32_t source[N], target[N];

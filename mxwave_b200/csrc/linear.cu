@@ -24,6 +24,12 @@
 // the SMs the CTAs of a cluster split K and add their fp32 partial tiles over
 // distributed shared memory in rank order, so results do not change from run
 // to run.
+//
+// Measured: one row, 5120 x 5120: 10 us (1.4 TB/s); 24 rows, 17408 x 5120: 21 us
+// (2.3 TB/s); both bound by shared memory, through which W passes three times
+// (copied, spread to twice its size, read by the products), and by 6 us of launch,
+// set-up, cluster sum and epilogue.  8192 rows, 5120 x 17408: 1.19 ms, 1.23
+// PFLOP/s of the product (twice that of the terms').
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
