@@ -39,9 +39,9 @@
 // log-sum-exp) in the workspace, two slots per block, and attention_join_kernel
 // adds them in block order.
 // Measured: 32 sequences of 1 to 65,536 keys, 40 heads over 8 of 128, one query
-// each: 187 us, 4.3 TB/s of cache and rows, 66% of the copy rate; bound by issue
-// slots (some 340 instructions a warp per 16 keys, half of them conversions and
-// matrix instructions).  One sequence of 517 keys: 12.4 us, of which the
+// each: 187 us, 4.3 TB/s of cache and rows, 66% of the copy rate; bound by its
+// instructions (some 340 a warp per 16 keys, half of them conversions and matrix
+// instructions; 61% of the issue slots with 16 warps an SM).  One sequence of 517 keys: 12.4 us, of which the
 // join's launch and chain are some 5.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
