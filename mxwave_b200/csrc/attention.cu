@@ -34,15 +34,15 @@
 //     synchronisation with the others until the end of a segment.
 // Work split: the (sequence, head, row group) units are cut into tiles of 128
 // keys, all tiles are laid end to end (each unit's behind the cost of starting
-// it), and each block takes an equal share, whatever the lengths.  A unit that
+// it), and each block takes an equal share, whatever the lengths (units of few
+// tiles stay whole, see kAttWhole).  A unit that
 // several blocks share leaves partial results (normalised rows and their
 // log-sum-exp) in the workspace, two slots per block, and attention_join_kernel
 // adds them in block order.
 // Measured: 32 sequences of 1 to 65,536 keys, 40 heads over 8 of 128, one query
 // each: 187 us, 4.3 TB/s of cache and rows, 66% of the copy rate; bound by its
 // instructions (some 340 a warp per 16 keys, half of them conversions and matrix
-// instructions; 61% of the issue slots with 16 warps an SM).  One sequence of 517 keys: 12.4 us, of which the
-// join's launch and chain are some 5.
+// instructions; 61% of the issue slots with 16 warps an SM).  One sequence of 517 keys: 12.2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -67,6 +67,12 @@ constexpr int kAttJoinThreads = 256;
 // finished last (393 us against 212 on 32 sequences of 1 to 65,536 keys; 325,
 // 253, 212 and 217 us with 1, 2, 4 and 8 here).
 constexpr int kAttStart = 4;
+// Short units are not shared between blocks, and nothing is joined: up to 12
+// tiles when there is a unit for every block that fits the GPU, up to 6 when
+// there are few (40 heads over 8, one query, whole against shared: 1 sequence of
+// 300, 516, 1000 keys 9.8, 12.2, 15.0 and 12.7, 12.4, 12.6 us; 64 sequences of 300,
+// 700, 1100 keys 17, 23, 30 and 25, 32, 39 us).
+constexpr int kAttWhole = 12, kAttWholeFew = 6;
 
 
 // One sequence's share of the work.
@@ -93,7 +99,7 @@ __device__ __forceinline__ AttSeq att_seq(const AttParams& P, int b) {
 }
 
 __device__ __forceinline__ int64_t att_work(const AttParams& P, const AttSeq& s) {
-  return static_cast<int64_t>(s.tiles + kAttStart) * s.row_groups * P.kv_heads;
+  return static_cast<int64_t>(P.whole ? 1 : s.tiles + kAttStart) * s.row_groups * P.kv_heads;
 }
 
 // Sum over the block (all threads get it); `red` holds one word per warp.
@@ -263,11 +269,11 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       rem -= att_work(P, seq);
       seq = att_seq<ROWS>(P, ++b);
     }
-    const int cost = seq.tiles + kAttStart;
+    const int cost = P.whole ? 1 : seq.tiles + kAttStart;
     const int64_t unit = rem / cost;
     const int c0 = static_cast<int>(rem % cost);
     const int c1 = static_cast<int>(min(static_cast<int64_t>(cost), c0 + (end - at)));
-    const int tile0 = max(0, c0 - kAttStart), tile1 = c1 - kAttStart;
+    const int tile0 = P.whole ? 0 : max(0, c0 - kAttStart), tile1 = P.whole ? seq.tiles : c1 - kAttStart;
     const bool opens = first_segment;
     at += c1 - c0;
     rem += c1 - c0;
@@ -759,23 +765,28 @@ struct AttPlan {
   int nt;            // groups of eight rows per unit
   int64_t units;     // at most, per sequence
   unsigned blocks;
+  bool whole;        // no unit is shared
   size_t bytes;      // of the workspace
 };
 
 // Bounds that the caller states (the longest sequence, the most queries of one)
 // fix the launch; the kernels read the true lengths.
 static AttPlan att_plan(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim, int64_t max_length,
-                        int64_t max_queries) {
+                        int64_t max_queries, int64_t window) {
   AttPlan plan{};
   const int64_t group = heads / kv_heads, rows = max_queries * group;
   plan.nt = rows <= 8 ? 1 : 2;
   const int64_t unit_rows = 8 * plan.nt;
   plan.units = (rows + unit_rows - 1) / unit_rows * kv_heads;
-  const int64_t deep = std::max<int64_t>(1, (max_length + kAttTile - 1) / kAttTile), units = plan.units * seqs;
+  // (A window's keys start anywhere in a tile.)
+  const int64_t reach = window > 0 ? std::min(max_length, window + max_queries + kAttTile) : max_length;
+  const int64_t deep = std::max<int64_t>(1, (reach + kAttTile - 1) / kAttTile), units = plan.units * seqs;
+  const int64_t slots = static_cast<int64_t>(num_sms()) * (plan.nt == 1 ? 4 : 3);
+  plan.whole = deep <= kAttWhole && deep * (slots - std::min(slots, units)) <= kAttWholeFew * slots;
   // At most 64 blocks per unit: joining more partial results costs what the split saves.
-  const int64_t tiles = std::min<int64_t>(deep, 64) * units;
-  plan.blocks = static_cast<unsigned>(std::min<int64_t>(tiles, static_cast<int64_t>(num_sms()) * (plan.nt == 1 ? 4 : 3)));
-  plan.bytes = static_cast<size_t>(plan.blocks) * 2 * static_cast<size_t>(unit_rows * dim + unit_rows) * sizeof(float);
+  const int64_t tiles = (plan.whole ? 1 : std::min<int64_t>(deep, 64)) * units;
+  plan.blocks = static_cast<unsigned>(std::min<int64_t>(tiles, slots));
+  plan.bytes = plan.whole ? 16 : static_cast<size_t>(plan.blocks) * 2 * static_cast<size_t>(unit_rows * dim + unit_rows) * sizeof(float);
   return plan;
 }
 
@@ -787,7 +798,7 @@ static int launch_attention(const AttParams& P, const AttPlan& plan, cudaStream_
   if (status != MXW_OK) return status;
   kernel<<<plan.blocks, kAttThreads, AttShape<D, NT>::kSmem, s>>>(P);
   status = check_launch();
-  if (status != MXW_OK) return status;
+  if (status != MXW_OK || plan.whole) return status;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(plan.units), static_cast<unsigned>(P.seqs));
   cfg.blockDim = dim3(kAttJoinThreads);
@@ -821,7 +832,7 @@ extern "C" size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads
                                                      int64_t max_length, int64_t max_queries) {
   if (!att_shape_ok(seqs, heads, kv_heads, dim, max_length, max_queries) || seqs == 0 || max_queries == 0) return 0;
   if (attention_prompt_fits(seqs, heads, kv_heads, max_queries)) return 16;  // nothing is shared between blocks
-  return att_plan(seqs, heads, kv_heads, dim, max_length, max_queries).bytes;
+  return att_plan(seqs, heads, kv_heads, dim, max_length, max_queries, 0).bytes;  // (a window needs no more)
 }
 
 extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens, int64_t heads, int64_t q_token,
@@ -849,7 +860,7 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   }
   if (!codes || !scales || !lengths || !start || (table_width > 0 && !table)) return MXW_EINVAL;
   if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0) return MXW_EINVAL;
-  const AttPlan plan = att_plan(seqs, heads, kv_heads, dim, max_length, max_queries);
+  const AttPlan plan = att_plan(seqs, heads, kv_heads, dim, max_length, max_queries, std::min<int64_t>(window, 0x3fffffff));
   const bool prompt = attention_prompt_fits(seqs, heads, kv_heads, max_queries);
   if (!prompt && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || workspace_bytes < plan.bytes)) return MXW_EINVAL;
   if (seqs > 65535 || plan.units > 0x7fffffff || tokens > 0x7fffffff) return MXW_EUNSUPPORTED;
@@ -878,6 +889,7 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   P.out = out;
   P.lse = lse;
   P.partial = static_cast<float*>(workspace);
+  P.whole = plan.whole;
   P.flags = flags;
   if (prompt) return launch_attention_prompt(P, dtype == MXW_BF16, static_cast<int>(dim), max_queries, s);
   if (dtype == MXW_BF16)

@@ -28,6 +28,7 @@ struct AttParams {
   int seqs, heads, kv_heads, group, page_shift;
   float scale_log2;  // softmax scale times log2(e)
   int causal, window;
+  int whole;   // units are not shared between blocks
   void* out;   // [tokens][heads][dim]
   float* lse;  // [tokens][heads] or null
   float* partial;

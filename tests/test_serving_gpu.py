@@ -384,6 +384,28 @@ def test_attention_matches_64_bits(lens, queries, heads, kv, page, dim, dtype) -
     case.check(*case.run())
 
 
+SHARED = [
+    # Units of more tiles than a block keeps to itself.
+    ([1700, 3, 2900], [1] * 3, 40, 8, 64, 128),
+    ([2000, 1300], [3, 1], 17, 1, 128, 64),
+    ([1500, 0, 1601, 5702], [7, 0, 5, 9], 6, 3, 16, 64),
+    ([4097, 1025], [33, 20], 5, 1, 32, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("window", [0, 1900])
+@pytest.mark.parametrize("lens, queries, heads, kv, page, dim", SHARED)
+def test_attention_over_shared_units(lens, queries, heads, kv, page, dim, window, dtype) -> None:
+    case = Case(22, lens, queries, heads, kv, page, dim, dtype)
+    out, lse = case.run(window=window)
+    case.check(out, lse, window=window)
+    again, lse2 = case.run(window=window)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    for bound in (1, 100, 100000):  # what the launch is sized for changes which blocks share, not the result
+        case.check(*case.run(window=window, max_length=bound), window=window)
+
+
 @pytest.mark.parametrize("window", [1, 16, 17, 100, 5000])
 @pytest.mark.parametrize("lens, queries, heads, kv, page, dim", [DECODE[3], DECODE[5], DECODE[8], PROMPT[1], PROMPT[2], PROMPT[3]])
 def test_sliding_windows(lens, queries, heads, kv, page, dim, window) -> None:
