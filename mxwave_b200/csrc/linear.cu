@@ -803,7 +803,9 @@ static int linear_split(int64_t tiles, int chunks, int per_sm) {
 }
 
 // Whether the wide tiles fill most of the SMs; below that the narrow kernel,
-// whose clusters split K, ends sooner.
+// whose clusters split K, ends sooner (wide against narrow, inner 5120: 300 rows
+// of 5120 outputs, 60 tiles, 44 and 40 us; 512 rows, 80 tiles, 46 and 78; 200 rows
+// of 17408, 136 tiles, 48 and 76; 333 x 1000 x 2080, 12 tiles, 43 and 15).
 static bool linear_wide(int64_t rows, int64_t outs) {
   return rows > 128 && (rows + 127) / 128 * ((outs + kWideN - 1) / kWideN) >= num_sms() / 2;
 }
