@@ -348,8 +348,11 @@ MXW_API int mxw_copy_pages(uint8_t* codes, uint8_t* scales, int64_t layers, int6
  * workspace: device memory, 16-byte aligned, of at least
  * mxw_paged_attention_workspace_size bytes for the same arguments; calls that
  * share one must not overlap on the device.
- * fp32 statistics and sums in a fixed order.  flags: MXW_FLAG_TIMEOUT or NULL;
- * outputs whose wait gave up are NaN.
+ * fp32 statistics and sums in a fixed order; probabilities are held to 2^-11 of
+ * themselves and 2^-32 of their row's largest, values exactly.  A key that a
+ * row's mask hides has no say in it, however large its value; rows of a head
+ * that see values of scales more than 2^20 apart take a slower path in fp32.
+ * flags: MXW_FLAG_TIMEOUT or NULL; outputs whose wait gave up are NaN.
  */
 MXW_API size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,
                                                   int64_t max_length, int64_t max_queries);

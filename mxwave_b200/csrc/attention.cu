@@ -24,7 +24,7 @@
 //     exact down to 2^-31 of the row's largest.  The values' scales run across
 //     the contraction, so they are multiplied into the codes, relative to the
 //     largest scale seen so far (times 2^13, below f16's maximum): exact down to
-//     2^-27 of it, zero below.
+//     2^-27 of it, and rows with smaller ones are done again (kAttSpan).
 //   * Probabilities are rounded to f16 as 2^(x - m + 7): 11 bits down to 2^-21
 //     of the largest, nothing lost above 2^-31.  Their sum is taken in fp32
 //     before the rounding.  m is raised only when a score passes it by 8
@@ -73,7 +73,11 @@ constexpr int kAttStart = 4;
 // 300, 516, 1000 keys 9.8, 12.2, 15.0 and 12.7, 12.4, 12.6 us; 64 sequences of 300,
 // 700, 1100 keys 17, 23, 30 and 25, 32, 39 us).
 constexpr int kAttWhole = 12, kAttWholeFew = 6;
-
+// Scales of values this many powers of two below the largest are not looked at
+// one by one: tracking the smallest in every step took 197 us where this takes
+// 192 (32 sequences of 1 to 65,536 keys; 187 without a look at the range).  A rise
+// of the largest by more than kAttSpan - kAttQuiet then counts as a wide range.
+constexpr int kAttQuiet = 10;
 
 // One sequence's share of the work.
 struct AttSeq {
@@ -205,8 +209,14 @@ struct AttShape {
   static constexpr int kSlot = kRows * D + kRows;  // floats of a partial result
 };
 
+// A call: its registers are not the kernel's.
+template <bool BF16, int D>
+__device__ __noinline__ float row_wide(const AttParams& P, int b, int head, const uint16_t* q, int from, int to, float (&o)[D / 32]) {
+  return att_row_wide<BF16, D>(P, b, head, q, from, to, o);
+}
+
 template <bool BF16, int D, int NT>
-__global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attention_kernel(const AttParams P) {
+__global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attention_kernel(const __grid_constant__ AttParams P) {
   using Shape = AttShape<D, NT>;
   constexpr int ROWS = Shape::kRows;
   constexpr int QREGS = D / 8;       // f16 pairs of a query row per lane
@@ -215,6 +225,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
   extern __shared__ __align__(128) uint8_t att_smem[];
   __shared__ int64_t red[kAttWarps];
   __shared__ float row_m[kAttWarps][ROWS], row_l[kAttWarps][ROWS];
+  __shared__ uint32_t warp_low[kAttWarps];  // the smallest scale but zero of the values so far, less one (or a bound: see kAttQuiet)
+  __shared__ int warp_wide[kAttWarps];
   grid_dependents_launch();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -410,6 +422,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       l[nt][0] = l[nt][1] = 0.0f;
     }
     int ref = 0;  // exponent byte that the values are relative to
+    if (lane == 0) warp_low[warp] = 0xffffu;
 
     int stage = 0;
     for (int step = skip; step < steps; ++step) {
@@ -498,10 +511,12 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
             if (!in || k + v_b < lo_min || k + v_b >= hi_max) sv[half][c] &= 0x0000ffffu;
           }
       }
+      // Scales outside [ref - kAttQuiet, ref] (zeros too) are looked at below; most steps have none.
+      const uint32_t base2 = (static_cast<uint32_t>(kAttQuiet - ref) & 0xffffu) * 0x10001u;
+      const uint32_t far2 = __vmaxu2(__viaddmax_u16x2(sv[0][1], base2, __vadd2(sv[0][0], base2)),
+                                     __viaddmax_u16x2(sv[1][1], base2, __vadd2(sv[1][0], base2)));
+      bool raise = max(far2 & 0xffffu, far2 >> 16) > static_cast<uint32_t>(kAttQuiet);
       // (The factors fq are positive: the largest raw score gives the largest.)
-      const uint32_t most2 = __vmaxu2(__vmaxu2(sv[0][0], sv[0][1]), __vmaxu2(sv[1][0], sv[1][1]));
-      const int lane_top = static_cast<int>(max(most2 & 0xffffu, most2 >> 16));
-      bool raise = lane_top > ref;
       float most[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -529,7 +544,17 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
               o[nt][k][2 + c] = __fmul_rn(o[nt][k][2 + c], f);
             }
           }
-        const int top = __reduce_max_sync(0xffffffffu, lane_top);
+        const uint32_t top2 = __vmaxu2(__vmaxu2(sv[0][0], sv[0][1]), __vmaxu2(sv[1][0], sv[1][1]));
+        const int top = __reduce_max_sync(0xffffffffu, static_cast<int>(max(top2 & 0xffffu, top2 >> 16)));
+        // (A zero byte is a block of zeros, or of values under 6 x 2^-127, which count as zeros next to larger ones.)
+        uint32_t low2 = 0xffffffffu;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) low2 = __viaddmin_u16x2(sv[half][c], 0xffffffffu, low2);
+        uint32_t low = __reduce_min_sync(0xffffffffu, min(low2 & 0xffffu, low2 >> 16));
+        if (top > ref && ref > 0) low = min(low, static_cast<uint32_t>(max(ref - kAttQuiet, 1) - 1));  // of the steps not looked at
+        if (lane == 0) warp_low[warp] = min(warp_low[warp], low);
         if (top > ref) {
           const float f = exp2i(max(ref - top, -149));
           ref = top;
@@ -607,6 +632,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           row_l[warp][8 * nt + 2 * t + c] = x;
         }
       }
+    const uint32_t low = (warp_low[warp] + 1u) & 0xffffu;
+    if (lane == 0) warp_wide[warp] = ref - static_cast<int>(low) > kAttSpan;  // (without any value both are zero)
     __syncthreads();  // (the rings are drained too: `join` takes their place)
     const float back = exp2i(max(ref - 140, -149));
 #pragma unroll
@@ -626,6 +653,36 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
     __syncthreads();
     const bool whole = tile0 == 0 && tile1 == seq.tiles;
     float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (opens ? 0 : 1)) * Shape::kSlot;
+    if (__builtin_expect(warp_wide[0] | warp_wide[1] | warp_wide[2] | warp_wide[3], 0)) {
+      const AttSeq seq = att_seq<ROWS>(P, b);  // (read again: kept over the steps above, it would cost them registers)
+      for (int r = warp; r < n_rows; r += kAttWarps) {
+        const int i_q = (row0 + r) / P.group, h = head * P.group + (row0 + r) - i_q * P.group;
+        const int pos = seq.length - seq.queries + i_q;
+        const int from = max(seq.lo + tile0 * kAttTile, P.window > 0 ? pos - P.window + 1 : 0);
+        const int to = min(min(seq.lo + tile1 * kAttTile, seq.length), P.causal ? pos + 1 : seq.length);
+        float v[D / 32];
+        const float lse2 = row_wide<BF16, D>(
+            P, b, head, static_cast<const uint16_t*>(P.query) + static_cast<int64_t>(seq.q0 + i_q) * P.q_token + static_cast<int64_t>(h) * P.q_head,
+            from, to, v);
+        const int64_t row = static_cast<int64_t>(seq.q0 + i_q) * P.heads + h;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          const int d = lane * (D / 32) + c;
+          if (whole)
+            att_store<BF16>(P.out, row * D + d, v[c]);
+          else
+            slot[r * D + d] = v[c];
+        }
+        if (lane == 0) {
+          if (!whole)
+            slot[ROWS * D + r] = lse2;
+          else if (P.lse)
+            P.lse[row] = __fmul_rn(lse2, 0.69314718055994531f);
+        }
+      }
+      __syncthreads();
+      continue;
+    }
     for (int i = threadIdx.x; i < n_rows * D; i += kAttThreads) {
       const int r = i / D, d = i % D;
       float top = row_m[0][r];

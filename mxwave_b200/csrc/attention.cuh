@@ -7,11 +7,22 @@
 
 #include "common.cuh"
 #include "f16mma.cuh"
+#include "terms.cuh"
 
 namespace mxw {
 
 constexpr float kAttLift = 7.0f;    // probabilities are held as 2^(x - m + 7)
 constexpr float kAttSlack = 8.0f;   // and x may pass m by 8 before m is raised: at most 2^15
+// Both kernels hold values and probabilities in f16, relative to the largest of
+// each.  A value 2^28 below the largest would be lost, and a probability keeps
+// 2^-32 of its row's largest: good for any rows whose values' scales lie within
+// this many powers of two of one another (the probability's part is then 2^-12
+// of the smallest scale).  Rows with a wider range are done again by
+// att_row_wide, so that a key counts by its probability alone, and one that a
+// row does not see not at all.  That is a path for odd data (an overflowed
+// value, say): it takes 11 ms where 32 sequences of 1 to 65,536 keys take 0.19,
+// and 139 where four prompts of up to 3001 tokens take 0.57.
+constexpr int kAttSpan = 20;
 
 struct AttParams {
   const void* query;
@@ -60,6 +71,96 @@ __device__ __forceinline__ void att_clear_rest(const AttParams& P, int dim, int6
     att_store<BF16>(P.out, token * width + i % width, 0.0f);
     if (P.lse && i % width < P.heads) P.lse[token * P.heads + i % width] = -INFINITY;
   }
+}
+
+// One row in fp32 throughout, for rows whose values differ widely in size: every
+// key in [from, to) counts (pages outside the pool do not).  `q`: the row's D
+// elements; `o`: the lane's D / 32 channels of the result, from lane D / 32 on;
+// returns the log2 of the sum of exponentials.  The whole warp calls.  A lane
+// takes a key of 32 for the scores, then all take the keys' values in turn.
+// Values are held as 2^-22 of themselves: sums of 2^22 of the largest, 6 x 2^127,
+// do not overflow.
+template <bool BF16, int D>
+__device__ __forceinline__ float att_row_wide(const AttParams& P, int b, int head, const uint16_t* q, int from, int to, float (&o)[D / 32]) {
+  constexpr int VPL = D / 32, BLOCKS = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
+  const int64_t values = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows from a key to its value
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int c = 0; c < VPL; ++c) o[c] = 0.0f;
+  for (int k0 = from; k0 < to; k0 += 32) {
+    const int key = k0 + lane;
+    int64_t row = -1;
+    if (key < to) {
+      const int32_t page = table[key >> P.page_shift];
+      if (static_cast<uint32_t>(page) < static_cast<uint64_t>(P.pages))
+        row = ((static_cast<int64_t>(page) * 2 * P.kv_heads + head) << P.page_shift) + (key & ((1 << P.page_shift) - 1));
+    }
+    float x = -INFINITY;
+    if (row >= 0) {
+      x = 0.0f;
+#pragma unroll 1
+      for (int k = 0; k < BLOCKS; ++k) {
+        const uint4 codes = reinterpret_cast<const uint4*>(P.codes + row * (D / 2))[k];
+        const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+        float acc = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint4 qw = load_x8(q + 32 * k + 8 * w, true, P.q_vec);
+          const uint32_t qs[4] = {qw.x, qw.y, qw.z, qw.w};
+          uint32_t h[4];
+          e2m1x8_to_f16x2(words[w], h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+            float2 e;
+            if constexpr (BF16)
+              e = make_float2(bits_f32(qs[i] << 16), bits_f32(qs[i] & 0xffff0000u));
+            else
+              e = __half22float2(*reinterpret_cast<const __half2*>(&qs[i]));
+            acc = __fmaf_rn(e.x, c.x, acc);
+            acc = __fmaf_rn(e.y, c.y, acc);
+          }
+        }
+        x = __fmaf_rn(acc, exp2i(static_cast<int>(P.scales[row * BLOCKS + k]) - 127), x);
+      }
+      x = __fmul_rn(x, P.scale_log2);
+    }
+    float up = fmaxf(m, x);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, s));
+    const float f = m == up ? 1.0f : ex2(__fsub_rn(m, up));
+    m = up;
+    const float p = x == -INFINITY ? 0.0f : ex2(__fsub_rn(x, m));
+    l = __fmaf_rn(l, f, p);
+#pragma unroll
+    for (int c = 0; c < VPL; ++c) o[c] = __fmul_rn(o[c], f);
+    const int n = min(32, to - k0);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const float pj = __shfl_sync(0xffffffffu, p, j);
+      const int64_t at = __shfl_sync(0xffffffffu, row, j);
+      if (at < 0) continue;  // (the same for all lanes)
+      // (A whole word: of a narrower load the compiler's conversion took other bytes.)
+      const uint32_t word = reinterpret_cast<const uint32_t*>(P.codes + (at + values) * (D / 2))[lane * VPL / 8] >> (lane * VPL % 8 * 4);
+      const float scale = exp2i(static_cast<int>(P.scales[(at + values) * BLOCKS + lane * VPL / 32]) - 149);
+      uint32_t h[4];
+      e2m1x8_to_f16x2(word, h);
+#pragma unroll
+      for (int c = 0; c < VPL; c += 2) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[c / 2]));
+        o[c] = __fmaf_rn(pj, __fmul_rn(v.x, scale), o[c]);
+        o[c + 1] = __fmaf_rn(pj, __fmul_rn(v.y, scale), o[c + 1]);
+      }
+    }
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, s));
+  const bool seen = !(l == 0.0f);  // NaN counts as seen
+#pragma unroll
+  for (int c = 0; c < VPL; ++c) o[c] = seen ? __fmul_rn(__fdiv_rn(o[c], l), 4194304.0f) : 0.0f;
+  return seen ? __fadd_rn(m, log2f(l)) : -INFINITY;
 }
 
 // Prompts (attention_prompt.cu): whether the call takes that kernel, and its launch.

@@ -8,8 +8,9 @@
 //               they are cached; Q is split into E4M3 terms once (terms.cuh)
 //   O += P V    kind::f16: P from TMEM, V decoded to f16 in shared memory.  V's
 //               scales run across the contraction, so they are multiplied into
-//               the codes relative to the tile's largest (times 2^13), and that
-//               one is folded into P: exact down to 2^-27 of the tile's largest.
+//               the codes relative to the largest so far (times 2^13): exact
+//               down to 2^-27 of it, and rows with smaller ones are done again
+//               (kAttSpan).
 // Warps 0-3 and 4-7 are the softmax of the two row tiles, a thread a row: no
 // exchange between threads.  P = 2^(x - m + 7) is rounded to f16 (11 bits; the
 // sum is taken in fp32 before); m is raised only when a score passes it by 8, so
@@ -101,7 +102,8 @@ struct PromptUnit {
   int q0, queries, length;
   int rows;    // of this block's 256 (0: none)
   int row0;    // first, among the sequence's queries x group
-  int lo, hi;  // keys that some row sees
+  int first;   // key that some row sees
+  int lo, hi;  // and from it, rounded down to 16, to the last
   int tiles;
 };
 
@@ -116,7 +118,8 @@ __device__ __forceinline__ PromptUnit prompt_unit(const AttParams& P, int b, int
   u.rows = max(0, min(2 * kPromptRows, u.queries * P.group - row0));
   const int pos0 = u.length - u.queries + row0 / P.group;
   const int pos1 = u.length - u.queries + (row0 + max(u.rows, 1) - 1) / P.group;
-  u.lo = P.window > 0 ? max(0, pos0 - P.window + 1) / 16 * 16 : 0;
+  u.first = P.window > 0 ? max(0, pos0 - P.window + 1) : 0;
+  u.lo = u.first / 16 * 16;
   u.hi = P.causal ? max(0, min(pos1 + 1, u.length)) : u.length;
   u.tiles = max(0, (u.hi - u.lo + kPromptKeys - 1) / kPromptKeys);
   return u;
@@ -140,10 +143,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
   uint64_t* s_free = s_full + 2;
   uint64_t* p_full = s_free + 2;
   uint64_t* o_done = p_full + 2;
-  int* tile_ref = reinterpret_cast<int*>(o_done + 2);  // [3] largest scale byte of the values
+  int* tile_ref = reinterpret_cast<int*>(o_done + 2);  // [3] largest scale byte of the values up to the tile
   uint32_t* tile_in = reinterpret_cast<uint32_t*>(tile_ref + kPromptKv);  // [3][2] keys whose page is one of the pool's, as bits
   int* warp_ref = reinterpret_cast<int*>(tile_in + 2 * kPromptKv);           // [2][4]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(warp_ref + 8);
+  uint32_t* tile_low = reinterpret_cast<uint32_t*>(warp_ref + 8);  // [3] and the smallest but zero, less one
+  uint32_t* warp_low = tile_low + kPromptKv;                       // [2][4]
+  uint32_t* tmem_slot = warp_low + 8;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int head = blockIdx.x, b = blockIdx.y;
@@ -224,6 +229,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         const uint32_t p_t = tmem + lanes + Shape::kP + x * (kPromptKeys / 2);
         float m = -INFINITY, l = 0.0f;
         int ref = 0;  // scale byte that the accumulator is relative to
+        uint32_t low = 0xffffffffu;  // the smallest but zero so far, less one
         for (int t = 0; t < u.tiles; ++t) {
           const int n = count[x] + t;
           if (!__all_sync(0xffffffffu, mbar_wait_cycles(&s_full[x], n & 1))) {
@@ -241,6 +247,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             break;
           }
           const int ref_t = *reinterpret_cast<volatile int*>(&tile_ref[buf]);
+          low = min(low, *reinterpret_cast<volatile uint32_t*>(&tile_low[buf]));
           const uint32_t in0 = *reinterpret_cast<volatile uint32_t*>(&tile_in[2 * buf]);
           const uint32_t in1 = *reinterpret_cast<volatile uint32_t*>(&tile_in[2 * buf + 1]);
           tmem_wait_load();
@@ -299,10 +306,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
               }
             }
           }
-          // P is relative to the accumulator's reference (in the exponent); its
-          // sum is not.  Values 2^-40 of the reference are as good as nothing.
-          const int drop = min(ref - ref_t, 40);
-          const float base = __fsub_rn(kAttLift - static_cast<float>(drop), m == -INFINITY ? 0.0f : m);
+          const float base = __fsub_rn(kAttLift, m == -INFINITY ? 0.0f : m);
           const unsigned long long f2 = pack2(P.scale_log2, P.scale_log2), b2 = pack2(base, base);
           unsigned long long sum2 = 0ull, sum3 = 0ull;
           uint32_t p0[16], p1[16];
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
           tmem_store16(p_t, p0);
           tmem_store16(p_t + 16, p1);
           const struct f2 sums = unpack2(add2(sum2, sum3));
-          l = __fmaf_rn(__fadd_rn(sums.x, sums.y), exp2i(drop), l);
+          l = __fadd_rn(l, __fadd_rn(sums.x, sums.y));
           tmem_wait_store();
           tc_fence_before();
           __syncwarp();
@@ -337,6 +341,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         if (u.tiles > 0 && ok) {
           if (!__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (count[x] + u.tiles - 1) & 1))) ok = false;
           tc_fence_after();
+        }
+        const bool wide = ok && ref - static_cast<int>(low + 1u) > kAttSpan;  // the same in all warps of the block
+        if (wide) {
+          for (int k = 0; k < 32 && x * kPromptRows + 32 * quarter + k < u.rows; ++k) {
+            const int at_k = u.row0 + x * kPromptRows + 32 * quarter + k, i_k = at_k / P.group;
+            const int h_k = head * P.group + at_k - i_k * P.group, pos_k = u.length - u.queries + i_k;
+            float v[D / 32];
+            const float lse2 = att_row_wide<BF16, D>(
+                P, b, head, static_cast<const uint16_t*>(P.query) + static_cast<int64_t>(u.q0 + i_k) * P.q_token + static_cast<int64_t>(h_k) * P.q_head,
+                P.window > 0 ? max(0, pos_k - P.window + 1) : 0, P.causal ? min(pos_k + 1, u.length) : u.length, v);
+            const int64_t row_k = static_cast<int64_t>(u.q0 + i_k) * P.heads + h_k;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) att_store<BF16>(P.out, row_k * D + lane * (D / 32) + c, v[c]);
+            if (lane == 0 && P.lse) P.lse[row_k] = __fmul_rn(lse2, 0.69314718055994531f);
+          }
         }
         if (!ok) l = NAN;  // a wait gave up: NaN, whether or not anybody reads the flags
         const bool seen = !(l == 0.0f);  // NaN counts as seen
@@ -351,7 +370,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             tmem_load32(o_t + c, o);
             tmem_wait_load();
           }
-          if (live) {
+          if (live && !wide) {
 #pragma unroll
             for (int j = 0; j < 32; j += 8) {
               uint32_t w[4];
@@ -370,7 +389,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             }
           }
         }
-        if (live && P.lse) P.lse[out_row] = seen ? __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(l), kAttLift)), 0.69314718055994531f) : -INFINITY;
+        if (live && !wide && P.lse) P.lse[out_row] = seen ? __fmul_rn(__fadd_rn(m, __fsub_rn(log2f(l), kAttLift)), 0.69314718055994531f) : -INFINITY;
         tc_fence_before();
       }
     } else if (warp < 12) {
@@ -428,21 +447,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         }
         cp_async_commit();
       };
-      // The largest scale byte of a tile's values, by warps, a tile ahead; bit
-      // 8: a stray page.  Keys that no row sees have no say.
-      int sv[PIECES], sv_next[PIECES];
+      // The largest scale byte of a tile's values (bit 8: a stray page) and the
+      // smallest but zero, by warps, a tile ahead.  Keys that no row sees have no
+      // say.  (A zero byte is a block of zeros, or of values under 6 x 2^-127,
+      // which count as zeros next to larger ones.)
+      int sv[PIECES], sv_next[PIECES], ref = 0;
       auto find_top = [&](int t) {
         if (t >= u.tiles) return;
         const int n = kv + t;
         const uint8_t* vs = raw_smem + (n % kPromptRaw) * Shape::kRawStage + 2 * Shape::kRawCodes + Shape::kRawScales;
         int top = 0;
+        uint32_t low = 0xffffffffu;
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-          sv_next[j] = u.lo + t * kPromptKeys + key_e + 128 / BLOCKS * j < u.hi ? vs[e + 128 * j] : 0;
+          const int key = u.lo + t * kPromptKeys + key_e + 128 / BLOCKS * j;
+          sv_next[j] = key >= u.first && key < u.hi ? vs[e + 128 * j] : 0;
           top = max(top, sv_next[j]);
+          low = min(low, static_cast<uint32_t>(sv_next[j]) - 1u);
         }
         top = __reduce_max_sync(0xffffffffu, top | static_cast<int>((strays >> (n & 3)) & 1u) << 8);
-        if (lane == 0) warp_ref[(n & 1) * 4 + warp - 8] = top;
+        low = __reduce_min_sync(0xffffffffu, low);
+        if (lane == 0) {
+          warp_ref[(n & 1) * 4 + warp - 8] = top;
+          warp_low[(n & 1) * 4 + warp - 8] = low;
+        }
       };
       look_up(0);
       issue(0);
@@ -461,8 +489,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         issue(t + 3);
         const int* found = warp_ref + (n & 1) * 4;
         int top = max(max(found[0], found[1]), max(found[2], found[3]));
+        const uint32_t* lows = warp_low + (n & 1) * 4;
+        const uint32_t low = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
         const bool stray = top >= 256;
         if (stray) top = max(max(found[0] & 255, found[1] & 255), max(found[2] & 255, found[3] & 255));
+        ref = max(ref, top);
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) sv[j] = sv_next[j];
         find_top(t + 1);
@@ -470,7 +501,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
         const uint8_t* ks = raw + 2 * Shape::kRawCodes;
         if (n >= kPromptKv) ok = __all_sync(0xffffffffu, mbar_wait_cycles(&kv_empty[buf], (n / kPromptKv - 1) & 1));
         if (!ok) continue;  // to the barrier, where the other warps learn of it
-        if (e == 0) tile_ref[buf] = top;
+        if (e == 0) {
+          tile_ref[buf] = ref;
+          tile_low[buf] = low;
+        }
         if (e < kPromptKeys) {
           uint32_t bits = 0xffffffffu;
           if (stray) {
@@ -495,7 +529,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
           *reinterpret_cast<uint2*>(row + (((2 * p + 1) ^ (key & 7)) << 4)) = make_uint2(kw.z, kw.w);
           // Values: 32 channels to four 16-byte slots of the key's row in a box of 64 channels.
           const uint4 vw = reinterpret_cast<const uint4*>(raw + Shape::kRawCodes)[unit];
-          const int drop = top - sv[j];
+          const int drop = ref - sv[j];
           const uint32_t factor = drop < 28 ? static_cast<uint32_t>(28 - drop) << 10 : 0u;  // f16 2^(13 - drop)
           const uint32_t f2 = factor * 0x10001u;
           uint8_t* box = vd + (p >> 1) * (kPromptKeys * 128) + key * 128;
