@@ -4,16 +4,16 @@
 //
 // Each function does the call when everything about it is ordinary -- plain
 // strided CUDA tensors of the expected shapes and types, laid out as the C ABI
-// wants them, nothing watching (no dispatch mode, no gradient asked for) -- and
-// returns None, with nothing done, when it is not.  The public functions
-// (mxwave_b200/linear.py, kvcache.py) then take their general path, which
-// copies, dispatches or raises.  So no check lives here alone.
+// wants them, nothing watching (no dispatch mode, tracer or functorch level, no
+// gradient asked for) -- and returns None, with nothing done, when it is not.
+// The public functions (mxwave_b200/linear.py, kvcache.py) then take their
+// general path, which copies, dispatches or raises.  So no check lives here alone.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -30,7 +30,12 @@ int dtype_code(at::ScalarType t) {
   return t == at::kBFloat16 ? MXW_BF16 : t == at::kHalf ? MXW_F16 : t == at::kFloat ? MXW_F32 : -1;
 }
 
-bool watched() { return c10::impl::TorchDispatchModeTLS::stack_len() != 0; }
+// Whether something records or transforms operators on this thread: each such
+// thing adds keys to those that every call dispatches through.
+bool watched() {
+  constexpr c10::DispatchKeySet always({c10::DispatchKey::BackendSelect, c10::DispatchKey::ADInplaceOrView});
+  return !(c10::impl::tls_local_dispatch_key_set().included_ - always).empty();
+}
 
 // A plain tensor with memory of its own kind, or null.
 const at::Tensor* plain(PyObject* o) {

@@ -263,10 +263,16 @@ except ImportError:
     binding = None
 
 
+# What every call dispatches through.  A dispatch mode (FakeTensor, make_fx, before the
+# dispatch or in it), torch.jit's tracer and a functorch level (vmap) each add keys.
+_UNWATCHED = (torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect) | torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView)).raw_repr()
+
+
 def plain_eager(t: Tensor) -> bool:
     """Whether a call on `t` may skip the operator dispatch: an ordinary tensor, and
-    nothing (FakeTensor, tracing, compilation, another dispatch mode) is watching."""
-    return type(t) is Tensor and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
+    nothing (FakeTensor, tracing, compilation, a functorch transform, another dispatch mode) is watching."""
+    return (type(t) is Tensor and not torch.compiler.is_compiling()
+            and not torch._C._dispatch_tls_local_include_set().raw_repr() & ~_UNWATCHED)
 
 
 def _call(fn, index: int, args: tuple, what: str) -> None:

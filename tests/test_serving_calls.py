@@ -1,0 +1,112 @@
+"""Calls of the serving operators that the ordinary path must not take as they come: recorded, transformed and
+unusually bounded ones."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+from torch.fx.experimental.proxy_tensor import make_fx
+
+from mxwave_b200 import _lib, kvcache, ops
+from mxwave_b200.core import quantize_mxfp4
+from mxwave_b200.linear import linear_mxfp4
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _watchers():
+    """Ways to run f(t) under something that records or transforms its operators."""
+    return {
+        "jit": lambda f, t: torch.jit.trace(f, (t,), check_trace=False),
+        "pre-dispatch": lambda f, t: make_fx(f, pre_dispatch=True)(t),
+        "dispatch": lambda f, t: make_fx(f)(t),
+        "vmap": lambda f, t: torch.vmap(f)(t),
+        "functionalize": lambda f, t: torch.func.functionalize(f)(t),
+    }
+
+
+def _gen(seed: int) -> torch.Generator:
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g: torch.Generator, *shape: int) -> torch.Tensor:
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def _pool(g: torch.Generator, lengths: list[int], heads: int = 2, page: int = 16, dim: int = 64):
+    """codes, scales, table, lengths of sequences of random rows."""
+    need = [-(-n // page) for n in lengths]
+    shape = (sum(need) + 1, 2, heads, page)
+    codes = torch.zeros(*shape, dim // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(*shape, dim // 32, dtype=torch.uint8, device="cuda")
+    rows = shape[0] * page
+    kvcache.append_mxfp4_(codes, scales, _randn(g, rows, heads, dim), _randn(g, rows, heads, dim), torch.arange(rows, device="cuda"))
+    table = torch.zeros(len(lengths), max(need), dtype=torch.int32, device="cuda")
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(sum(need[:b]), sum(need[:b]) + n)
+    return codes, scales, table, torch.tensor(lengths, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("name", sorted(_watchers()))
+def test_what_watches_is_noticed(name: str) -> None:
+    found = []
+
+    def f(t: torch.Tensor) -> torch.Tensor:
+        found.append(ops.plain_eager(t))
+        return t + 1
+
+    assert ops.plain_eager(torch.ones(3))
+    with torch.inference_mode():
+        assert ops.plain_eager(torch.ones(3))
+    with torch.autocast("cpu", dtype=BF):
+        assert ops.plain_eager(torch.ones(3))
+    _watchers()[name](f, torch.ones(3))
+    assert found and not any(found)
+    assert ops.plain_eager(torch.ones(3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["jit", "pre-dispatch", "dispatch"])
+def test_recorded_calls_run_the_operators(name: str) -> None:
+    g = _gen(1)
+    packed, scales = quantize_mxfp4(_randn(g, 96, 64), method="rtn")
+    pool = _pool(g, [40, 3])
+    start = torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda")
+
+    def product(x: torch.Tensor) -> torch.Tensor:
+        return linear_mxfp4(x, packed, scales, activation="silu", residual=x[:, :1].expand(-1, 96))
+
+    def attention(q: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return kvcache.paged_attention_mxfp4(q, *pool, start, max_length=40, max_queries=2, return_lse=True)
+
+    def rows(r: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        codes, sc = torch.zeros_like(pool[0]), torch.zeros_like(pool[1])
+        slots = torch.arange(5, device="cuda")
+        kvcache.append_mxfp4_(codes, sc, r, r + 1, slots)
+        kvcache.copy_pages_(codes[None], sc[None], torch.tensor([0]), torch.tensor([2]))
+        return kvcache.gather_mxfp4(codes, sc, slots + 32, torch.float32)
+
+    for f, shape in ((product, (5, 64)), (attention, (3, 4, 64)), (rows, (5, 2, 64))):
+        first, other = _randn(g, *shape).to(BF), _randn(g, *shape).to(BF)
+        graph = _watchers()[name](f, first)
+        for t in (other, first):
+            torch.empty(1 << 20, device="cuda").fill_(float("nan"))  # what an unwritten output would be made of
+            got, want = graph(t), f(t)
+            for a, b in zip((got,) if torch.is_tensor(got) else got, (want,) if torch.is_tensor(want) else want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_vmap_runs_slice_by_slice() -> None:
+    g = _gen(2)
+    packed, scales = quantize_mxfp4(_randn(g, 96, 64), method="rtn")
+    x = _randn(g, 4, 5, 64).to(BF)
+    got = torch.vmap(lambda t: linear_mxfp4(t, packed, scales))(x)
+    assert torch.equal(got, torch.stack([linear_mxfp4(t, packed, scales) for t in x]))
+    pool = _pool(g, [40, 3])
+    start = torch.tensor([0, 2, 3], dtype=torch.int32, device="cuda")
+    q = _randn(g, 4, 3, 4, 64).to(BF)
+    attend = lambda t: kvcache.paged_attention_mxfp4(t, *pool, start, max_length=40, max_queries=2)  # noqa: E731
+    assert torch.equal(torch.vmap(attend)(q), torch.stack([attend(t) for t in q]))
