@@ -887,7 +887,8 @@ using namespace mxw;
 
 extern "C" size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,
                                                      int64_t max_length, int64_t max_queries) {
-  if (!att_shape_ok(seqs, heads, kv_heads, dim, max_length, max_queries) || seqs == 0 || max_queries == 0) return 0;
+  if (!att_shape_ok(seqs, heads, kv_heads, dim, max_length, max_queries) || seqs == 0) return 0;
+  max_queries = std::max<int64_t>(max_queries, 1);  // (0 may be wrong too: the starts decide)
   if (attention_prompt_fits(seqs, heads, kv_heads, max_queries)) return 16;  // nothing is shared between blocks
   return att_plan(seqs, heads, kv_heads, dim, max_length, max_queries, 0).bytes;  // (a window needs no more)
 }
@@ -908,13 +909,14 @@ extern "C" int mxw_paged_attention(const void* query, int dtype, int64_t tokens,
   if (tokens == 0) return MXW_OK;
   if (!query || !out || reinterpret_cast<uintptr_t>(out) % 16 != 0) return MXW_EINVAL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (seqs == 0 || max_queries == 0) {
-    // No sequence has a query: every row is one that no key reaches.
+  if (seqs == 0) {
+    // Every row is one that no key reaches.
     return lse ? MXW_EUNSUPPORTED
                : (cudaMemsetAsync(out, 0, static_cast<size_t>(tokens * heads * dim) * 2, s) == cudaSuccess
                       ? MXW_OK
                       : record_cuda_error(cudaGetLastError()));
   }
+  max_queries = std::max<int64_t>(max_queries, 1);
   if (!codes || !scales || !lengths || !start || (table_width > 0 && !table)) return MXW_EINVAL;
   if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0) return MXW_EINVAL;
   const AttPlan plan = att_plan(seqs, heads, kv_heads, dim, max_length, max_queries, std::min<int64_t>(window, 0x3fffffff));

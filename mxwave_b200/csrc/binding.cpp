@@ -222,7 +222,7 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const double scale = args[8] == Py_None ? 1.0 / std::sqrt(static_cast<double>(p.dim)) : PyFloat_CheckExact(args[8]) ? PyFloat_AS_DOUBLE(args[8]) : 0.0;
   const bool causal = PyObject_IsTrue(args[9]) == 1, want_lse = PyObject_IsTrue(args[11]) == 1;
-  if (max_length < 0 || max_queries < 1 || window < 0 || (window > 0 && !causal) || !(scale > 0.0) || !std::isfinite(scale)) return none();
+  if (max_length < 0 || max_queries < 0 || window < 0 || (window > 0 && !causal) || !(scale > 0.0) || !std::isfinite(scale)) return none();
   const c10::cuda::CUDAGuard guard(device);
   at::Tensor out = at::empty({tokens, heads, p.dim}, query->options());
   at::Tensor lse = want_lse ? at::empty({tokens, heads}, query->options().dtype(at::kFloat)) : at::Tensor();

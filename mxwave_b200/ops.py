@@ -390,7 +390,7 @@ def _paged_attention_mxfp4(query: Tensor, codes: Tensor, scales: Tensor, table: 
     tokens, heads, dim = query.shape
     pages, _two, kv_heads, page, _half = codes.shape
     seqs, width = table.shape
-    if tokens == 0 or seqs == 0 or max_queries == 0:
+    if tokens == 0 or seqs == 0:
         if lse is not None:
             lse.fill_(float("-inf"))
         return query.new_zeros((tokens, heads, dim))

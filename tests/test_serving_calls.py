@@ -110,3 +110,27 @@ def test_vmap_runs_slice_by_slice() -> None:
     q = _randn(g, 4, 3, 4, 64).to(BF)
     attend = lambda t: kvcache.paged_attention_mxfp4(t, *pool, start, max_length=40, max_queries=2)  # noqa: E731
     assert torch.equal(torch.vmap(attend)(q), torch.stack([attend(t) for t in q]))
+
+
+@pytest.mark.parametrize("lengths", [100, 5000])
+def test_a_bound_of_no_queries_sizes_the_launch_for_one(lengths: int) -> None:
+    lib = _lib.load()
+    assert lib.mxw_paged_attention_workspace_size(2, 8, 2, 64, lengths, 0) == lib.mxw_paged_attention_workspace_size(2, 8, 2, 64, lengths, 1) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("queries", [[1, 1], [3, 0], [90, 40], [0, 0]])
+def test_a_bound_of_no_queries_costs_speed_only(queries: list[int], monkeypatch) -> None:
+    g = _gen(3)
+    codes, scales, table, lengths = _pool(g, [200, 77])
+    start = torch.tensor([0, queries[0], sum(queries)], dtype=torch.int32, device="cuda")
+    q = _randn(g, sum(queries) + 2, 4, 64).to(BF)
+    run = lambda most: kvcache.paged_attention_mxfp4(q, codes, scales, table, lengths, start, max_length=200, max_queries=most,  # noqa: E731
+                                                     return_lse=True)
+    want = run(1)
+    assert (want[0][: sum(queries)] != 0).any() == (sum(queries) > 0)
+    for _ in range(2):
+        out, lse = run(0)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        assert (out[sum(queries) :] == 0).all() and (lse[sum(queries) :] == -math.inf).all()
+        monkeypatch.setattr(ops, "binding", None)
