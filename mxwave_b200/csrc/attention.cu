@@ -650,12 +650,21 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         for (int k = 0; k < STEPS; ++k)
           dst[k] = make_float2(__fmul_rn(__fmul_rn(o[nt][k][c], f), back), __fmul_rn(__fmul_rn(o[nt][k][2 + c], f), back));
       }
-    __syncthreads();
+    // A row without a sum sees no key of the segment, or its infinite query made every score -infinity and it is NaN.
+    auto empty = [&](int r) {
+      bool none = true;
+#pragma unroll
+      for (int w = 0; w < kAttWarps; ++w) none &= row_l[w][r] == 0.0f;
+      return none;
+    };
+    const bool again = __syncthreads_or(threadIdx.x < n_rows && empty(threadIdx.x));
+    const bool wide = warp_wide[0] | warp_wide[1] | warp_wide[2] | warp_wide[3];
     const bool whole = tile0 == 0 && tile1 == seq.tiles;
     float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (opens ? 0 : 1)) * Shape::kSlot;
-    if (__builtin_expect(warp_wide[0] | warp_wide[1] | warp_wide[2] | warp_wide[3], 0)) {
+    if (__builtin_expect(again | wide, 0)) {
       const AttSeq seq = att_seq<ROWS>(P, b);  // (read again: kept over the steps above, it would cost them registers)
       for (int r = warp; r < n_rows; r += kAttWarps) {
+        if (!wide && !empty(r)) continue;
         const int i_q = (row0 + r) / P.group, h = head * P.group + (row0 + r) - i_q * P.group;
         const int pos = seq.length - seq.queries + i_q;
         const int from = max(seq.lo + tile0 * kAttTile, P.window > 0 ? pos - P.window + 1 : 0);
@@ -680,10 +689,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
             P.lse[row] = __fmul_rn(lse2, 0.69314718055994531f);
         }
       }
-      __syncthreads();
-      continue;
     }
-    for (int i = threadIdx.x; i < n_rows * D; i += kAttThreads) {
+    for (int i = threadIdx.x; i < n_rows * D && !wide; i += kAttThreads) {
       const int r = i / D, d = i % D;
       float top = row_m[0][r];
 #pragma unroll
@@ -695,9 +702,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         sum = __fadd_rn(sum, __fmul_rn(row_l[w][r], f));
         acc = __fadd_rn(acc, join[(w * ROWS + r) * D + d]);
       }
-      const bool seen = !(sum == 0.0f);  // NaN counts as seen
-      const float v = seen ? __fdiv_rn(acc, sum) : 0.0f;
-      const float lse2 = seen ? __fadd_rn(top, __fsub_rn(log2f(sum), kAttLift)) : -INFINITY;
+      if (empty(r)) continue;  // (done above)
+      const float v = __fdiv_rn(acc, sum);
+      const float lse2 = __fadd_rn(top, __fsub_rn(log2f(sum), kAttLift));
       if (whole) {
         const int i_q = (row0 + r) / P.group;
         const int64_t row = static_cast<int64_t>(seq.q0 + i_q) * P.heads + head * P.group + (row0 + r) - i_q * P.group;

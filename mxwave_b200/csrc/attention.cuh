@@ -24,6 +24,10 @@ constexpr float kAttSlack = 8.0f;   // and x may pass m by 8 before m is raised:
 // and 139 where four prompts of up to 3001 tokens take 0.57.
 constexpr int kAttSpan = 20;
 
+// The bits of infinity in the queries' type; what has more is NaN.
+template <bool BF16>
+constexpr uint32_t kAttInf = BF16 ? 0x7f80u : 0x7c00u;
+
 struct AttParams {
   const void* query;
   int64_t q_token, q_head;  // strides in elements
@@ -87,8 +91,13 @@ __device__ __forceinline__ float att_row_wide(const AttParams& P, int b, int hea
   const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
   const int64_t values = static_cast<int64_t>(P.kv_heads) << P.page_shift;  // rows from a key to its value
   float m = -INFINITY, l = 0.0f;
+  bool odd = false;
 #pragma unroll
-  for (int c = 0; c < VPL; ++c) o[c] = 0.0f;
+  for (int c = 0; c < VPL; ++c) {
+    o[c] = 0.0f;
+    odd |= (q[lane * VPL + c] & 0x7fffu) >= kAttInf<BF16>;
+  }
+  odd = __any_sync(0xffffffffu, odd);  // the row is NaN if it sees a key
   for (int k0 = from; k0 < to; k0 += 32) {
     const int key = k0 + lane;
     int64_t row = -1;
@@ -125,7 +134,7 @@ __device__ __forceinline__ float att_row_wide(const AttParams& P, int b, int hea
         }
         x = __fmaf_rn(acc, exp2i(static_cast<int>(P.scales[row * BLOCKS + k]) - 127), x);
       }
-      x = __fmul_rn(x, P.scale_log2);
+      x = odd ? NAN : __fmul_rn(x, P.scale_log2);
     }
     float up = fmaxf(m, x);
 #pragma unroll

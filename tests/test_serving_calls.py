@@ -134,3 +134,30 @@ def test_a_bound_of_no_queries_costs_speed_only(queries: list[int], monkeypatch)
         assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
         assert (out[sum(queries) :] == 0).all() and (lse[sum(queries) :] == -math.inf).all()
         monkeypatch.setattr(ops, "binding", None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("length, queries", [(40, 1), (3000, 3), (300, 150)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_an_infinite_query_gives_nan(dtype: torch.dtype, length: int, queries: int, wide: bool) -> None:
+    """Also where the infinity makes every score -infinity; rows that no key reaches stay zero."""
+    g = _gen(4)
+    codes, scales, table, lengths = _pool(g, [length, length], heads=16)
+    codes[:, 0, ..., 0] = 0xAA  # the first two channels of every key: -1 times the scale
+    if wide:
+        scales[:, 1, ..., 3, :] = 20  # values far smaller than the others
+    lengths[1] = 0
+    start = torch.tensor([0, queries, 2 * queries], dtype=torch.int32, device="cuda")
+    q = _randn(g, 2 * queries, 16, 64).to(dtype)
+    run = lambda: kvcache.paged_attention_mxfp4(q, codes, scales, table, lengths, start, max_length=length, max_queries=queries,  # noqa: E731
+                                                return_lse=True)
+    clean, _ = run()
+    bad = torch.zeros(2 * queries, 16, dtype=torch.bool, device="cuda")
+    for row, head, value in ((0, 0, math.inf), (queries - 1, 3, -math.inf), (queries, 5, math.inf)):
+        q[row, head, 0] = value
+        bad[row, head] = True
+    out, lse = run()
+    assert out[:queries][bad[:queries]].isnan().all() and lse[:queries][bad[:queries]].isnan().all()
+    assert torch.equal(out[~bad], clean[~bad])
+    assert (out[queries:] == 0).all() and (lse[queries:] == -math.inf).all()
