@@ -47,7 +47,7 @@ const at::Tensor* on_cuda(PyObject* o) {
   const at::Tensor* t = plain(o);
   return t && t->is_cuda() ? t : nullptr;
 }
-bool wants_gradient(const at::Tensor* t) { return t && c10::GradMode::is_enabled() && t->requires_grad(); }
+bool wants_gradient(const at::Tensor* t) { return t && ((c10::GradMode::is_enabled() && t->requires_grad()) || t->_fw_grad(0).defined()); }
 bool aligned16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 bool bytes_like(const at::Tensor& t, int64_t dim) { return t.scalar_type() == at::kByte && t.dim() == dim && t.is_contiguous(); }
 

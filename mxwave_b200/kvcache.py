@@ -200,7 +200,7 @@ def paged_attention_mxfp4(
     scale = dim**-0.5 if softmax_scale is None else float(softmax_scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
-    if torch.is_grad_enabled() and query.requires_grad:
+    if ops.wants_gradient(query):
         raise RuntimeError("paged_attention_mxfp4 has no gradient: call it under torch.no_grad()")
     if table.stride(1) != 1 or table.stride(0) < table.shape[1]:
         table = table.contiguous()

@@ -78,7 +78,7 @@ def _check(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, bias: to
     for t in (packed, scales, bias, residual):
         if t is not None and t.device != device:
             raise ValueError(f"x is on {device}, another argument is on {t.device}")
-    if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad or residual is not None and residual.requires_grad):
+    if ops.wants_gradient(x, bias, residual):
         raise RuntimeError("linear_mxfp4 has no gradient: call it under torch.no_grad()")
 
 

@@ -49,6 +49,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -273,6 +274,13 @@ def plain_eager(t: Tensor) -> bool:
     nothing (FakeTensor, tracing, compilation, a functorch transform, another dispatch mode) is watching."""
     return (type(t) is Tensor and not torch.compiler.is_compiling()
             and not torch._C._dispatch_tls_local_include_set().raw_repr() & ~_UNWATCHED)
+
+
+def wants_gradient(*tensors: Tensor | None) -> bool:
+    """Whether a derivative is asked for: a backward pass, or the tangents of a forward one."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _call(fn, index: int, args: tuple, what: str) -> None:

@@ -161,3 +161,22 @@ def test_an_infinite_query_gives_nan(dtype: torch.dtype, length: int, queries: i
     assert out[:queries][bad[:queries]].isnan().all() and lse[:queries][bad[:queries]].isnan().all()
     assert torch.equal(out[~bad], clean[~bad])
     assert (out[queries:] == 0).all() and (lse[queries:] == -math.inf).all()
+
+
+@pytest.mark.gpu
+def test_forward_mode_gradients_are_refused() -> None:
+    import torch.autograd.forward_ad as forward
+
+    g = _gen(5)
+    packed, scales = quantize_mxfp4(_randn(g, 32, 64), method="rtn")
+    pool = _pool(g, [20])
+    start = torch.tensor([0, 2], dtype=torch.int32, device="cuda")
+    x, bias, q = _randn(g, 2, 64).to(BF), _randn(g, 32).to(BF), _randn(g, 2, 4, 64).to(BF)
+    with forward.dual_level():
+        dual = lambda t: forward.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: linear_mxfp4(dual(x), packed, scales), lambda: linear_mxfp4(x, packed, scales, dual(bias)),
+                     lambda: linear_mxfp4(x, packed, scales, residual=dual(x[:, :32])),
+                     lambda: kvcache.paged_attention_mxfp4(dual(q), *pool, start, max_length=20, max_queries=2)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+        assert linear_mxfp4(x, packed, scales, bias).isfinite().all()  # nothing asks for one here
