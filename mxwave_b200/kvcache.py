@@ -19,6 +19,7 @@ from __future__ import annotations
 import heapq
 from collections.abc import Iterable, Sequence
 from dataclasses import dataclass, field
+from operator import index
 
 import torch
 
@@ -116,16 +117,8 @@ def copy_pages_(
     """
     if ops.binding is not None and not torch.compiler.is_compiling() and ops.binding.copy_pages(codes, scales, source, target):
         return
+    source, target = _page_numbers("source", source), _page_numbers("target", target)
     _check_pool(codes, scales, layers=True)
-    if not isinstance(source, torch.Tensor):
-        source = torch.tensor(source, dtype=torch.int64)
-    if not isinstance(target, torch.Tensor):
-        target = torch.tensor(target, dtype=torch.int64)
-    if source.dtype.is_floating_point or target.dtype.is_floating_point:
-        raise ValueError("source and target must hold whole numbers")
-    source, target = source.to(torch.int64), target.to(torch.int64)
-    if source.device.type != "cpu" or target.device.type != "cpu":
-        raise ValueError("source and target are page numbers on the host")
     if source.ndim != 1 or source.shape != target.shape:
         raise ValueError(f"source and target must be vectors of one length, got {tuple(source.shape)} and {tuple(target.shape)}")
     args = (codes, scales, source.contiguous(), target.contiguous())
@@ -221,6 +214,17 @@ def _written(*tensors: torch.Tensor) -> None:
             torch.autograd.graph.increment_version(t)
 
 
+def _page_numbers(name: str, pages: torch.Tensor | Sequence[int]) -> torch.Tensor:
+    """Page numbers as a host tensor of int64."""
+    if not isinstance(pages, torch.Tensor):
+        pages = torch.tensor([index(page) for page in pages], dtype=torch.int64)
+    if pages.dtype == torch.bool or pages.dtype.is_floating_point or pages.dtype.is_complex:
+        raise ValueError(f"{name} must hold whole numbers, got {pages.dtype}")
+    if pages.device.type != "cpu":
+        raise ValueError(f"{name} holds page numbers on the host, got a tensor on {pages.device}")
+    return pages.to(torch.int64)
+
+
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     """`t` with unit stride over its last dimension (other strides may be anything)."""
     return t if t.stride(-1) == 1 else t.contiguous()
@@ -296,7 +300,7 @@ class PageBooks:
 
     def truncate(self, seq: int, length: int) -> None:
         """Drop the tokens from `length` on."""
-        held = self._get(seq)
+        held, length = self._get(seq), index(length)
         if not 0 <= length <= held.length:
             raise ValueError(f"length must be in [0, {held.length}], got {length}")
         keep = -(-length // self.page_tokens)
@@ -310,6 +314,7 @@ class PageBooks:
 
         Raises, and changes nothing, when the free pages do not suffice.
         """
+        tokens = [index(n) for n in tokens]
         if len(seqs) != len(tokens):
             raise ValueError(f"{len(seqs)} sequences, {len(tokens)} token counts")
         if len(set(seqs)) != len(seqs):
@@ -428,7 +433,7 @@ class PagedKVCache:
 
         Raises RuntimeError, and changes nothing, when the pool is full.
         """
-        seqs, new_tokens = list(seqs), [int(n) for n in new_tokens]
+        seqs, new_tokens = list(seqs), [index(n) for n in new_tokens]
         if not seqs:
             raise ValueError("a step needs at least one sequence")
         copies = self.books.grow(seqs, new_tokens)

@@ -180,3 +180,25 @@ def test_forward_mode_gradients_are_refused() -> None:
             with pytest.raises(RuntimeError, match="no gradient"):
                 call()
         assert linear_mxfp4(x, packed, scales, bias).isfinite().all()  # nothing asks for one here
+
+
+@pytest.mark.parametrize("source, target, error", [
+    ([0.5], [1], TypeError), ([0], [1.9], TypeError), (["0"], [1], TypeError), (torch.tensor([0.0]), [1], ValueError),
+    ([0], torch.tensor([True]), ValueError),
+])
+def test_page_numbers_are_whole(source, target, error: type) -> None:
+    codes, scales = torch.zeros(2, 4, 2, 1, 16, 32, dtype=torch.uint8), torch.zeros(2, 4, 2, 1, 16, 2, dtype=torch.uint8)
+    with pytest.raises(error):
+        kvcache.copy_pages_(codes, scales, source, target)
+
+
+def test_token_counts_are_whole() -> None:
+    cache = kvcache.PagedKVCache(8, kv_heads=1, head_dim=64, page_tokens=16, device="cpu")
+    seq = cache.add()
+    with pytest.raises(TypeError):
+        cache.plan([seq], [1.9])
+    with pytest.raises(TypeError):
+        cache.books.grow([seq], [1.9])
+    with pytest.raises(TypeError):
+        cache.truncate(seq, 0.0)
+    assert cache.books.length(seq) == 0 and cache.plan([seq], torch.tensor([2])).lengths.tolist() == [2]
