@@ -4,6 +4,9 @@ unusually bounded ones."""
 from __future__ import annotations
 
 import math
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -202,3 +205,15 @@ def test_token_counts_are_whole() -> None:
     with pytest.raises(TypeError):
         cache.truncate(seq, 0.0)
     assert cache.books.length(seq) == 0 and cache.plan([seq], torch.tensor([2])).lengths.tolist() == [2]
+
+
+def test_the_library_builds_without_the_binding(tmp_path: Path) -> None:
+    """Users of the C ABI alone need no torch headers: `make` ends well without the host binding, `make binding` says so."""
+    root = Path(__file__).resolve().parents[1]
+    shutil.copytree(root / "mxwave_b200" / "csrc", tmp_path / "mxwave_b200" / "csrc")
+    shutil.copytree(root / "include", tmp_path / "include")
+    make = ["make", "-C", str(tmp_path / "mxwave_b200" / "csrc"), "NVCC=true", "CXX=false", "PYTHON=false"]
+    done = subprocess.run(make, capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
+    assert "built ../_native/libmxwave_b200.so" in done.stdout and "torch's headers" in done.stdout
+    assert subprocess.run([*make, "binding"], capture_output=True).returncode != 0
