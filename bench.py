@@ -685,6 +685,10 @@ def run_decoder_layer(args, dev) -> dict:
     from mxwave_b200.core import quantize_into
 
     _reference_importable()
+    try:
+        import mxwave.calibration_stream  # noqa: F401  -- the planner that calibration_stream runs
+    except ImportError:
+        return {"unavailable": "reference package not installed in baseline/_ref"}
     cfg = synthetic.decoder_config(layers=1)
     seqs, length = 128, 2048
     g = torch.Generator().manual_seed(44)
