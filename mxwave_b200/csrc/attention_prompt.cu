@@ -181,9 +181,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
   int kv = 0;     // key tiles so far (all roles count alike)
   int count[2] = {0, 0};  // key tiles so far of each row tile
   int made[2] = {0, 0};   // and its sets of queries
-  for (int z = n_units - 1 - static_cast<int>(blockIdx.z); z >= 0 && ok; z -= static_cast<int>(gridDim.z)) {
+  for (int z = n_units - 1 - static_cast<int>(blockIdx.z); z >= 0; z -= static_cast<int>(gridDim.z)) {
     const PromptUnit u = prompt_unit(P, b, z * 2 * kPromptRows);
     if (u.rows == 0) continue;
+    if (!ok) {  // a wait gave up: no more waits, and what this warp would have written is NaN
+      for (int r = 32 * warp; warp < 8 && r < min(32 * warp + 32, u.rows); ++r) {
+        const int at = u.row0 + r, i_q = at / P.group;
+        const int64_t row = static_cast<int64_t>(u.q0 + i_q) * P.heads + head * P.group + (at - i_q * P.group);
+        for (int c = lane; c < D; c += 32) att_store<BF16>(P.out, row * D + c, NAN);
+        if (lane == 0 && P.lse) P.lse[row] = NAN;
+      }
+      continue;
+    }
     const bool second = u.rows > kPromptRows;
 
     if (warp < 8) {
