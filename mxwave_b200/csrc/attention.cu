@@ -78,6 +78,8 @@ constexpr int kAttWhole = 12, kAttWholeFew = 6;
 // 192 (32 sequences of 1 to 65,536 keys; 187 without a look at the range).  A rise
 // of the largest by more than kAttSpan - kAttQuiet then counts as a wide range.
 constexpr int kAttQuiet = 10;
+// Partial results are this much of themselves: 6 x 2^127, an overflowed value, is finite, and nothing where its share weighs nothing.
+constexpr float kAttPartial = 0.0625f;
 
 // One sequence's share of the work.
 struct AttSeq {
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
   __shared__ int64_t red[kAttWarps];
   __shared__ float row_m[kAttWarps][ROWS], row_l[kAttWarps][ROWS];
   __shared__ uint32_t warp_low[kAttWarps];  // the smallest scale but zero of the values so far, less one (or a bound: see kAttQuiet)
-  __shared__ int warp_wide[kAttWarps];
+  __shared__ int warp_ref[kAttWarps];       // ref below; 256 where the range is wide
   grid_dependents_launch();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -633,9 +635,10 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         }
       }
     const uint32_t low = (warp_low[warp] + 1u) & 0xffffu;
-    if (lane == 0) warp_wide[warp] = ref - static_cast<int>(low) > kAttSpan;  // (without any value both are zero)
+    if (lane == 0) warp_ref[warp] = ref - static_cast<int>(low) > kAttSpan ? 256 : ref;  // (without any value both are zero)
     __syncthreads();  // (the rings are drained too: `join` takes their place)
-    const float back = exp2i(max(ref - 140, -149));
+    const int ref_all = max(max(warp_ref[0], warp_ref[1]), max(warp_ref[2], warp_ref[3]));
+    const float back = exp2i(max(ref - ref_all, -149));  // (to the values' own size only when divided: the sums could overflow)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -658,7 +661,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       return none;
     };
     const bool again = __syncthreads_or(threadIdx.x < n_rows && empty(threadIdx.x));
-    const bool wide = warp_wide[0] | warp_wide[1] | warp_wide[2] | warp_wide[3];
+    const bool wide = ref_all == 256;
     const bool whole = tile0 == 0 && tile1 == seq.tiles;
     float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (opens ? 0 : 1)) * Shape::kSlot;
     if (__builtin_expect(again | wide, 0)) {
@@ -678,9 +681,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         for (int c = 0; c < D / 32; ++c) {
           const int d = lane * (D / 32) + c;
           if (whole)
-            att_store<BF16>(P.out, row * D + d, v[c]);
+            att_store<BF16>(P.out, row * D + d, __fmul_rn(v[c], kAttWideUnit));
           else
-            slot[r * D + d] = v[c];
+            slot[r * D + d] = __fmul_rn(v[c], kAttWideUnit * kAttPartial);
         }
         if (lane == 0) {
           if (!whole)
@@ -704,14 +707,15 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       }
       if (empty(r)) continue;  // (done above)
       const float v = __fdiv_rn(acc, sum);
+      const int unit = ref_all - 140;  // exponent of the values' unit
       const float lse2 = __fadd_rn(top, __fsub_rn(log2f(sum), kAttLift));
       if (whole) {
         const int i_q = (row0 + r) / P.group;
         const int64_t row = static_cast<int64_t>(seq.q0 + i_q) * P.heads + head * P.group + (row0 + r) - i_q * P.group;
-        att_store<BF16>(P.out, row * D + d, v);
+        att_store<BF16>(P.out, row * D + d, __fmul_rn(v, exp2i(unit)));
         if (P.lse && d == 0) P.lse[row] = __fmul_rn(lse2, 0.69314718055994531f);
       } else {
-        slot[r * D + d] = v;
+        slot[r * D + d] = __fmul_rn(v, exp2i(unit - 4));  // (kAttPartial)
         if (d == 0) slot[ROWS * D + r] = lse2;
       }
     }
@@ -816,7 +820,7 @@ __global__ void __launch_bounds__(kAttJoinThreads) attention_join_kernel(const A
         const int64_t row = static_cast<int64_t>(seq.q0 + i_q) * P.heads + head * P.group + (row0 + r) - i_q * P.group;
         const float v[4] = {acc[e].x, acc[e].y, acc[e].z, acc[e].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) att_store<BF16>(P.out, row * D + d + k, seen ? __fdiv_rn(v[k], sum) : 0.0f);
+        for (int k = 0; k < 4; ++k) att_store<BF16>(P.out, row * D + d + k, seen ? __fmul_rn(__fdiv_rn(v[k], sum), 1.0f / kAttPartial) : 0.0f);
         if (P.lse && d == 0) P.lse[row] = seen ? __fmul_rn(__fadd_rn(row_top[r], log2f(sum)), 0.69314718055994531f) : -INFINITY;
       }
     }

@@ -82,8 +82,9 @@ __device__ __forceinline__ void att_clear_rest(const AttParams& P, int dim, int6
 // elements; `o`: the lane's D / 32 channels of the result, from lane D / 32 on;
 // returns the log2 of the sum of exponentials.  The whole warp calls.  A lane
 // takes a key of 32 for the scores, then all take the keys' values in turn.
-// Values are held as 2^-22 of themselves: sums of 2^22 of the largest, 6 x 2^127,
-// do not overflow.
+// Values, and the result, are 2^-22 of themselves: sums of 2^22 of the largest,
+// 6 x 2^127, do not overflow.
+constexpr float kAttWideUnit = 4194304.0f;
 template <bool BF16, int D>
 __device__ __forceinline__ float att_row_wide(const AttParams& P, int b, int head, const uint16_t* q, int from, int to, float (&o)[D / 32]) {
   constexpr int VPL = D / 32, BLOCKS = D / 32;
@@ -168,7 +169,7 @@ __device__ __forceinline__ float att_row_wide(const AttParams& P, int b, int hea
   for (int s = 16; s > 0; s >>= 1) l = __fadd_rn(l, __shfl_xor_sync(0xffffffffu, l, s));
   const bool seen = !(l == 0.0f);  // NaN counts as seen
 #pragma unroll
-  for (int c = 0; c < VPL; ++c) o[c] = seen ? __fmul_rn(__fdiv_rn(o[c], l), 4194304.0f) : 0.0f;
+  for (int c = 0; c < VPL; ++c) o[c] = seen ? __fdiv_rn(o[c], l) : 0.0f;
   return seen ? __fadd_rn(m, log2f(l)) : -INFINITY;
 }
 

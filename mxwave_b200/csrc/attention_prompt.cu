@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
                 P.window > 0 ? max(0, pos_k - P.window + 1) : 0, P.causal ? min(pos_k + 1, u.length) : u.length, v);
             const int64_t row_k = static_cast<int64_t>(u.q0 + i_k) * P.heads + h_k;
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) att_store<BF16>(P.out, row_k * D + lane * (D / 32) + c, v[c]);
+            for (int c = 0; c < D / 32; ++c) att_store<BF16>(P.out, row_k * D + lane * (D / 32) + c, __fmul_rn(v[c], kAttWideUnit));
             if (lane == 0 && P.lse) P.lse[row_k] = __fmul_rn(lse2, 0.69314718055994531f);
           }
         }

@@ -188,3 +188,28 @@ def test_wide_values_give_equal_bits() -> None:
     fused = torch.zeros(306, 8, 131, dtype=BF, device="cuda")
     fused[..., 3:] = case.query
     assert all(torch.equal(a, b) for a, b in zip(first, case.run(query=fused[..., 3:])))
+
+
+@pytest.mark.parametrize("lens, queries, heads, kv, page, dim", DECODE[:10] + PROMPTS)
+@pytest.mark.parametrize("by", [118, -112])
+def test_values_near_the_ends_of_the_range(lens, queries, heads, kv, page, dim, by) -> None:
+    """Sums in the units of the probabilities would overflow where the values themselves do not."""
+    case = RowCase(39, lens, queries, heads, kv, page, dim, BF)
+    for b, n in enumerate(lens):
+        if n:
+            case.raise_values(b, list(range(n)), by)
+    case.check_rows(*case.run())
+
+
+@pytest.mark.parametrize("queries", [1, 6])
+def test_an_overflowed_value_in_a_share_of_little_weight(queries) -> None:
+    """A value past fp32's range, in a block's share of the keys that next to nothing of the probability falls on."""
+    heads, n, page, dim = 2, 30000, 64, 128
+    case = RowCase(40, [n], [queries], heads, heads, page, dim, BF)
+    case.query[:] = case.query[:1]
+    far = torch.arange(0, 20000, device="cuda")
+    key = (-20.0 * case.query[:1].float()).expand(len(far), -1, -1).contiguous()
+    value = randn(gen(41), len(far), heads, dim)
+    value[7777] = math.inf
+    kvcache.append_mxfp4_(case.codes, case.scales, key, value, case.slots(0)[far])
+    case.check_rows(*case.run())
