@@ -283,7 +283,8 @@ MXW_API int mxw_finalize_block_hessian(const float* gram, int full, int64_t cols
  *             mxw_linear_workspace_size(rows, inner, dtype) bytes; calls that
  *             share one must not overlap on the device
  * inner % 32 == 0; packed 16-byte aligned.  fp32 accumulation; the fixed order
- * of additions makes results reproducible.  A row of x that holds a NaN or an
+ * of additions makes results reproducible.  Elements of x under 2^-13 of the
+ * largest of their 32 are taken to within 2^-22 of it, all others exactly.  A row of x that holds a NaN or an
  * infinity gives NaN in all its outputs; so does a scale byte 255.
  * flags: MXW_FLAG_TIMEOUT or NULL; outputs whose wait gave up are NaN.
  */

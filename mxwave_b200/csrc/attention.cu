@@ -40,9 +40,9 @@
 // log-sum-exp) in the workspace, two slots per block, and attention_join_kernel
 // adds them in block order.
 // Measured: 32 sequences of 1 to 65,536 keys, 40 heads over 8 of 128, one query
-// each: 187 us, 4.3 TB/s of cache and rows, 66% of the copy rate; bound by its
+// each: 192 us, 4.2 TB/s of cache and rows, 65% of the copy rate; bound by its
 // instructions (some 340 a warp per 16 keys, half of them conversions and matrix
-// instructions; 61% of the issue slots with 16 warps an SM).  One sequence of 517 keys: 12.2 us.
+// instructions; 61% of the issue slots with 16 warps an SM).  One sequence of 517 keys: 13.2 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       const uint8_t* sc = scales + static_cast<uint64_t>(at) * page_scales + in_page * BLOCKS;
 #pragma unroll
       for (int k = 0; k < Shape::kCodes / 512; ++k) {
-        cp_async<16>(st + key_put + (k * 512), kc + k * 512, bytes);
-        cp_async<16>(st + value_put + (Shape::kCodes + k * 512), vc + k * 512, bytes);
+        cp_async16(st + key_put + (k * 512), kc + k * 512, bytes);
+        cp_async16(st + value_put + (Shape::kCodes + k * 512), vc + k * 512, bytes);
       }
       cp_async16_if(lane < 2 * SC, st + lane * 16 + 2 * Shape::kCodes, sc, bytes);
       return ok ? 1u : 0u;

@@ -19,10 +19,11 @@
 // tile), spread K's codes and decode V; warps 12 and 13 issue the products of a
 // row tile each, so that one's waits are covered by the other's products.
 // What bounds it: the chain of a row tile from scores to probabilities to the
-// next scores, some 2700 cycles per 64 keys, in which the products take 1300
+// next scores, some 2600 cycles per 64 keys, in which the products take 1300
 // (the scores' narrow ones are held back by their operands' shared-memory reads)
 // and the 16,384 exponentials 1024.  Four prompts of up to 3001 new tokens over
-// up to 1000 cached ones, 40 heads over 8 of 128, bf16: 598 us, 500 TFLOP/s.
+// up to 1000 cached ones, 40 heads over 8 of 128, bf16: 575 us, 520 TFLOP/s; f16, with
+// three terms, 624 us.
 #include "attention.cuh"
 #include "blockscale.cuh"
 #include "common.cuh"
@@ -443,13 +444,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
             const int offset = (key + key_e + 128 / BLOCKS * j) & page_mask;
             const uint8_t* kc = codes + static_cast<uint64_t>(in ? static_cast<uint32_t>(next[j]) : 0u) * page_codes + offset * (D / 2);
             const uint32_t bytes = in ? 16u : 0u;
-            cp_async<16>(st + (e + 128 * j) * 16, kc, bytes);
-            cp_async<16>(st + Shape::kRawCodes + (e + 128 * j) * 16, kc + to_values, bytes);
+            cp_async16(st + (e + 128 * j) * 16, kc, bytes);
+            cp_async16(st + Shape::kRawCodes + (e + 128 * j) * 16, kc + to_values, bytes);
           }
           if (e < 2 * SCALES) {
             const bool in = static_cast<uint32_t>(next_scale) < static_cast<uint32_t>(P.pages);
             const uint8_t* sc = scales + static_cast<uint64_t>(in ? static_cast<uint32_t>(next_scale) : 0u) * page_scales + ((key + scale_key) & page_mask) * BLOCKS;
-            cp_async<16>(st + 2 * Shape::kRawCodes + e * 16, sc, in ? 16u : 0u);
+            cp_async16(st + 2 * Shape::kRawCodes + e * 16, sc, in ? 16u : 0u);
           }
           strays = (strays & ~(1u << (n & 3))) | (stray << (n & 3));
           look_up(t + 1);

@@ -257,7 +257,6 @@ struct PageCopy {
   uint8_t* scales;
   int64_t pages, layers;
   int64_t code_vec, scale_vec;  // 16-byte vectors of one page
-  int n;
 };
 
 constexpr int kCopyVecs = 4;  // vectors per thread: enough loads in flight to cover HBM's latency
@@ -291,17 +290,17 @@ __global__ void __launch_bounds__(kKvThreads) copy_pages_kernel(const PageCopy P
 }
 
 template <int N>
-static int launch_copy(PageCopy P, const int64_t* source, const int64_t* target, int64_t n, cudaStream_t s) {
+static int launch_copy(const PageCopy& P, const int64_t* source, const int64_t* target, int64_t n, cudaStream_t s) {
   const unsigned blocks =
       static_cast<unsigned>((P.code_vec + P.scale_vec + kKvThreads * kCopyVecs - 1) / (kKvThreads * kCopyVecs));
   PagePairs<N> pairs;
   for (int64_t done = 0; done < n; done += N) {
-    P.n = static_cast<int>(std::min<int64_t>(N, n - done));
+    const int now = static_cast<int>(std::min<int64_t>(N, n - done));
     for (int i = 0; i < N; ++i) {
-      pairs.source[i] = i < P.n ? static_cast<int32_t>(source[done + i]) : 0;
-      pairs.target[i] = i < P.n ? static_cast<int32_t>(target[done + i]) : 0;
+      pairs.source[i] = i < now ? static_cast<int32_t>(source[done + i]) : 0;
+      pairs.target[i] = i < now ? static_cast<int32_t>(target[done + i]) : 0;
     }
-    copy_pages_kernel<N><<<dim3(blocks, static_cast<unsigned>(P.n), static_cast<unsigned>(P.layers)), kKvThreads, 0, s>>>(
+    copy_pages_kernel<N><<<dim3(blocks, static_cast<unsigned>(now), static_cast<unsigned>(P.layers)), kKvThreads, 0, s>>>(
         P, pairs);
     const int status = check_launch();
     if (status != MXW_OK) return status;

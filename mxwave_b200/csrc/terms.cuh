@@ -33,8 +33,8 @@ template <int NT, int TERMS>
 struct LinearTile {
   static constexpr bool kFused = NT == 16;  // terms made in the product's kernel
   // Small tiles take the terms as rows of one operand (and add up their columns
-  // at the end): a quarter of the instructions, which one thread issues at some
-  // 65 cycles each.
+  // at the end): a half or a third of the products' instructions, which are issued
+  // one after the other.
   static constexpr bool kMerged = NT < 128;
   static constexpr int kTermBytes = NT * kLinK;
   static constexpr int kN = kMerged ? TERMS * NT : NT;               // columns of the accumulator

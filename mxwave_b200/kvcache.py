@@ -161,7 +161,8 @@ def paged_attention_mxfp4(
     reaches, and a row of `query` behind the last sequence, gives zeros (and
     -inf).  Equal calls give equal bits.  There is no gradient.
 
-    Scores, statistics and sums are fp32; values times their scales are exact,
+    Scores, statistics and sums are fp32 (long prompts take queries as
+    ``linear_mxfp4`` takes x); values times their scales are exact,
     and probabilities are held to 2^-11 of themselves and 2^-32 of their row's
     largest (f16).  A key that a row's mask hides has no say in it, however
     large its value.  Where the values' scales that the rows of a head see span

@@ -37,8 +37,10 @@ def linear_mxfp4(
     uint8 as ``quantize_mxfp4`` returns them; bias [out] and residual
     [..., out] of x's type.  Returns [..., out] of x's type.  Sums are fp32 and
     rounded once, after the residual; the order of additions is fixed, so equal
-    calls give equal bits.  A row of x that holds a NaN or an infinity gives
-    NaN in all its outputs.  There is no gradient.
+    calls give equal bits.  Products are taken of x as it is where an element is
+    at least 2^-13 of the largest of its 32, and of x to within 2^-22 of that
+    largest where it is smaller.  A row of x that holds a NaN or an infinity
+    gives NaN in all its outputs.  There is no gradient.
     """
     act = ACTIVATIONS.get(activation)
     if act is None:

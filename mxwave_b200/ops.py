@@ -310,7 +310,7 @@ def _linear_mxfp4(x: Tensor, packed: Tensor, scales: Tensor, bias: Tensor | None
     lib = _lib.load()
     code = _DTYPE_CODES[x.dtype]
     nbytes = lib.mxw_linear_workspace_size(rows, inner, code)
-    # Up to 16 rows the kernel needs none: any address will do.
+    # Up to four rows the kernel needs none: any address will do.
     workspace = packed if nbytes <= 16 else packed.new_empty(nbytes)
     _call(lib.mxw_linear_mxfp4, x.device.index, (
         x.data_ptr(), code, rows, inner, x.stride(0) if rows > 1 else inner, packed.data_ptr(), scales.data_ptr(), outs,
