@@ -352,7 +352,8 @@ MXW_API int mxw_copy_pages(uint8_t* codes, uint8_t* scales, int64_t layers, int6
  * fp32 statistics and sums in a fixed order; probabilities are held to 2^-11 of
  * themselves and 2^-32 of their row's largest, values exactly.  A key that a
  * row's mask hides has no say in it, however large its value; rows of a head
- * that see values of scales more than 2^20 apart take a slower path in fp32.
+ * that see values of scales more than 2^20 apart within 32 channels, or 2^27 over
+ * all, take a far slower path in fp32.
  * flags: MXW_FLAG_TIMEOUT or NULL; outputs whose wait gave up are NaN.
  */
 MXW_API size_t mxw_paged_attention_workspace_size(int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim,

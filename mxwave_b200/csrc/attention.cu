@@ -73,11 +73,12 @@ constexpr int kAttStart = 4;
 // 300, 516, 1000 keys 9.8, 12.2, 15.0 and 12.7, 12.4, 12.6 us; 64 sequences of 300,
 // 700, 1100 keys 17, 23, 30 and 25, 32, 39 us).
 constexpr int kAttWhole = 12, kAttWholeFew = 6;
-// Scales of values this many powers of two below the largest are not looked at
-// one by one: tracking the smallest in every step took 197 us where this takes
-// 192 (32 sequences of 1 to 65,536 keys; 187 without a look at the range).  A rise
-// of the largest by more than kAttSpan - kAttQuiet then counts as a wide range.
-constexpr int kAttQuiet = 10;
+// Scales of values up to this many powers of two below the largest so far are not
+// looked at one by one: tracking the smallest in every step took 197 us where this
+// takes 192 (32 sequences of 1 to 65,536 keys; 187 without a look at the range).
+// So the range is looked at closer when the largest rises by more than kAttSpan
+// - kAttQuiet.
+constexpr int kAttQuiet = 16;
 // Partial results are this much of themselves: 6 x 2^127, an overflowed value, is finite, and nothing where its share weighs nothing.
 constexpr float kAttPartial = 0.0625f;
 
@@ -211,10 +212,18 @@ struct AttShape {
   static constexpr int kSlot = kRows * D + kRows;  // floats of a partial result
 };
 
-// A call: its registers are not the kernel's.
+// What odd data needs, as calls: their registers are not the kernel's (inline, the
+// ragged batch took 196 us instead of 192).
 template <bool BF16, int D>
 __device__ __noinline__ float row_wide(const AttParams& P, int b, int head, const uint16_t* q, int from, int to, float (&o)[D / 32]) {
   return att_row_wide<BF16, D>(P, b, head, q, from, to, o);
+}
+
+template <int D>
+__device__ __noinline__ uint64_t segment_range(const AttParams& P, int b, int head, int from, int to, int warp) {
+  AttRange<D> range;
+  range.look(P, b, head, from, to, warp, kAttWarps);
+  return static_cast<uint64_t>(range.top) << 32 | range.low;
 }
 
 template <bool BF16, int D, int NT>
@@ -227,8 +236,8 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
   extern __shared__ __align__(128) uint8_t att_smem[];
   __shared__ int64_t red[kAttWarps];
   __shared__ float row_m[kAttWarps][ROWS], row_l[kAttWarps][ROWS];
-  __shared__ uint32_t warp_low[kAttWarps];  // the smallest scale but zero of the values so far, less one (or a bound: see kAttQuiet)
-  __shared__ int warp_ref[kAttWarps];       // ref below; 256 where the range is wide
+  __shared__ int warp_first[kAttWarps];     // ref at its first value; 0 once a scale below kAttQuiet has been met
+  __shared__ int warp_ref[kAttWarps];       // ref below, and 256 where the range may be wide
   grid_dependents_launch();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -424,7 +433,7 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       l[nt][0] = l[nt][1] = 0.0f;
     }
     int ref = 0;  // exponent byte that the values are relative to
-    if (lane == 0) warp_low[warp] = 0xffffu;
+    if (lane == 0) warp_first[warp] = 0;
 
     int stage = 0;
     for (int step = skip; step < steps; ++step) {
@@ -554,9 +563,9 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int c = 0; c < 2; ++c) low2 = __viaddmin_u16x2(sv[half][c], 0xffffffffu, low2);
-        uint32_t low = __reduce_min_sync(0xffffffffu, min(low2 & 0xffffu, low2 >> 16));
-        if (top > ref && ref > 0) low = min(low, static_cast<uint32_t>(max(ref - kAttQuiet, 1) - 1));  // of the steps not looked at
-        if (lane == 0) warp_low[warp] = min(warp_low[warp], low);
+        if (ref == 0 && lane == 0) warp_first[warp] = top;
+        __syncwarp();
+        if (static_cast<int>(min(low2 & 0xffffu, low2 >> 16)) + 1 < max(ref, top) - kAttQuiet) warp_first[warp] = 0;
         if (top > ref) {
           const float f = exp2i(max(ref - top, -149));
           ref = top;
@@ -634,10 +643,10 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
           row_l[warp][8 * nt + 2 * t + c] = x;
         }
       }
-    const uint32_t low = (warp_low[warp] + 1u) & 0xffffu;
-    if (lane == 0) warp_ref[warp] = ref - static_cast<int>(low) > kAttSpan ? 256 : ref;  // (without any value both are zero)
+    __syncwarp();
+    if (lane == 0) warp_ref[warp] = ref + (ref - warp_first[warp] > kAttSpan - kAttQuiet ? 256 : 0);
     __syncthreads();  // (the rings are drained too: `join` takes their place)
-    const int ref_all = max(max(warp_ref[0], warp_ref[1]), max(warp_ref[2], warp_ref[3]));
+    const int ref_all = max(max(warp_ref[0] & 255, warp_ref[1] & 255), max(warp_ref[2] & 255, warp_ref[3] & 255));
     const float back = exp2i(max(ref - ref_all, -149));  // (to the values' own size only when divided: the sums could overflow)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -660,12 +669,24 @@ __global__ void __launch_bounds__(kAttThreads, AttShape<D, NT>::kBlocks) attenti
       for (int w = 0; w < kAttWarps; ++w) none &= row_l[w][r] == 0.0f;
       return none;
     };
-    const bool again = __syncthreads_or(threadIdx.x < n_rows && empty(threadIdx.x));
-    const bool wide = ref_all == 256;
+    const bool again = __syncthreads_or((threadIdx.x < n_rows && empty(threadIdx.x)) || warp_ref[warp] >= 256);
+    bool wide = false;
     const bool whole = tile0 == 0 && tile1 == seq.tiles;
     float* slot = P.partial + (2 * static_cast<int64_t>(blockIdx.x) + (opens ? 0 : 1)) * Shape::kSlot;
-    if (__builtin_expect(again | wide, 0)) {
+    if (__builtin_expect(again, 0)) {
       const AttSeq seq = att_seq<ROWS>(P, b);  // (read again: kept over the steps above, it would cost them registers)
+      if (((warp_ref[0] | warp_ref[1] | warp_ref[2] | warp_ref[3]) & 256) != 0) {
+        const int pos0 = seq.length - seq.queries + row0 / P.group, pos1 = seq.length - seq.queries + (row0 + n_rows - 1) / P.group;
+        const int from = max(seq.lo + tile0 * kAttTile, P.window > 0 ? pos0 - P.window + 1 : 0);
+        const int to = min(min(seq.lo + tile1 * kAttTile, seq.length), P.causal ? pos1 + 1 : seq.length);
+        AttRange<D> range;
+        const uint64_t part = segment_range<D>(P, b, head, from, to, warp);
+        if (lane == 0) red[warp] = static_cast<int64_t>(part);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kAttWarps; ++w) range.add(static_cast<uint32_t>(red[w] >> 32), static_cast<uint32_t>(red[w]));
+        wide = range.wide();
+      }
       for (int r = warp; r < n_rows; r += kAttWarps) {
         if (!wide && !empty(r)) continue;
         const int i_q = (row0 + r) / P.group, h = head * P.group + (row0 + r) - i_q * P.group;

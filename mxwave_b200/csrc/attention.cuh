@@ -14,15 +14,17 @@ namespace mxw {
 constexpr float kAttLift = 7.0f;    // probabilities are held as 2^(x - m + 7)
 constexpr float kAttSlack = 8.0f;   // and x may pass m by 8 before m is raised: at most 2^15
 // Both kernels hold values and probabilities in f16, relative to the largest of
-// each.  A value 2^28 below the largest would be lost, and a probability keeps
-// 2^-32 of its row's largest: good for any rows whose values' scales lie within
-// this many powers of two of one another (the probability's part is then 2^-12
-// of the smallest scale).  Rows with a wider range are done again by
-// att_row_wide, so that a key counts by its probability alone, and one that a
-// row does not see not at all.  That is a path for odd data (an overflowed
-// value, say): it takes 11 ms where 32 sequences of 1 to 65,536 keys take 0.19,
-// and 139 where four prompts of up to 3001 tokens take 0.57.
-constexpr int kAttSpan = 20;
+// each.  A value is exact down to 2^-27 of the largest scale, and a probability
+// keeps 2^-32 of its row's largest: good for any rows whose values' scales lie
+// within kAttExact powers of two of one another, and those of the same 32
+// channels within kAttSpan (the probability's part is then 2^-12 of the smallest
+// scale).  Rows with a wider range are done again by att_row_wide, so that a key
+// counts by its probability alone, and one that a row does not see not at all.
+// That is a path for odd data (an overflowed value, say): it takes 11 ms where 32
+// sequences of 1 to 65,536 keys take 0.19, and 137 where four prompts of up to
+// 3001 tokens take 0.59.  The kernels only watch whether the range over all
+// channels may exceed kAttSpan; AttRange then looks closer.
+constexpr int kAttSpan = 20, kAttExact = 27;
 
 // The bits of infinity in the queries' type; what has more is NaN.
 template <bool BF16>
@@ -76,6 +78,43 @@ __device__ __forceinline__ void att_clear_rest(const AttParams& P, int dim, int6
     if (P.lse && i % width < P.heads) P.lse[token * P.heads + i % width] = -INFINITY;
   }
 }
+
+// The range of the values' scales over keys, by blocks of 32 channels: a byte for
+// each of the D / 32 blocks.
+template <int D>
+struct AttRange {
+  uint32_t top = 0, low = 0xffffffffu;  // the largest, and the smallest but zero, less one
+  // This warp's part of the keys in [from, to): 32 of every 32 `warps`, from the `warp`-th 32 on.
+  __device__ __forceinline__ void look(const AttParams& P, int b, int head, int from, int to, int warp, int warps) {
+    const int32_t* table = P.table + static_cast<int64_t>(b) * P.table_ld;
+#pragma unroll 4
+    for (int key = from + 32 * warp + static_cast<int>(threadIdx.x & 31); key < to; key += 32 * warps) {
+      const int32_t page = table[key >> P.page_shift];
+      if (static_cast<uint32_t>(page) >= static_cast<uint64_t>(P.pages)) continue;
+      const int64_t row = (((static_cast<int64_t>(page) * 2 + 1) * P.kv_heads + head) << P.page_shift) + (key & ((1 << P.page_shift) - 1));
+      const uint32_t word = D == 128 ? reinterpret_cast<const uint32_t*>(P.scales)[row] : reinterpret_cast<const uint16_t*>(P.scales)[row];
+      add(word, __vsub4(word, 0x01010101u));
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) add(__shfl_xor_sync(0xffffffffu, top, s), __shfl_xor_sync(0xffffffffu, low, s));
+  }
+  __device__ __forceinline__ void add(uint32_t more_top, uint32_t more_low) {
+    top = __vmaxu4(top, more_top);
+    low = __vminu4(low, more_low);
+  }
+  __device__ __forceinline__ bool wide() const {
+    int all_top = 0, all_low = 256;
+    bool wide = false;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      const int t = (top >> (8 * k)) & 255, least = static_cast<int>(((low >> (8 * k)) + 1u) & 255u);  // both 0: none
+      wide |= t - least > kAttSpan;
+      all_top = max(all_top, t);
+      if (least > 0) all_low = min(all_low, least);
+    }
+    return wide || all_top - all_low > kAttExact;
+  }
+};
 
 // One row in fp32 throughout, for rows whose values differ widely in size: every
 // key in [from, to) counts (pages outside the pool do not).  `q`: the row's D

@@ -19,11 +19,11 @@
 // tile), spread K's codes and decode V; warps 12 and 13 issue the products of a
 // row tile each, so that one's waits are covered by the other's products.
 // What bounds it: the chain of a row tile from scores to probabilities to the
-// next scores, some 2600 cycles per 64 keys, in which the products take 1300
+// next scores, some 2700 cycles per 64 keys, in which the products take 1300
 // (the scores' narrow ones are held back by their operands' shared-memory reads)
 // and the 16,384 exponentials 1024.  Four prompts of up to 3001 new tokens over
-// up to 1000 cached ones, 40 heads over 8 of 128, bf16: 575 us, 520 TFLOP/s; f16, with
-// three terms, 624 us.
+// up to 1000 cached ones, 40 heads over 8 of 128, bf16: 590 us, 507 TFLOP/s; f16, with
+// three terms, 610 us.
 #include "attention.cuh"
 #include "blockscale.cuh"
 #include "common.cuh"
@@ -352,7 +352,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attention_prompt_kernel(con
           if (!__all_sync(0xffffffffu, mbar_wait_cycles(&o_done[x], (count[x] + u.tiles - 1) & 1))) ok = false;
           tc_fence_after();
         }
-        const bool wide = ok && ref - static_cast<int>(low + 1u) > kAttSpan;  // the same in all warps of the block
+        bool wide = ok && ref - static_cast<int>(low + 1u) > kAttSpan;  // may be: the same in all warps of the block
+        if (wide) {
+          AttRange<D> range;
+          range.look(P, b, head, u.first, u.hi, 0, 1);
+          wide = range.wide();
+        }
         if (wide) {
           for (int k = 0; k < 32 && x * kPromptRows + 32 * quarter + k < u.rows; ++k) {
             const int at_k = u.row0 + x * kPromptRows + 32 * quarter + k, i_k = at_k / P.group;

@@ -165,8 +165,9 @@ def paged_attention_mxfp4(
     ``linear_mxfp4`` takes x); values times their scales are exact,
     and probabilities are held to 2^-11 of themselves and 2^-32 of their row's
     largest (f16).  A key that a row's mask hides has no say in it, however
-    large its value.  Where the values' scales that the rows of a head see span
-    more than 2^20, those rows take fp32 throughout, which is far slower.
+    large its value.  Where the scales of the values that the rows of a head see
+    span more than 2^20 within 32 channels, or 2^27 over all, those rows take
+    fp32 throughout, which is far slower.
     """
     if ops.binding is not None and not torch.compiler.is_compiling():
         got = ops.binding.attention(query, codes, scales, table, lengths, query_start, max_length, max_queries, softmax_scale, causal, window,

@@ -126,7 +126,7 @@ def test_improbable_keys_count_by_their_probability(queries, size, by, n) -> Non
     case.check_rows(*case.run())
 
 
-@pytest.mark.parametrize("dtype, by", [(BF, -60), (BF, 50), (HF, -14), (HF, 30)])
+@pytest.mark.parametrize("dtype, by", [(BF, -60), (BF, 50), (BF, -24), (BF, 22), (HF, -14), (HF, 30)])
 @pytest.mark.parametrize("lens, queries, heads, kv, page, dim", DRAFTS[:2] + PROMPTS[1:])
 def test_channel_blocks_of_different_size(lens, queries, heads, kv, page, dim, dtype, by) -> None:
     """The first 32 channels of every value are 2^by times the others."""
